@@ -81,6 +81,15 @@ int qimm_stream_synchronize(qimm_ctx *ctx, void *stream);
 
 /* ---------------- quantized weights ---------------- */
 
+/* One GGUF tensor in host memory, as the quantized VarBuilder returns it. */
+typedef struct {
+    int ggml_type;
+    int64_t rows;      /* out features (GGUF ne[1]) */
+    int64_t cols;      /* in features (GGUF ne[0]) */
+    const void *data;  /* NULL = absent */
+    size_t nbytes;
+} qimm_tensor;
+
 /* Whether the weights uploaded through ctx from here on (by themselves or with a
  * block or a model) keep their values as bf16 rows beside the codes: 2 bytes a
  * value, for which the products of many tokens run 1.1 to 1.5 times faster (f32
@@ -167,6 +176,38 @@ typedef struct {
 int qimm_qmatmul_route(int ggml_type, int64_t rows, int64_t cols, int bf16_rows, int64_t m,
                        int cus, qimm_gemm_route *out);
 
+/* ---------------- low-rank adapters ---------------- */
+
+/* Low-rank adapters (LoRA) of a projection whose weight stays shared and quantized: of a
+ * batch of requests, each row of the product takes its own request's adapter, or none. A
+ * qimm_adapters holds the adapters of one projection [rows, cols]: a [rank, cols] and b
+ * [rows, rank], F32, F16 or BF16 in host memory, kept as bf16 (nearest even) on the device;
+ * scale multiplies their product (alpha / rank of the usual files). Ranks may differ, 1 to
+ * QIMM_ADAPTER_MAX_RANK; rows a multiple of 128, cols of 64; 1 to 65535 adapters. No
+ * counterpart in the reference. */
+typedef struct qimm_adapters qimm_adapters;
+#define QIMM_ADAPTER_MAX_RANK 1024
+typedef struct {
+    float scale;
+    qimm_tensor a, b;
+} qimm_adapter;
+int qimm_adapters_create(qimm_ctx *ctx, int64_t rows, int64_t cols, const qimm_adapter *list, int64_t n,
+                         qimm_adapters **out);
+int qimm_adapters_destroy(qimm_adapters *ad);
+int64_t qimm_adapters_device_bytes(const qimm_adapters *ad);
+
+/* y[m] = x[m] W^T + scale_a (x[m] A_a^T) B_a^T with a = ids[m], int32 [m] on the device;
+ * an id outside [0, n) is a row without an adapter. The rest as qimm_qmatmul (the same
+ * checks, the same products of W); sums are f32, y is rounded once. Rows of one adapter
+ * next to each other are fastest: a tile of rows is multiplied once per adapter in it.
+ * Scratch is the context's and grows like qimm_qmatmul's; after a
+ * qimm_qmatmul_adapters_reserve with at least this m (same weight, adapters and out_type)
+ * the call neither allocates nor synchronizes and can be captured. ids, x and the adapters'
+ * choice may change between replays. */
+int qimm_qmatmul_adapters(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapters *ad, const int32_t *ids,
+                          const void *x_bf16, int64_t m, int64_t lda, void *y, int out_type, void *stream);
+int qimm_qmatmul_adapters_reserve(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapters *ad, int64_t m, int out_type);
+
 /* ---------------- host-side layout and RoPE ---------------- */
 
 /* JointLayout::new (src/joint_layout.rs:52-103). text_image_mask may be NULL
@@ -223,6 +264,31 @@ int qimm_kv_is_host(const qimm_kv *kv);
  * src/transformer.rs:43-45; the prefetch is this library's overlap of it.) */
 int qimm_kv_prefetch(qimm_kv *kv, int64_t layer, void *stream);
 
+/* The cache held in 4 bits: the same object with every layer in 4.25 bits a value,
+ * 3.76 times smaller than bf16, for long prefixes and for many requests at once. Blocks
+ * of 32 values share one power of two 2^s, s the smallest integer with max|x| <= 7 2^s,
+ * within [-120, 125]; a value stands for the nearest of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} 2^s,
+ * ties to the even code. A key's blocks run along its dimensions, a value's along 32
+ * consecutive keys of one dimension (keys 32 i .. 32 i + 31 of the prefix).
+ * Every call that takes a qimm_kv works on it. qimm_kv_store_layer encodes a layer,
+ * qimm_kv_load_layer gives what it stands for (exact in bf16); k and v must be 16-byte
+ * aligned in both. The attention of up to 64 queries multiplies the codes as they lie; with
+ * more, and in the block and the model, the layer is expanded first into one bf16 layer that
+ * the cache keeps for it. Nothing is allocated after the creation. That layer and the
+ * attention's scratch belong to the cache: calls with one cache must not overlap on the
+ * device, two replayed graphs neither. The values of 32 keys share a scale, so one that is
+ * no number does not spoil its neighbours: a NaN is stored as 0, an infinity as +-6 2^s of
+ * the block's numbers. A key's block with a NaN or an infinity stands for NaN: its score is
+ * NaN unless a mask hides the key. qimm_model_prefix_fill stores the keys and values of
+ * tokens that key_valid hides as zeros; through qimm_kv_store_layer they are stored as they
+ * are, so very large values of hidden tokens would coarsen their 31 neighbours'.
+ * batch * heads at most 65535. No counterpart in the reference. */
+int qimm_kv_create_q4(qimm_ctx *ctx, int64_t layers, int64_t batch, int64_t heads,
+                      int64_t prefix_len, int64_t head_dim, qimm_kv **out);
+/* Bits of a stored value: 16 or 4 (-1 for NULL); device memory the cache holds. */
+int qimm_kv_bits(const qimm_kv *kv);
+int64_t qimm_kv_device_bytes(const qimm_kv *kv);
+
 /* ---------------- attention ---------------- */
 
 /* Per-head RmsNorm (eps 1e-6, weight norm_w[128] device f32) then RoPE with
@@ -272,15 +338,6 @@ typedef struct {
     int64_t head_dim;  /* must be 128 */
     int64_t mlp;       /* Config::mlp_hidden_size = 3 * hidden (src/transformer.rs:86-88) */
 } qimm_block_config;
-
-/* One GGUF tensor in host memory, as the quantized VarBuilder returns it. */
-typedef struct {
-    int ggml_type;
-    int64_t rows;      /* out features (GGUF ne[1]) */
-    int64_t cols;      /* in features (GGUF ne[0]) */
-    const void *data;  /* NULL = absent */
-    size_t nbytes;
-} qimm_tensor;
 
 /* The tensors of transformer_blocks.{i} (src/quantized_transformer.rs:99-111,
  * 173-188): attn.to_q/to_k/to_v/to_out.0, attn.norm_q/norm_k [128],

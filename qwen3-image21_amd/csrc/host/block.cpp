@@ -514,6 +514,27 @@ int qimm_quantize_act(qimm_ctx *ctx, int weight_type, const float *x, int64_t m,
     return QIMM_OK;
 }
 
+}  // extern "C"
+
+namespace {
+
+// Few queries over a 4-bit cache: the kernel that multiplies its codes. Many take the
+// expanded layer like any other cache's.
+bool takes_codes(const qimm_kv *kv, int64_t sq) { return kv && kv->bits4 && qimm::attn4_takes(sq); }
+
+int attention_codes(qimm_ctx *ctx, const uint16_t *q, int64_t batch, int64_t heads, int64_t sq, const qimm_kv *kv,
+                    int64_t layer, const uint16_t *k_own, const uint16_t *vt_own, int64_t so, float scale,
+                    const uint8_t *kvalid, uint16_t *out, hipStream_t s) {
+    QIMM_HIP(ctx, hipSetDevice(ctx->device));
+    QIMM_HIP(ctx, qimm::launch_attn4(q, kv->q4 + layer * kv->q4_layer(), kv->prefix, k_own, vt_own, so, kvalid, batch, heads,
+                                     sq, scale, kv->q4_part, out, s));
+    return QIMM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
 int qimm_attention(qimm_ctx *ctx, const uint16_t *q, int64_t batch, int64_t heads, int64_t sq, const qimm_kv *kv,
                    int64_t layer, const uint16_t *k_own, const uint16_t *vt_own, int64_t so, float scale,
                    uint16_t *out, void *stream) {
@@ -530,6 +551,8 @@ int qimm_attention(qimm_ctx *ctx, const uint16_t *q, int64_t batch, int64_t head
     }
     if (P + so == 0) return set_err(ctx, QIMM_ERR_SHAPE, "attention: no keys");
     const hipStream_t s = (hipStream_t)stream;
+    if (takes_codes(kv, sq))
+        return attention_codes(ctx, q, batch, heads, sq, kv, layer, k_own, vt_own, so, scale, nullptr, out, s);
     qimm::KeySeg prefix{};
     if (kv) {
         const int rc = kv_layer(kv, layer, s, &prefix);
@@ -559,6 +582,8 @@ int qimm_attention_masked(qimm_ctx *ctx, const uint16_t *q, int64_t batch, int64
     if (mask->image_ids && (P != 0 || so != sq))
         return set_err(ctx, QIMM_ERR_SHAPE, "attention: the block-causal mask needs no prefix and so == sq");
     const hipStream_t s = (hipStream_t)stream;
+    if (takes_codes(kv, sq) && !mask->image_ids)
+        return attention_codes(ctx, q, batch, heads, sq, kv, layer, k_own, vt_own, so, scale, mask->key_valid, out, s);
     int32_t *lim = nullptr;
     if (mask->image_ids) {
         QIMM_HIP(ctx, hipSetDevice(ctx->device));

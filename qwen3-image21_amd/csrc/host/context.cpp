@@ -191,7 +191,12 @@ hipError_t kv_alloc_norms(qimm_kv *kv) {
 void kv_free(qimm_kv *kv) {
     if (kv->knorm) (void)hipFree(kv->knorm);
     if (kv->knorm_part) (void)hipFree(kv->knorm_part);
-    if (kv->host) {
+    if (kv->q4) (void)hipFree(kv->q4);
+    if (kv->q4_part) (void)hipFree(kv->q4_part);
+    if (kv->bits4) {
+        if (kv->slot[0].k) (void)hipFree(kv->slot[0].k);
+        if (kv->slot[0].vt) (void)hipFree(kv->slot[0].vt);
+    } else if (kv->host) {
         if (kv->k) (void)hipHostFree(kv->k);
         if (kv->vt) (void)hipHostFree(kv->vt);
         for (auto &sl : kv->slot) {
@@ -242,6 +247,15 @@ namespace qimm_host {
 
 int kv_layer(const qimm_kv *kv, int64_t layer, hipStream_t s, qimm::KeySeg *seg) {
     *seg = qimm::KeySeg{nullptr, nullptr, kv->prefix, qimm::vt_ld(kv->prefix)};
+    if (kv->bits4) {
+        if (!kv->layer_elems()) return QIMM_OK;
+        seg->k = kv->slot[0].k;
+        seg->vt = kv->slot[0].vt;
+        QIMM_HIP(kv->ctx, hipSetDevice(kv->ctx->device));
+        QIMM_HIP(kv->ctx, qimm::launch_load4(kv->q4 + layer * kv->q4_layer(), kv->batch * kv->heads, kv->prefix, seg->ld,
+                                             kv->slot[0].k, kv->slot[0].vt, s));
+        return QIMM_OK;
+    }
     if (!kv->host) {
         seg->k = kv->k + layer * kv->layer_elems();
         seg->vt = kv->vt + layer * kv->vt_elems();
@@ -297,6 +311,43 @@ int qimm_kv_create(qimm_ctx *ctx, int64_t layers, int64_t batch, int64_t heads, 
     return QIMM_OK;
 }
 
+int qimm_kv_create_q4(qimm_ctx *ctx, int64_t layers, int64_t batch, int64_t heads, int64_t prefix_len,
+                      int64_t head_dim, qimm_kv **out) {
+    if (!ctx || !out) return QIMM_ERR_ARG;
+    *out = nullptr;
+    if (batch > 0 && heads > 65535 / batch)
+        return set_err(ctx, QIMM_ERR_SHAPE, "kv cache in 4 bits: batch * heads must be at most 65535");
+    if (prefix_len > (int64_t)1 << 36) return set_err(ctx, QIMM_ERR_SHAPE, "kv cache in 4 bits: prefix too long");
+    qimm_kv *kv;
+    int rc = kv_new(ctx, layers, batch, heads, prefix_len, head_dim, &kv);
+    if (rc) return rc;
+    kv->bits4 = true;
+    hipError_t e = hipSetDevice(ctx->device);
+    if (kv->layer_elems()) {
+        if (e == hipSuccess) e = hipMalloc((void **)&kv->q4, (size_t)(layers * kv->q4_layer()));
+        if (e == hipSuccess) e = hipMalloc((void **)&kv->slot[0].k, (size_t)kv->layer_elems() * 2);
+        if (e == hipSuccess) e = hipMalloc((void **)&kv->slot[0].vt, (size_t)kv->vt_elems() * 2);
+        if (e == hipSuccess) e = kv_alloc_norms(kv);
+    }
+    if (e == hipSuccess) e = hipMalloc((void **)&kv->q4_part, qimm::attn4_scratch_bytes());
+    if (e != hipSuccess) {
+        kv_free(kv);
+        return hip_err(ctx, e, "hipMalloc(kv cache in 4 bits)");
+    }
+    *out = kv;
+    return QIMM_OK;
+}
+
+int qimm_kv_bits(const qimm_kv *kv) { return !kv ? -1 : kv->bits4 ? 4 : 16; }
+
+int64_t qimm_kv_device_bytes(const qimm_kv *kv) {
+    if (!kv) return -1;
+    const int64_t layer = (kv->layer_elems() + kv->vt_elems()) * 2;
+    const int64_t norms = kv->knorm ? kv->layers * 4 * (1 + qimm::QK_NORM_PARTS) : 0;
+    if (kv->bits4) return norms + kv->layers * kv->q4_layer() + layer + (int64_t)qimm::attn4_scratch_bytes();
+    return norms + layer * (kv->host ? 2 : kv->layers);
+}
+
 int qimm_kv_create_host(qimm_ctx *ctx, int64_t layers, int64_t batch, int64_t heads, int64_t prefix_len,
                         int64_t head_dim, qimm_kv **out) {
     if (!ctx || !out) return QIMM_ERR_ARG;
@@ -345,6 +396,14 @@ int qimm_kv_store_layer(qimm_kv *kv, int64_t layer, const uint16_t *k_bhpd, cons
     const int64_t n = kv->layer_elems(), nv = kv->vt_elems();
     if (!n) return QIMM_OK;
     hipStream_t s = (hipStream_t)stream;
+    if (kv->bits4) {
+        if (((uintptr_t)k_bhpd | (uintptr_t)v_bhpd) & 15)
+            return set_err(ctx, QIMM_ERR_ARG, "kv store: k and v must be 16-byte aligned for a 4-bit cache");
+        QIMM_HIP(ctx, hipSetDevice(ctx->device));
+        QIMM_HIP(ctx, qimm::launch_store4(k_bhpd, v_bhpd, 0, kv->batch, kv->heads, kv->prefix, nullptr, 0,
+                                          kv->q4 + layer * kv->q4_layer(), kv->knorm + layer, s));
+        return QIMM_OK;
+    }
     // the layer's largest key norm: the attention's score bound
     QIMM_HIP(ctx, qimm::launch_row_norm_max(k_bhpd, n / 128, kv->knorm_part + layer * qimm::QK_NORM_PARTS,
                                             kv->knorm + layer, s));
@@ -380,6 +439,14 @@ int qimm_kv_load_layer(const qimm_kv *kv, int64_t layer, uint16_t *k_bhpd, uint1
     const int64_t n = kv->layer_elems();
     if (!n) return QIMM_OK;
     hipStream_t s = (hipStream_t)stream;
+    if (kv->bits4) {
+        if (((uintptr_t)k_bhpd | (uintptr_t)v_bhpd) & 15)
+            return set_err(ctx, QIMM_ERR_ARG, "kv load: k and v must be 16-byte aligned for a 4-bit cache");
+        QIMM_HIP(ctx, hipSetDevice(ctx->device));
+        QIMM_HIP(ctx, qimm::launch_load4(kv->q4 + layer * kv->q4_layer(), kv->batch * kv->heads, kv->prefix, 0, k_bhpd,
+                                         v_bhpd, s));
+        return QIMM_OK;
+    }
     qimm::KeySeg seg;
     int rc = kv_layer(kv, layer, s, &seg);
     if (rc) return rc;

@@ -58,6 +58,13 @@ struct qimm_kv {
     mutable Slot slot[2];
     mutable int next = 0;
     hipEvent_t written = nullptr;
+    // 4-bit cache: layers of kv4_layer_bytes each (k, vt unused); slot[0] takes a layer
+    // expanded to bf16 where a kernel reads that, q4_part is the scratch of the attention
+    // of few queries
+    bool bits4 = false;
+    uint8_t *q4 = nullptr;
+    float *q4_part = nullptr;
+    int64_t q4_layer() const { return qimm::kv4_layer_bytes(batch * heads, prefix); }
     int64_t layer_elems() const { return batch * heads * prefix * head_dim; }
     int64_t vt_elems() const { return batch * heads * qimm::vt_ld(prefix) * head_dim; }
 };
@@ -92,6 +99,10 @@ int ensure_part_workspace(qimm_ctx *ctx, size_t bytes);
 int upload_weight_rows(qimm_ctx *ctx, int type, int64_t rows, int64_t cols, const uint8_t *bytes,
                        qimm_weight **out);
 int64_t row_bytes(int type, int64_t cols);
+// n values of a float type (F32, F16, BF16) rounded to bf16 (nearest even)
+void to_bf16(int type, const uint8_t *src, int64_t n, uint16_t *dst);
+// the checks of a product's arguments
+int qmatmul_check(qimm_ctx *ctx, const qimm_weight *w, const void *x_bf16, int64_t m, int64_t lda, void *y, int out_type);
 int block_values(int type);
 
 // The key segment of cache layer `layer` for kernels launched on stream s. A

@@ -289,12 +289,20 @@ int qimm_model_prefix_fill(qimm_model *m, const float *txt, int64_t text_len, co
         QIMM_HIP(ctx, qimm::launch_set_floats(kv->knorm, bound.data(), m->cfg.layers, s));
         for (int64_t i = 0; i < m->cfg.layers; i++) {
             qimm_block *blk = m->blocks[(size_t)i];
+            if (kv->bits4) {
+                // through the cache's bf16 slot; the keys that the prompt's padding hides are stored as zeros
+                rc = block_prefix_forward(blk, x, batch, P, modv, pe, mk, kv->slot[0].k, kv->slot[0].vt, stream);
+                if (rc) return rc;
+                QIMM_HIP(ctx, qimm::launch_store4(kv->slot[0].k, kv->slot[0].vt, qimm::vt_ld(P), batch, H, P, key_valid, P,
+                                                  kv->q4 + i * kv->q4_layer(), kv->knorm + i, s));
+                continue;
+            }
             rc = block_prefix_forward(blk, x, batch, P, modv, pe, mk, kv->k + i * kv->layer_elems(),
                                       kv->vt + i * kv->vt_elems(), stream);
             if (rc) return rc;
             if (blk->k_norm_bound < INFINITY) bound[(size_t)i] = blk->k_norm_bound;
         }
-        QIMM_HIP(ctx, qimm::launch_set_floats(kv->knorm, bound.data(), m->cfg.layers, s));
+        if (!kv->bits4) QIMM_HIP(ctx, qimm::launch_set_floats(kv->knorm, bound.data(), m->cfg.layers, s));
         return QIMM_OK;
     }
     for (int64_t i = 0; i < m->cfg.layers; i++) {

@@ -58,6 +58,21 @@ static inline float f16_to_f32(uint16_t h) {
     return f;
 }
 
+void to_bf16(int type, const uint8_t *src, int64_t n, uint16_t *dst) {
+    for (int64_t i = 0; i < n; i++) {
+        if (type == QIMM_TYPE_BF16) memcpy(&dst[i], src + 2 * i, 2);
+        else if (type == QIMM_TYPE_F16) {
+            uint16_t h;
+            memcpy(&h, src + 2 * i, 2);
+            dst[i] = f32_to_bf16_rne(f16_to_f32(h));
+        } else {
+            float f;
+            memcpy(&f, src + 4 * i, 4);
+            dst[i] = f32_to_bf16_rne(f);
+        }
+    }
+}
+
 // Lays the values of a quantized weight out as bf16 rows beside its codes, for
 // the products of many tokens: a matrix kernel over bf16 rows runs 1.38-1.52
 // PFLOP/s, one that decodes beside its MFMAs 1.10-1.18, while a few tokens are
@@ -157,19 +172,7 @@ int upload_weight_rows(qimm_ctx *ctx, int type, int64_t rows, int64_t cols, cons
             // F32 rounded to bf16 (nearest even).
             fmt = qimm::WF_BF16;
             main_bytes.resize((size_t)(rows * cols) * 2);
-            uint16_t *dst = (uint16_t *)main_bytes.data();
-            for (int64_t i = 0; i < rows * cols; i++) {
-                if (type == QIMM_TYPE_BF16) memcpy(&dst[i], src + 2 * i, 2);
-                else if (type == QIMM_TYPE_F16) {
-                    uint16_t h;
-                    memcpy(&h, src + 2 * i, 2);
-                    dst[i] = f32_to_bf16_rne(f16_to_f32(h));
-                } else {
-                    float f;
-                    memcpy(&f, src + 4 * i, 4);
-                    dst[i] = f32_to_bf16_rne(f);
-                }
-            }
+            to_bf16(type, src, rows * cols, (uint16_t *)main_bytes.data());
         }
     } catch (const std::bad_alloc &) {
         delete w;
@@ -240,9 +243,11 @@ int qimm_dequant(qimm_ctx *ctx, int ggml_type, const void *dev_bytes, int64_t n,
     return QIMM_OK;
 }
 
-namespace {
+}  // extern "C"
 
 static_assert(qimm::NOALLOC_SCRATCH_BYTES == QIMM_NOALLOC_SCRATCH_BYTES, "static scratch size of qimm.h");
+
+namespace qimm_host {
 
 int qmatmul_check(qimm_ctx *ctx, const qimm_weight *w, const void *x_bf16, int64_t m, int64_t lda, void *y,
                   int out_type) {
@@ -256,7 +261,9 @@ int qmatmul_check(qimm_ctx *ctx, const qimm_weight *w, const void *x_bf16, int64
     return QIMM_OK;
 }
 
-}  // namespace
+}  // namespace qimm_host
+
+extern "C" {
 
 int qimm_qmatmul(qimm_ctx *ctx, const qimm_weight *w, const void *x_bf16, int64_t m, int64_t lda, void *y,
                  int out_type, void *stream) {

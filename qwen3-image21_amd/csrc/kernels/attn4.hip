@@ -1,0 +1,431 @@
+// Attention of few queries over a prefix cache held in 4 bits (kv4.h) and own bf16 keys,
+// gfx950. Many queries take attention.hip over the expanded layer (attn4_takes).
+//
+// O = softmax(scale Q [K4 ; K]^T) [V4 ; V], hidden keys at -inf. One pass over the keys
+// with the running maximum and sum; f32 scores, sums and output, rounded to bf16 once.
+//
+// What bounds it: the cache's bytes, 4.25 bits a value, as long as the arithmetic beside
+// them stays below: HBM gives a CU about 13 B a clock, 25 values, so a decoding of two VALU
+// operations a value would already use up the SIMDs. The matrix pipe takes the codes and
+// their powers of two as they lie (v_mfma_scale_f32_16x16x128_f8f6f4, A = keys or values
+// in e2m1), so nothing is decoded. The other operand is e4m3 there, four significant bits:
+// queries and probabilities go in as the sum of two, x = hi + lo 2^-5, hi = e4m3(x) and
+// lo = e4m3((x - hi) 2^5), which holds a bf16 query's eight bits exactly (down to 2^-22
+// of its row's largest) and a probability to 2^-9, as the rounding to bf16 of the other
+// kernels does. Two products of 128 deep cost the matrix pipe what the bf16 ones would.
+//
+// A workgroup is 16 NQ queries of one head and a share of the keys, four waves taking
+// tiles of 128 keys in turn (64 own keys); a tile's 17 KB go straight into registers, the
+// next tile's keys while this one's softmax and P V run, its values after that: nothing
+// waits on a barrier until the waves' sums are joined through LDS. With several shares
+// (few rows, long caches) a second launch joins them.
+#include <algorithm>
+
+#include "kernels.h"
+#include "kv4.h"
+
+namespace qimm {
+namespace {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int OWN_KEYS = 64;
+
+__device__ __forceinline__ i32x8 widen(u32x4 c) {
+    return i32x8{(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
+}
+
+// four values below 448 as e4m3 hi (one word) and lo 2^5
+__device__ __forceinline__ void split4(float a, float b, float c, float d, int &hi, int &lo) {
+    int h = 0;
+    h = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, h, false);
+    h = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, h, true);
+    const f32x2 ab = __builtin_amdgcn_cvt_pk_f32_fp8(h, false), cd = __builtin_amdgcn_cvt_pk_f32_fp8(h, true);
+    int l = 0;
+    l = __builtin_amdgcn_cvt_pk_fp8_f32((a - ab[0]) * 32.f, (b - ab[1]) * 32.f, l, false);
+    l = __builtin_amdgcn_cvt_pk_fp8_f32((c - cd[0]) * 32.f, (d - cd[1]) * 32.f, l, true);
+    hi = h;
+    lo = l;
+}
+
+struct Attn4 {
+    const uint16_t *q;      // [B,H,Sq,128]
+    const uint8_t *tiles;   // [B*H][T] tiles
+    int64_t P, T;
+    const uint16_t *k_own;  // [B,H,So,128]
+    const uint16_t *vt_own; // [B,H,128,So]
+    int64_t So;
+    const uint8_t *kvalid;  // [B][P + So] or null
+    int64_t H, Sq;
+    float sl2;              // softmax scale * log2 e, >= 0 (q's sign is turned with `flip`)
+    uint32_t flip;          // 0x80008000 where the scale is negative
+    uint16_t *out;          // [B,Sq,H*128]
+    float *part;            // shares > 1: O [share][B*H*Sq][128], then (m, l) [share][B*H*Sq]
+    int shares;
+};
+
+template <int NQ, bool MASKED>
+__global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attn4_kernel(const Attn4 a) {
+    constexpr int PITCH = 132;  // floats per query row in LDS
+    __shared__ __attribute__((aligned(16))) float so[4 * 16 * NQ * PITCH];
+    __shared__ float sm[4][16 * NQ], sl[4][16 * NQ];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int l16 = lane & 15, lg = lane >> 4;
+    const int64_t bh = blockIdx.x / a.shares, b = bh / a.H;
+    const int share = (int)(blockIdx.x % a.shares);
+    const int64_t q0 = (int64_t)blockIdx.y * 16 * NQ;
+    const int64_t items = a.T + (a.So + OWN_KEYS - 1) / OWN_KEYS;
+    const int64_t first = items * share / a.shares, last = items * (share + 1) / a.shares;
+    const uint8_t *tiles = a.tiles + bh * a.T * KV4_TILE;
+
+    // ---- queries: lane (l16, lg) holds dimensions 16 lg .. + 15 and 64 + 16 lg .. + 15 of query
+    // l16, scaled by a power of two so that the row's largest lies in [128, 256) ----
+    i32x8 qhi[NQ], qlo[NQ];
+    int qsc[NQ];  // scale bytes: hi, lo
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        const int64_t qi = min(q0 + 16 * n + l16, a.Sq - 1);
+        const u32x4 *src = (const u32x4 *)(a.q + (bh * a.Sq + qi) * 128 + 16 * lg);
+        u32x4 w[4];
+        uint32_t mag = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            w[e] = src[8 * (e >> 1) + (e & 1)];
+#pragma unroll
+            for (int x = 0; x < 4; x++) mag = max(mag, max(w[e][x] & 0x7fffu, (w[e][x] >> 16) & 0x7fffu));
+        }
+        mag = max(mag, (uint32_t)__shfl_xor((int)mag, 16));
+        mag = max(mag, (uint32_t)__shfl_xor((int)mag, 32));
+        const int ex = (int)(mag >> 7);                            // biased exponent of the row's largest
+        const int by = ex == 255 ? 255 : max(ex - 7, 6);           // 2^(ex - 134), biased; no number: NaN
+        const float up = __uint_as_float((uint32_t)(254 - min(by, 253)) << 23);
+        qsc[n] = by | (by == 255 ? 255 : by - 5) << 8;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const uint32_t x = w[e >> 1][2 * (e & 1)] ^ a.flip, y = w[e >> 1][2 * (e & 1) + 1] ^ a.flip;
+            int hi, lo;
+            split4(__uint_as_float(x << 16) * up, __uint_as_float(x & 0xffff0000u) * up, __uint_as_float(y << 16) * up,
+                   __uint_as_float(y & 0xffff0000u) * up, hi, lo);
+            qhi[n][e] = hi;
+            qlo[n][e] = lo;
+        }
+    }
+
+    f32x4 o[NQ][8];  // [d tile]: dimensions 16 j + 4 lg + r of query l16
+    float m[NQ], l[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        m[n] = -INFINITY;
+        l[n] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) o[n][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    u32x4 kc[8], vc[8];
+    int ks[2], vs[2];
+    auto load_k = [&](int64_t it) __attribute__((always_inline)) {
+        const uint8_t *t = tiles + it * KV4_TILE;
+#pragma unroll
+        for (int i = 0; i < 8; i++) kc[i] = *(const u32x4 *)(t + (i * 64 + lane) * 16);
+#pragma unroll
+        for (int i = 0; i < 2; i++) ks[i] = *(const int *)(t + KV4_KS + (i * 64 + lane) * 4);
+    };
+    auto load_v = [&](int64_t it) __attribute__((always_inline)) {
+        const uint8_t *t = tiles + it * KV4_TILE + KV4_V;
+#pragma unroll
+        for (int j = 0; j < 8; j++) vc[j] = *(const u32x4 *)(t + (j * 64 + lane) * 16);
+#pragma unroll
+        for (int j = 0; j < 2; j++) vs[j] = *(const int *)(t + (KV4_VS - KV4_V) + (j * 64 + lane) * 4);
+    };
+    // The running maximum over the N scores of a lane's query and its three other lanes',
+    // with the sums taken along; the scores become 2^8 exp(scale (s - max)), hidden ones 0.
+    // `seen` has a bit per score.
+    auto softmax = [&](float *s, auto count, int n, bool some, uint32_t seen) __attribute__((always_inline)) {
+        constexpr int N = decltype(count)::value;
+        if (some)
+#pragma unroll
+            for (int e = 0; e < N; e++) s[e] = (seen >> e) & 1u ? s[e] : -INFINITY;
+        float mx = s[0];
+#pragma unroll
+        for (int e = 1; e < N; e++) mx = fmaxf(mx, s[e]);
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        mx = fmaxf(mx, m[n]);
+        if (__ballot(mx > m[n])) {
+            // a lane without a visible key so far has sums of 0
+            const float al = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[n] - mx) * a.sl2);
+            m[n] = mx;
+            l[n] *= al;
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) o[n][j][r] *= al;
+        }
+        const float c = 8.f - (mx == -INFINITY ? 0.f : mx * a.sl2);
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], a.sl2, c));
+            if (some) p = (seen >> e) & 1u ? p : 0.f;
+            s[e] = p;
+            sum += p;
+        }
+        l[n] += sum;
+    };
+    // visible keys of 64 from key k0 of the P + So, the first `have` of them there
+    auto validity = [&](int64_t k0, int have) __attribute__((always_inline)) -> uint64_t {
+        bool ok = lane < have;
+        if constexpr (MASKED) {
+            const uint8_t byte = a.kvalid[b * (a.P + a.So) + k0 + min(lane, have - 1)];
+            ok = ok && byte != 0;
+        }
+        return __ballot(ok);
+    };
+
+    int64_t it = first + wave;
+    if (it < last && it < a.T) {
+        load_k(it);
+        load_v(it);
+    }
+    for (; it < last && it < a.T; it += 4) {
+        const int64_t key0 = it * KV4_KEYS;
+        const int have = (int)min(a.P - key0, (int64_t)KV4_KEYS);
+        uint32_t seen = 0xffffffffu;
+        bool some = false;
+        if (MASKED || have < KV4_KEYS) {
+            const uint64_t lo = validity(key0, min(have, 64)), hi = have > 64 ? validity(key0 + 64, have - 64) : 0;
+            some = (lo & hi) != ~0ull;
+            seen = (uint32_t)((lo >> (16 * lg)) & 0xffffu) | (uint32_t)((hi >> (16 * lg)) & 0xffffu) << 16;
+        }
+        const bool more = it + 4 < last && it + 4 < a.T;
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+            float s[32];
+            f32x4 acc[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#define QK(i) \
+    acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(kc[i]), qhi[n], acc[i], 4, 0, i & 3, ks[i >> 2], 0, qsc[n]);
+            QK(0) QK(1) QK(2) QK(3) QK(4) QK(5) QK(6) QK(7)
+#undef QK
+#define QK(i) \
+    acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(kc[i]), qlo[n], acc[i], 4, 0, i & 3, ks[i >> 2], 1, qsc[n]);
+            QK(0) QK(1) QK(2) QK(3) QK(4) QK(5) QK(6) QK(7)
+#undef QK
+            if (n == NQ - 1 && more) load_k(it + 4);
+#pragma unroll
+            for (int e = 0; e < 32; e++) s[e] = acc[e >> 2][e & 3];
+            softmax(s, std::integral_constant<int, 32>{}, n, some, seen);
+            i32x8 ph, pl;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                int hi, lo;
+                split4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3], hi, lo);
+                ph[i] = hi;
+                pl[i] = lo;
+            }
+            constexpr int psc = 127 | 122 << 8;
+#define PV(j) \
+    o[n][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(vc[j]), ph, o[n][j], 4, 0, j & 3, vs[j >> 2], 0, psc);
+            PV(0) PV(1) PV(2) PV(3) PV(4) PV(5) PV(6) PV(7)
+#undef PV
+#define PV(j) \
+    o[n][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(vc[j]), pl, o[n][j], 4, 0, j & 3, vs[j >> 2], 1, psc);
+            PV(0) PV(1) PV(2) PV(3) PV(4) PV(5) PV(6) PV(7)
+#undef PV
+            if (n == NQ - 1 && more) load_v(it + 4);
+        }
+    }
+
+    // ---- own keys, 64 at a time in two groups of 32 (bf16 products of 32 deep): row m of
+    // product i is key 8 (m / 4) + 4 i + m % 4, so the lane's scores are the eight keys
+    // 8 lg .. of its probability operand ----
+    for (; it < last; it += 4) {
+        const int64_t key0 = (it - a.T) * OWN_KEYS;
+        const int have = (int)min(a.So - key0, (int64_t)OWN_KEYS);
+        const uint64_t ok = validity(a.P + key0, have);
+        const uint16_t *kb = a.k_own + (bh * a.So + key0) * 128;
+        const uint16_t *vb = a.vt_own + bh * 128 * a.So + key0;
+        const bool some = ok != ~0ull;
+        const uint32_t seen = (uint32_t)((ok >> (8 * lg)) & 0xffu) | (uint32_t)((ok >> (32 + 8 * lg)) & 0xffu) << 8;
+        const bool rows16 = (a.So & 7) == 0;
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+            const int64_t qi = min(q0 + 16 * n + l16, a.Sq - 1);
+            const uint16_t *qp = a.q + (bh * a.Sq + qi) * 128 + 8 * lg;
+            bf16x8 qf[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) qf[e] = __builtin_bit_cast(bf16x8, *(const u32x4 *)(qp + 32 * e) ^ a.flip);
+            float s[16];
+#pragma unroll
+            for (int g = 0; g < 2; g++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int key = min(32 * g + 8 * (l16 >> 2) + 4 * i + (l16 & 3), have - 1);
+                    const uint16_t *kp = kb + (int64_t)key * 128 + 8 * lg;
+                    f32x4 acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8 *)(kp + 32 * e), qf[e], acc, 0, 0, 0);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) s[8 * g + 4 * i + r] = acc[r];
+                }
+            softmax(s, std::integral_constant<int, 16>{}, n, some, seen);
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+                if (32 * g >= have) continue;
+                const u32x4 p = u32x4{pack_bf16x2(s[8 * g], s[8 * g + 1]), pack_bf16x2(s[8 * g + 2], s[8 * g + 3]),
+                                      pack_bf16x2(s[8 * g + 4], s[8 * g + 5]), pack_bf16x2(s[8 * g + 6], s[8 * g + 7])};
+                const int k8 = 32 * g + 8 * lg;  // the lane's eight keys
+                const uint32_t keep = (seen >> (8 * g)) & 0xffu;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const uint16_t *vp = vb + (int64_t)(16 * j + l16) * a.So + k8;
+                    u32x4 v{};
+                    if (rows16 && k8 + 8 <= have) {
+                        v = *(const u32x4 *)vp;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            if (k8 + e < have) v[e >> 1] |= (uint32_t)vp[e] << (16 * (e & 1));
+                    }
+                    if (some)  // what a hidden key holds does not count, a NaN either
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            v[e] &= ((keep >> (2 * e)) & 1u ? 0xffffu : 0u) | ((keep >> (2 * e + 1)) & 1u ? 0xffff0000u : 0u);
+                    o[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v), __builtin_bit_cast(bf16x8, p),
+                                                                      o[n][j], 0, 0, 0);
+                }
+            }
+        }
+    }
+
+    // ---- the four waves' sums ----
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        l[n] += __shfl_xor(l[n], 16);
+        l[n] += __shfl_xor(l[n], 32);
+        if (lg == 0) {
+            sm[wave][16 * n + l16] = m[n];
+            sl[wave][16 * n + l16] = l[n];
+        }
+        float *row = so + (wave * 16 * NQ + 16 * n + l16) * PITCH + 4 * lg;
+#pragma unroll
+        for (int j = 0; j < 8; j++) *(f32x4 *)(row + 16 * j) = o[n][j];
+    }
+    __syncthreads();
+    constexpr int TPQ = 16 / NQ, DPT = 128 / TPQ;  // threads per query, dimensions per thread
+    const int ql = tid / TPQ, d0 = (tid % TPQ) * 4;
+    const int64_t qi = q0 + ql;
+    if (qi >= a.Sq) return;
+    float mm = fmaxf(fmaxf(sm[0][ql], sm[1][ql]), fmaxf(sm[2][ql], sm[3][ql])), ll = 0.f, f[4];
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        f[w] = sm[w][ql] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((sm[w][ql] - mm) * a.sl2);
+        ll += sl[w][ql] * f[w];
+    }
+    const int64_t row = bh * a.Sq + qi, rows = (int64_t)gridDim.x / a.shares * a.Sq;
+    if (a.shares > 1 && tid % TPQ == 0) {
+        float *ml = a.part + (int64_t)a.shares * rows * 128 + ((int64_t)share * rows + row) * 2;
+        ml[0] = mm;
+        ml[1] = ll;
+    }
+    const float inv = 1.0f / ll;  // a query that sees no key: 0 / 0, as the softmax of -inf
+#pragma unroll
+    for (int e = 0; e < DPT / 4; e++) {
+        const int d = d0 + 4 * TPQ * e;
+        f32x4 v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const f32x4 x = *(const f32x4 *)(so + (w * 16 * NQ + ql) * PITCH + d);
+#pragma unroll
+            for (int r = 0; r < 4; r++) v[r] += x[r] * f[w];
+        }
+        if (a.shares > 1)
+            *(f32x4 *)(a.part + ((int64_t)share * rows + row) * 128 + d) = v;
+        else
+            *(u32x2 *)(a.out + ((b * a.Sq + qi) * a.H + bh % a.H) * 128 + d) =
+                u32x2{pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv)};
+    }
+}
+
+// Joins the shares of a row, one wave per row, two dimensions per lane.
+__global__ __launch_bounds__(256) void attn4_join_kernel(const float *__restrict__ part, int shares, int64_t rows, int64_t H,
+                                                         int64_t Sq, float sl2, uint16_t *__restrict__ out) {
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const int lane = threadIdx.x & 63;
+    const f32x2 *ml = (const f32x2 *)(part + (int64_t)shares * rows * 128);
+    // lane s has share s's maximum and sum (at most 64 shares)
+    const f32x2 mine = lane < shares ? ml[lane * rows + row] : f32x2{-INFINITY, 0.f};
+    float mm = mine[0];
+    for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o));
+    const float f = mine[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mine[0] - mm) * sl2);
+    const float ll = wave_sum(mine[1] * f);
+    f32x2 v{0.f, 0.f};
+    for (int s = 0; s < shares; s++) {
+        const f32x2 x = *(const f32x2 *)(part + ((int64_t)s * rows + row) * 128 + 2 * lane);
+        const float fs = __shfl(f, s);
+        v[0] += x[0] * fs;
+        v[1] += x[1] * fs;
+    }
+    const float inv = 1.0f / ll;
+    const int64_t bh = row / Sq, qi = row % Sq;
+    *(uint32_t *)(out + ((bh / H * Sq + qi) * H + bh % H) * 128 + 2 * lane) = pack_bf16x2(v[0] * inv, v[1] * inv);
+}
+
+// Query tiles of 16 per workgroup, and shares of the keys: two workgroups per CU (one with
+// four tiles, whose registers fill it), each with at least a tile for every wave, at most 64.
+struct Plan {
+    int nq;
+    int shares;
+};
+Plan plan_of(int64_t bh, int64_t sq, int64_t items) {
+    const int nq = sq <= 16 ? 1 : sq <= 32 ? 2 : 4;
+    const int64_t cus = std::max(device_cu_count(), 1), want = nq == 4 ? cus : 2 * cus;
+    const int64_t wgs = bh * ((sq + 16 * nq - 1) / (16 * nq));
+    return {nq, (int)std::max<int64_t>(1, std::min<int64_t>({want / wgs, (items + 3) / 4, 64}))};
+}
+
+template <bool MASKED>
+void launch_nq(int nq, dim3 grid, const Attn4 &a, hipStream_t stream) {
+    if (nq == 1)
+        attn4_kernel<1, MASKED><<<grid, dim3(256), 0, stream>>>(a);
+    else if (nq == 2)
+        attn4_kernel<2, MASKED><<<grid, dim3(256), 0, stream>>>(a);
+    else
+        attn4_kernel<4, MASKED><<<grid, dim3(256), 0, stream>>>(a);
+}
+
+}  // namespace
+
+// more than one share only with at most `want` workgroups of 16 nq rows: 2 x 16 or 64 per CU
+size_t attn4_scratch_bytes() { return (size_t)std::max(device_cu_count(), 1) * 64 * (128 + 2) * 4; }
+
+bool attn4_takes(int64_t sq) { return sq <= 64; }
+
+hipError_t launch_attn4(const uint16_t *q, const uint8_t *tiles, int64_t p, const uint16_t *k_own, const uint16_t *vt_own,
+                        int64_t so, const uint8_t *kvalid, int64_t b, int64_t h, int64_t sq, float scale, float *scratch,
+                        uint16_t *out, hipStream_t stream) {
+    if (sq <= 0 || b <= 0 || h <= 0) return hipSuccess;
+    if (p < 0 || so < 0 || p + so <= 0 || !scratch) return hipErrorInvalidValue;
+    const int64_t bh = b * h, T = (p + KV4_KEYS - 1) / KV4_KEYS, items = T + (so + OWN_KEYS - 1) / OWN_KEYS;
+    const Plan pl = plan_of(bh, sq, items);
+    const int64_t qt = (sq + 16 * pl.nq - 1) / (16 * pl.nq);
+    if (bh * pl.shares >= ((int64_t)1 << 31) || qt > 65535) return hipErrorInvalidValue;
+    const float sl2 = scale * 1.4426950408889634f;
+    const Attn4 a{q, tiles, p, T, k_own, vt_own, so, kvalid, h, sq, sl2 < 0.f ? -sl2 : sl2,
+                  sl2 < 0.f ? 0x80008000u : 0u, out, scratch, pl.shares};
+    const dim3 grid((unsigned)(bh * pl.shares), (unsigned)qt);
+    if (kvalid)
+        launch_nq<true>(pl.nq, grid, a, stream);
+    else
+        launch_nq<false>(pl.nq, grid, a, stream);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || pl.shares == 1) return e;
+    attn4_join_kernel<<<dim3((unsigned)((bh * sq + 3) / 4)), dim3(256), 0, stream>>>(scratch, pl.shares, bh * sq, h, sq, a.sl2, out);
+    return hipGetLastError();
+}
+
+}  // namespace qimm

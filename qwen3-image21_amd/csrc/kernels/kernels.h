@@ -272,6 +272,45 @@ hipError_t launch_qk_prep(const float *x, int64_t b, int64_t s, int64_t h, const
 hipError_t launch_transpose_sd(const uint16_t *in, int64_t bh, int64_t s, int64_t ld, uint16_t *out,
                                int inverse, hipStream_t stream);
 
+// ---- low-rank adapters beside a projection (lora.hip) ----
+struct AdapterDev {
+    const uint16_t *a;  // bf16 [rank][K]
+    const uint16_t *b;  // bf16 [N][ldb], zeros past the rank
+    int32_t rank;
+    int32_t ldb;        // rank rounded up to 8
+    float scale;
+    int32_t pad;
+};
+// t[row][0:ldt) (f32, ldt the largest rank rounded up to 32) = scale x A^T with the adapter
+// ids[row] of each row, zeros past its rank up to a multiple of 32; rows without one are not
+// written. x [m][k] bf16, row stride lda.
+hipError_t launch_lora_down(const uint16_t *x, int64_t lda, int64_t m, int64_t k, const AdapterDev *ad, int count,
+                            const int32_t *ids, float *t, int64_t ldt, hipStream_t stream);
+// y [m][n] = base [m][n] (f32) + t B^T, to y32 (f32, may be base) when set, else bf16 to y16
+hipError_t launch_lora_up(const float *t, int64_t ldt, int64_t m, int64_t n, const AdapterDev *ad, int count,
+                          const int32_t *ids, const float *base, float *y32, uint16_t *y16, hipStream_t stream);
+
+// ---- the prefix cache held in 4 bits (kv4.hip, attn4.hip; the layout is in kv4.h) ----
+// Bytes of one layer: b * h heads of p keys.
+int64_t kv4_layer_bytes(int64_t bh, int64_t p);
+// Stores one layer: k [B,H,P,128] bf16 and v, [B,H,P,128] with vt_ld 0 or [B,H,128,vt_ld]
+// (vt_ld a multiple of 8, >= p). Of the transposed form, keys with kvalid[b * valid_ld +
+// key] == 0 are stored as zeros (kvalid may be null). *norm (device): a bound of the stored
+// keys' norms, NaN or infinite keys +inf.
+hipError_t launch_store4(const uint16_t *k, const uint16_t *v, int64_t vt_ld, int64_t b, int64_t h, int64_t p,
+                         const uint8_t *kvalid, int64_t valid_ld, uint8_t *tiles, float *norm, hipStream_t stream);
+// Reads one layer back: k [BH,P,128] and v [BH,P,128] (vt_ld 0) or [BH,128,vt_ld].
+hipError_t launch_load4(const uint8_t *tiles, int64_t bh, int64_t p, int64_t vt_ld, uint16_t *k, uint16_t *v,
+                        hipStream_t stream);
+// Attention of sq queries q [B,H,sq,128] over [4-bit layer ; own], out [B,sq,H*128] bf16;
+// own keys dense (vt_own [B,H,128,so]), kvalid [B][p + so] or null, scratch
+// attn4_scratch_bytes(). For few queries (attn4_takes).
+bool attn4_takes(int64_t sq);
+size_t attn4_scratch_bytes();
+hipError_t launch_attn4(const uint16_t *q, const uint8_t *tiles, int64_t p, const uint16_t *k_own, const uint16_t *vt_own,
+                        int64_t so, const uint8_t *kvalid, int64_t b, int64_t h, int64_t sq, float scale, float *scratch,
+                        uint16_t *out, hipStream_t stream);
+
 // ---- the denoising step around the blocks (step.hip), all f32 ----
 enum : int { ACT_NONE = 0, ACT_SILU = 1, ACT_GELU_TANH = 2 };
 // y[m][n] (row stride ldy) = act(sum_k x[m][k] * w[n][k]); x row stride ldx, w [n][k] dense.

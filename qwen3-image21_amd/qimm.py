@@ -50,6 +50,11 @@ SIGNATURES = [
     ("qimm_qmatmul_noalloc", _i32, [_vp, _vp, _vp, _i64, _i64, _vp, _i32, _vp]),
     ("qimm_qmatmul_scratch_bytes", _i64, [_vp, _i64]),
     ("qimm_qmatmul_route", _i32, [_i32, _i64, _i64, _i32, _i64, _i32, _vp]),
+    ("qimm_adapters_create", _i32, [_vp, _i64, _i64, _vp, _i64, C.POINTER(_vp)]),
+    ("qimm_adapters_destroy", _i32, [_vp]),
+    ("qimm_adapters_device_bytes", _i64, [_vp]),
+    ("qimm_qmatmul_adapters", _i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i32, _vp]),
+    ("qimm_qmatmul_adapters_reserve", _i32, [_vp, _vp, _vp, _i64, _i32]),
     ("qimm_joint_layout", _i32, [_i64, _vp, _vp, _i64, _i64, _i64, _vp, _i64,
                                  C.POINTER(_i64), C.POINTER(_i64), C.POINTER(_i64)]),
     ("qimm_rope_table", _i32, [_vp, _i64, _vp, _i64, _vp, C.c_double, _vp]),
@@ -60,6 +65,9 @@ SIGNATURES = [
     ("qimm_kv_prefix_len", _i64, [_vp]),
     ("qimm_kv_create_host", _i32, [_vp, _i64, _i64, _i64, _i64, _i64, C.POINTER(_vp)]),
     ("qimm_kv_is_host", _i32, [_vp]),
+    ("qimm_kv_create_q4", _i32, [_vp, _i64, _i64, _i64, _i64, _i64, C.POINTER(_vp)]),
+    ("qimm_kv_bits", _i32, [_vp]),
+    ("qimm_kv_device_bytes", _i64, [_vp]),
     ("qimm_kv_prefetch", _i32, [_vp, _i64, _vp]),
     ("qimm_qk_norm_rope", _i32, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
     ("qimm_v_transpose", _i32, [_vp, _vp, _i64, _i64, _i64, _vp, _vp]),
@@ -113,6 +121,11 @@ class Tensor(C.Structure):
     """qimm_tensor: one GGUF tensor in host memory."""
     _fields_ = [("ggml_type", _i32), ("rows", _i64), ("cols", _i64), ("data", _vp),
                 ("nbytes", C.c_size_t)]
+
+
+class Adapter(C.Structure):
+    """qimm_adapter: scale, a [rank, cols], b [rows, rank]."""
+    _fields_ = [("scale", _f32), ("a", Tensor), ("b", Tensor)]
 
 
 class BlockTensors(C.Structure):
@@ -255,6 +268,30 @@ class Context:
         """Device scratch bytes of the product of w with m rows (qimm_qmatmul_scratch_bytes)."""
         return int(self.lib.qimm_qmatmul_scratch_bytes(w.h, m))
 
+    # -- low-rank adapters --
+    def adapters_create(self, rows: int, cols: int, adapters) -> "Adapters":
+        """adapters: (scale, type, a bytes [rank, cols], b bytes [rows, rank]) each, type F32, F16 or BF16."""
+        keep, arr = [], (Adapter * max(1, len(adapters)))()
+        for i, (scale, t, a, b) in enumerate(adapters):
+            size = 4 if t == F32 else 2
+            rank = len(a) // (cols * size) if cols > 0 else 0
+            arr[i] = Adapter(scale, make_tensor(t, rank, cols, a, keep), make_tensor(t, rows, rank, b, keep))
+        h = C.c_void_p()
+        self.check(self.lib.qimm_adapters_create(self.h, rows, cols, C.byref(arr), len(adapters), C.byref(h)),
+                   "qimm_adapters_create")
+        return Adapters(self, h, rows, cols)
+
+    def qmatmul_adapters(self, w: "Weight", adapters: "Adapters", ids_dev: int, x_dev: int, m: int, lda: int,
+                         y_dev: int, out_type: int, stream: int = 0):
+        """y = x W^T + scale (x A^T) B^T, the adapter of each row by its id (int32 [m], outside the
+        adapters: none) (qimm_qmatmul_adapters)."""
+        self.check(self.lib.qimm_qmatmul_adapters(self.h, w.h, adapters.h, ids_dev, x_dev, m, lda, y_dev, out_type,
+                                                  stream), "qimm_qmatmul_adapters")
+
+    def qmatmul_adapters_reserve(self, w: "Weight", adapters: "Adapters", m: int, out_type: int):
+        self.check(self.lib.qimm_qmatmul_adapters_reserve(self.h, w.h, adapters.h, m, out_type),
+                   "qimm_qmatmul_adapters_reserve")
+
     # -- cache --
     def kv_create(self, layers: int, batch: int, heads: int, prefix_len: int, head_dim: int = 128) -> "KvCache":
         h = C.c_void_p()
@@ -288,6 +325,14 @@ class Context:
         h = C.c_void_p()
         self.check(self.lib.qimm_kv_create_host(self.h, layers, batch, heads, prefix_len, head_dim, C.byref(h)),
                    "qimm_kv_create_host")
+        return KvCache(self, h, layers, batch, heads, prefix_len)
+
+    def kv_create_q4(self, layers: int, batch: int, heads: int, prefix_len: int,
+                     head_dim: int = 128) -> "KvCache":
+        """The cache held in 4 bits: 4.25 bits a value in blocks of 32 (qimm_kv_create_q4)."""
+        h = C.c_void_p()
+        self.check(self.lib.qimm_kv_create_q4(self.h, layers, batch, heads, prefix_len, head_dim, C.byref(h)),
+                   "qimm_kv_create_q4")
         return KvCache(self, h, layers, batch, heads, prefix_len)
 
     # -- attention --
@@ -330,6 +375,21 @@ class Weight:
             self.h = None
 
 
+class Adapters:
+    """The low-rank adapters of one projection (qimm_adapters)."""
+
+    def __init__(self, ctx, h, rows, cols):
+        self.ctx, self.h, self.rows, self.cols = ctx, h, rows, cols
+
+    def device_bytes(self) -> int:
+        return int(self.ctx.lib.qimm_adapters_device_bytes(self.h))
+
+    def free(self):
+        if self.h:
+            self.ctx.lib.qimm_adapters_destroy(self.h)
+            self.h = None
+
+
 class KvCache:
     def __init__(self, ctx, h, layers, batch, heads, prefix_len):
         self.ctx, self.h = ctx, h
@@ -347,6 +407,14 @@ class KvCache:
     @property
     def is_host(self) -> bool:
         return bool(self.ctx.lib.qimm_kv_is_host(self.h))
+
+    @property
+    def bits(self) -> int:
+        """Bits of a stored value, 16 or 4."""
+        return self.ctx.lib.qimm_kv_bits(self.h)
+
+    def device_bytes(self) -> int:
+        return int(self.ctx.lib.qimm_kv_device_bytes(self.h))
 
     def free(self):
         if self.h:
