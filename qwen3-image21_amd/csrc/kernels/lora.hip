@@ -115,11 +115,80 @@ __global__ __launch_bounds__(256) void lora_up_kernel(const float *__restrict__ 
     }
 }
 
+// ---- few rows: every row by itself ----
+
+__device__ __forceinline__ float dot8(u32x4 a, u32x4 b, float s) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        s = __builtin_fmaf(__uint_as_float(a[e] << 16), __uint_as_float(b[e] << 16), s);
+        s = __builtin_fmaf(__uint_as_float(a[e] & 0xffff0000u), __uint_as_float(b[e] & 0xffff0000u), s);
+    }
+    return s;
+}
+
+// t of row blockIdx.y, one rank per wave.
+__global__ __launch_bounds__(256) void lora_down_row_kernel(const uint16_t *__restrict__ x, int64_t lda, int64_t K,
+                                                           const AdapterDev *__restrict__ ad, int count,
+                                                           const int32_t *__restrict__ ids, float *__restrict__ t, int64_t ldt) {
+    const int64_t row = blockIdx.y;
+    const int id = ids[row];
+    if (id < 0 || id >= count) return;
+    const AdapterDev d = ad[id];
+    const int lane = threadIdx.x & 63, r = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (r >= d.rank) return;
+    const uint16_t *xr = x + row * lda, *ar = d.a + (int64_t)r * K;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};  // four chains: a row's loads are all in flight at once
+    int64_t k = 8 * lane;
+    for (; k + 3 * 512 < K; k += 4 * 512) {
+#pragma unroll
+        for (int u = 0; u < 4; u++) s[u] = dot8(*(const u32x4 *)(xr + k + 512 * u), *(const u32x4 *)(ar + k + 512 * u), s[u]);
+    }
+    for (; k < K; k += 512) s[0] = dot8(*(const u32x4 *)(xr + k), *(const u32x4 *)(ar + k), s[0]);
+    const float sum = wave_sum((s[0] + s[1]) + (s[2] + s[3]));
+    if (lane == 0) t[row * ldt + r] = sum * d.scale;
+}
+
+// y of row blockIdx.y, one column per thread: a thread reads its row of B, 16 B at a time.
+__global__ __launch_bounds__(256) void lora_up_row_kernel(const float *__restrict__ t, int64_t ldt, int64_t N,
+                                                         const AdapterDev *__restrict__ ad, int count,
+                                                         const int32_t *__restrict__ ids, const float *base, float *y32,
+                                                         uint16_t *y16) {
+    const int64_t row = blockIdx.y, n = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int id = ids[row];
+    if (n >= N) return;
+    const float b0 = base[row * N + n];
+    float s = 0.f;
+    if (id >= 0 && id < count) {
+        const AdapterDev d = ad[id];
+        const float *tr = t + row * ldt;
+        const uint16_t *br = d.b + n * d.ldb;
+        for (int r = 0; r < d.rank; r += 8) {
+            const u32x4 b = *(const u32x4 *)(br + r);  // zeros past the rank, where t is not written
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (r + e < d.rank)
+                    s = __builtin_fmaf(tr[r + e], __uint_as_float(e & 1 ? b[e >> 1] & 0xffff0000u : b[e >> 1] << 16), s);
+        }
+    }
+    s += b0;
+    if (y32)
+        y32[row * N + n] = s;
+    else
+        y16[row * N + n] = (uint16_t)(pack_bf16x2(s, 0.f) & 0xffffu);
+}
+
+// Up to this many rows each row is taken by itself.
+constexpr int64_t FEW_ROWS = 64;
+
 }  // namespace
 
 hipError_t launch_lora_down(const uint16_t *x, int64_t lda, int64_t m, int64_t k, const AdapterDev *ad, int count,
                             const int32_t *ids, float *t, int64_t ldt, hipStream_t stream) {
     if (m <= 0) return hipSuccess;
+    if (m <= FEW_ROWS) {
+        lora_down_row_kernel<<<dim3((unsigned)((ldt + 3) / 4), (unsigned)m), dim3(256), 0, stream>>>(x, lda, k, ad, count, ids, t, ldt);
+        return hipGetLastError();
+    }
     lora_down_kernel<<<dim3((unsigned)((m + 15) / 16)), dim3(256), 0, stream>>>(x, lda, m, k, ad, count, ids, t, ldt);
     return hipGetLastError();
 }
@@ -128,6 +197,11 @@ hipError_t launch_lora_up(const float *t, int64_t ldt, int64_t m, int64_t n, con
                           const int32_t *ids, const float *base, float *y32, uint16_t *y16, hipStream_t stream) {
     if (m <= 0) return hipSuccess;
     if (n % 128 || (m + 15) / 16 > 65535) return hipErrorInvalidValue;
+    if (m <= FEW_ROWS) {
+        lora_up_row_kernel<<<dim3((unsigned)((n + 255) / 256), (unsigned)m), dim3(256), 0, stream>>>(t, ldt, n, ad, count, ids,
+                                                                                                    base, y32, y16);
+        return hipGetLastError();
+    }
     lora_up_kernel<<<dim3((unsigned)((n + 255) / 256), (unsigned)((m + 15) / 16)), dim3(256), 0, stream>>>(t, ldt, m, n, ad, count,
                                                                                                           ids, base, y32, y16);
     return hipGetLastError();
