@@ -15,23 +15,44 @@ struct qimm_adapters {
     void *dev = nullptr;                // the table of AdapterDev, then every A and B
     size_t bytes = 0;
     const qimm::AdapterDev *table() const { return (const qimm::AdapterDev *)dev; }
-    int64_t ldt() const { return (max_rank + 31) / 32 * 32; }
+    const uint16_t *zeros() const { return (const uint16_t *)dev + bytes / 2 - 128; }  // the last 256 B
 };
 
 namespace {
 
 size_t align_up(size_t v) { return (v + 255) & ~(size_t)255; }
 
-// Scratch of one product in the context's growable workspace: t, and for bf16 outputs the
-// f32 sums.
-struct Scratch {
-    size_t base, total;
+// How a product of m rows is taken: each row by itself beside the product's f32 sums (few), as
+// k steps of the product over bf16 rows (steps), or a pass over its f32 sums; and the scratch
+// in the context's growable workspace: t, the first product's shares, the f32 sums of a bf16
+// output; the partial sums of a split product.
+struct Route {
+    bool few, steps;
+    qimm::Bf16Plan plan;
+    size_t shares, sums, total, part;
 };
-Scratch scratch_of(const qimm_adapters *ad, int64_t m, int out_type) {
-    Scratch s{};
-    s.base = align_up((size_t)(m * ad->ldt()) * 4);
-    s.total = s.base + (out_type == QIMM_TYPE_F32 ? 0 : (size_t)(m * ad->rows) * 4);
-    return s;
+Route route_of(const qimm_weight *w, const qimm_adapters *ad, int64_t m, int out_type) {
+    Route r{};
+    r.few = qimm::lora_few(m);
+    const int64_t kt = (ad->max_rank + 63) / 64 * 64;
+    if (r.few) {
+        r.shares = align_up((size_t)(m * ad->max_rank) * 4);
+        r.sums = r.shares;
+    } else {
+        r.shares = align_up((size_t)(m * 2 * kt) * 2);
+        r.sums = r.shares + align_up(qimm::lora_down_scratch(m, w->cols, ad->max_rank));
+        r.steps = qimm::qgemm_bf16_fits(w->gw);
+    }
+    r.total = r.sums;
+    if (r.steps) {
+        r.plan = qimm::qgemm_bf16_plan(w->gw, m, true);
+        if (r.plan.splits > 1)
+            r.part = qimm::STREAM_COUNTER_BYTES + (size_t)r.plan.splits * (size_t)m * (size_t)w->rows * 4;
+    } else {
+        r.part = qimm::qgemm_workspace(w->gw, m);
+        if (out_type != QIMM_TYPE_F32) r.total += (size_t)(m * ad->rows) * 4;
+    }
+    return r;
 }
 
 int check_pair(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapters *ad) {
@@ -42,12 +63,9 @@ int check_pair(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapters *ad) {
     return QIMM_OK;
 }
 
-int reserve(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapters *ad, int64_t m, int out_type) {
-    QIMM_HIP(ctx, hipSetDevice(ctx->device));
-    if (const int rc = ensure_workspace(ctx, scratch_of(ad, m, out_type).total)) return rc;
-    if (const size_t need = qimm::qgemm_workspace(w->gw, m))
-        if (const int rc = ensure_part_workspace(ctx, need)) return rc;
-    return QIMM_OK;
+int reserve(qimm_ctx *ctx, const Route &r) {
+    if (const int rc = ensure_workspace(ctx, r.total)) return rc;
+    return r.part ? ensure_part_workspace(ctx, r.part) : QIMM_OK;
 }
 
 }  // namespace
@@ -91,6 +109,7 @@ int qimm_adapters_create(qimm_ctx *ctx, int64_t rows, int64_t cols, const qimm_a
             off += align_up((size_t)(rows * ldb) * 2);
             ad->max_rank = std::max(ad->max_rank, r);
         }
+        off += 256;  // zeros, which the tiles of other adapters' rows read
         ad->bytes = off;
         // A as it is; B's rows padded with zeros to 16 bytes
         std::vector<uint8_t> host(off, 0);
@@ -99,6 +118,15 @@ int qimm_adapters_create(qimm_ctx *ctx, int64_t rows, int64_t cols, const qimm_a
             to_bf16(list[i].a.ggml_type, (const uint8_t *)list[i].a.data, r * cols, (uint16_t *)&host[at_a[(size_t)i]]);
             std::vector<uint16_t> b((size_t)(rows * r));
             to_bf16(list[i].b.ggml_type, (const uint8_t *)list[i].b.data, rows * r, b.data());
+            for (const uint16_t *p : {(const uint16_t *)&host[at_a[(size_t)i]], (const uint16_t *)b.data()}) {
+                const int64_t count = p == b.data() ? rows * r : r * cols;
+                bool numbers = true;
+                for (int64_t q = 0; q < count; q++) numbers &= (p[q] & 0x7f80u) != 0x7f80u;
+                if (!numbers) {
+                    delete ad;
+                    return set_err(ctx, QIMM_ERR_ARG, "adapters: values must be numbers within the bf16 range");
+                }
+            }
             for (int64_t row = 0; row < rows; row++)
                 memcpy(&host[at_b[(size_t)i] + (size_t)(row * ldb) * 2], &b[(size_t)(row * r)], (size_t)r * 2);
         }
@@ -140,7 +168,9 @@ int qimm_qmatmul_adapters_reserve(qimm_ctx *ctx, const qimm_weight *w, const qim
     if (out_type != QIMM_TYPE_F32 && out_type != QIMM_TYPE_BF16)
         return set_err(ctx, QIMM_ERR_TYPE, "qmatmul: output must be F32 or BF16");
     if (const int rc = check_pair(ctx, w, ad)) return rc;
-    return reserve(ctx, w, ad, m, out_type);
+    if (m == 0) return QIMM_OK;
+    QIMM_HIP(ctx, hipSetDevice(ctx->device));
+    return reserve(ctx, route_of(w, ad, m, out_type));
 }
 
 int qimm_qmatmul_adapters(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapters *ad, const int32_t *ids,
@@ -150,28 +180,40 @@ int qimm_qmatmul_adapters(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapte
     if (const int rc = check_pair(ctx, w, ad)) return rc;
     if ((uintptr_t)ids & 3) return set_err(ctx, QIMM_ERR_ARG, "qmatmul with adapters: ids must be 4-byte aligned");
     if (m == 0) return QIMM_OK;
-    if (const int rc = reserve(ctx, w, ad, m, out_type)) return rc;
+    QIMM_HIP(ctx, hipSetDevice(ctx->device));
+    const Route r = route_of(w, ad, m, out_type);
+    if (const int rc = reserve(ctx, r)) return rc;
     const hipStream_t s = (hipStream_t)stream;
-    const Scratch sc = scratch_of(ad, m, out_type);
-    float *t = (float *)ctx->ws;
-    float *base = out_type == QIMM_TYPE_F32 ? (float *)y : (float *)((char *)ctx->ws + sc.base);
-    QIMM_HIP(ctx, qimm::launch_lora_down((const uint16_t *)x_bf16, lda, m, w->cols, ad->table(), (int)ad->count, ids, t,
-                                         ad->ldt(), s));
+    const uint16_t *x = (const uint16_t *)x_bf16;
+    const bool f32 = out_type == QIMM_TYPE_F32;
+    const int64_t K = w->cols, N = w->rows, kt = (ad->max_rank + 63) / 64 * 64;
+    const int n = (int)ad->count;
+    char *ws = (char *)ctx->ws;
+    if (r.few)
+        QIMM_HIP(ctx, qimm::launch_lora_few_down(x, lda, m, K, ad->table(), n, ids, (float *)ws, ad->max_rank, s));
+    else
+        QIMM_HIP(ctx, qimm::launch_lora_down(x, lda, m, K, ad->max_rank, ad->table(), n, ids, (float *)(ws + r.shares),
+                                             (uint16_t *)ws, s));
     qimm::EpiParams ep{};
-    ep.out = base;
-    ep.ldo = w->rows;
-    if (qimm::qgemm_workspace(w->gw, m)) {
+    ep.out = y;
+    ep.ldo = N;
+    if (r.part) {
         ep.part_ws = (float *)ctx->ws_part;
         ep.part_ws_bytes = ctx->ws_part_bytes;
     }
-    QIMM_HIP(ctx, qimm::launch_qgemm(w->gw, (const uint16_t *)x_bf16, m, lda, qimm::EPI_F32, ep, s));
-    // rows a launch at a time within the grid's limit
-    constexpr int64_t MOST = 16 * 65535;
-    for (int64_t r = 0; r < m; r += MOST)
-        QIMM_HIP(ctx, qimm::launch_lora_up(t + r * ad->ldt(), ad->ldt(), std::min(m - r, MOST), w->rows, ad->table(),
-                                           (int)ad->count, ids + r, base + r * w->rows,
-                                           out_type == QIMM_TYPE_F32 ? (float *)y + r * w->rows : nullptr,
-                                           (uint16_t *)y + r * w->rows, s));
+    if (r.steps) {
+        const qimm::AdapterSteps st{(const uint16_t *)ws, (int)(kt / 64), ad->table(), n, ids, ad->zeros()};
+        QIMM_HIP(ctx, qimm::launch_qgemm_bf16_adapters(w->gw, x, m, lda, f32 ? qimm::EPI_F32 : qimm::EPI_BF16, ep, r.plan, st, s));
+        return QIMM_OK;
+    }
+    float *sums = f32 ? (float *)y : (float *)(ws + r.sums);
+    ep.out = sums;
+    QIMM_HIP(ctx, qimm::launch_qgemm(w->gw, x, m, lda, qimm::EPI_F32, ep, s));
+    float *y32 = f32 ? sums : nullptr;
+    if (r.few)
+        QIMM_HIP(ctx, qimm::launch_lora_few_up((const float *)ws, ad->max_rank, m, N, ad->table(), n, ids, sums, y32, (uint16_t *)y, s));
+    else
+        QIMM_HIP(ctx, qimm::launch_lora_up((const uint16_t *)ws, kt, m, N, ad->table(), n, ids, sums, y32, (uint16_t *)y, s));
     return QIMM_OK;
 }
 

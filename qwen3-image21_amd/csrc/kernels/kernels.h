@@ -281,14 +281,34 @@ struct AdapterDev {
     float scale;
     int32_t pad;
 };
-// t[row][0:ldt) (f32, ldt the largest rank rounded up to 32) = scale x A^T with the adapter
-// ids[row] of each row, zeros past its rank up to a multiple of 32; rows without one are not
-// written. x [m][k] bf16, row stride lda.
-hipError_t launch_lora_down(const uint16_t *x, int64_t lda, int64_t m, int64_t k, const AdapterDev *ad, int count,
-                            const int32_t *ids, float *t, int64_t ldt, hipStream_t stream);
-// y [m][n] = base [m][n] (f32) + t B^T, to y32 (f32, may be base) when set, else bf16 to y16
-hipError_t launch_lora_up(const float *t, int64_t ldt, int64_t m, int64_t n, const AdapterDev *ad, int count,
+// Few rows (lora_few): t[row][0:rank) (f32, row stride ldt, the largest rank) = scale x A^T
+// with the adapter ids[row] of each row; x [m][k] bf16, row stride lda. Then y [m][n] = base
+// (f32) + t B^T, to y32 (f32, may be base) when set, else bf16 to y16.
+bool lora_few(int64_t m);
+hipError_t launch_lora_few_down(const uint16_t *x, int64_t lda, int64_t m, int64_t k, const AdapterDev *ad, int count,
+                                const int32_t *ids, float *t, int64_t ldt, hipStream_t stream);
+hipError_t launch_lora_few_up(const float *t, int64_t ldt, int64_t m, int64_t n, const AdapterDev *ad, int count,
+                              const int32_t *ids, const float *base, float *y32, uint16_t *y16, hipStream_t stream);
+// Many rows: t16[row] = t as two bf16 rows of kt = the largest rank rounded up to 64, the bf16
+// rounding and then what it leaves, zeros past the adapter's rank; rows without an adapter are
+// not written. scratch: lora_down_scratch bytes.
+size_t lora_down_scratch(int64_t m, int64_t k, int64_t max_rank);
+hipError_t launch_lora_down(const uint16_t *x, int64_t lda, int64_t m, int64_t k, int64_t max_rank, const AdapterDev *ad, int count,
+                            const int32_t *ids, float *scratch, uint16_t *t16, hipStream_t stream);
+hipError_t launch_lora_up(const uint16_t *t16, int64_t kt, int64_t m, int64_t n, const AdapterDev *ad, int count,
                           const int32_t *ids, const float *base, float *y32, uint16_t *y16, hipStream_t stream);
+// The product over bf16 rows with the adapters' second product as further k steps
+// (launch_qgemm_bf16's plain outputs): y = A W^T + t B^T.
+struct AdapterSteps {
+    const uint16_t *t;     // t16
+    int kb;                // kt / 64
+    const AdapterDev *ad;
+    int count;
+    const int32_t *ids;    // [m]
+    const uint16_t *zero;  // 128 B of zeros
+};
+hipError_t launch_qgemm_bf16_adapters(const GemmWeight &w, const uint16_t *a, int64_t m, int64_t lda, int epi,
+                                      const EpiParams &ep, const Bf16Plan &plan, const AdapterSteps &x, hipStream_t stream);
 
 // ---- the prefix cache held in 4 bits (kv4.hip, attn4.hip; the layout is in kv4.h) ----
 // Bytes of one layer: b * h heads of p keys.

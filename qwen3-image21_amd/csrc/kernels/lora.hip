@@ -2,14 +2,18 @@
 //   y[m] = x[m] W^T + scale_a (x[m] A_a^T) B_a^T,   a = ids[m] (none outside [0, n)).
 //
 // Two products: t = scale x A^T (ranks wide, K deep), then t B^T (N wide, ranks deep)
-// added to the projection's f32 sums before the one rounding of y. t is held in f32 and
-// enters the second product as the sum of two bf16 numbers, hi = bf16(t) and lo = bf16(t -
-// hi): 2^-17 of t, so that f32 outputs keep the precision of their sums.
+// added to the projection's f32 sums before the one rounding of y. Where the matrix pipe
+// takes the second product t is the sum of two bf16 numbers, hi = bf16(t) and lo = bf16(t -
+// hi): 2^-16 of t at most, so that f32 outputs keep the precision of their sums.
 //
-// Rows of any adapters may lie next to each other: a tile of 16 rows is multiplied once per
+// Rows of any adapters may lie next to each other: a tile of rows is multiplied once per
 // adapter among its ids; of t the rows of other adapters are not written, in the second
-// product they enter as zeros.
+// product they enter as zeros (adapters hold numbers only). Few rows are taken each by
+// itself, so that many adapters are not multiplied one after the other. The second product
+// of many rows runs as further k steps of the projection where that is over bf16 rows
+// (qgemm_bf16.hip), else as a pass over its f32 sums (lora_up_kernel).
 #include <algorithm>
+#include <type_traits>
 
 #include "device_common.h"
 #include "kernels.h"
@@ -23,50 +27,142 @@ __device__ __forceinline__ int row_id(const int32_t *ids, int64_t row, int64_t m
     return id >= 0 && id < count ? id : -1;
 }
 
-// t[row][0 .. 32 ceil(rank / 32)) for a tile of 16 rows; the four waves share K, 64 ranks at
-// a time. A = the adapter's rows (ranks past the last repeat it, their sums become 0), B = x.
-__global__ __launch_bounds__(256) void lora_down_kernel(const uint16_t *__restrict__ x, int64_t lda, int64_t m, int64_t K,
-                                                       const AdapterDev *__restrict__ ad, int count,
-                                                       const int32_t *__restrict__ ids, float *__restrict__ t, int64_t ldt) {
-    __shared__ f32x4 red[4][4][64];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
-    const int64_t row = (int64_t)blockIdx.x * 16 + l16;
-    const int id = row_id(ids, row, m, count);
-    const uint16_t *xr = x + min(row, m - 1) * lda + 8 * lg;
-    uint64_t todo = __ballot(id >= 0) & 0xffffu;
-    while (todo) {
-        const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
-        todo &= ~__ballot(id == a);
+// ---- many rows: shares of K, 16 RT ranks at a time ----
+
+// part[share][row][ldp] = x A^T over a share of K, for 128 rows and 16 RT ranks (from 64
+// blockIdx.z) per workgroup, once per adapter among the rows' ids; rows of other adapters are
+// not written. Bound by the bytes of x: both operands are copied HBM -> LDS by direct loads in
+// whole 128 B rows of 64 deep (XOR-swizzled slots, three stages), since lanes that load their
+// operand straight from 16 rows of x 64 B at a time reach half the bandwidth however many are
+// in flight (4096 rows of 12288, 64 ranks: 46-52 us). A wave multiplies its 32 rows
+// (v_mfma_f32_16x16x32_bf16, A = the adapter's rows; ranks past the last repeat it).
+template <int RT>
+__global__ __launch_bounds__(256, 2) void lora_down_kernel(const uint16_t *__restrict__ x, int64_t lda, int64_t m, int64_t K,
+                                                          const AdapterDev *__restrict__ ad, int count,
+                                                          const int32_t *__restrict__ ids, float *__restrict__ part, int64_t ldp) {
+    constexpr int XB = 128 * 128, STAGE = XB + RT * 16 * 128;  // bytes of x rows and of a stage
+    constexpr int AI = RT == 4 ? 2 : 1, NI = 4 + AI;           // direct loads of a wave and stage
+    __shared__ __attribute__((aligned(16))) uint8_t lds[3 * STAGE];
+    const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t tile0 = (int64_t)blockIdx.x * 128, row0 = tile0 + 32 * wave + l16;
+    const int r0 = 64 * (int)blockIdx.z;
+    const int64_t steps = K / 64, first = steps * blockIdx.y / gridDim.y, last = steps * (blockIdx.y + 1) / gridDim.y;
+    part += (int64_t)blockIdx.y * m * ldp;
+    const int id[2] = {row_id(ids, row0, m, count), row_id(ids, row0 + 16, m, count)};
+    int all[2];  // of rows lane and lane + 64 of the tile
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        all[u] = row_id(ids, tile0 + 64 * u + lane, m, count);
+        if (all[u] < 0) all[u] = 0x7fffffff;
+    }
+    uint32_t off[2];
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++) off[ks] = (uint32_t)(l16 * 128 + (((4 * ks + lg) ^ swz_key(l16)) << 4));
+    for (int a = -1;;) {
+        // the next adapter of the tile: the smallest id above the last one
+        int next = min(all[0] > a ? all[0] : 0x7fffffff, all[1] > a ? all[1] : 0x7fffffff);
+        for (int o = 32; o > 0; o >>= 1) next = min(next, __shfl_xor(next, o));
+        a = __builtin_amdgcn_readfirstlane(next);
+        if (a == 0x7fffffff) break;
         const AdapterDev d = ad[a];
-        for (int r0 = 0; r0 < d.rank; r0 += 64) {
-            f32x4 acc[4] = {};
-            const uint16_t *ar[4];
+        if (r0 >= d.rank) continue;
+        // one instruction fills 8 rows, lane l row l / 8 at slot l % 8, which holds chunk (l % 8) ^ key(row)
+        const uint16_t *xs[4], *as[AI];
 #pragma unroll
-            for (int i = 0; i < 4; i++) ar[i] = d.a + (int64_t)min(r0 + 16 * i + l16, d.rank - 1) * K + 8 * lg;
-            for (int64_t k = 32 * wave; k < K; k += 128) {
-                const bf16x8 b = *(const bf16x8 *)(xr + k);
+        for (int i = 0; i < 4; i++) {
+            const int r = 32 * wave + 8 * i + (lane >> 3);
+            xs[i] = x + min(tile0 + r, m - 1) * lda + 8 * ((lane & 7) ^ swz_key(r));
+        }
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8 *)(ar[i] + k), b, acc[i], 0, 0, 0);
+        for (int i = 0; i < AI; i++) {  // RT 1: two instructions, each issued by two waves
+            const int r = (AI * wave + i) % (2 * RT) * 8 + (lane >> 3);
+            as[i] = d.a + (int64_t)min(r0 + r, d.rank - 1) * K + 8 * ((lane & 7) ^ swz_key(r));
+        }
+        auto dma = [&](int s, int64_t step) __attribute__((always_inline)) {
+            const int64_t k = min(step, last - 1) * 64;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                __builtin_amdgcn_global_load_lds((const void *)(xs[i] + k), (lds_ptr_t)(lds + s * STAGE + (32 * wave + 8 * i) * 128), 16, 0, 0);
+#pragma unroll
+            for (int i = 0; i < AI; i++)
+                __builtin_amdgcn_global_load_lds((const void *)(as[i] + k),
+                                                 (lds_ptr_t)(lds + s * STAGE + XB + (AI * wave + i) % (2 * RT) * 1024), 16, 0, 0);
+        };
+        f32x4 acc[2][RT] = {};
+        dma(0, first);
+        dma(1, first + 1);
+        int s = 0;
+        for (int64_t step = first; step < last; step++) {
+            __builtin_amdgcn_s_waitcnt(WAIT_VM0 | NI);  // this step's rows have landed
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            dma(s == 0 ? 2 : s - 1, step + 2);  // the stage that the last step read
+            const uint8_t *st = lds + s * STAGE;
+            bf16x8 b[2][2], w[2][RT];
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) {
+#pragma unroll
+                for (int u = 0; u < 2; u++) b[ks][u] = *(const bf16x8 *)(st + (32 * wave + 16 * u) * 128 + off[ks]);
+#pragma unroll
+                for (int i = 0; i < RT; i++) w[ks][i] = *(const bf16x8 *)(st + XB + 16 * i * 128 + off[ks]);
             }
 #pragma unroll
-            for (int i = 0; i < 4; i++) red[wave][i][lane] = acc[i];
-            __syncthreads();
-            // wave i adds rank tile i: ranks r0 + 16 i + 4 lg + e of token l16
-            f32x4 s = red[0][wave][lane];
+            for (int ks = 0; ks < 2; ks++)
 #pragma unroll
-            for (int w = 1; w < 4; w++) s += red[w][wave][lane];
-            const int r = r0 + 16 * wave + 4 * lg;
+                for (int i = 0; i < RT; i++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[e] = r + e < d.rank ? s[e] * d.scale : 0.f;
-            if (id == a && r < ((d.rank + 31) & ~31)) *(f32x4 *)(t + row * ldt + r) = s;
-            __syncthreads();
+                    for (int u = 0; u < 2; u++)
+                        acc[u][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[ks][i], b[ks][u], acc[u][i], 0, 0, 0);
+            s = s == 2 ? 0 : s + 1;
         }
+        __builtin_amdgcn_s_waitcnt(WAIT_VM0_LGKM0);  // no load into LDS still in flight
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+            if (id[u] == a)
+#pragma unroll
+                for (int i = 0; i < RT; i++) *(f32x4 *)(part + (row0 + 16 * u) * ldp + r0 + 16 * i + 4 * lg) = acc[u][i];
     }
 }
 
-// y = base + t B^T for 16 rows x 256 columns, 64 columns per wave. A = B's rows, B = t.
-__global__ __launch_bounds__(256) void lora_up_kernel(const float *__restrict__ t, int64_t ldt, int64_t m, int64_t N,
+// The shares' sums times the scale as two bf16 rows, t16[row][hi 0 .. ldp | lo 0 .. ldp), zeros
+// past the rank; four ranks per thread. Rows without an adapter are not written.
+__global__ __launch_bounds__(256) void lora_split_kernel(const float *__restrict__ part, int shares, int64_t m, int64_t ldp,
+                                                        const AdapterDev *__restrict__ ad, int count,
+                                                        const int32_t *__restrict__ ids, uint16_t *__restrict__ t16, int64_t kt) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = kt / 4, row = i / per;
+    if (row >= m) return;
+    const int id = row_id(ids, row, m, count), r = (int)(i % per) * 4;
+    if (id < 0) return;
+    const int rank = ad[id].rank;
+    const float scale = ad[id].scale;
+    f32x4 s{};
+    if (r < rank)  // written by every share: r < 16 RT ceil(rank / (16 RT))
+    {
+        int p = 0;
+        for (; p + 4 <= shares; p += 4) {  // four loads in flight
+            f32x4 v[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) v[u] = *(const f32x4 *)(part + ((int64_t)(p + u) * m + row) * ldp + r);
+            s += (v[0] + v[1]) + (v[2] + v[3]);
+        }
+        for (; p < shares; p++) s += *(const f32x4 *)(part + ((int64_t)p * m + row) * ldp + r);
+    }
+    float hi[4], lo[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float v = r + e < rank ? s[e] * scale : 0.f;
+        hi[e] = __uint_as_float(pack_bf16x2(v, 0.f) << 16);
+        lo[e] = v - hi[e];
+    }
+    *(u32x2 *)(t16 + row * 2 * kt + r) = u32x2{pack_bf16x2(hi[0], hi[1]), pack_bf16x2(hi[2], hi[3])};
+    *(u32x2 *)(t16 + row * 2 * kt + kt + r) = u32x2{pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3])};
+}
+
+// y = base + t B^T for 16 rows x 256 columns, 64 columns per wave. A = B's rows, B = t's.
+__global__ __launch_bounds__(256) void lora_up_kernel(const uint16_t *__restrict__ t16, int64_t kt, int64_t m, int64_t N,
                                                      const AdapterDev *__restrict__ ad, int count,
                                                      const int32_t *__restrict__ ids, const float *base,
                                                      float *y32, uint16_t *y16) {
@@ -82,24 +178,17 @@ __global__ __launch_bounds__(256) void lora_up_kernel(const float *__restrict__ 
         const AdapterDev d = ad[a];
         for (int r0 = 0; r0 < d.rank; r0 += 32) {
             const int r = r0 + 8 * lg;
-            f32x4 u{}, v{};
+            bf16x8 hi = {}, lo = {};
             if (id == a) {
-                u = *(const f32x4 *)(t + row * ldt + r);
-                v = *(const f32x4 *)(t + row * ldt + r + 4);
-            }
-            const u32x4 hi = u32x4{pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3]), pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-            u32x4 lo;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float p = e < 2 ? u[2 * e] : v[2 * e - 4], q = e < 2 ? u[2 * e + 1] : v[2 * e - 3];
-                lo[e] = pack_bf16x2(p - __uint_as_float(hi[e] << 16), q - __uint_as_float(hi[e] & 0xffff0000u));
+                hi = *(const bf16x8 *)(t16 + row * 2 * kt + r);
+                lo = *(const bf16x8 *)(t16 + row * 2 * kt + kt + r);
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                u32x4 b{};
-                if (r < d.ldb) b = *(const u32x4 *)(d.b + (n0 + 16 * i + l16) * d.ldb + r);
-                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, hi), acc[i], 0, 0, 0);
-                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, lo), acc[i], 0, 0, 0);
+                bf16x8 b = {};
+                if (r < d.ldb) b = *(const bf16x8 *)(d.b + (n0 + 16 * i + l16) * d.ldb + r);
+                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, hi, acc[i], 0, 0, 0);
+                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, lo, acc[i], 0, 0, 0);
             }
         }
     }
@@ -182,29 +271,70 @@ constexpr int64_t FEW_ROWS = 64;
 
 }  // namespace
 
-hipError_t launch_lora_down(const uint16_t *x, int64_t lda, int64_t m, int64_t k, const AdapterDev *ad, int count,
-                            const int32_t *ids, float *t, int64_t ldt, hipStream_t stream) {
+bool lora_few(int64_t m) { return m <= FEW_ROWS; }
+
+hipError_t launch_lora_few_down(const uint16_t *x, int64_t lda, int64_t m, int64_t k, const AdapterDev *ad, int count,
+                                const int32_t *ids, float *t, int64_t ldt, hipStream_t stream) {
     if (m <= 0) return hipSuccess;
-    if (m <= FEW_ROWS) {
-        lora_down_row_kernel<<<dim3((unsigned)((ldt + 3) / 4), (unsigned)m), dim3(256), 0, stream>>>(x, lda, k, ad, count, ids, t, ldt);
-        return hipGetLastError();
-    }
-    lora_down_kernel<<<dim3((unsigned)((m + 15) / 16)), dim3(256), 0, stream>>>(x, lda, m, k, ad, count, ids, t, ldt);
+    if (m > FEW_ROWS) return hipErrorInvalidValue;
+    lora_down_row_kernel<<<dim3((unsigned)((ldt + 3) / 4), (unsigned)m), dim3(256), 0, stream>>>(x, lda, k, ad, count, ids, t, ldt);
     return hipGetLastError();
 }
 
-hipError_t launch_lora_up(const float *t, int64_t ldt, int64_t m, int64_t n, const AdapterDev *ad, int count,
-                          const int32_t *ids, const float *base, float *y32, uint16_t *y16, hipStream_t stream) {
+hipError_t launch_lora_few_up(const float *t, int64_t ldt, int64_t m, int64_t n, const AdapterDev *ad, int count,
+                              const int32_t *ids, const float *base, float *y32, uint16_t *y16, hipStream_t stream) {
     if (m <= 0) return hipSuccess;
-    if (n % 128 || (m + 15) / 16 > 65535) return hipErrorInvalidValue;
-    if (m <= FEW_ROWS) {
-        lora_up_row_kernel<<<dim3((unsigned)((n + 255) / 256), (unsigned)m), dim3(256), 0, stream>>>(t, ldt, n, ad, count, ids,
-                                                                                                    base, y32, y16);
-        return hipGetLastError();
-    }
-    lora_up_kernel<<<dim3((unsigned)((n + 255) / 256), (unsigned)((m + 15) / 16)), dim3(256), 0, stream>>>(t, ldt, m, n, ad, count,
-                                                                                                          ids, base, y32, y16);
+    if (m > FEW_ROWS) return hipErrorInvalidValue;
+    lora_up_row_kernel<<<dim3((unsigned)((n + 255) / 256), (unsigned)m), dim3(256), 0, stream>>>(t, ldt, n, ad, count, ids, base,
+                                                                                                y32, y16);
     return hipGetLastError();
+}
+
+// Ranks per workgroup: 16, 32 or 64 at a time; shares of K: as many as give every CU two
+// workgroups, each of at least 4 steps of 64.
+namespace {
+int rank_tile(int64_t max_rank) { return max_rank <= 16 ? 16 : max_rank <= 32 ? 32 : 64; }
+int down_shares(int64_t m, int64_t k, int64_t max_rank) {
+    const int64_t rt = rank_tile(max_rank), wgs = (m + 127) / 128 * ((max_rank + rt - 1) / rt);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(2 * std::max(device_cu_count(), 1) / wgs, k / 256));
+}
+}  // namespace
+
+size_t lora_down_scratch(int64_t m, int64_t k, int64_t max_rank) {
+    const int64_t rt = rank_tile(max_rank);
+    return (size_t)(down_shares(m, k, max_rank) * m * ((max_rank + rt - 1) / rt * rt)) * 4;
+}
+
+hipError_t launch_lora_down(const uint16_t *x, int64_t lda, int64_t m, int64_t k, int64_t max_rank, const AdapterDev *ad, int count,
+                            const int32_t *ids, float *scratch, uint16_t *t16, hipStream_t stream) {
+    if (m <= 0) return hipSuccess;
+    const int64_t kt = (max_rank + 63) / 64 * 64, rt = rank_tile(max_rank), groups = (max_rank + rt - 1) / rt, ldp = groups * rt;
+    const int shares = down_shares(m, k, max_rank);
+    const dim3 grid((unsigned)((m + 127) / 128), (unsigned)shares, (unsigned)groups);
+    if (rt == 16)
+        lora_down_kernel<1><<<grid, dim3(256), 0, stream>>>(x, lda, m, k, ad, count, ids, scratch, ldp);
+    else if (rt == 32)
+        lora_down_kernel<2><<<grid, dim3(256), 0, stream>>>(x, lda, m, k, ad, count, ids, scratch, ldp);
+    else
+        lora_down_kernel<4><<<grid, dim3(256), 0, stream>>>(x, lda, m, k, ad, count, ids, scratch, ldp);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    lora_split_kernel<<<dim3((unsigned)((m * (kt / 4) + 255) / 256)), dim3(256), 0, stream>>>(scratch, shares, m, ldp, ad, count, ids, t16, kt);
+    return hipGetLastError();
+}
+
+hipError_t launch_lora_up(const uint16_t *t16, int64_t kt, int64_t m, int64_t n, const AdapterDev *ad, int count,
+                          const int32_t *ids, const float *base, float *y32, uint16_t *y16, hipStream_t stream) {
+    if (n % 128) return hipErrorInvalidValue;
+    constexpr int64_t MOST = 16 * 65535;  // rows of one grid
+    for (int64_t r = 0; r < m; r += MOST) {
+        const int64_t rows = std::min(m - r, MOST);
+        lora_up_kernel<<<dim3((unsigned)((n + 255) / 256), (unsigned)((rows + 15) / 16)), dim3(256), 0, stream>>>(
+            t16 + r * 2 * kt, kt, rows, n, ad, count, ids + r, base + r * n, y32 ? y32 + r * n : nullptr,
+            y16 ? y16 + r * n : nullptr);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace qimm

@@ -32,6 +32,8 @@
 // tokens against the 128x128 kernel 4096 x 4096 95 -> 62, 4096 x 12288 (Q6_K)
 // 313 -> 172; bf16 weights 12288 x 4096 at 2050 tokens against the four-wave
 // kernel of qgemm_large.hip 219 -> 191.
+#include <stddef.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -79,25 +81,41 @@ struct Shape {
 
 // EPI's epilogue of tile (m0, n0); `head` tiles of 16 * 4 WT tokens first, then,
 // with SMALL, tiles of half as many.
-template <int EPI, bool SMALL>
+//
+// AD: the rows' low-rank adapters as further k steps, so that their product is summed in
+// the same accumulators and costs neither a pass over the outputs nor its rounding. For
+// each adapter among the tile's ids (in ascending order, the list in LDS) 2 kb steps: the
+// token operand is x.t's row, hi part and then lo part, a zero row for tokens of other
+// adapters; the weight operand the adapter's B rows, zeros past the rank. Two steps of 64
+// for 4096 (rank up to 64): 3% of the products, against 134 MB read and written by a pass
+// over 4096 x 4096 outputs.
+template <int EPI, bool SMALL, bool AD>
 __global__ __launch_bounds__(64 * NWAVE, 1) void qgemm_bf16_kernel(const uint16_t *__restrict__ A, int64_t M, int64_t lda,
                                                                  const uint16_t *__restrict__ W, int64_t N, int64_t K,
-                                                                 EpiParams ep, int head) {
+                                                                 EpiParams ep, int head, AdapterSteps x) {
     constexpr int WN = waves_n<EPI>();
     constexpr int LDS_BYTES = Shape<WN, 4>::LDS > (SMALL ? Shape<WN, 2>::LDS : 0) ? Shape<WN, 4>::LDS : Shape<WN, 2>::LDS;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[LDS_BYTES];
+    constexpr int LIST = AD ? Shape<WN, 4>::BM : 0;  // adapters of a tile, at most one per token
+    __shared__ __attribute__((aligned(16))) uint8_t lds[LDS_BYTES + 4 * LIST];
+    int *list = (int *)(lds + LDS_BYTES);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nt = (int)(N / (128 * WN));
     // a split product (EPI_F32): share blockIdx.y of the k steps, its sums to
     // out [share][M][ldo]
     int KT = (int)(K / BK);
     int64_t k_first = 0;
+    [[maybe_unused]] bool last_share = true;  // whose products the adapters' steps join
     if constexpr (EPI == EPI_F32) {
-        const int sh = blockIdx.y, n = gridDim.y, k0 = KT * sh / n;
+        // with adapters the last share has their steps too (one adapter's counted; the loads
+        // ahead of the list need two steps of K)
+        const int sh = blockIdx.y, n = gridDim.y, all = AD && n > 1 ? KT + 2 * x.kb : KT;
+        const int k0 = AD ? min(all * sh / n, KT - 2) : all * sh / n, k1 = AD && sh < n - 1 ? min(all * (sh + 1) / n, KT - 2) : all * (sh + 1) / n;
         k_first = (int64_t)k0 * BK;
-        KT = KT * (sh + 1) / n - k0;
+        KT = (AD && sh == n - 1 ? KT : k1) - k0;
         ep.out = (float *)ep.out + (int64_t)sh * M * ep.ldo;
+        last_share = sh == n - 1;
     }
+    [[maybe_unused]] const int KB = KT;  // steps over K itself
 
     auto tiles = [&](auto tt_, int idx, int mt, int64_t row0) __attribute__((always_inline)) {
         constexpr int TT = decltype(tt_)::value;
@@ -145,8 +163,86 @@ __global__ __launch_bounds__(64 * NWAVE, 1) void qgemm_bf16_kernel(const uint16_
             const int q = WI * wave + i, r = q / 8 * 128 + q % 8 * 8 + (lane >> 3);
             wsrc[i] = (uint32_t)r * (uint32_t)(2 * K) + 16 * ((lane & 7) ^ swz_key(r));
         }
+        [[maybe_unused]] int tid_of[NTP][TI];  // AD: the adapters of the lane's rows
+        [[maybe_unused]] int slot_at = -1, ad_at = -1, ldb_at = 0;
+        [[maybe_unused]] const uint16_t *b_at = nullptr;
+        [[maybe_unused]] int mine[BM / 64];  // AD: the ids of rows lane, lane + 64, ..
+        if constexpr (AD) {
+#pragma unroll
+            for (int i = 0; i < BM / 64; i++) mine[i] = 64 * i + lane <= mlast ? x.ids[m0 + 64 * i + lane] : -1;
+#pragma unroll
+            for (int i = 0; i < TI; i++) {
+                const int q = TI * wave + i, r = q / (RT / 8) * 16 * TT + q % (RT / 8) * 8 + (lane >> 3);
+#pragma unroll
+                for (int h = 0; h < NTP; h++) tid_of[h][i] = x.ids[m0 + min(r + h * RT, mlast)];
+            }
+        }
+        // the current adapter and its B, in scalar registers: no load of them may be pending in
+        // the loop, whose waits count the direct loads (with one, every phase waited for all of
+        // them: 4096 x 12288 at 4096 tokens 290 -> 690 us)
+        [[maybe_unused]] auto take = [&](int a) __attribute__((always_inline)) {
+            const u32x4 e = *(const u32x4 *)(x.ad + a), f = *((const u32x4 *)(x.ad + a) + 1);
+            static_assert(offsetof(AdapterDev, b) == 8 && offsetof(AdapterDev, ldb) == 20, "as read here");
+            ad_at = a;
+            b_at = (const uint16_t *)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)e[2]) |
+                                      (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)e[3]) << 32);
+            ldb_at = __builtin_amdgcn_readfirstlane((int)f[1]);
+        };
+        // AD, with the first loads in flight: every wave lists the tile's adapters (the smallest id
+        // above the last one, until none is left); the first one's B is looked up here, ahead of its steps
+        auto list_adapters = [&]() __attribute__((always_inline)) {
+            if constexpr (AD) {
+                int n = 0;
+#pragma unroll
+                for (int i = 0; i < BM / 64; i++)
+                    if ((uint32_t)mine[i] >= (uint32_t)x.count) mine[i] = 0x7fffffff;
+                if (last_share)
+                    for (int at = -1;; n++) {
+                        int next = 0x7fffffff;
+#pragma unroll
+                        for (int i = 0; i < BM / 64; i++) next = min(next, mine[i] > at ? mine[i] : 0x7fffffff);
+                        for (int o = 32; o > 0; o >>= 1) next = min(next, __shfl_xor(next, o));
+                        at = __builtin_amdgcn_readfirstlane(next);
+                        if (at == 0x7fffffff) break;
+                        if (n == 0) {
+                            slot_at = 0;
+                            take(at);
+                        }
+                        if (wave == 0 && lane == 0) list[n] = at;
+                    }
+                KT = KB + n * 2 * x.kb;
+#pragma unroll
+                for (int i = 0; i < TI; i++)
+#pragma unroll
+                    for (int h = 0; h < NTP; h++) asm volatile("" : "+v"(tid_of[h][i]));  // arrived
+                __builtin_amdgcn_s_waitcnt(WAIT_LGKM0);  // the list, before the barrier that follows
+            }
+        };
+        // AD: the adapter of step e past K, kept until another one's step comes; its B
+        [[maybe_unused]] auto adapter_of = [&](int e) __attribute__((always_inline)) -> int {
+            const int slot = e / (2 * x.kb);
+            if (slot != slot_at) {
+                slot_at = slot;
+                take(__builtin_amdgcn_readfirstlane(list[slot]));
+            }
+            return e - slot * 2 * x.kb;
+        };
         auto dma_t = [&](int s, int h, int kt) __attribute__((always_inline)) {
-            const char *b = abase + (int64_t)min(kt, KT - 1) * (2 * BK);
+            kt = min(kt, KT - 1);
+            if constexpr (AD)
+                if (kt >= KB) {
+                    const int rem = adapter_of(kt - KB), row = 128 * x.kb;  // elements of a t row
+#pragma unroll
+                    for (int i = 0; i < TI; i++) {
+                        const int q = TI * wave + i, r = q / (RT / 8) * 16 * TT + q % (RT / 8) * 8 + h * RT;
+                        const int rl = r + (lane >> 3), c = 8 * ((lane & 7) ^ swz_key(rl));
+                        const uint16_t *src = x.t + (m0 + min(rl, mlast)) * row + 64 * rem + c;
+                        if (tid_of[h][i] != ad_at) src = x.zero + c;
+                        __builtin_amdgcn_global_load_lds((const void *)src, (lds_ptr_t)(lds + s * TB + r * ROWB), 16, 0, 0);
+                    }
+                    return;
+                }
+            const char *b = abase + (int64_t)kt * (2 * BK);
 #pragma unroll
             for (int i = 0; i < TI; i++) {
                 const int q = TI * wave + i, r = q / (RT / 8) * 16 * TT + q % (RT / 8) * 8 + h * RT;
@@ -154,7 +250,21 @@ __global__ __launch_bounds__(64 * NWAVE, 1) void qgemm_bf16_kernel(const uint16_
             }
         };
         auto dma_w = [&](int s, int h, int kt) __attribute__((always_inline)) {
-            const char *b = wbase + (int64_t)min(kt, KT - 1) * (2 * BK) + (int64_t)h * 64 * 2 * K;
+            kt = min(kt, KT - 1);
+            if constexpr (AD)
+                if (kt >= KB) {
+                    const int blk = adapter_of(kt - KB) % x.kb;
+#pragma unroll
+                    for (int i = 0; i < WI; i++) {
+                        const int q = WI * wave + i, r = q / 8 * 128 + q % 8 * 8 + h * 64;
+                        const int rl = r + (lane >> 3), c = 8 * ((lane & 7) ^ swz_key(rl)), rank = 64 * blk + c;
+                        const uint16_t *src = rank < ldb_at ? b_at + (n0 + rl) * ldb_at + rank : x.zero + c;
+                        __builtin_amdgcn_global_load_lds((const void *)src, (lds_ptr_t)(lds + NS * TB + s * WB + r * ROWB),
+                                                         16, 0, 0);
+                    }
+                    return;
+                }
+            const char *b = wbase + (int64_t)kt * (2 * BK) + (int64_t)h * 64 * 2 * K;
 #pragma unroll
             for (int i = 0; i < WI; i++) {
                 const int q = WI * wave + i, r = q / 8 * 128 + q % 8 * 8 + h * 64;
@@ -226,6 +336,7 @@ __global__ __launch_bounds__(64 * NWAVE, 1) void qgemm_bf16_kernel(const uint16_
             dma_w(0, 1, 0);
             dma_t(1, 0, 1);
             dma_w(1, 0, 1);
+            list_adapters();
             __builtin_amdgcn_s_waitcnt(WAIT_VM0 | (TI + WI));  // step 0 has landed
             barrier();
             if (wave >= 4) barrier();  // waves 4-7 run one barrier behind
@@ -251,6 +362,7 @@ __global__ __launch_bounds__(64 * NWAVE, 1) void qgemm_bf16_kernel(const uint16_
             dma_t(1, 0, 1);
             dma_w(1, 0, 1);
             dma_w(1, 1, 1);
+            list_adapters();
             __builtin_amdgcn_s_waitcnt(WAIT_VM0 | (TI + 2 * WI));
             barrier();
             if (wave >= 4) barrier();
@@ -604,14 +716,14 @@ __global__ __launch_bounds__(256) void weight_rows_bf16_kernel(GemmWeight w, uin
     }
 }
 
-template <int EPI>
+template <int EPI, bool AD = false>
 hipError_t launch_one(const GemmWeight &w, const uint16_t *a, int64_t m, int64_t lda, const EpiParams &ep, int64_t head,
-                      int splits, hipStream_t stream) {
+                      int splits, hipStream_t stream, const AdapterSteps &x = {}) {
     constexpr int WN = waves_n<EPI>(), BM = Shape<WN, 4>::BM, BS = Shape<WN, 2>::BM;
     const int64_t nt = w.n / (128 * WN), rest = std::max<int64_t>(m - head * BM, 0);
     const int64_t wgs = WN == 4 ? (m + BM - 1) / BM * nt : (head + (rest + BS - 1) / BS) * nt;
-    qgemm_bf16_kernel<EPI, WN == 2><<<dim3((unsigned)wgs, (unsigned)splits), dim3(64 * NWAVE), 0, stream>>>(
-        a, m, lda, w.bf16, w.n, w.k, ep, (int)(WN == 4 ? (m + BM - 1) / BM : head));
+    qgemm_bf16_kernel<EPI, WN == 2, AD><<<dim3((unsigned)wgs, (unsigned)splits), dim3(64 * NWAVE), 0, stream>>>(
+        a, m, lda, w.bf16, w.n, w.k, ep, (int)(WN == 4 ? (m + BM - 1) / BM : head), x);
     return hipGetLastError();
 }
 
@@ -711,6 +823,21 @@ hipError_t launch_qgemm_bf16(const GemmWeight &w, const uint16_t *a, int64_t m, 
         return launch_one<EPI_SWIGLU>(w, a, m, lda, ep, plan.head, 1, stream);
     default: return hipErrorInvalidValue;
     }
+}
+
+hipError_t launch_qgemm_bf16_adapters(const GemmWeight &w, const uint16_t *a, int64_t m, int64_t lda, int epi,
+                                      const EpiParams &ep, const Bf16Plan &plan, const AdapterSteps &x, hipStream_t stream) {
+    if (!qgemm_bf16_fits(w) || lda > ((int64_t)1 << 22) || (epi != EPI_F32 && epi != EPI_BF16)) return hipErrorInvalidValue;
+    if (plan.splits > 1) {
+        float *part = (float *)((char *)ep.part_ws + STREAM_COUNTER_BYTES);
+        EpiParams pe{};
+        pe.out = part;
+        pe.ldo = w.n;
+        const hipError_t e = launch_one<EPI_F32, true>(w, a, m, lda, pe, 0, plan.splits, stream, x);
+        return e == hipSuccess ? launch_split_epilogue(part, plan.splits, m, w.n, epi, ep, stream) : e;
+    }
+    return epi == EPI_F32 ? launch_one<EPI_F32, true>(w, a, m, lda, ep, plan.head, 1, stream, x)
+                          : launch_one<EPI_BF16, true>(w, a, m, lda, ep, plan.head, 1, stream, x);
 }
 
 }  // namespace qimm
