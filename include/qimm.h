@@ -272,9 +272,10 @@ int qimm_kv_prefetch(qimm_kv *kv, int64_t layer, void *stream);
  * consecutive keys of one dimension (keys 32 i .. 32 i + 31 of the prefix).
  * Every call that takes a qimm_kv works on it. qimm_kv_store_layer encodes a layer,
  * qimm_kv_load_layer gives what it stands for (exact in bf16); k and v must be 16-byte
- * aligned in both. The attention of up to 64 queries multiplies the codes as they lie; with
- * more, and in the block and the model, the layer is expanded first into one bf16 layer that
- * the cache keeps for it. Nothing is allocated after the creation. That layer and the
+ * aligned in both. Attention (qimm_attention, qimm_attention_masked) multiplies the codes as
+ * they lie or, where that is estimated to be faster (many queries and own keys), expands
+ * the layer first into one bf16 layer that the cache keeps for it, as the block and the
+ * model always do. Nothing is allocated after the creation. That layer and the
  * attention's scratch belong to the cache: calls with one cache must not overlap on the
  * device, two replayed graphs neither. The values of 32 keys share a scale, so one that is
  * no number does not spoil its neighbours: a NaN is stored as 0, an infinity as +-6 2^s of

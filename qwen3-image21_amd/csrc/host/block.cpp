@@ -520,7 +520,9 @@ namespace {
 
 // Few queries over a 4-bit cache: the kernel that multiplies its codes. Many take the
 // expanded layer like any other cache's.
-bool takes_codes(const qimm_kv *kv, int64_t sq) { return kv && kv->bits4 && qimm::attn4_takes(sq); }
+bool takes_codes(const qimm_kv *kv, int64_t sq, int64_t so, bool masked) {
+    return kv && kv->bits4 && qimm::attn4_takes(kv->batch * kv->heads, sq, kv->prefix, so, masked);
+}
 
 int attention_codes(qimm_ctx *ctx, const uint16_t *q, int64_t batch, int64_t heads, int64_t sq, const qimm_kv *kv,
                     int64_t layer, const uint16_t *k_own, const uint16_t *vt_own, int64_t so, float scale,
@@ -551,7 +553,7 @@ int qimm_attention(qimm_ctx *ctx, const uint16_t *q, int64_t batch, int64_t head
     }
     if (P + so == 0) return set_err(ctx, QIMM_ERR_SHAPE, "attention: no keys");
     const hipStream_t s = (hipStream_t)stream;
-    if (takes_codes(kv, sq))
+    if (takes_codes(kv, sq, so, false))
         return attention_codes(ctx, q, batch, heads, sq, kv, layer, k_own, vt_own, so, scale, nullptr, out, s);
     qimm::KeySeg prefix{};
     if (kv) {
@@ -582,7 +584,7 @@ int qimm_attention_masked(qimm_ctx *ctx, const uint16_t *q, int64_t batch, int64
     if (mask->image_ids && (P != 0 || so != sq))
         return set_err(ctx, QIMM_ERR_SHAPE, "attention: the block-causal mask needs no prefix and so == sq");
     const hipStream_t s = (hipStream_t)stream;
-    if (takes_codes(kv, sq) && !mask->image_ids)
+    if (!mask->image_ids && takes_codes(kv, sq, so, true))
         return attention_codes(ctx, q, batch, heads, sq, kv, layer, k_own, vt_own, so, scale, mask->key_valid, out, s);
     int32_t *lim = nullptr;
     if (mask->image_ids) {

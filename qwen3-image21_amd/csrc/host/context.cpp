@@ -401,7 +401,8 @@ int qimm_kv_store_layer(qimm_kv *kv, int64_t layer, const uint16_t *k_bhpd, cons
             return set_err(ctx, QIMM_ERR_ARG, "kv store: k and v must be 16-byte aligned for a 4-bit cache");
         QIMM_HIP(ctx, hipSetDevice(ctx->device));
         QIMM_HIP(ctx, qimm::launch_store4(k_bhpd, v_bhpd, 0, kv->batch, kv->heads, kv->prefix, nullptr, 0,
-                                          kv->q4 + layer * kv->q4_layer(), kv->knorm + layer, s));
+                                          kv->q4 + layer * kv->q4_layer(), kv->knorm_part + layer * qimm::QK_NORM_PARTS,
+                                          kv->knorm + layer, s));
         return QIMM_OK;
     }
     // the layer's largest key norm: the attention's score bound

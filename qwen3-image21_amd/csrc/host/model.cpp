@@ -294,7 +294,7 @@ int qimm_model_prefix_fill(qimm_model *m, const float *txt, int64_t text_len, co
                 rc = block_prefix_forward(blk, x, batch, P, modv, pe, mk, kv->slot[0].k, kv->slot[0].vt, stream);
                 if (rc) return rc;
                 QIMM_HIP(ctx, qimm::launch_store4(kv->slot[0].k, kv->slot[0].vt, qimm::vt_ld(P), batch, H, P, key_valid, P,
-                                                  kv->q4 + i * kv->q4_layer(), kv->knorm + i, s));
+                                                  kv->q4 + i * kv->q4_layer(), kv->knorm_part + i * qimm::QK_NORM_PARTS, kv->knorm + i, s));
                 continue;
             }
             rc = block_prefix_forward(blk, x, batch, P, modv, pe, mk, kv->k + i * kv->layer_elems(),

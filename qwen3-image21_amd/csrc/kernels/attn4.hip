@@ -14,7 +14,7 @@
 // of its row's largest) and a probability to 2^-9, as the rounding to bf16 of the other
 // kernels does. Two products of 128 deep cost the matrix pipe what the bf16 ones would.
 //
-// A workgroup is 16 NQ queries of one head and a share of the keys, four waves taking
+// A workgroup is 16 queries of one head and a share of the keys, four waves taking
 // tiles of 128 keys in turn (64 own keys); a tile's 17 KB go straight into registers, the
 // next tile's keys while this one's softmax and P V run, its values after that: nothing
 // waits on a barrier until the waves' sums are joined through LDS. With several shares
@@ -63,29 +63,39 @@ struct Attn4 {
     uint16_t *out;          // [B,Sq,H*128]
     float *part;            // shares > 1: O [share][B*H*Sq][128], then (m, l) [share][B*H*Sq]
     int shares;
+    uint32_t qtiles;        // tiles of 16 queries
+    uint32_t spread;        // heads x shares are a multiple of the XCDs
 };
 
-template <int NQ, bool MASKED>
-__global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attn4_kernel(const Attn4 a) {
+template <bool MASKED>
+__global__ __launch_bounds__(256, 2) void attn4_kernel(const Attn4 a) {
     constexpr int PITCH = 132;  // floats per query row in LDS
-    __shared__ __attribute__((aligned(16))) float so[4 * 16 * NQ * PITCH];
-    __shared__ float sm[4][16 * NQ], sl[4][16 * NQ];
+    __shared__ __attribute__((aligned(16))) float so[4 * 16 * PITCH];
+    __shared__ float sm[4][16], sl[4][16];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int l16 = lane & 15, lg = lane >> 4;
-    const int64_t bh = blockIdx.x / a.shares, b = bh / a.H;
-    const int share = (int)(blockIdx.x % a.shares);
-    const int64_t q0 = (int64_t)blockIdx.y * 16 * NQ;
+    // The query tiles of one share of a head run next to each other on one XCD (workgroups
+    // go to the eight in turn), where the second one finds the keys in L2.
+    uint32_t at = blockIdx.x, qt;
+    if (a.spread) {
+        qt = (at >> 3) % a.qtiles;
+        at = (at >> 3) / a.qtiles * 8 + (at & 7);
+    } else {
+        qt = at % a.qtiles;
+        at /= a.qtiles;
+    }
+    const int share = (int)(at % a.shares);
+    const int64_t bh = at / a.shares, b = bh / a.H, q0 = (int64_t)qt * 16;
     const int64_t items = a.T + (a.So + OWN_KEYS - 1) / OWN_KEYS;
     const int64_t first = items * share / a.shares, last = items * (share + 1) / a.shares;
     const uint8_t *tiles = a.tiles + bh * a.T * KV4_TILE;
 
     // ---- queries: lane (l16, lg) holds dimensions 16 lg .. + 15 and 64 + 16 lg .. + 15 of query
     // l16, scaled by a power of two so that the row's largest lies in [128, 256) ----
-    i32x8 qhi[NQ], qlo[NQ];
-    int qsc[NQ];  // scale bytes: hi, lo
-#pragma unroll
-    for (int n = 0; n < NQ; n++) {
-        const int64_t qi = min(q0 + 16 * n + l16, a.Sq - 1);
+    i32x8 qhi, qlo;
+    int qsc;  // scale bytes: hi, lo
+    {
+        const int64_t qi = min(q0 + l16, a.Sq - 1);
         const u32x4 *src = (const u32x4 *)(a.q + (bh * a.Sq + qi) * 128 + 16 * lg);
         u32x4 w[4];
         uint32_t mag = 0;
@@ -100,27 +110,20 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attn4_kernel(const Attn4
         const int ex = (int)(mag >> 7);                            // biased exponent of the row's largest
         const int by = ex == 255 ? 255 : max(ex - 7, 6);           // 2^(ex - 134), biased; no number: NaN
         const float up = __uint_as_float((uint32_t)(254 - min(by, 253)) << 23);
-        qsc[n] = by | (by == 255 ? 255 : by - 5) << 8;
+        qsc = by | (by == 255 ? 255 : by - 5) << 8;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const uint32_t x = w[e >> 1][2 * (e & 1)] ^ a.flip, y = w[e >> 1][2 * (e & 1) + 1] ^ a.flip;
             int hi, lo;
             split4(__uint_as_float(x << 16) * up, __uint_as_float(x & 0xffff0000u) * up, __uint_as_float(y << 16) * up,
                    __uint_as_float(y & 0xffff0000u) * up, hi, lo);
-            qhi[n][e] = hi;
-            qlo[n][e] = lo;
+            qhi[e] = hi;
+            qlo[e] = lo;
         }
     }
 
-    f32x4 o[NQ][8];  // [d tile]: dimensions 16 j + 4 lg + r of query l16
-    float m[NQ], l[NQ];
-#pragma unroll
-    for (int n = 0; n < NQ; n++) {
-        m[n] = -INFINITY;
-        l[n] = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; j++) o[n][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+    f32x4 o[8] = {};  // [d tile]: dimensions 16 j + 4 lg + r of query l16
+    float m = -INFINITY, l = 0.f;
 
     u32x4 kc[8], vc[8];
     int ks[2], vs[2];
@@ -141,7 +144,7 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attn4_kernel(const Attn4
     // The running maximum over the N scores of a lane's query and its three other lanes',
     // with the sums taken along; the scores become 2^8 exp(scale (s - max)), hidden ones 0.
     // `seen` has a bit per score.
-    auto softmax = [&](float *s, auto count, int n, bool some, uint32_t seen) __attribute__((always_inline)) {
+    auto softmax = [&](float *s, auto count, bool some, uint32_t seen) __attribute__((always_inline)) {
         constexpr int N = decltype(count)::value;
         if (some)
 #pragma unroll
@@ -151,16 +154,16 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attn4_kernel(const Attn4
         for (int e = 1; e < N; e++) mx = fmaxf(mx, s[e]);
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        mx = fmaxf(mx, m[n]);
-        if (__ballot(mx > m[n])) {
+        mx = fmaxf(mx, m);
+        if (__ballot(mx > m)) {
             // a lane without a visible key so far has sums of 0
-            const float al = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[n] - mx) * a.sl2);
-            m[n] = mx;
-            l[n] *= al;
+            const float al = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mx) * a.sl2);
+            m = mx;
+            l *= al;
 #pragma unroll
             for (int j = 0; j < 8; j++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) o[n][j][r] *= al;
+                for (int r = 0; r < 4; r++) o[j][r] *= al;
         }
         const float c = 8.f - (mx == -INFINITY ? 0.f : mx * a.sl2);
         float sum = 0.f;
@@ -171,52 +174,63 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attn4_kernel(const Attn4
             s[e] = p;
             sum += p;
         }
-        l[n] += sum;
+        l += sum;
     };
-    // visible keys of 64 from key k0 of the P + So, the first `have` of them there
+    // visible keys of 64 from key k0 of the P + So, the first `have` of them there (have >= 1)
     auto validity = [&](int64_t k0, int have) __attribute__((always_inline)) -> uint64_t {
         bool ok = lane < have;
-        if constexpr (MASKED) {
-            const uint8_t byte = a.kvalid[b * (a.P + a.So) + k0 + min(lane, have - 1)];
-            ok = ok && byte != 0;
-        }
+        if constexpr (MASKED) ok = ok && a.kvalid[b * (a.P + a.So) + k0 + min(lane, have - 1)] != 0;
         return __ballot(ok);
+    };
+    // the same of tile i's 128 keys in two steps: the bytes, and the masks. A tile without a
+    // visible key is neither read nor multiplied.
+    struct Bytes {
+        uint32_t lo, hi;
+    };
+    auto bytes_of = [&](int64_t i) __attribute__((always_inline)) -> Bytes {
+        if constexpr (!MASKED) return {1, 1};
+        const int64_t left = a.P - 1 - i * KV4_KEYS;
+        const uint8_t *p = a.kvalid + b * (a.P + a.So) + i * KV4_KEYS;
+        return {p[min((int64_t)lane, left)], p[min((int64_t)lane + 64, left)]};
+    };
+    uint64_t seen_lo = 0, seen_hi = 0;
+    auto masks_of = [&](int64_t i, Bytes y) __attribute__((always_inline)) {
+        const int have = (int)min(a.P - i * KV4_KEYS, (int64_t)KV4_KEYS);
+        seen_lo = __ballot(lane < have && y.lo != 0);
+        seen_hi = __ballot(lane + 64 < have && y.hi != 0);
     };
 
     int64_t it = first + wave;
-    if (it < last && it < a.T) {
-        load_k(it);
-        load_v(it);
-    }
-    for (; it < last && it < a.T; it += 4) {
-        const int64_t key0 = it * KV4_KEYS;
-        const int have = (int)min(a.P - key0, (int64_t)KV4_KEYS);
-        uint32_t seen = 0xffffffffu;
-        bool some = false;
-        if (MASKED || have < KV4_KEYS) {
-            const uint64_t lo = validity(key0, min(have, 64)), hi = have > 64 ? validity(key0 + 64, have - 64) : 0;
-            some = (lo & hi) != ~0ull;
-            seen = (uint32_t)((lo >> (16 * lg)) & 0xffffu) | (uint32_t)((hi >> (16 * lg)) & 0xffffu) << 16;
+    const int64_t end = min(last, a.T);
+    if (it < end) {
+        masks_of(it, bytes_of(it));
+        if (seen_lo | seen_hi) {
+            load_k(it);
+            load_v(it);
         }
-        const bool more = it + 4 < last && it + 4 < a.T;
-#pragma unroll
-        for (int n = 0; n < NQ; n++) {
+    }
+    for (; it < end; it += 4) {
+        const int64_t next = it + 4;
+        const Bytes ny = next < end ? bytes_of(next) : Bytes{0, 0};
+        const bool any = seen_lo | seen_hi, some = (seen_lo & seen_hi) != ~0ull;
+        const uint32_t seen = (uint32_t)((seen_lo >> (16 * lg)) & 0xffffu) | (uint32_t)((seen_hi >> (16 * lg)) & 0xffffu) << 16;
+        f32x4 acc[8] = {};
+        if (any) {
+#define QK(i, q, sel) \
+    acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(kc[i]), q, acc[i], 4, 0, i & 3, ks[i >> 2], sel, qsc);
+            QK(0, qhi, 0) QK(1, qhi, 0) QK(2, qhi, 0) QK(3, qhi, 0) QK(4, qhi, 0) QK(5, qhi, 0) QK(6, qhi, 0) QK(7, qhi, 0)
+            QK(0, qlo, 1) QK(1, qlo, 1) QK(2, qlo, 1) QK(3, qlo, 1) QK(4, qlo, 1) QK(5, qlo, 1) QK(6, qlo, 1) QK(7, qlo, 1)
+#undef QK
+        }
+        seen_lo = seen_hi = 0;
+        if (next < end) masks_of(next, ny);
+        const bool more = seen_lo | seen_hi;
+        if (more) load_k(next);
+        if (any) {
             float s[32];
-            f32x4 acc[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#define QK(i) \
-    acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(kc[i]), qhi[n], acc[i], 4, 0, i & 3, ks[i >> 2], 0, qsc[n]);
-            QK(0) QK(1) QK(2) QK(3) QK(4) QK(5) QK(6) QK(7)
-#undef QK
-#define QK(i) \
-    acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(kc[i]), qlo[n], acc[i], 4, 0, i & 3, ks[i >> 2], 1, qsc[n]);
-            QK(0) QK(1) QK(2) QK(3) QK(4) QK(5) QK(6) QK(7)
-#undef QK
-            if (n == NQ - 1 && more) load_k(it + 4);
 #pragma unroll
             for (int e = 0; e < 32; e++) s[e] = acc[e >> 2][e & 3];
-            softmax(s, std::integral_constant<int, 32>{}, n, some, seen);
+            softmax(s, std::integral_constant<int, 32>{}, some, seen);
             i32x8 ph, pl;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
@@ -226,16 +240,13 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attn4_kernel(const Attn4
                 pl[i] = lo;
             }
             constexpr int psc = 127 | 122 << 8;
-#define PV(j) \
-    o[n][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(vc[j]), ph, o[n][j], 4, 0, j & 3, vs[j >> 2], 0, psc);
-            PV(0) PV(1) PV(2) PV(3) PV(4) PV(5) PV(6) PV(7)
+#define PV(j, p, sel) \
+    o[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(vc[j]), p, o[j], 4, 0, j & 3, vs[j >> 2], sel, psc);
+            PV(0, ph, 0) PV(1, ph, 0) PV(2, ph, 0) PV(3, ph, 0) PV(4, ph, 0) PV(5, ph, 0) PV(6, ph, 0) PV(7, ph, 0)
+            PV(0, pl, 1) PV(1, pl, 1) PV(2, pl, 1) PV(3, pl, 1) PV(4, pl, 1) PV(5, pl, 1) PV(6, pl, 1) PV(7, pl, 1)
 #undef PV
-#define PV(j) \
-    o[n][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(vc[j]), pl, o[n][j], 4, 0, j & 3, vs[j >> 2], 1, psc);
-            PV(0) PV(1) PV(2) PV(3) PV(4) PV(5) PV(6) PV(7)
-#undef PV
-            if (n == NQ - 1 && more) load_v(it + 4);
         }
+        if (more) load_v(next);
     }
 
     // ---- own keys, 64 at a time in two groups of 32 (bf16 products of 32 deep): row m of
@@ -250,9 +261,8 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attn4_kernel(const Attn4
         const bool some = ok != ~0ull;
         const uint32_t seen = (uint32_t)((ok >> (8 * lg)) & 0xffu) | (uint32_t)((ok >> (32 + 8 * lg)) & 0xffu) << 8;
         const bool rows16 = (a.So & 7) == 0;
-#pragma unroll
-        for (int n = 0; n < NQ; n++) {
-            const int64_t qi = min(q0 + 16 * n + l16, a.Sq - 1);
+        {
+            const int64_t qi = min(q0 + l16, a.Sq - 1);
             const uint16_t *qp = a.q + (bh * a.Sq + qi) * 128 + 8 * lg;
             bf16x8 qf[4];
 #pragma unroll
@@ -271,7 +281,7 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attn4_kernel(const Attn4
 #pragma unroll
                     for (int r = 0; r < 4; r++) s[8 * g + 4 * i + r] = acc[r];
                 }
-            softmax(s, std::integral_constant<int, 16>{}, n, some, seen);
+            softmax(s, std::integral_constant<int, 16>{}, some, seen);
 #pragma unroll
             for (int g = 0; g < 2; g++) {
                 if (32 * g >= have) continue;
@@ -294,28 +304,25 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attn4_kernel(const Attn4
 #pragma unroll
                         for (int e = 0; e < 4; e++)
                             v[e] &= ((keep >> (2 * e)) & 1u ? 0xffffu : 0u) | ((keep >> (2 * e + 1)) & 1u ? 0xffff0000u : 0u);
-                    o[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v), __builtin_bit_cast(bf16x8, p),
-                                                                      o[n][j], 0, 0, 0);
+                    o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v), __builtin_bit_cast(bf16x8, p),
+                                                                      o[j], 0, 0, 0);
                 }
             }
         }
     }
 
     // ---- the four waves' sums ----
-#pragma unroll
-    for (int n = 0; n < NQ; n++) {
-        l[n] += __shfl_xor(l[n], 16);
-        l[n] += __shfl_xor(l[n], 32);
-        if (lg == 0) {
-            sm[wave][16 * n + l16] = m[n];
-            sl[wave][16 * n + l16] = l[n];
-        }
-        float *row = so + (wave * 16 * NQ + 16 * n + l16) * PITCH + 4 * lg;
-#pragma unroll
-        for (int j = 0; j < 8; j++) *(f32x4 *)(row + 16 * j) = o[n][j];
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (lg == 0) {
+        sm[wave][l16] = m;
+        sl[wave][l16] = l;
     }
+    float *mine = so + (wave * 16 + l16) * PITCH + 4 * lg;
+#pragma unroll
+    for (int j = 0; j < 8; j++) *(f32x4 *)(mine + 16 * j) = o[j];
     __syncthreads();
-    constexpr int TPQ = 16 / NQ, DPT = 128 / TPQ;  // threads per query, dimensions per thread
+    constexpr int TPQ = 16, DPT = 8;  // threads per query, dimensions per thread
     const int ql = tid / TPQ, d0 = (tid % TPQ) * 4;
     const int64_t qi = q0 + ql;
     if (qi >= a.Sq) return;
@@ -325,7 +332,7 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attn4_kernel(const Attn4
         f[w] = sm[w][ql] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((sm[w][ql] - mm) * a.sl2);
         ll += sl[w][ql] * f[w];
     }
-    const int64_t row = bh * a.Sq + qi, rows = (int64_t)gridDim.x / a.shares * a.Sq;
+    const int64_t row = bh * a.Sq + qi, rows = (int64_t)(gridDim.x / (a.qtiles * (uint32_t)a.shares)) * a.Sq;
     if (a.shares > 1 && tid % TPQ == 0) {
         float *ml = a.part + (int64_t)a.shares * rows * 128 + ((int64_t)share * rows + row) * 2;
         ml[0] = mm;
@@ -338,7 +345,7 @@ __global__ __launch_bounds__(256, NQ == 4 ? 1 : 2) void attn4_kernel(const Attn4
         f32x4 v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-            const f32x4 x = *(const f32x4 *)(so + (w * 16 * NQ + ql) * PITCH + d);
+            const f32x4 x = *(const f32x4 *)(so + (w * 16 + ql) * PITCH + d);
 #pragma unroll
             for (int r = 0; r < 4; r++) v[r] += x[r] * f[w];
         }
@@ -375,35 +382,37 @@ __global__ __launch_bounds__(256) void attn4_join_kernel(const float *__restrict
     *(uint32_t *)(out + ((bh / H * Sq + qi) * H + bh % H) * 128 + 2 * lane) = pack_bf16x2(v[0] * inv, v[1] * inv);
 }
 
-// Query tiles of 16 per workgroup, and shares of the keys: two workgroups per CU (one with
-// four tiles, whose registers fill it), each with at least a tile for every wave, at most 64.
-struct Plan {
-    int nq;
-    int shares;
-};
-Plan plan_of(int64_t bh, int64_t sq, int64_t items) {
-    const int nq = sq <= 16 ? 1 : sq <= 32 ? 2 : 4;
-    const int64_t cus = std::max(device_cu_count(), 1), want = nq == 4 ? cus : 2 * cus;
-    const int64_t wgs = bh * ((sq + 16 * nq - 1) / (16 * nq));
-    return {nq, (int)std::max<int64_t>(1, std::min<int64_t>({want / wgs, (items + 3) / 4, 64}))};
-}
-
-template <bool MASKED>
-void launch_nq(int nq, dim3 grid, const Attn4 &a, hipStream_t stream) {
-    if (nq == 1)
-        attn4_kernel<1, MASKED><<<grid, dim3(256), 0, stream>>>(a);
-    else if (nq == 2)
-        attn4_kernel<2, MASKED><<<grid, dim3(256), 0, stream>>>(a);
-    else
-        attn4_kernel<4, MASKED><<<grid, dim3(256), 0, stream>>>(a);
+// Shares of the keys: two workgroups per CU, each share at least a tile for every wave, at most 64.
+int shares_of(int64_t wgs, int64_t items) {
+    const int64_t want = 2 * (int64_t)std::max(device_cu_count(), 1);
+    return (int)std::max<int64_t>(1, std::min<int64_t>({want / wgs, (items + 3) / 4, 64}));
 }
 
 }  // namespace
 
-// more than one share only with at most `want` workgroups of 16 nq rows: 2 x 16 or 64 per CU
-size_t attn4_scratch_bytes() { return (size_t)std::max(device_cu_count(), 1) * 64 * (128 + 2) * 4; }
+// more than one share only with at most two workgroups of 16 rows per CU
+size_t attn4_scratch_bytes() { return (size_t)std::max(device_cu_count(), 1) * 2 * 16 * (128 + 2) * 4; }
 
-bool attn4_takes(int64_t sq) { return sq <= 64; }
+// Which calls this kernel takes: those it is estimated to do before the expansion of the layer
+// and attention.hip, in us. Here 16 queries over 128 keys of the cache take 1.39 ns with the
+// card full, over 64 own keys 4 ns (8 requests of 32 heads, 4299 keys: 256 queries 193 and with
+// as many own keys 232, 1024 queries 772). There the expansion moves 2.53 B a value at 5 TB/s
+// and two launches take about 12; a round of 256-query tiles takes 2.15 per 64 keys (masked
+// 1.8 and no half tiles) and 8, 0.63 of that where half tiles fill at most one per CU.
+// Measured, here / there: 1 x 32 heads over 333 keys, 64 queries 7 / 20, 512 with as many own
+// 39 / 31; over 4299, 512 with as many own 76 / 121, 1024 200 / 132 and without own keys 102 /
+// 122; 8 x 32 heads over 4299 with as many own, 256 232 / 332, 512 625 / 461.
+bool attn4_takes(int64_t bh, int64_t sq, int64_t p, int64_t so, bool masked) {
+    const double cus = (double)std::max(device_cu_count(), 1), part = 256.0 / cus;
+    const double tiles = (double)bh * (double)((sq + 15) / 16);
+    const double here = 8.0 + part * tiles * (1.39e-3 * (double)((p + KV4_KEYS - 1) / KV4_KEYS) +
+                                              4.0e-3 * (double)((so + OWN_KEYS - 1) / OWN_KEYS));
+    const double blocks = (double)((p + 63) / 64 + (so + 63) / 64), n8 = (double)((sq + 255) / 256 * bh);
+    const bool half = !masked && (double)((sq + 127) / 128 * bh) <= cus;
+    const double rounds = half ? 0.63 : (double)(int64_t)((n8 + cus - 1) / cus);
+    const double there = 12.0 + (double)bh * (double)p * 256.0 * 2.53 / 5e6 + rounds * ((masked ? 1.8 : 2.15) * blocks + 8.0);
+    return here <= there;
+}
 
 hipError_t launch_attn4(const uint16_t *q, const uint8_t *tiles, int64_t p, const uint16_t *k_own, const uint16_t *vt_own,
                         int64_t so, const uint8_t *kvalid, int64_t b, int64_t h, int64_t sq, float scale, float *scratch,
@@ -411,20 +420,20 @@ hipError_t launch_attn4(const uint16_t *q, const uint8_t *tiles, int64_t p, cons
     if (sq <= 0 || b <= 0 || h <= 0) return hipSuccess;
     if (p < 0 || so < 0 || p + so <= 0 || !scratch) return hipErrorInvalidValue;
     const int64_t bh = b * h, T = (p + KV4_KEYS - 1) / KV4_KEYS, items = T + (so + OWN_KEYS - 1) / OWN_KEYS;
-    const Plan pl = plan_of(bh, sq, items);
-    const int64_t qt = (sq + 16 * pl.nq - 1) / (16 * pl.nq);
-    if (bh * pl.shares >= ((int64_t)1 << 31) || qt > 65535) return hipErrorInvalidValue;
+    const int64_t qt = (sq + 15) / 16;
+    const int shares = shares_of(bh * qt, items);
+    if (bh * qt * shares >= ((int64_t)1 << 31)) return hipErrorInvalidValue;
     const float sl2 = scale * 1.4426950408889634f;
     const Attn4 a{q, tiles, p, T, k_own, vt_own, so, kvalid, h, sq, sl2 < 0.f ? -sl2 : sl2,
-                  sl2 < 0.f ? 0x80008000u : 0u, out, scratch, pl.shares};
-    const dim3 grid((unsigned)(bh * pl.shares), (unsigned)qt);
+                  sl2 < 0.f ? 0x80008000u : 0u, out, scratch, shares, (uint32_t)qt, (uint32_t)(bh * shares % 8 == 0)};
+    const dim3 grid((unsigned)(bh * qt * shares));
     if (kvalid)
-        launch_nq<true>(pl.nq, grid, a, stream);
+        attn4_kernel<true><<<grid, dim3(256), 0, stream>>>(a);
     else
-        launch_nq<false>(pl.nq, grid, a, stream);
+        attn4_kernel<false><<<grid, dim3(256), 0, stream>>>(a);
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || pl.shares == 1) return e;
-    attn4_join_kernel<<<dim3((unsigned)((bh * sq + 3) / 4)), dim3(256), 0, stream>>>(scratch, pl.shares, bh * sq, h, sq, a.sl2, out);
+    if (e != hipSuccess || shares == 1) return e;
+    attn4_join_kernel<<<dim3((unsigned)((bh * sq + 3) / 4)), dim3(256), 0, stream>>>(scratch, shares, bh * sq, h, sq, a.sl2, out);
     return hipGetLastError();
 }
 

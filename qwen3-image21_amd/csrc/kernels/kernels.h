@@ -316,16 +316,17 @@ int64_t kv4_layer_bytes(int64_t bh, int64_t p);
 // Stores one layer: k [B,H,P,128] bf16 and v, [B,H,P,128] with vt_ld 0 or [B,H,128,vt_ld]
 // (vt_ld a multiple of 8, >= p). Of the transposed form, keys with kvalid[b * valid_ld +
 // key] == 0 are stored as zeros (kvalid may be null). *norm (device): a bound of the stored
-// keys' norms, NaN or infinite keys +inf.
+// keys' norms, +inf with NaN or infinite keys; norm_part: QK_NORM_PARTS floats of scratch.
 hipError_t launch_store4(const uint16_t *k, const uint16_t *v, int64_t vt_ld, int64_t b, int64_t h, int64_t p,
-                         const uint8_t *kvalid, int64_t valid_ld, uint8_t *tiles, float *norm, hipStream_t stream);
+                         const uint8_t *kvalid, int64_t valid_ld, uint8_t *tiles, float *norm_part, float *norm,
+                         hipStream_t stream);
 // Reads one layer back: k [BH,P,128] and v [BH,P,128] (vt_ld 0) or [BH,128,vt_ld].
 hipError_t launch_load4(const uint8_t *tiles, int64_t bh, int64_t p, int64_t vt_ld, uint16_t *k, uint16_t *v,
                         hipStream_t stream);
 // Attention of sq queries q [B,H,sq,128] over [4-bit layer ; own], out [B,sq,H*128] bf16;
 // own keys dense (vt_own [B,H,128,so]), kvalid [B][p + so] or null, scratch
-// attn4_scratch_bytes(). For few queries (attn4_takes).
-bool attn4_takes(int64_t sq);
+// attn4_scratch_bytes(). attn4_takes: whether it is the faster way for a call.
+bool attn4_takes(int64_t bh, int64_t sq, int64_t p, int64_t so, bool masked);
 size_t attn4_scratch_bytes();
 hipError_t launch_attn4(const uint16_t *q, const uint8_t *tiles, int64_t p, const uint16_t *k_own, const uint16_t *vt_own,
                         int64_t so, const uint8_t *kvalid, int64_t b, int64_t h, int64_t sq, float scale, float *scratch,

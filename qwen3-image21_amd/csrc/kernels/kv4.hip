@@ -12,6 +12,8 @@
 // other way round. 16 B accesses, one block per thread and step; V is taken from rows
 // [P][128] by threads that hold four dimensions of 32 keys, so that rows are read 256 B
 // at a time.
+#include <algorithm>
+
 #include "kernels.h"
 #include "kv4.h"
 
@@ -52,61 +54,76 @@ __device__ __forceinline__ int scale_at(int base, int i, int lane) { return base
 
 // ---- storing ----
 
-// Keys [BH][P][128] (bf16) of one tile per workgroup, one block of 32 dimensions per thread
-// and step. A block with a NaN or an infinity gets the scale byte 255 and stands for NaN
-// throughout: the key's scores are NaN, as they would be from the bf16 cache. A key with
-// kvalid[b][key] == 0 is stored as zeros. norm: the largest norm of a stored key (the bits
-// of a float >= 0, which order as integers), set to 0 before this launch.
+// Keys [BH][P][128] (bf16), one block of 32 dimensions per thread and step, the tiles in turn
+// over the workgroups. A block with a NaN or an infinity gets the scale byte 255 and stands for
+// NaN throughout: the key's scores are NaN, as they would be from the bf16 cache. A key with
+// kvalid[b][key] == 0 is stored as zeros. part[workgroup]: the largest norm of its keys; the
+// kernel that stores the values comes after this one and takes their maximum (an atomic
+// maximum of every tile into one address took 5-10 ns each: 8395 keys of 32 heads 36 us).
 __global__ __launch_bounds__(256) void store_k4_kernel(const uint16_t *__restrict__ k, int64_t P, int64_t heads,
-                                                       const uint8_t *__restrict__ kvalid, int64_t valid_ld,
-                                                       uint8_t *__restrict__ tiles, uint32_t *__restrict__ norm) {
+                                                       const uint8_t *__restrict__ kvalid, int64_t valid_ld, int64_t T,
+                                                       int64_t count, uint8_t *__restrict__ tiles, float *__restrict__ part) {
     __shared__ float top[4];
-    const int64_t bh = blockIdx.y, T = gridDim.x;
+    __shared__ __attribute__((aligned(16))) uint8_t scales[512];
     const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
-    uint8_t *tile = tiles + (bh * T + blockIdx.x) * KV4_TILE;
     float most = 0.f;
+    for (int64_t at = blockIdx.x; at < count; at += gridDim.x) {
+        const int64_t bh = at / T, t = at % T;
+        uint8_t *tile = tiles + at * KV4_TILE;
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const int i = (tid >> 6) + 4 * h;
-        const int64_t key = (int64_t)blockIdx.x * KV4_KEYS + kv4_key(i, l16);
-        u32x4 w[4] = {};
-        if (key < P && (!kvalid || kvalid[bh / heads * valid_ld + key])) {
-            const u32x4 *src = (const u32x4 *)(k + (bh * P + key) * 128 + 32 * lg);
+        for (int h = 0; h < 2; h++) {
+            const int i = (tid >> 6) + 4 * h;
+            const int64_t key = t * KV4_KEYS + kv4_key(i, l16);
+            u32x4 w[4] = {};
+            if (key < P && (!kvalid || kvalid[bh / heads * valid_ld + key])) {
+                const u32x4 *src = (const u32x4 *)(k + (bh * P + key) * 128 + 32 * lg);
 #pragma unroll
-            for (int e = 0; e < 4; e++) w[e] = src[e];
-        }
-        uint32_t mag = 0;
-#pragma unroll
-        for (int e = 0; e < 16; e++) mag = max_mag(mag, w[e >> 2][e & 3]);
-        const uint32_t byte = mag < 0x7f80u ? scale_byte(mag) : 255u;
-        const float sc = scale_of(mag < 0x7f80u ? byte : 127u);
-        u32x4 c;
-        float ss = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            c[e] = encode8(w[e], sc);
-            const u32x4 v = decode8(c[e], sc);
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const float a = __uint_as_float(v[q] << 16), b = __uint_as_float(v[q] & 0xffff0000u);
-                ss += a * a + b * b;
+                for (int e = 0; e < 4; e++) w[e] = src[e];
             }
+            uint32_t mag = 0;
+#pragma unroll
+            for (int e = 0; e < 16; e++) mag = max_mag(mag, w[e >> 2][e & 3]);
+            const uint32_t byte = mag < 0x7f80u ? scale_byte(mag) : 255u;
+            const float sc = scale_of(mag < 0x7f80u ? byte : 127u);
+            u32x4 c;
+            float ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                c[e] = encode8(w[e], sc);
+                const u32x4 v = decode8(c[e], sc);
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const float a = __uint_as_float(v[q] << 16), b = __uint_as_float(v[q] & 0xffff0000u);
+                    ss += a * a + b * b;
+                }
+            }
+            if (byte == 255u) ss = INFINITY;
+            *(u32x4 *)(tile + chunk_of(0, i, lane)) = c;
+            scales[scale_at(0, i, lane)] = (uint8_t)byte;
+            ss += __shfl_xor(ss, 16);
+            ss += __shfl_xor(ss, 32);
+            most = fmaxf(most, ss);
         }
-        if (byte == 255u) ss = INFINITY;
-        *(u32x4 *)(tile + chunk_of(0, i, lane)) = c;
-        tile[scale_at(KV4_KS, i, lane)] = (uint8_t)byte;
-        ss += __shfl_xor(ss, 16);
-        ss += __shfl_xor(ss, 32);
-        most = fmaxf(most, ss);
+        __syncthreads();
+        if (tid < 32) *(u32x4 *)(tile + KV4_KS + 16 * tid) = *(const u32x4 *)(scales + 16 * tid);
+        __syncthreads();
     }
     for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
     if (lane == 0) top[tid >> 6] = most;
     __syncthreads();
-    if (tid == 0) {
-        most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        // a bound: the f32 sum of 128 squares and the root are off by less than 2^-16
-        atomicMax(norm, __float_as_uint(sqrtf(most) * 1.0001f));
-    }
+    // a bound: the f32 sum of 128 squares and the root are off by less than 2^-16
+    if (tid == 0) part[blockIdx.x] = sqrtf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))) * 1.0001f;
+}
+
+// the maximum of store_k4_kernel's parts, by one workgroup of the kernel launched after it
+__device__ __forceinline__ void join_norms(const float *part, int parts, float *norm) {
+    __shared__ float top[4];
+    float most = 0.f;
+    for (int i = threadIdx.x; i < parts; i += 256) most = fmaxf(most, part[i]);
+    for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
+    if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) *norm = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
 }
 
 // One block of values: its scale byte, and the codes. 32 keys share it, so a value that is
@@ -151,10 +168,12 @@ __device__ __forceinline__ u32x4 encode_v(u32x4 (&w)[4], uint32_t &byte) {
 
 // Values [BH][P][128] (bf16): a thread holds four dimensions of 32 keys, a workgroup two tiles.
 __global__ __launch_bounds__(256) void store_v4_kernel(const uint16_t *__restrict__ v, int64_t P, int64_t T,
-                                                       uint8_t *__restrict__ tiles, uint32_t *__restrict__ norm) {
-    const int64_t bh = blockIdx.y, t = (int64_t)blockIdx.x * 2 + (threadIdx.x >> 7);
-    if (norm && blockIdx.x == 0 && bh == 0 && threadIdx.x == 0) *norm = 0u;  // for store_k4_kernel, launched next
-    if (t >= T) return;
+                                                       uint8_t *__restrict__ tiles, const float *__restrict__ part,
+                                                       int parts, float *__restrict__ norm) {
+    __shared__ __attribute__((aligned(16))) uint8_t scales[2][512];
+    const int half = threadIdx.x >> 7;
+    const int64_t bh = blockIdx.y, t = (int64_t)blockIdx.x * 2 + half;
+    if (blockIdx.x == 0 && bh == 0) join_norms(part, parts, norm);
     const int d4 = threadIdx.x & 31, lg = (threadIdx.x >> 5) & 3;
     const int64_t key0 = t * KV4_KEYS + 32 * lg;
     const uint16_t *src = v + (bh * P + key0) * 128 + 4 * d4;
@@ -176,18 +195,21 @@ __global__ __launch_bounds__(256) void store_v4_kernel(const uint16_t *__restric
         uint32_t byte;
         const u32x4 c = encode_v(w, byte);
         const int dim = 4 * d4 + d, j = dim >> 4, lane = 16 * lg + (dim & 15);
-        *(u32x4 *)(tile + chunk_of(KV4_V, j, lane)) = c;
-        tile[scale_at(KV4_VS, j, lane)] = (uint8_t)byte;
+        if (t < T) *(u32x4 *)(tile + chunk_of(KV4_V, j, lane)) = c;
+        scales[half][scale_at(0, j, lane)] = (uint8_t)byte;
     }
+    __syncthreads();
+    const int q = threadIdx.x & 127;
+    if (t < T && q < 32) *(u32x4 *)(tile + KV4_VS + 16 * q) = *(const u32x4 *)(scales[half] + 16 * q);
 }
 
 // Values already transposed, vt [BH][128][ld] (ld a multiple of 8): one block per thread and step.
 __global__ __launch_bounds__(256) void store_vt4_kernel(const uint16_t *__restrict__ vt, int64_t ld, int64_t P,
                                                         int64_t heads, const uint8_t *__restrict__ kvalid,
                                                         int64_t valid_ld, uint8_t *__restrict__ tiles,
-                                                        uint32_t *__restrict__ norm) {
+                                                        const float *__restrict__ part, int parts, float *__restrict__ norm) {
     const int64_t bh = blockIdx.y, T = gridDim.x;
-    if (norm && blockIdx.x == 0 && bh == 0 && threadIdx.x == 0) *norm = 0u;
+    if (blockIdx.x == 0 && bh == 0) join_norms(part, parts, norm);
     const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
     uint8_t *tile = tiles + (bh * T + blockIdx.x) * KV4_TILE;
     const int64_t key0 = (int64_t)blockIdx.x * KV4_KEYS + 32 * lg;
@@ -221,55 +243,51 @@ template <bool VT>
 __global__ __launch_bounds__(256) void load4_kernel(const uint8_t *__restrict__ tiles, int64_t P, int64_t ld,
                                                     uint16_t *__restrict__ k, uint16_t *__restrict__ v) {
     const int64_t bh = blockIdx.y, T = gridDim.x;
-    const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
+    const int tid = threadIdx.x;
     const uint8_t *tile = tiles + (bh * T + blockIdx.x) * KV4_TILE;
     const int64_t first = (int64_t)blockIdx.x * KV4_KEYS;
+    // 16 B of the output per thread and step, 16 threads a row of 256 B: eight dimensions of
+    // a key or, transposed, eight keys of a dimension, one word of codes
     if (blockIdx.z == 0) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int i = (tid >> 6) + 4 * h;
-            const int64_t key = first + kv4_key(i, l16);
-            if (key >= P) continue;
-            const u32x4 c = *(const u32x4 *)(tile + chunk_of(0, i, lane));
+        for (int h = 0; h < 8; h++) {
+            const int at = (tid >> 4) + 16 * h, piece = tid & 15;  // key of the tile
+            const int i = 4 * (at >> 6) + ((at >> 2) & 3), lane = 16 * (piece >> 2) + 4 * ((at >> 4) & 3) + (at & 3);
+            if (first + at >= P) continue;
+            const uint32_t c = *(const uint32_t *)(tile + chunk_of(0, i, lane) + 4 * (piece & 3));
             const uint32_t byte = tile[scale_at(KV4_KS, i, lane)];
-            u32x4 *dst = (u32x4 *)(k + (bh * P + key) * 128 + 32 * lg);
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                dst[e] = byte == 255u ? u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u} : decode8(c[e], scale_of(byte));
+            *(u32x4 *)(k + (bh * P + first + at) * 128 + 8 * piece) =
+                byte == 255u ? u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u} : decode8(c, scale_of(byte));
         }
     } else if constexpr (VT) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int j = (tid >> 6) + 4 * h;
-            const u32x4 c = *(const u32x4 *)(tile + chunk_of(KV4_V, j, lane));
-            const float sc = scale_of(tile[scale_at(KV4_VS, j, lane)]);
-            const int64_t key0 = first + 32 * lg;
-            uint16_t *dst = v + (bh * 128 + 16 * j + l16) * ld + key0;
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (key0 + 8 * e < ld) *(u32x4 *)(dst + 8 * e) = decode8(c[e], sc);  // zeros past P
+        for (int h = 0; h < 8; h++) {
+            const int dim = (tid >> 4) + 16 * h, piece = tid & 15, lane = 16 * (piece >> 2) + (dim & 15);
+            if (first + 8 * piece >= ld) continue;
+            const uint32_t c = *(const uint32_t *)(tile + chunk_of(KV4_V, h, lane) + 4 * (piece & 3));
+            *(u32x4 *)(v + (bh * 128 + dim) * ld + first + 8 * piece) =
+                decode8(c, scale_of(tile[scale_at(KV4_VS, h, lane)]));  // zeros past P
         }
     } else {
-        if (tid >= 128) return;
-        // four dimensions of 32 keys per thread, as store_v4_kernel
-        const int d4 = tid & 31, g = tid >> 5;
-        u32x4 w[4][4];  // [dimension][8 keys each]
+        // four dimensions of eight keys per thread and step: rows of 256 B by 32 threads
 #pragma unroll
-        for (int d = 0; d < 4; d++) {
-            const int dim = 4 * d4 + d, j = dim >> 4, ln = 16 * g + (dim & 15);
-            const u32x4 c = *(const u32x4 *)(tile + chunk_of(KV4_V, j, ln));
-            const float sc = scale_of(tile[scale_at(KV4_VS, j, ln)]);
+        for (int h = 0; h < 2; h++) {
+            const int d4 = tid & 31, oct = (tid >> 5) + 8 * h, g = oct >> 2;
+            u32x4 w[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) w[d][e] = decode8(c[e], sc);
-        }
-        const int64_t key0 = first + 32 * g;
+            for (int d = 0; d < 4; d++) {
+                const int dim = 4 * d4 + d, j = dim >> 4, lane = 16 * g + (dim & 15);
+                w[d] = decode8(*(const uint32_t *)(tile + chunk_of(KV4_V, j, lane) + 4 * (oct & 3)),
+                               scale_of(tile[scale_at(KV4_VS, j, lane)]));
+            }
+            const int64_t key0 = first + 8 * oct;
 #pragma unroll
-        for (int n = 0; n < 32; n++) {
-            if (key0 + n >= P) break;
-            const uint32_t sel = n & 1 ? 0x07060302u : 0x05040100u;
-            const int e = n >> 3, q = (n & 7) >> 1;
-            *(u32x2 *)(v + (bh * P + key0 + n) * 128 + 4 * d4) =
-                u32x2{__builtin_amdgcn_perm(w[1][e][q], w[0][e][q], sel), __builtin_amdgcn_perm(w[3][e][q], w[2][e][q], sel)};
+            for (int n = 0; n < 8; n++) {
+                if (key0 + n >= P) break;
+                const uint32_t sel = n & 1 ? 0x07060302u : 0x05040100u;
+                *(u32x2 *)(v + (bh * P + key0 + n) * 128 + 4 * d4) =
+                    u32x2{__builtin_amdgcn_perm(w[1][n >> 1], w[0][n >> 1], sel), __builtin_amdgcn_perm(w[3][n >> 1], w[2][n >> 1], sel)};
+            }
         }
     }
 }
@@ -279,20 +297,21 @@ __global__ __launch_bounds__(256) void load4_kernel(const uint8_t *__restrict__ 
 int64_t kv4_layer_bytes(int64_t bh, int64_t p) { return bh * ((p + KV4_KEYS - 1) / KV4_KEYS) * KV4_TILE; }
 
 hipError_t launch_store4(const uint16_t *k, const uint16_t *v, int64_t vt_ld, int64_t b, int64_t h, int64_t p,
-                         const uint8_t *kvalid, int64_t valid_ld, uint8_t *tiles, float *norm, hipStream_t stream) {
+                         const uint8_t *kvalid, int64_t valid_ld, uint8_t *tiles, float *norm_part, float *norm,
+                         hipStream_t stream) {
     const int64_t bh = b * h, T = (p + KV4_KEYS - 1) / KV4_KEYS;
     if (bh <= 0 || p <= 0) return hipSuccess;
     if (bh > 65535 || T > (int64_t)1 << 30 || (vt_ld && (vt_ld < p || vt_ld % 8))) return hipErrorInvalidValue;
+    const int parts = (int)std::min<int64_t>(T * bh, QK_NORM_PARTS);
+    store_k4_kernel<<<dim3((unsigned)parts), dim3(256), 0, stream>>>(k, p, h, kvalid, valid_ld, T, T * bh, tiles, norm_part);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
     if (vt_ld)
         store_vt4_kernel<<<dim3((unsigned)T, (unsigned)bh), dim3(256), 0, stream>>>(v, vt_ld, p, h, kvalid, valid_ld, tiles,
-                                                                                   (uint32_t *)norm);
+                                                                                   norm_part, parts, norm);
     else
-        store_v4_kernel<<<dim3((unsigned)((T + 1) / 2), (unsigned)bh), dim3(256), 0, stream>>>(v, p, T, tiles,
-                                                                                              (uint32_t *)norm);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    store_k4_kernel<<<dim3((unsigned)T, (unsigned)bh), dim3(256), 0, stream>>>(k, p, h, kvalid, valid_ld, tiles,
-                                                                              (uint32_t *)norm);
+        store_v4_kernel<<<dim3((unsigned)((T + 1) / 2), (unsigned)bh), dim3(256), 0, stream>>>(v, p, T, tiles, norm_part,
+                                                                                              parts, norm);
     return hipGetLastError();
 }
 

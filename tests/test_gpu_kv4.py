@@ -167,7 +167,7 @@ def assert_near(got, want, a):
     (1, 1, 1, 1, 0), (1, 1, 1, 1, 1), (2, 3, 1, 128, 0), (1, 2, 1, 129, 1), (1, 2, 1, 127, 3), (2, 2, 16, 300, 16),
     (1, 3, 17, 333, 17), (1, 2, 15, 64, 0), (1, 1, 32, 1000, 33), (1, 2, 33, 511, 33), (1, 2, 48, 640, 64),
     (2, 1, 64, 1025, 65), (1, 1, 64, 31, 200), (1, 2, 5, 0, 9), (1, 1, 64, 0, 64), (1, 1, 3, 8191, 0),
-    (3, 5, 7, 77, 250), (1, 1, 1, 40, 2049)])
+    (3, 5, 7, 77, 250), (1, 1, 1, 40, 2049), (2, 2, 65, 140, 65), (1, 3, 300, 333, 129), (1, 1, 1000, 600, 0)])
 def test_attention_over_codes(torch_cuda, qctx, b, h, sq, p, so):
     assert_near(*attn_case(torch_cuda, qctx, b, h, sq, p, so, seed=sq * 1000 + p + so))
 
@@ -179,7 +179,7 @@ def test_attention_over_codes_scales(torch_cuda, qctx, scale, sharp):
 
 
 @pytest.mark.parametrize("fill", [None, float("nan"), float("inf"), -3.0e38])
-@pytest.mark.parametrize("sq,p,so", [(1, 200, 1), (20, 700, 70), (64, 130, 64), (9, 129, 0)])
+@pytest.mark.parametrize("sq,p,so", [(1, 200, 1), (20, 700, 70), (64, 130, 64), (9, 129, 0), (150, 400, 33)])
 def test_attention_over_codes_masked(torch_cuda, qctx, sq, p, so, fill):
     """Padded prompts: the tail of one, scattered keys and whole tiles of another; hidden keys
     may hold anything."""
@@ -192,14 +192,15 @@ def test_attention_over_codes_masked(torch_cuda, qctx, sq, p, so, fill):
     assert_near(*attn_case(torch_cuda, qctx, 3, 2, sq, p, so, seed=p, valid=valid, fill=fill))
 
 
-@pytest.mark.parametrize("sq,so", [(1, 0), (5, 3), (64, 64), (65, 8), (300, 40)])
-def test_a_row_without_a_visible_key_is_nan(torch_cuda, qctx, sq, so):
-    """As on the other caches (the softmax of -inf); the other entries are as without it."""
+@pytest.mark.parametrize("h,sq,so", [(2, 1, 0), (2, 5, 3), (2, 64, 64), (2, 300, 40), (8, 1300, 1300)])
+def test_a_row_without_a_visible_key_is_nan(torch_cuda, qctx, h, sq, so):
+    """As on the other caches (the softmax of -inf); the other entries are as without it. The
+    last case takes the expanded layer."""
     valid = np.ones((2, 140 + so), np.uint8)
     valid[1] = 0
-    got, want, a = attn_case(torch_cuda, qctx, 2, 2, sq, 140, so, seed=so, valid=valid)
+    got, want, a = attn_case(torch_cuda, qctx, 2, h, sq, 140, so, seed=so, valid=valid)
     assert np.isnan(got[1]).all() and np.isnan(want[1]).all()
-    if sq <= 64:
+    if sq < 1000:
         assert_near(got[:1], want[:1], a[:1])
     else:
         kv_close(got[:1], want[:1])
@@ -244,9 +245,10 @@ def two_caches(torch, qctx, b, h, p, seed):
     return kv4, kv16
 
 
-@pytest.mark.parametrize("b,h,sq,p,so,padded", [(1, 2, 65, 40, 65, False), (2, 2, 300, 333, 300, False), (1, 2, 256, 128, 256, True),
-                                                (2, 1, 100, 217, 7, True), (1, 1, 128, 500, 0, False)])
+@pytest.mark.parametrize("b,h,sq,p,so,padded", [(1, 8, 1536, 333, 1536, False), (2, 8, 1200, 128, 1200, True),
+                                                (1, 16, 1100, 217, 1101, True), (1, 8, 2100, 40, 2100, False)])
 def test_many_queries_equal_the_bf16_cache_of_the_same_values(torch_cuda, qctx, b, h, sq, p, so, padded):
+    """Where the layer is expanded the attention is the bf16 cache's, bit for bit."""
     torch = torch_cuda
     caches = two_caches(torch, qctx, b, h, p, seed=sq)
     rng = np.random.default_rng(sq + 1)
@@ -293,21 +295,21 @@ def test_replays_of_a_graph_equal_eager_calls(torch_cuda, qctx):
     """Store, few and many queries captured on a stream of their own, replayed on new inputs
     with the program's own work in between."""
     torch = torch_cuda
-    b, h, p, so = 2, 4, 700, 3
+    b, h, p, so, sq = 2, 8, 700, 1500, 1500
     gen = torch.Generator(device="cuda").manual_seed(1)
 
     def draw(*shape):
         return torch.randn(*shape, device="cuda", generator=gen).to(torch.bfloat16)
 
-    k, v, q, ko, vo = draw(b, h, p, 128), draw(b, h, p, 128), draw(b, h, 80, 128), draw(b, h, so, 128), draw(b, h, 128, so)
-    few, many = torch.empty(b, 3, h * 128, dtype=torch.bfloat16, device="cuda"), torch.empty(b, 80, h * 128, dtype=torch.bfloat16, device="cuda")
+    k, v, q, ko, vo = draw(b, h, p, 128), draw(b, h, p, 128), draw(b, h, sq, 128), draw(b, h, so, 128), draw(b, h, 128, so)
+    few, many = torch.empty(b, 3, h * 128, dtype=torch.bfloat16, device="cuda"), torch.empty(b, sq, h * 128, dtype=torch.bfloat16, device="cuda")
     kv = qctx.kv_create_q4(2, b, h, p)
 
     def step():
         s = stream(torch)
         kv.store(1, k.data_ptr(), v.data_ptr(), s)
         qctx.attention(q.data_ptr(), b, h, 3, kv, 1, ko.data_ptr(), vo.data_ptr(), so, 0.088, few.data_ptr(), s)
-        qctx.attention(q.data_ptr(), b, h, 80, kv, 1, ko.data_ptr(), vo.data_ptr(), so, 0.088, many.data_ptr(), s)
+        qctx.attention(q.data_ptr(), b, h, sq, kv, 1, ko.data_ptr(), vo.data_ptr(), so, 0.088, many.data_ptr(), s)
 
     side = torch.cuda.Stream()
     with torch.cuda.stream(side):
