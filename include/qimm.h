@@ -201,9 +201,9 @@ int64_t qimm_adapters_device_bytes(const qimm_adapters *ad);
  * checks, the same products of W); sums are f32, y is rounded once. Rows of one adapter
  * next to each other are fastest: a tile of rows is multiplied once per adapter in it.
  * Scratch is the context's and grows like qimm_qmatmul's; after a
- * qimm_qmatmul_adapters_reserve with at least this m (same weight, adapters and out_type)
- * the call neither allocates nor synchronizes and can be captured. ids, x and the adapters'
- * choice may change between replays. */
+ * qimm_qmatmul_adapters_reserve with the call's weight, adapters, m and out_type it neither
+ * allocates nor synchronizes and can be captured (as for a captured block forward, no later
+ * call may grow the scratch: reserve every size first). ids and x may change between replays. */
 int qimm_qmatmul_adapters(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapters *ad, const int32_t *ids,
                           const void *x_bf16, int64_t m, int64_t lda, void *y, int out_type, void *stream);
 int qimm_qmatmul_adapters_reserve(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapters *ad, int64_t m, int out_type);

@@ -22,36 +22,45 @@ namespace {
 
 size_t align_up(size_t v) { return (v + 255) & ~(size_t)255; }
 
-// How a product of m rows is taken: each row by itself beside the product's f32 sums (few), as
-// k steps of the product over bf16 rows (steps), or a pass over its f32 sums; and the scratch
-// in the context's growable workspace: t, the first product's shares, the f32 sums of a bf16
-// output; the partial sums of a split product.
+// How a product of m rows is taken: each row by itself beside the product's f32 sums (few); or
+// t of all rows first, then the rows before the product's tail and the tail, each as k steps of
+// the product over bf16 rows (steps) or with a pass over its f32 sums. The pass is for what runs
+// over the codes or split over K: its sums are in memory for the reduction anyway (4096 x 12288
+// Q4_K at 128 / 512 rows 51 / 79 us, 63 / 84 as steps), while 1024 x 12288 x 4096 takes 106 as
+// steps and 121 with it. Offsets into the context's growable workspace: t16 of the steps,
+// t's shares, the f32 sums of a bf16 output; `part`: the split products' own scratch.
 struct Route {
     bool few, steps;
-    qimm::Bf16Plan plan;
+    int64_t head, tiles;  // rows before the tail; their tiles of 256
+    int parts;
     size_t shares, sums, total, part;
 };
-Route route_of(const qimm_weight *w, const qimm_adapters *ad, int64_t m, int out_type) {
+Route route_of(const qimm_weight *w, const qimm_adapters *ad, int64_t m, int64_t lda, int out_type) {
     Route r{};
-    r.few = qimm::lora_few(m);
+    const bool f32 = out_type == QIMM_TYPE_F32;
     const int64_t kt = (ad->max_rank + 63) / 64 * 64;
-    if (r.few) {
-        r.shares = align_up((size_t)(m * ad->max_rank) * 4);
-        r.sums = r.shares;
-    } else {
-        r.shares = align_up((size_t)(m * 2 * kt) * 2);
+    r.few = qimm::lora_few(m);
+    r.parts = f32 ? 3 : 2;
+    r.head = m;
+    r.part = qimm::qgemm_workspace(w->gw, m);
+    qimm::EpiParams ep{};
+    ep.ldo = w->rows;
+    ep.part_ws_bytes = r.part;
+    static float some;  // an address: the plans only test for one
+    if (r.part) ep.part_ws = &some;
+    int64_t pass = m;  // rows with a pass
+    if (!r.few) {
+        r.head = m - qimm::qgemm_route(w->gw, m, lda, qimm::EPI_F32, ep).tail;
+        const qimm::GemmRoute g = qimm::qgemm_route(w->gw, r.head, lda, qimm::EPI_F32, ep);
+        r.steps = g.kernel == qimm::GEMM_BF16_ROWS && g.splits == 1;
+        r.tiles = g.head;
+        if (r.steps) pass = m - r.head;
+        r.shares = r.steps ? align_up((size_t)(m * r.parts * kt) * 2) : 0;
         r.sums = r.shares + align_up(qimm::lora_down_scratch(m, w->cols, ad->max_rank));
-        r.steps = qimm::qgemm_bf16_fits(w->gw);
-    }
-    r.total = r.sums;
-    if (r.steps) {
-        r.plan = qimm::qgemm_bf16_plan(w->gw, m, true);
-        if (r.plan.splits > 1)
-            r.part = qimm::STREAM_COUNTER_BYTES + (size_t)r.plan.splits * (size_t)m * (size_t)w->rows * 4;
     } else {
-        r.part = qimm::qgemm_workspace(w->gw, m);
-        if (out_type != QIMM_TYPE_F32) r.total += (size_t)(m * ad->rows) * 4;
+        r.sums = align_up((size_t)(m * ad->max_rank) * 4);
     }
+    r.total = r.sums + (f32 ? 0 : (size_t)(pass * w->rows) * 4);
     return r;
 }
 
@@ -170,7 +179,8 @@ int qimm_qmatmul_adapters_reserve(qimm_ctx *ctx, const qimm_weight *w, const qim
     if (const int rc = check_pair(ctx, w, ad)) return rc;
     if (m == 0) return QIMM_OK;
     QIMM_HIP(ctx, hipSetDevice(ctx->device));
-    return reserve(ctx, route_of(w, ad, m, out_type));
+    if (const int rc = reserve(ctx, route_of(w, ad, m, w->cols, out_type))) return rc;
+    return reserve(ctx, route_of(w, ad, m, (int64_t)1 << 40, out_type));  // rows too far apart for the bf16 rows' kernel
 }
 
 int qimm_qmatmul_adapters(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapters *ad, const int32_t *ids,
@@ -181,39 +191,45 @@ int qimm_qmatmul_adapters(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapte
     if ((uintptr_t)ids & 3) return set_err(ctx, QIMM_ERR_ARG, "qmatmul with adapters: ids must be 4-byte aligned");
     if (m == 0) return QIMM_OK;
     QIMM_HIP(ctx, hipSetDevice(ctx->device));
-    const Route r = route_of(w, ad, m, out_type);
+    const Route r = route_of(w, ad, m, lda, out_type);
     if (const int rc = reserve(ctx, r)) return rc;
     const hipStream_t s = (hipStream_t)stream;
     const uint16_t *x = (const uint16_t *)x_bf16;
     const bool f32 = out_type == QIMM_TYPE_F32;
     const int64_t K = w->cols, N = w->rows, kt = (ad->max_rank + 63) / 64 * 64;
+    const qimm::AdapterDev *table = ad->table();
     const int n = (int)ad->count;
     char *ws = (char *)ctx->ws;
-    if (r.few)
-        QIMM_HIP(ctx, qimm::launch_lora_few_down(x, lda, m, K, ad->table(), n, ids, (float *)ws, ad->max_rank, s));
-    else
-        QIMM_HIP(ctx, qimm::launch_lora_down(x, lda, m, K, ad->max_rank, ad->table(), n, ids, (float *)(ws + r.shares),
-                                             (uint16_t *)ws, s));
+    uint16_t *t16 = (uint16_t *)ws;
+    float *shares = (float *)(ws + r.shares);
+    const qimm::LoraShares sh = qimm::lora_shares(m, K, ad->max_rank);
     qimm::EpiParams ep{};
-    ep.out = y;
     ep.ldo = N;
     if (r.part) {
         ep.part_ws = (float *)ctx->ws_part;
         ep.part_ws_bytes = ctx->ws_part_bytes;
     }
-    if (r.steps) {
-        const qimm::AdapterSteps st{(const uint16_t *)ws, (int)(kt / 64), ad->table(), n, ids, ad->zeros()};
-        QIMM_HIP(ctx, qimm::launch_qgemm_bf16_adapters(w->gw, x, m, lda, f32 ? qimm::EPI_F32 : qimm::EPI_BF16, ep, r.plan, st, s));
-        return QIMM_OK;
-    }
-    float *sums = f32 ? (float *)y : (float *)(ws + r.sums);
-    ep.out = sums;
-    QIMM_HIP(ctx, qimm::launch_qgemm(w->gw, x, m, lda, qimm::EPI_F32, ep, s));
-    float *y32 = f32 ? sums : nullptr;
     if (r.few)
-        QIMM_HIP(ctx, qimm::launch_lora_few_up((const float *)ws, ad->max_rank, m, N, ad->table(), n, ids, sums, y32, (uint16_t *)y, s));
+        QIMM_HIP(ctx, qimm::launch_lora_few_down(x, lda, m, K, table, n, ids, shares, ad->max_rank, s));
     else
-        QIMM_HIP(ctx, qimm::launch_lora_up((const uint16_t *)ws, kt, m, N, ad->table(), n, ids, sums, y32, (uint16_t *)y, s));
+        QIMM_HIP(ctx, qimm::launch_lora_down(x, lda, m, K, ad->max_rank, table, n, ids, shares, s));
+    int64_t row0 = 0;
+    if (r.steps) {
+        QIMM_HIP(ctx, qimm::launch_lora_split(shares, sh, m, kt, r.parts, table, n, ids, t16, s));
+        const qimm::AdapterSteps st{t16, (int)(kt / 64), (int)(kt / 64) * r.parts, table, n, ids, ad->zeros()};
+        ep.out = y;
+        QIMM_HIP(ctx, qimm::launch_qgemm_bf16_adapters(w->gw, x, r.head, lda, f32 ? qimm::EPI_F32 : qimm::EPI_BF16, ep, r.tiles, st, s));
+        row0 = r.head;
+    }
+    if (row0 == m) return QIMM_OK;
+    float *y32 = f32 ? (float *)y + row0 * N : nullptr, *sums = f32 ? y32 : (float *)(ws + r.sums);
+    uint16_t *y16 = (uint16_t *)y + row0 * N;
+    ep.out = sums;
+    QIMM_HIP(ctx, qimm::launch_qgemm(w->gw, x + row0 * lda, m - row0, lda, qimm::EPI_F32, ep, s));
+    if (r.few)
+        QIMM_HIP(ctx, qimm::launch_lora_few_up(shares, ad->max_rank, m, N, table, n, ids, sums, y32, y16, s));
+    else
+        QIMM_HIP(ctx, qimm::launch_lora_up(shares, sh, m, row0, m - row0, N, table, n, ids + row0, sums, y32, y16, s));
     return QIMM_OK;
 }
 

@@ -289,26 +289,37 @@ hipError_t launch_lora_few_down(const uint16_t *x, int64_t lda, int64_t m, int64
                                 const int32_t *ids, float *t, int64_t ldt, hipStream_t stream);
 hipError_t launch_lora_few_up(const float *t, int64_t ldt, int64_t m, int64_t n, const AdapterDev *ad, int count,
                               const int32_t *ids, const float *base, float *y32, uint16_t *y16, hipStream_t stream);
-// Many rows: t16[row] = t as two bf16 rows of kt = the largest rank rounded up to 64, the bf16
-// rounding and then what it leaves, zeros past the adapter's rank; rows without an adapter are
-// not written. scratch: lora_down_scratch bytes.
+// Many rows: partial sums of t in scratch, lora_down_scratch bytes: [shares][m][ldp] f32 over
+// shares of K, without the scale; rows without an adapter are not written.
+struct LoraShares {
+    int shares;
+    int64_t ldp;  // the largest rank rounded up to what the kernel takes at a time
+};
+LoraShares lora_shares(int64_t m, int64_t k, int64_t max_rank);
 size_t lora_down_scratch(int64_t m, int64_t k, int64_t max_rank);
 hipError_t launch_lora_down(const uint16_t *x, int64_t lda, int64_t m, int64_t k, int64_t max_rank, const AdapterDev *ad, int count,
-                            const int32_t *ids, float *scratch, uint16_t *t16, hipStream_t stream);
-hipError_t launch_lora_up(const uint16_t *t16, int64_t kt, int64_t m, int64_t n, const AdapterDev *ad, int count,
-                          const int32_t *ids, const float *base, float *y32, uint16_t *y16, hipStream_t stream);
+                            const int32_t *ids, float *part, hipStream_t stream);
+// y = base + t B^T of rows row0 .. row0 + rows (of part's m rows; ids, base and y are the rows'
+// own), to y32 (f32, may be base) when set, else bf16 to y16
+hipError_t launch_lora_up(const float *part, LoraShares sh, int64_t m, int64_t row0, int64_t rows, int64_t n, const AdapterDev *ad,
+                          int count, const int32_t *ids, const float *base, float *y32, uint16_t *y16, hipStream_t stream);
+// t16[row][parts][kt] (kt the largest rank rounded up to 64) = t as a sum of bf16 numbers, each
+// the rounding of what the ones before leave: two parts keep 2^-16 of t, three 2^-24; zeros past
+// the adapter's rank; rows without one are not written.
+hipError_t launch_lora_split(const float *part, LoraShares sh, int64_t m, int64_t kt, int parts, const AdapterDev *ad, int count,
+                             const int32_t *ids, uint16_t *t16, hipStream_t stream);
 // The product over bf16 rows with the adapters' second product as further k steps
-// (launch_qgemm_bf16's plain outputs): y = A W^T + t B^T.
+// (launch_qgemm_bf16's plain outputs, `head` tiles of 256 tokens): y = A W^T + t B^T.
 struct AdapterSteps {
     const uint16_t *t;     // t16
-    int kb;                // kt / 64
+    int kb, steps;         // kt / 64; parts of them
     const AdapterDev *ad;
     int count;
     const int32_t *ids;    // [m]
     const uint16_t *zero;  // 128 B of zeros
 };
 hipError_t launch_qgemm_bf16_adapters(const GemmWeight &w, const uint16_t *a, int64_t m, int64_t lda, int epi,
-                                      const EpiParams &ep, const Bf16Plan &plan, const AdapterSteps &x, hipStream_t stream);
+                                      const EpiParams &ep, int64_t head, const AdapterSteps &x, hipStream_t stream);
 
 // ---- the prefix cache held in 4 bits (kv4.hip, attn4.hip; the layout is in kv4.h) ----
 // Bytes of one layer: b * h heads of p keys.

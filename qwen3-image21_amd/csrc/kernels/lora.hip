@@ -3,15 +3,16 @@
 //
 // Two products: t = scale x A^T (ranks wide, K deep), then t B^T (N wide, ranks deep)
 // added to the projection's f32 sums before the one rounding of y. Where the matrix pipe
-// takes the second product t is the sum of two bf16 numbers, hi = bf16(t) and lo = bf16(t -
-// hi): 2^-16 of t at most, so that f32 outputs keep the precision of their sums.
+// takes the second product t is the sum of bf16 numbers, each the rounding of what the ones
+// before leave: two (2^-16 of t) for bf16 outputs, three (2^-24) for f32 ones, which keep the
+// precision of their sums (with two 1.1e-6 instead of 2e-7 of 64 bits at 514 x 4096 x 4096).
 //
 // Rows of any adapters may lie next to each other: a tile of rows is multiplied once per
 // adapter among its ids; of t the rows of other adapters are not written, in the second
 // product they enter as zeros (adapters hold numbers only). Few rows are taken each by
 // itself, so that many adapters are not multiplied one after the other. The second product
-// of many rows runs as further k steps of the projection where that is over bf16 rows
-// (qgemm_bf16.hip), else as a pass over its f32 sums (lora_up_kernel).
+// of many rows runs as further k steps of the projection where that is over bf16 rows and not
+// split over K (qgemm_bf16.hip), else as a pass over its f32 sums (lora_up_kernel).
 #include <algorithm>
 #include <type_traits>
 
@@ -127,8 +128,30 @@ __global__ __launch_bounds__(256, 2) void lora_down_kernel(const uint16_t *__res
     }
 }
 
-// The shares' sums times the scale as two bf16 rows, t16[row][hi 0 .. ldp | lo 0 .. ldp), zeros
-// past the rank; four ranks per thread. Rows without an adapter are not written.
+// four ranks' sums over the shares
+__device__ __forceinline__ f32x4 add_shares(const float *p, int shares, int64_t stride) {
+    f32x4 s{};
+    int i = 0;
+    for (; i + 4 <= shares; i += 4, p += 4 * stride) {  // four loads in flight
+        f32x4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) v[u] = *(const f32x4 *)(p + u * stride);
+        s += (v[0] + v[1]) + (v[2] + v[3]);
+    }
+    for (; i < shares; i++, p += stride) s += *(const f32x4 *)p;
+    return s;
+}
+// the bf16 rounding of v (two in a word), and what it leaves
+__device__ __forceinline__ uint32_t take_bf16x2(float &a, float &b) {
+    const uint32_t w = pack_bf16x2(a, b);
+    a -= __uint_as_float(w << 16);
+    b -= __uint_as_float(w & 0xffff0000u);
+    return w;
+}
+
+// The shares' sums times the scale as PARTS bf16 rows of kt, zeros past the rank; four ranks per
+// thread. Rows without an adapter are not written.
+template <int PARTS>
 __global__ __launch_bounds__(256) void lora_split_kernel(const float *__restrict__ part, int shares, int64_t m, int64_t ldp,
                                                         const AdapterDev *__restrict__ ad, int count,
                                                         const int32_t *__restrict__ ids, uint16_t *__restrict__ t16, int64_t kt) {
@@ -139,38 +162,32 @@ __global__ __launch_bounds__(256) void lora_split_kernel(const float *__restrict
     const int rank = ad[id].rank;
     const float scale = ad[id].scale;
     f32x4 s{};
-    if (r < rank)  // written by every share: r < 16 RT ceil(rank / (16 RT))
-    {
-        int p = 0;
-        for (; p + 4 <= shares; p += 4) {  // four loads in flight
-            f32x4 v[4];
+    if (r < rank) s = add_shares(part + row * ldp + r, shares, m * ldp);  // written up to the rank's tile of 16
 #pragma unroll
-            for (int u = 0; u < 4; u++) v[u] = *(const f32x4 *)(part + ((int64_t)(p + u) * m + row) * ldp + r);
-            s += (v[0] + v[1]) + (v[2] + v[3]);
-        }
-        for (; p < shares; p++) s += *(const f32x4 *)(part + ((int64_t)p * m + row) * ldp + r);
-    }
-    float hi[4], lo[4];
+    for (int e = 0; e < 4; e++) s[e] = r + e < rank ? s[e] * scale : 0.f;
+    uint16_t *dst = t16 + row * PARTS * kt + r;
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-        const float v = r + e < rank ? s[e] * scale : 0.f;
-        hi[e] = __uint_as_float(pack_bf16x2(v, 0.f) << 16);
-        lo[e] = v - hi[e];
+    for (int p = 0; p < PARTS; p++) {
+        float a = s[0], b = s[1], c = s[2], d = s[3];
+        *(u32x2 *)(dst + p * kt) = u32x2{take_bf16x2(a, b), take_bf16x2(c, d)};
+        s = f32x4{a, b, c, d};
     }
-    *(u32x2 *)(t16 + row * 2 * kt + r) = u32x2{pack_bf16x2(hi[0], hi[1]), pack_bf16x2(hi[2], hi[3])};
-    *(u32x2 *)(t16 + row * 2 * kt + kt + r) = u32x2{pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3])};
 }
 
-// y = base + t B^T for 16 rows x 256 columns, 64 columns per wave. A = B's rows, B = t's.
-__global__ __launch_bounds__(256) void lora_up_kernel(const uint16_t *__restrict__ t16, int64_t kt, int64_t m, int64_t N,
-                                                     const AdapterDev *__restrict__ ad, int count,
+// y = base + t B^T for 16 rows x 256 columns, 64 columns per wave; t from the shares' sums,
+// in PARTS bf16 operands. A = B's rows, B = t's.
+template <int PARTS>
+__global__ __launch_bounds__(256) void lora_up_kernel(const float *__restrict__ part, int shares, int64_t m, int64_t ldp,
+                                                     int64_t rows, int64_t N, const AdapterDev *__restrict__ ad, int count,
                                                      const int32_t *__restrict__ ids, const float *base,
                                                      float *y32, uint16_t *y16) {
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
     const int64_t row = (int64_t)blockIdx.y * 16 + l16, n0 = (int64_t)blockIdx.x * 256 + 64 * wave;
     if (n0 >= N) return;  // N is a multiple of 128
-    const int id = row_id(ids, row, m, count);
-    f32x4 acc[4] = {};
+    const int id = row_id(ids, row, rows, count);
+    f32x4 acc[4] = {}, base4[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) base4[i] = *(const f32x4 *)(base + min(row, rows - 1) * N + n0 + 16 * i + 4 * lg);
     uint64_t todo = __ballot(id >= 0) & 0xffffu;
     while (todo) {
         const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
@@ -178,25 +195,39 @@ __global__ __launch_bounds__(256) void lora_up_kernel(const uint16_t *__restrict
         const AdapterDev d = ad[a];
         for (int r0 = 0; r0 < d.rank; r0 += 32) {
             const int r = r0 + 8 * lg;
-            bf16x8 hi = {}, lo = {};
-            if (id == a) {
-                hi = *(const bf16x8 *)(t16 + row * 2 * kt + r);
-                lo = *(const bf16x8 *)(t16 + row * 2 * kt + kt + r);
+            f32x4 u{}, v{};
+            if (id == a && r < d.rank) {
+                u = add_shares(part + row * ldp + r, shares, m * ldp);
+                if (r + 4 < d.rank) v = add_shares(part + row * ldp + r + 4, shares, m * ldp);
             }
 #pragma unroll
+            for (int e = 0; e < 4; e++) {
+                u[e] = r + e < d.rank ? u[e] * d.scale : 0.f;
+                v[e] = r + 4 + e < d.rank ? v[e] * d.scale : 0.f;
+            }
+            bf16x8 b[4];
+#pragma unroll
             for (int i = 0; i < 4; i++) {
-                bf16x8 b = {};
-                if (r < d.ldb) b = *(const bf16x8 *)(d.b + (n0 + 16 * i + l16) * d.ldb + r);
-                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, hi, acc[i], 0, 0, 0);
-                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, lo, acc[i], 0, 0, 0);
+                b[i] = bf16x8{};
+                if (r < d.ldb) b[i] = *(const bf16x8 *)(d.b + (n0 + 16 * i + l16) * d.ldb + r);
+            }
+#pragma unroll
+            for (int p = 0; p < PARTS; p++) {
+                float t[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
+                const u32x4 w = u32x4{take_bf16x2(t[0], t[1]), take_bf16x2(t[2], t[3]), take_bf16x2(t[4], t[5]), take_bf16x2(t[6], t[7])};
+                u = f32x4{t[0], t[1], t[2], t[3]};
+                v = f32x4{t[4], t[5], t[6], t[7]};
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[i], __builtin_bit_cast(bf16x8, w), acc[i], 0, 0, 0);
             }
         }
     }
-    if (row >= m) return;
+    if (row >= rows) return;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int64_t at = row * N + n0 + 16 * i + 4 * lg;
-        const f32x4 s = *(const f32x4 *)(base + at) + acc[i];
+        const f32x4 s = base4[i] + acc[i];
         if (y32)
             *(f32x4 *)(y32 + at) = s;
         else
@@ -300,38 +331,58 @@ int down_shares(int64_t m, int64_t k, int64_t max_rank) {
 }
 }  // namespace
 
-size_t lora_down_scratch(int64_t m, int64_t k, int64_t max_rank) {
+LoraShares lora_shares(int64_t m, int64_t k, int64_t max_rank) {
     const int64_t rt = rank_tile(max_rank);
-    return (size_t)(down_shares(m, k, max_rank) * m * ((max_rank + rt - 1) / rt * rt)) * 4;
+    return {down_shares(m, k, max_rank), (max_rank + rt - 1) / rt * rt};
+}
+
+size_t lora_down_scratch(int64_t m, int64_t k, int64_t max_rank) {
+    const LoraShares s = lora_shares(m, k, max_rank);
+    return (size_t)(s.shares * m * s.ldp) * 4;
 }
 
 hipError_t launch_lora_down(const uint16_t *x, int64_t lda, int64_t m, int64_t k, int64_t max_rank, const AdapterDev *ad, int count,
-                            const int32_t *ids, float *scratch, uint16_t *t16, hipStream_t stream) {
+                            const int32_t *ids, float *part, hipStream_t stream) {
     if (m <= 0) return hipSuccess;
-    const int64_t kt = (max_rank + 63) / 64 * 64, rt = rank_tile(max_rank), groups = (max_rank + rt - 1) / rt, ldp = groups * rt;
-    const int shares = down_shares(m, k, max_rank);
-    const dim3 grid((unsigned)((m + 127) / 128), (unsigned)shares, (unsigned)groups);
+    const int64_t rt = rank_tile(max_rank);
+    const LoraShares s = lora_shares(m, k, max_rank);
+    const dim3 grid((unsigned)((m + 127) / 128), (unsigned)s.shares, (unsigned)(s.ldp / rt));
     if (rt == 16)
-        lora_down_kernel<1><<<grid, dim3(256), 0, stream>>>(x, lda, m, k, ad, count, ids, scratch, ldp);
+        lora_down_kernel<1><<<grid, dim3(256), 0, stream>>>(x, lda, m, k, ad, count, ids, part, s.ldp);
     else if (rt == 32)
-        lora_down_kernel<2><<<grid, dim3(256), 0, stream>>>(x, lda, m, k, ad, count, ids, scratch, ldp);
+        lora_down_kernel<2><<<grid, dim3(256), 0, stream>>>(x, lda, m, k, ad, count, ids, part, s.ldp);
     else
-        lora_down_kernel<4><<<grid, dim3(256), 0, stream>>>(x, lda, m, k, ad, count, ids, scratch, ldp);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    lora_split_kernel<<<dim3((unsigned)((m * (kt / 4) + 255) / 256)), dim3(256), 0, stream>>>(scratch, shares, m, ldp, ad, count, ids, t16, kt);
+        lora_down_kernel<4><<<grid, dim3(256), 0, stream>>>(x, lda, m, k, ad, count, ids, part, s.ldp);
     return hipGetLastError();
 }
 
-hipError_t launch_lora_up(const uint16_t *t16, int64_t kt, int64_t m, int64_t n, const AdapterDev *ad, int count,
-                          const int32_t *ids, const float *base, float *y32, uint16_t *y16, hipStream_t stream) {
+hipError_t launch_lora_split(const float *part, LoraShares sh, int64_t m, int64_t kt, int parts, const AdapterDev *ad, int count,
+                             const int32_t *ids, uint16_t *t16, hipStream_t stream) {
+    if (m <= 0) return hipSuccess;
+    const dim3 grid((unsigned)((m * (kt / 4) + 255) / 256));
+    if (parts == 2)
+        lora_split_kernel<2><<<grid, dim3(256), 0, stream>>>(part, sh.shares, m, sh.ldp, ad, count, ids, t16, kt);
+    else if (parts == 3)
+        lora_split_kernel<3><<<grid, dim3(256), 0, stream>>>(part, sh.shares, m, sh.ldp, ad, count, ids, t16, kt);
+    else
+        return hipErrorInvalidValue;
+    return hipGetLastError();
+}
+
+hipError_t launch_lora_up(const float *part, LoraShares sh, int64_t m, int64_t row0, int64_t rows, int64_t n, const AdapterDev *ad,
+                          int count, const int32_t *ids, const float *base, float *y32, uint16_t *y16, hipStream_t stream) {
     if (n % 128) return hipErrorInvalidValue;
     constexpr int64_t MOST = 16 * 65535;  // rows of one grid
-    for (int64_t r = 0; r < m; r += MOST) {
-        const int64_t rows = std::min(m - r, MOST);
-        lora_up_kernel<<<dim3((unsigned)((n + 255) / 256), (unsigned)((rows + 15) / 16)), dim3(256), 0, stream>>>(
-            t16 + r * 2 * kt, kt, rows, n, ad, count, ids + r, base + r * n, y32 ? y32 + r * n : nullptr,
-            y16 ? y16 + r * n : nullptr);
+    for (int64_t r = 0; r < rows; r += MOST) {
+        const int64_t some = std::min(rows - r, MOST);
+        const dim3 grid((unsigned)((n + 255) / 256), (unsigned)((some + 15) / 16));
+        const float *p = part + (row0 + r) * sh.ldp;
+        if (y32)
+            lora_up_kernel<3><<<grid, dim3(256), 0, stream>>>(p, sh.shares, m, sh.ldp, some, n, ad, count, ids + r, base + r * n,
+                                                             y32 + r * n, nullptr);
+        else
+            lora_up_kernel<2><<<grid, dim3(256), 0, stream>>>(p, sh.shares, m, sh.ldp, some, n, ad, count, ids + r, base + r * n,
+                                                             nullptr, y16 + r * n);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
     return hipSuccess;

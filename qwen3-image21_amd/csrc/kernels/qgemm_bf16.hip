@@ -83,12 +83,12 @@ struct Shape {
 // with SMALL, tiles of half as many.
 //
 // AD: the rows' low-rank adapters as further k steps, so that their product is summed in
-// the same accumulators and costs neither a pass over the outputs nor its rounding. For
-// each adapter among the tile's ids (in ascending order, the list in LDS) 2 kb steps: the
-// token operand is x.t's row, hi part and then lo part, a zero row for tokens of other
-// adapters; the weight operand the adapter's B rows, zeros past the rank. Two steps of 64
-// for 4096 (rank up to 64): 3% of the products, against 134 MB read and written by a pass
-// over 4096 x 4096 outputs.
+// the same accumulators and costs no pass over the outputs. For each adapter among the
+// tile's ids (in ascending order, the list in LDS) x.steps of them: the token operand is
+// x.t's row, the parts of t one after the other, a zero row for tokens of other adapters;
+// the weight operand the adapter's B rows, zeros past the rank. Measured, with one adapter of
+// rank 64 / without: 4096 tokens x 4096 x 12288 295 / 287 us; 16384 x 12288 x 4096 with three of
+// rank 32 1253 / 1226 (and 377 for the pass).
 template <int EPI, bool SMALL, bool AD>
 __global__ __launch_bounds__(64 * NWAVE, 1) void qgemm_bf16_kernel(const uint16_t *__restrict__ A, int64_t M, int64_t lda,
                                                                  const uint16_t *__restrict__ W, int64_t N, int64_t K,
@@ -104,16 +104,11 @@ __global__ __launch_bounds__(64 * NWAVE, 1) void qgemm_bf16_kernel(const uint16_
     // out [share][M][ldo]
     int KT = (int)(K / BK);
     int64_t k_first = 0;
-    [[maybe_unused]] bool last_share = true;  // whose products the adapters' steps join
     if constexpr (EPI == EPI_F32) {
-        // with adapters the last share has their steps too (one adapter's counted; the loads
-        // ahead of the list need two steps of K)
-        const int sh = blockIdx.y, n = gridDim.y, all = AD && n > 1 ? KT + 2 * x.kb : KT;
-        const int k0 = AD ? min(all * sh / n, KT - 2) : all * sh / n, k1 = AD && sh < n - 1 ? min(all * (sh + 1) / n, KT - 2) : all * (sh + 1) / n;
+        const int sh = blockIdx.y, n = gridDim.y, k0 = KT * sh / n;
         k_first = (int64_t)k0 * BK;
-        KT = (AD && sh == n - 1 ? KT : k1) - k0;
+        KT = KT * (sh + 1) / n - k0;
         ep.out = (float *)ep.out + (int64_t)sh * M * ep.ldo;
-        last_share = sh == n - 1;
     }
     [[maybe_unused]] const int KB = KT;  // steps over K itself
 
@@ -164,7 +159,7 @@ __global__ __launch_bounds__(64 * NWAVE, 1) void qgemm_bf16_kernel(const uint16_
             wsrc[i] = (uint32_t)r * (uint32_t)(2 * K) + 16 * ((lane & 7) ^ swz_key(r));
         }
         [[maybe_unused]] int tid_of[NTP][TI];  // AD: the adapters of the lane's rows
-        [[maybe_unused]] int slot_at = -1, ad_at = -1, ldb_at = 0;
+        [[maybe_unused]] int slots = 0, slot_at = -1, ad_at = -1, ldb_at = 0;
         [[maybe_unused]] const uint16_t *b_at = nullptr;
         [[maybe_unused]] int mine[BM / 64];  // AD: the ids of rows lane, lane + 64, ..
         if constexpr (AD) {
@@ -192,46 +187,51 @@ __global__ __launch_bounds__(64 * NWAVE, 1) void qgemm_bf16_kernel(const uint16_
         // above the last one, until none is left); the first one's B is looked up here, ahead of its steps
         auto list_adapters = [&]() __attribute__((always_inline)) {
             if constexpr (AD) {
-                int n = 0;
 #pragma unroll
                 for (int i = 0; i < BM / 64; i++)
                     if ((uint32_t)mine[i] >= (uint32_t)x.count) mine[i] = 0x7fffffff;
-                if (last_share)
-                    for (int at = -1;; n++) {
-                        int next = 0x7fffffff;
+                for (int at = -1;; slots++) {
+                    int next = 0x7fffffff;
 #pragma unroll
-                        for (int i = 0; i < BM / 64; i++) next = min(next, mine[i] > at ? mine[i] : 0x7fffffff);
-                        for (int o = 32; o > 0; o >>= 1) next = min(next, __shfl_xor(next, o));
-                        at = __builtin_amdgcn_readfirstlane(next);
-                        if (at == 0x7fffffff) break;
-                        if (n == 0) {
-                            slot_at = 0;
-                            take(at);
-                        }
-                        if (wave == 0 && lane == 0) list[n] = at;
+                    for (int i = 0; i < BM / 64; i++) next = min(next, mine[i] > at ? mine[i] : 0x7fffffff);
+                    for (int o = 32; o > 0; o >>= 1) next = min(next, __shfl_xor(next, o));
+                    at = __builtin_amdgcn_readfirstlane(next);
+                    if (at == 0x7fffffff) break;
+                    if (slots == 0) {
+                        slot_at = 0;
+                        take(at);
                     }
-                KT = KB + n * 2 * x.kb;
+                    if (wave == 0 && lane == 0) list[slots] = at;
+                }
+                KT = KB + slots * x.steps;
+                if (TT == 4) KT += KT & 1;  // steps come in pairs there: one of zeros
 #pragma unroll
                 for (int i = 0; i < TI; i++)
 #pragma unroll
-                    for (int h = 0; h < NTP; h++) asm volatile("" : "+v"(tid_of[h][i]));  // arrived
+                    for (int h = 0; h < NTP; h++) {
+                        asm volatile("" : "+v"(tid_of[h][i]));  // arrived
+                        if ((uint32_t)tid_of[h][i] >= (uint32_t)x.count) tid_of[h][i] = -1;
+                    }
                 __builtin_amdgcn_s_waitcnt(WAIT_LGKM0);  // the list, before the barrier that follows
             }
         };
         // AD: the adapter of step e past K, kept until another one's step comes; its B
         [[maybe_unused]] auto adapter_of = [&](int e) __attribute__((always_inline)) -> int {
-            const int slot = e / (2 * x.kb);
+            const int slot = e / x.steps;
             if (slot != slot_at) {
                 slot_at = slot;
-                take(__builtin_amdgcn_readfirstlane(list[slot]));
+                if (slot < slots)
+                    take(__builtin_amdgcn_readfirstlane(list[slot]));
+                else
+                    ad_at = -2;  // no row's
             }
-            return e - slot * 2 * x.kb;
+            return slot < slots ? e - slot * x.steps : 0;
         };
         auto dma_t = [&](int s, int h, int kt) __attribute__((always_inline)) {
             kt = min(kt, KT - 1);
             if constexpr (AD)
                 if (kt >= KB) {
-                    const int rem = adapter_of(kt - KB), row = 128 * x.kb;  // elements of a t row
+                    const int rem = adapter_of(kt - KB), row = 64 * x.steps;  // elements of a t row
 #pragma unroll
                     for (int i = 0; i < TI; i++) {
                         const int q = TI * wave + i, r = q / (RT / 8) * 16 * TT + q % (RT / 8) * 8 + h * RT;
@@ -826,18 +826,12 @@ hipError_t launch_qgemm_bf16(const GemmWeight &w, const uint16_t *a, int64_t m, 
 }
 
 hipError_t launch_qgemm_bf16_adapters(const GemmWeight &w, const uint16_t *a, int64_t m, int64_t lda, int epi,
-                                      const EpiParams &ep, const Bf16Plan &plan, const AdapterSteps &x, hipStream_t stream) {
-    if (!qgemm_bf16_fits(w) || lda > ((int64_t)1 << 22) || (epi != EPI_F32 && epi != EPI_BF16)) return hipErrorInvalidValue;
-    if (plan.splits > 1) {
-        float *part = (float *)((char *)ep.part_ws + STREAM_COUNTER_BYTES);
-        EpiParams pe{};
-        pe.out = part;
-        pe.ldo = w.n;
-        const hipError_t e = launch_one<EPI_F32, true>(w, a, m, lda, pe, 0, plan.splits, stream, x);
-        return e == hipSuccess ? launch_split_epilogue(part, plan.splits, m, w.n, epi, ep, stream) : e;
-    }
-    return epi == EPI_F32 ? launch_one<EPI_F32, true>(w, a, m, lda, ep, plan.head, 1, stream, x)
-                          : launch_one<EPI_BF16, true>(w, a, m, lda, ep, plan.head, 1, stream, x);
+                                      const EpiParams &ep, int64_t head, const AdapterSteps &x, hipStream_t stream) {
+    if (!qgemm_bf16_fits(w) || lda > ((int64_t)1 << 22) || (epi != EPI_F32 && epi != EPI_BF16) || head < 0 ||
+        x.kb < 1 || x.steps % x.kb)
+        return hipErrorInvalidValue;
+    return epi == EPI_F32 ? launch_one<EPI_F32, true>(w, a, m, lda, ep, head, 1, stream, x)
+                          : launch_one<EPI_BF16, true>(w, a, m, lda, ep, head, 1, stream, x);
 }
 
 }  // namespace qimm
