@@ -322,12 +322,13 @@ hipError_t launch_lora_few_up(const float *t, int64_t ldt, int64_t m, int64_t n,
 }
 
 // Ranks per workgroup: 16, 32 or 64 at a time; shares of K: as many as give every CU two
-// workgroups, each of at least 4 steps of 64.
+// workgroups, each of at least 4 steps of 64, and at most 16 (the second product adds them:
+// 48 shares of 12288 at 1024 rows took it 29 us).
 namespace {
 int rank_tile(int64_t max_rank) { return max_rank <= 16 ? 16 : max_rank <= 32 ? 32 : 64; }
 int down_shares(int64_t m, int64_t k, int64_t max_rank) {
     const int64_t rt = rank_tile(max_rank), wgs = (m + 127) / 128 * ((max_rank + rt - 1) / rt);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(2 * std::max(device_cu_count(), 1) / wgs, k / 256));
+    return (int)std::max<int64_t>(1, std::min<int64_t>({2 * std::max(device_cu_count(), 1) / wgs, k / 256, 16}));
 }
 }  // namespace
 
