@@ -90,38 +90,6 @@ __global__ __launch_bounds__(256, 2) void attn4_kernel(const Attn4 a) {
     const int64_t first = items * share / a.shares, last = items * (share + 1) / a.shares;
     const uint8_t *tiles = a.tiles + bh * a.T * KV4_TILE;
 
-    // ---- queries: lane (l16, lg) holds dimensions 16 lg .. + 15 and 64 + 16 lg .. + 15 of query
-    // l16, scaled by a power of two so that the row's largest lies in [128, 256) ----
-    i32x8 qhi, qlo;
-    int qsc;  // scale bytes: hi, lo
-    {
-        const int64_t qi = min(q0 + l16, a.Sq - 1);
-        const u32x4 *src = (const u32x4 *)(a.q + (bh * a.Sq + qi) * 128 + 16 * lg);
-        u32x4 w[4];
-        uint32_t mag = 0;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            w[e] = src[8 * (e >> 1) + (e & 1)];
-#pragma unroll
-            for (int x = 0; x < 4; x++) mag = max(mag, max(w[e][x] & 0x7fffu, (w[e][x] >> 16) & 0x7fffu));
-        }
-        mag = max(mag, (uint32_t)__shfl_xor((int)mag, 16));
-        mag = max(mag, (uint32_t)__shfl_xor((int)mag, 32));
-        const int ex = (int)(mag >> 7);                            // biased exponent of the row's largest
-        const int by = ex == 255 ? 255 : max(ex - 7, 6);           // 2^(ex - 134), biased; no number: NaN
-        const float up = __uint_as_float((uint32_t)(254 - min(by, 253)) << 23);
-        qsc = by | (by == 255 ? 255 : by - 5) << 8;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const uint32_t x = w[e >> 1][2 * (e & 1)] ^ a.flip, y = w[e >> 1][2 * (e & 1) + 1] ^ a.flip;
-            int hi, lo;
-            split4(__uint_as_float(x << 16) * up, __uint_as_float(x & 0xffff0000u) * up, __uint_as_float(y << 16) * up,
-                   __uint_as_float(y & 0xffff0000u) * up, hi, lo);
-            qhi[e] = hi;
-            qlo[e] = lo;
-        }
-    }
-
     f32x4 o[8] = {};  // [d tile]: dimensions 16 j + 4 lg + r of query l16
     float m = -INFINITY, l = 0.f;
 
@@ -209,6 +177,39 @@ __global__ __launch_bounds__(256, 2) void attn4_kernel(const Attn4 a) {
             load_v(it);
         }
     }
+
+    // ---- queries: lane (l16, lg) holds dimensions 16 lg .. + 15 and 64 + 16 lg .. + 15 of query
+    // l16, scaled by a power of two so that the row's largest lies in [128, 256) ----
+    i32x8 qhi, qlo;
+    int qsc;  // scale bytes: hi, lo
+    {
+        const int64_t qi = min(q0 + l16, a.Sq - 1);
+        const u32x4 *src = (const u32x4 *)(a.q + (bh * a.Sq + qi) * 128 + 16 * lg);
+        u32x4 w[4];
+        uint32_t mag = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            w[e] = src[8 * (e >> 1) + (e & 1)];
+#pragma unroll
+            for (int x = 0; x < 4; x++) mag = max(mag, max(w[e][x] & 0x7fffu, (w[e][x] >> 16) & 0x7fffu));
+        }
+        mag = max(mag, (uint32_t)__shfl_xor((int)mag, 16));
+        mag = max(mag, (uint32_t)__shfl_xor((int)mag, 32));
+        const int ex = (int)(mag >> 7);                            // biased exponent of the row's largest
+        const int by = ex == 255 ? 255 : max(ex - 7, 6);           // 2^(ex - 134), biased; no number: NaN
+        const float up = __uint_as_float((uint32_t)(254 - min(by, 253)) << 23);
+        qsc = by | (by == 255 ? 255 : by - 5) << 8;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const uint32_t x = w[e >> 1][2 * (e & 1)] ^ a.flip, y = w[e >> 1][2 * (e & 1) + 1] ^ a.flip;
+            int hi, lo;
+            split4(__uint_as_float(x << 16) * up, __uint_as_float(x & 0xffff0000u) * up, __uint_as_float(y << 16) * up,
+                   __uint_as_float(y & 0xffff0000u) * up, hi, lo);
+            qhi[e] = hi;
+            qlo[e] = lo;
+        }
+    }
+
     for (; it < end; it += 4) {
         const int64_t next = it + 4;
         const Bytes ny = next < end ? bytes_of(next) : Bytes{0, 0};
@@ -260,53 +261,74 @@ __global__ __launch_bounds__(256, 2) void attn4_kernel(const Attn4 a) {
         const uint16_t *vb = a.vt_own + bh * 128 * a.So + key0;
         const bool some = ok != ~0ull;
         const uint32_t seen = (uint32_t)((ok >> (8 * lg)) & 0xffu) | (uint32_t)((ok >> (32 + 8 * lg)) & 0xffu) << 8;
-        const bool rows16 = (a.So & 7) == 0;
-        {
-            const int64_t qi = min(q0 + l16, a.Sq - 1);
-            const uint16_t *qp = a.q + (bh * a.Sq + qi) * 128 + 8 * lg;
-            bf16x8 qf[4];
+        // the loads of the keys and half of the values together, then the other half
+        bf16x8 qf[4], kq[2][2][4];
+        u32x4 vq[2][8];
+        const uint16_t *qp = a.q + (bh * a.Sq + min(q0 + l16, a.Sq - 1)) * 128 + 8 * lg;
 #pragma unroll
-            for (int e = 0; e < 4; e++) qf[e] = __builtin_bit_cast(bf16x8, *(const u32x4 *)(qp + 32 * e) ^ a.flip);
-            float s[16];
+        for (int e = 0; e < 4; e++) qf[e] = __builtin_bit_cast(bf16x8, *(const u32x4 *)(qp + 32 * e) ^ a.flip);
 #pragma unroll
-            for (int g = 0; g < 2; g++)
+        for (int g = 0; g < 2; g++)
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const int key = min(32 * g + 8 * (l16 >> 2) + 4 * i + (l16 & 3), have - 1);
-                    const uint16_t *kp = kb + (int64_t)key * 128 + 8 * lg;
-                    f32x4 acc{0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < 2; i++) {
+                const uint16_t *kp = kb + (int64_t)min(32 * g + 8 * (l16 >> 2) + 4 * i + (l16 & 3), have - 1) * 128 + 8 * lg;
+#pragma unroll
+                for (int e = 0; e < 4; e++) kq[g][i][e] = *(const bf16x8 *)(kp + 32 * e);
+            }
+        auto load_vq = [&](int g) __attribute__((always_inline)) {
+            const int k8 = 32 * g + 8 * lg;  // the lane's eight keys
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const uint16_t *row = vb + (int64_t)(16 * j + l16) * a.So;  // from key0 on
+                if (have == OWN_KEYS) {
+                    __builtin_memcpy(&vq[g][j], row + k8, 16);  // at any alignment
+                } else if (32 * g >= have) {
+                    vq[g][j] = u32x4{};
+                } else if (a.So >= 8) {
+                    // the row's last eight keys, shifted down to the lane's, zeros after them
+                    const int from = min(k8, have - 8), drop = min(k8 - from, 8);
+                    uint64_t v[2];
+                    __builtin_memcpy(v, row + from, 16);
+                    const int d = 16 * (drop & 3);
+                    const uint64_t lo = drop & 4 ? v[1] : v[0], hi = drop & 4 ? 0 : v[1];
+                    v[0] = drop == 8 ? 0 : d ? lo >> d | hi << (64 - d) : lo;
+                    v[1] = drop == 8 ? 0 : hi >> d;
+                    __builtin_memcpy(&vq[g][j], v, 16);
+                } else {  // fewer than eight in all: the first lanes'
+                    vq[g][j] = u32x4{};
+#pragma unroll
+                    for (int e = 0; e < 7; e++)
+                        if (e < have && lg == 0) vq[g][j][e >> 1] |= (uint32_t)row[e] << (16 * (e & 1));
+                }
+            }
+        };
+        load_vq(0);
+        float s[16];
+#pragma unroll
+        for (int g = 0; g < 2; g++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                f32x4 acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kq[g][i][e], qf[e], acc, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; r++) s[8 * g + 4 * i + r] = acc[r];
+            }
+        load_vq(1);
+        softmax(s, std::integral_constant<int, 16>{}, some, seen);
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            const u32x4 p = u32x4{pack_bf16x2(s[8 * g], s[8 * g + 1]), pack_bf16x2(s[8 * g + 2], s[8 * g + 3]),
+                                  pack_bf16x2(s[8 * g + 4], s[8 * g + 5]), pack_bf16x2(s[8 * g + 6], s[8 * g + 7])};
+            const uint32_t keep = (seen >> (8 * g)) & 0xffu;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                if (some)  // what a hidden key holds does not count, a NaN either
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8 *)(kp + 32 * e), qf[e], acc, 0, 0, 0);
-#pragma unroll
-                    for (int r = 0; r < 4; r++) s[8 * g + 4 * i + r] = acc[r];
-                }
-            softmax(s, std::integral_constant<int, 16>{}, some, seen);
-#pragma unroll
-            for (int g = 0; g < 2; g++) {
-                if (32 * g >= have) continue;
-                const u32x4 p = u32x4{pack_bf16x2(s[8 * g], s[8 * g + 1]), pack_bf16x2(s[8 * g + 2], s[8 * g + 3]),
-                                      pack_bf16x2(s[8 * g + 4], s[8 * g + 5]), pack_bf16x2(s[8 * g + 6], s[8 * g + 7])};
-                const int k8 = 32 * g + 8 * lg;  // the lane's eight keys
-                const uint32_t keep = (seen >> (8 * g)) & 0xffu;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const uint16_t *vp = vb + (int64_t)(16 * j + l16) * a.So + k8;
-                    u32x4 v{};
-                    if (rows16 && k8 + 8 <= have) {
-                        v = *(const u32x4 *)vp;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; e++)
-                            if (k8 + e < have) v[e >> 1] |= (uint32_t)vp[e] << (16 * (e & 1));
-                    }
-                    if (some)  // what a hidden key holds does not count, a NaN either
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            v[e] &= ((keep >> (2 * e)) & 1u ? 0xffffu : 0u) | ((keep >> (2 * e + 1)) & 1u ? 0xffff0000u : 0u);
-                    o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v), __builtin_bit_cast(bf16x8, p),
-                                                                      o[j], 0, 0, 0);
-                }
+                        vq[g][j][e] &= ((keep >> (2 * e)) & 1u ? 0xffffu : 0u) | ((keep >> (2 * e + 1)) & 1u ? 0xffff0000u : 0u);
+                o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vq[g][j]), __builtin_bit_cast(bf16x8, p),
+                                                               o[j], 0, 0, 0);
             }
         }
     }
@@ -395,18 +417,18 @@ size_t attn4_scratch_bytes() { return (size_t)std::max(device_cu_count(), 1) * 2
 
 // Which calls this kernel takes: those it is estimated to do before the expansion of the layer
 // and attention.hip, in us. Here 16 queries over 128 keys of the cache take 1.39 ns with the
-// card full, over 64 own keys 4 ns (8 requests of 32 heads, 4299 keys: 256 queries 193 and with
-// as many own keys 232, 1024 queries 772). There the expansion moves 2.53 B a value at 5 TB/s
-// and two launches take about 12; a round of 256-query tiles takes 2.15 per 64 keys (masked
-// 1.8 and no half tiles) and 8, 0.63 of that where half tiles fill at most one per CU.
-// Measured, here / there: 1 x 32 heads over 333 keys, 64 queries 7 / 20, 512 with as many own
-// 39 / 31; over 4299, 512 with as many own 76 / 121, 1024 200 / 132 and without own keys 102 /
-// 122; 8 x 32 heads over 4299 with as many own, 256 232 / 332, 512 625 / 461.
+// card full, over 64 own keys 2.7 ns (8 requests of 32 heads, 4299 keys: 256 queries 194 and
+// with as many own keys 231, 1024 queries 787 and 1469). There the expansion moves 2.53 B a
+// value at 5 TB/s and two launches take about 12; a round of 256-query tiles takes 2.15 per 64
+// keys (masked 1.8 and no half tiles) and 8, 0.63 of that where half tiles fill at most one
+// per CU. Measured, here / there: 1 x 32 heads over 333 keys, 64 queries 7 / 20, 512 with as
+// many own 39 / 31; over 4299, 512 with as many own 74 / 121, 1024 190 / 132 and without own
+// keys 99 / 122; 8 x 32 heads over 4299 with as many own, 256 231 / 332, 512 560 / 461.
 bool attn4_takes(int64_t bh, int64_t sq, int64_t p, int64_t so, bool masked) {
     const double cus = (double)std::max(device_cu_count(), 1), part = 256.0 / cus;
     const double tiles = (double)bh * (double)((sq + 15) / 16);
     const double here = 8.0 + part * tiles * (1.39e-3 * (double)((p + KV4_KEYS - 1) / KV4_KEYS) +
-                                              4.0e-3 * (double)((so + OWN_KEYS - 1) / OWN_KEYS));
+                                              2.7e-3 * (double)((so + OWN_KEYS - 1) / OWN_KEYS));
     const double blocks = (double)((p + 63) / 64 + (so + 63) / 64), n8 = (double)((sq + 255) / 256 * bh);
     const bool half = !masked && (double)((sq + 127) / 128 * bh) <= cus;
     const double rounds = half ? 0.63 : (double)(int64_t)((n8 + cus - 1) / cus);

@@ -128,17 +128,17 @@ __global__ __launch_bounds__(256, 2) void lora_down_kernel(const uint16_t *__res
     }
 }
 
-// four ranks' sums over the shares
+// four ranks' sums over the shares (stride apart), eight loads in flight
 __device__ __forceinline__ f32x4 add_shares(const float *p, int shares, int64_t stride) {
     f32x4 s{};
-    int i = 0;
-    for (; i + 4 <= shares; i += 4, p += 4 * stride) {  // four loads in flight
-        f32x4 v[4];
+    for (int i = 0; i < shares; i += 8) {
+        f32x4 v[8];
 #pragma unroll
-        for (int u = 0; u < 4; u++) v[u] = *(const f32x4 *)(p + u * stride);
-        s += (v[0] + v[1]) + (v[2] + v[3]);
+        for (int u = 0; u < 8; u++) v[u] = *(const f32x4 *)(p + min(i + u, shares - 1) * stride);
+#pragma unroll
+        for (int u = 0; u < 8; u++)
+            if (i + u < shares) s += v[u];
     }
-    for (; i < shares; i++, p += stride) s += *(const f32x4 *)p;
     return s;
 }
 // the bf16 rounding of v (two in a word), and what it leaves
