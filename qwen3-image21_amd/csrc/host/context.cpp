@@ -317,7 +317,7 @@ int qimm_kv_create_q4(qimm_ctx *ctx, int64_t layers, int64_t batch, int64_t head
     *out = nullptr;
     if (batch > 0 && heads > 65535 / batch)
         return set_err(ctx, QIMM_ERR_SHAPE, "kv cache in 4 bits: batch * heads must be at most 65535");
-    if (prefix_len > (int64_t)1 << 36) return set_err(ctx, QIMM_ERR_SHAPE, "kv cache in 4 bits: prefix too long");
+    if (prefix_len >= (int64_t)1 << 31) return set_err(ctx, QIMM_ERR_SHAPE, "kv cache in 4 bits: prefix too long");
     qimm_kv *kv;
     int rc = kv_new(ctx, layers, batch, heads, prefix_len, head_dim, &kv);
     if (rc) return rc;

@@ -427,6 +427,7 @@ size_t attn4_scratch_bytes() { return (size_t)std::max(device_cu_count(), 1) * 2
 bool attn4_takes(int64_t bh, int64_t sq, int64_t p, int64_t so, bool masked) {
     const double cus = (double)std::max(device_cu_count(), 1), part = 256.0 / cus;
     const double tiles = (double)bh * (double)((sq + 15) / 16);
+    if (tiles >= (double)(1 << 24)) return false;  // 2^32 threads
     const double here = 8.0 + part * tiles * (1.39e-3 * (double)((p + KV4_KEYS - 1) / KV4_KEYS) +
                                               2.7e-3 * (double)((so + OWN_KEYS - 1) / OWN_KEYS));
     const double blocks = (double)((p + 63) / 64 + (so + 63) / 64), n8 = (double)((sq + 255) / 256 * bh);
@@ -444,7 +445,7 @@ hipError_t launch_attn4(const uint16_t *q, const uint8_t *tiles, int64_t p, cons
     const int64_t bh = b * h, T = (p + KV4_KEYS - 1) / KV4_KEYS, items = T + (so + OWN_KEYS - 1) / OWN_KEYS;
     const int64_t qt = (sq + 15) / 16;
     const int shares = shares_of(bh * qt, items);
-    if (bh * qt * shares >= ((int64_t)1 << 31)) return hipErrorInvalidValue;
+    if (bh * qt * shares >= (int64_t)1 << 24) return hipErrorInvalidValue;
     const float sl2 = scale * 1.4426950408889634f;
     const Attn4 a{q, tiles, p, T, k_own, vt_own, so, kvalid, h, sq, sl2 < 0.f ? -sl2 : sl2,
                   sl2 < 0.f ? 0x80008000u : 0u, out, scratch, shares, (uint32_t)qt, (uint32_t)(bh * shares % 8 == 0)};

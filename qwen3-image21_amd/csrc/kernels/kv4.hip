@@ -301,7 +301,7 @@ hipError_t launch_store4(const uint16_t *k, const uint16_t *v, int64_t vt_ld, in
                          hipStream_t stream) {
     const int64_t bh = b * h, T = (p + KV4_KEYS - 1) / KV4_KEYS;
     if (bh <= 0 || p <= 0) return hipSuccess;
-    if (bh > 65535 || T > (int64_t)1 << 30 || (vt_ld && (vt_ld < p || vt_ld % 8))) return hipErrorInvalidValue;
+    if (bh > 65535 || T >= (int64_t)1 << 24 || (vt_ld && (vt_ld < p || vt_ld % 8))) return hipErrorInvalidValue;
     const int parts = (int)std::min<int64_t>(T * bh, QK_NORM_PARTS);
     store_k4_kernel<<<dim3((unsigned)parts), dim3(256), 0, stream>>>(k, p, h, kvalid, valid_ld, T, T * bh, tiles, norm_part);
     const hipError_t e = hipGetLastError();
@@ -319,7 +319,7 @@ hipError_t launch_load4(const uint8_t *tiles, int64_t bh, int64_t p, int64_t vt_
                         hipStream_t stream) {
     const int64_t T = (p + KV4_KEYS - 1) / KV4_KEYS;
     if (bh <= 0 || p <= 0) return hipSuccess;
-    if (bh > 65535 || T > (int64_t)1 << 30 || (vt_ld && (vt_ld < p || vt_ld % 8))) return hipErrorInvalidValue;
+    if (bh > 65535 || T >= (int64_t)1 << 24 || (vt_ld && (vt_ld < p || vt_ld % 8))) return hipErrorInvalidValue;
     const dim3 grid((unsigned)T, (unsigned)bh, 2);
     if (vt_ld)
         load4_kernel<true><<<grid, dim3(256), 0, stream>>>(tiles, p, vt_ld, k, v);

@@ -153,11 +153,11 @@ __device__ __forceinline__ uint32_t take_bf16x2(float &a, float &b) {
 // thread. Rows without an adapter are not written.
 template <int PARTS>
 __global__ __launch_bounds__(256) void lora_split_kernel(const float *__restrict__ part, int shares, int64_t m, int64_t ldp,
-                                                        const AdapterDev *__restrict__ ad, int count,
+                                                        int64_t rows, const AdapterDev *__restrict__ ad, int count,
                                                         const int32_t *__restrict__ ids, uint16_t *__restrict__ t16, int64_t kt) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = kt / 4, row = i / per;
-    if (row >= m) return;
-    const int id = row_id(ids, row, m, count), r = (int)(i % per) * 4;
+    if (row >= rows) return;
+    const int id = row_id(ids, row, rows, count), r = (int)(i % per) * 4;
     if (id < 0) return;
     const int rank = ad[id].rank;
     const float scale = ad[id].scale;
@@ -360,14 +360,20 @@ hipError_t launch_lora_down(const uint16_t *x, int64_t lda, int64_t m, int64_t k
 hipError_t launch_lora_split(const float *part, LoraShares sh, int64_t m, int64_t kt, int parts, const AdapterDev *ad, int count,
                              const int32_t *ids, uint16_t *t16, hipStream_t stream) {
     if (m <= 0) return hipSuccess;
-    const dim3 grid((unsigned)((m * (kt / 4) + 255) / 256));
-    if (parts == 2)
-        lora_split_kernel<2><<<grid, dim3(256), 0, stream>>>(part, sh.shares, m, sh.ldp, ad, count, ids, t16, kt);
-    else if (parts == 3)
-        lora_split_kernel<3><<<grid, dim3(256), 0, stream>>>(part, sh.shares, m, sh.ldp, ad, count, ids, t16, kt);
-    else
-        return hipErrorInvalidValue;
-    return hipGetLastError();
+    if (parts != 2 && parts != 3) return hipErrorInvalidValue;
+    constexpr int64_t MOST = 1 << 20;  // rows of one grid (2^28 threads at rank 1024)
+    for (int64_t r = 0; r < m; r += MOST) {
+        const int64_t rows = std::min(m - r, MOST);
+        const dim3 grid((unsigned)((rows * (kt / 4) + 255) / 256));
+        const float *p = part + r * sh.ldp;
+        uint16_t *t = t16 + r * parts * kt;
+        if (parts == 2)
+            lora_split_kernel<2><<<grid, dim3(256), 0, stream>>>(p, sh.shares, m, sh.ldp, rows, ad, count, ids + r, t, kt);
+        else
+            lora_split_kernel<3><<<grid, dim3(256), 0, stream>>>(p, sh.shares, m, sh.ldp, rows, ad, count, ids + r, t, kt);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 hipError_t launch_lora_up(const float *part, LoraShares sh, int64_t m, int64_t row0, int64_t rows, int64_t n, const AdapterDev *ad,

@@ -120,6 +120,50 @@ def test_quantized_weights(torch_cuda, qctx, qctx_codes, t, m, codes_only):
     c.free()
 
 
+@pytest.mark.parametrize("out_type", [qimm.F32, qimm.BF16])
+@pytest.mark.parametrize("m,n,k,ranks", [
+    (4096, 4096, 256, (64,)), (700, 12288, 128, (16, 3)), (1030, 12288, 256, (8, 65, 130)), (4299, 4096, 256, (33, 16)),
+    (2051, 4096, 512, tuple([1, 2, 5] * 100)), (6889, 4096, 128, (16,) * 7)])
+def test_steps_of_the_product_over_bf16_rows(torch_cuda, qctx, m, n, k, ranks, out_type):
+    """Large and small tiles, tails, several adapters and up to a tile's worth of them, an odd
+    number of steps; rows that are no numbers stay alone."""
+    torch = torch_cuda
+    rng = np.random.default_rng(m)
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    route = qimm.qmatmul_route(qimm.BF16, n, k, m, cus)
+    route = qimm.qmatmul_route(qimm.BF16, n, k, m - route.tail, cus)
+    assert route.kernel == qimm.GEMM_BF16_ROWS and route.splits == 1
+    c = Case(torch, qctx, synth.BF16, n, k, ranks, seed=m + k)
+    x_d, _ = bf16_dev(torch, rng.standard_normal((m, k)))
+    for kind in ("requests", "any", "one", "none"):
+        ids = ids_of(kind, m, len(ranks), rng)
+        ids_d = dev(torch, ids.astype(np.int32))
+        got = c.call(x_d, m, ids_d, out_type)
+        # the bar of Case.check, on the device
+        x, w = x_d.double(), dev(torch, c.wv)
+        want, tol = x @ w.t(), (k / 32 + 32) * 2.0 ** -24 * (x.abs() @ w.abs().t())
+        for i in np.unique(ids):
+            if 0 <= i < len(ranks):
+                rows = dev(torch, np.flatnonzero(ids == i))
+                a, b, s = dev(torch, c.a[i]), dev(torch, c.b[i]), c.scale[i]
+                t = s * (x[rows] @ a.t())
+                want[rows] += t @ b.t()
+                tol[rows] += ((k / 32 + 32) * 2.0 ** -24 * abs(s) * (x[rows].abs() @ a.abs().t()) +
+                              (2.0 ** -16 + (len(a) / 32 + 32) * 2.0 ** -24) * t.abs()) @ b.abs().t()
+        tol += 33 * 2.0 ** -24 * want.abs()
+        if out_type == qimm.BF16:
+            tol = tol * (1 + 2.0 ** -8) + 2.0 ** -8 * want.abs()
+        worst = float(((got.double() - want).abs() / tol).max())
+        assert worst <= 1.0, (kind, worst)
+        bad = x_d.clone()
+        bad[5], bad[min(m - 1, 300), 7] = float("inf"), float("nan")
+        after = c.call(bad, m, ids_d, out_type)
+        keep = torch.ones(m, dtype=torch.bool, device="cuda")
+        keep[5] = keep[min(m - 1, 300)] = False
+        assert torch.equal(got[keep], after[keep]) and bool(after[min(m - 1, 300)].isnan().all()), kind
+    c.free()
+
+
 def test_rows_without_adapters_equal_the_plain_product_within_rounding(torch_cuda, qctx):
     torch = torch_cuda
     c = Case(torch, qctx, synth.Q8_0, 512, 1024, (16,), seed=1)
@@ -227,6 +271,8 @@ def test_refusals(torch_cuda, qctx):
     product(m=0)
     refused("QIMM_ERR_SHAPE", lambda: qctx.adapters_create(250, 512, [(1.0, qimm.BF16, a, b)]))
     refused("QIMM_ERR_SHAPE", lambda: qctx.adapters_create(256, 520, [(1.0, qimm.BF16, a, b)]))
+    refused("QIMM_ERR_ARG", lambda: qctx.adapters_create(256, 512, [(1.0, qimm.BF16, b"\x80\x7f" + a[2:], b)]))  # an infinity
+    refused("QIMM_ERR_ARG", lambda: qctx.adapters_create(256, 512, [(1.0, qimm.BF16, a, b[:-2] + b"\xc0\x7f")]))  # a NaN
     refused("QIMM_ERR_SHAPE", lambda: qctx.adapters_create(256, 512, []))
     refused("QIMM_ERR_SHAPE", lambda: qctx.adapters_create(256, 512, [(1.0, qimm.BF16, a, b[:-2])]))
     refused("QIMM_ERR_TYPE", lambda: qctx.adapters_create(256, 512, [(1.0, qimm.Q8_0, a, b)]))
