@@ -392,6 +392,29 @@ int qimm_block_forward(qimm_block *blk, const float *x, float *x_out, int64_t ba
 int qimm_block_set_act_mode(qimm_block *blk, int mode);
 int qimm_block_act_mode(const qimm_block *blk);
 
+/* Low-rank adapters of a block's projections, for batches whose entries belong to requests
+ * with adapters of their own. list: n adapters, each with one scale and a pair (a [rank, in],
+ * b [out, rank]: F32, F16 or BF16, kept as bf16) for the projections it has, data NULL for the
+ * others; gate_up [2 mlp] as in qimm_block_tensors, or proj and gate_layer. They replace the
+ * block's earlier ones (n = 0: none); on an error those stay. Ranks of q, k and v together, and
+ * of proj and gate_layer, at most QIMM_ADAPTER_MAX_RANK. Sizes the scratch of later forwards:
+ * call it before qimm_block_reserve, and not while a captured forward may still be replayed.
+ * ids: int32 [batch] on the device, the adapter of each batch entry in every later forward of
+ * the block (also by a model's forward or prefix fill), an id outside [0, n) none; read by the
+ * forwards, so it must stay; NULL, the default: no adapters. Each projection becomes
+ * y = x W^T + scale (x A^T) B^T, with x the operand that W multiplies (rounded as the activation
+ * mode says) and the sums going through the projection's own epilogue. No counterpart in the
+ * reference. */
+typedef struct {
+    qimm_tensor a, b;
+} qimm_adapter_pair;
+typedef struct {
+    float scale;
+    qimm_adapter_pair to_q, to_k, to_v, to_out, gate_up, proj, gate_layer, mlp_out;
+} qimm_block_adapter;
+int qimm_block_set_adapters(qimm_block *blk, const qimm_block_adapter *list, int64_t n);
+int qimm_block_set_adapter_ids(qimm_block *blk, const int32_t *ids);
+
 /* Sizes the context's device scratch for forwards of this block with up to
  * batch x seq tokens and mod_rows modulation rows (1 or seq). A forward that
  * needs more than the scratch holds grows it, which synchronizes the device

@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <new>
+#include <utility>
 #include <vector>
 
 #include "internal.h"
@@ -61,8 +62,68 @@ bool tensor_ok(const qimm_tensor &t, int64_t rows, int64_t cols) {
     return rb > 0 && (size_t)(rb * rows) == t.nbytes;
 }
 
+void free_adapters(qimm_block *b) {
+    for (qimm_adapters **ad : {&b->ad_qkv, &b->ad_q, &b->ad_k, &b->ad_v, &b->ad_out, &b->ad_gate_up, &b->ad_down}) {
+        if (*ad) qimm_adapters_destroy(*ad);
+        *ad = nullptr;
+    }
+}
+
+// One projection's tensors of a block adapter as part of a product's: output row i of the
+// projection is row at(i) of the product.
+struct AdapterPart {
+    const qimm_adapter_pair *pair;
+    int64_t rows;
+    int64_t (*at)(int64_t i, int64_t rows);
+};
+int64_t rows_0(int64_t i, int64_t) { return i; }
+int64_t rows_1(int64_t i, int64_t n) { return n + i; }
+int64_t rows_2(int64_t i, int64_t n) { return 2 * n + i; }
+// gate and up rows interleaved per 64, and both of a fused [gate ; up]
+int64_t rows_gate(int64_t i, int64_t) { return i / 64 * 128 + i % 64; }
+int64_t rows_up(int64_t i, int64_t) { return i / 64 * 128 + 64 + i % 64; }
+int64_t rows_gate_up(int64_t i, int64_t n) { return i < n / 2 ? rows_gate(i, n) : rows_up(i - n / 2, n); }
+
+// The adapters of one product: A stacked over the parts that an adapter has, B with each
+// part's columns in its rows; an adapter without any is one of zeros. Null if none has any.
+int product_adapters(qimm_ctx *ctx, int64_t rows, int64_t cols, const std::vector<float> &scale,
+                     const std::vector<std::vector<AdapterPart>> &list, qimm_adapters **out) {
+    std::vector<HostAdapter> all(list.size());
+    bool any = false;
+    for (size_t i = 0; i < list.size(); i++) {
+        HostAdapter &h = all[i];
+        h.rank = 0;
+        h.scale = scale[i];
+        for (const AdapterPart &p : list[i]) {
+            if (!p.pair->a.data && !p.pair->b.data) continue;
+            if (const int rc = adapter_tensors(ctx, p.pair->a, p.pair->b, p.rows, cols)) return rc;
+            h.rank += p.pair->a.rows;
+        }
+        if (h.rank > QIMM_ADAPTER_MAX_RANK)
+            return set_err(ctx, QIMM_ERR_SHAPE, "block adapters: q, k and v (or gate and up) together have at most rank " +
+                                                    std::to_string(QIMM_ADAPTER_MAX_RANK));
+        any = any || h.rank > 0;
+        const int64_t rank = std::max<int64_t>(h.rank, 1);
+        h.a.assign((size_t)(rank * cols), 0);
+        h.b.assign((size_t)(rows * rank), 0);
+        int64_t r0 = 0;
+        for (const AdapterPart &p : list[i]) {
+            if (!p.pair->a.data) continue;
+            const std::vector<uint16_t> a = tensor_bf16(p.pair->a), b = tensor_bf16(p.pair->b);
+            const int64_t r = p.pair->a.rows;
+            memcpy(&h.a[(size_t)(r0 * cols)], a.data(), (size_t)(r * cols) * 2);
+            for (int64_t row = 0; row < p.rows; row++)
+                memcpy(&h.b[(size_t)(p.at(row, p.rows) * rank + r0)], &b[(size_t)(row * r)], (size_t)r * 2);
+            r0 += r;
+        }
+        h.rank = rank;
+    }
+    return any ? adapters_build(ctx, rows, cols, all, out) : QIMM_OK;
+}
+
 void free_block(qimm_block *b) {
     if (!b) return;
+    free_adapters(b);
     for (qimm_weight *w : {b->qkv, b->q, b->k, b->v, b->out, b->gate_up, b->down})
         if (w) qimm_weight_free(w);
     if (b->norm_q) (void)hipFree(b->norm_q);
@@ -184,7 +245,7 @@ namespace {
 // rounding (candle mode only), and the split-K scratch of the short- and mid-M
 // GEMM paths, sized for the largest projection.
 struct WsLayout {
-    size_t modp, xn, q, k, vt, att, h, lim, keys, f32, total, part;
+    size_t modp, xn, q, k, vt, att, h, lim, keys, f32, ids, lora, total, part;
 };
 
 // The activation block of candle's vec-dot type for weight w under the
@@ -222,6 +283,17 @@ WsLayout ws_layout(const qimm_block *blk, int64_t batch, int64_t seq, int64_t mo
     L.f32 = off;
     if (act_qblk(blk, blk->out) || act_qblk(blk, blk->down))
         off += align_up((size_t)(M * std::max(hid, F)) * 4);
+    // the tokens' adapters and their products' scratch
+    L.ids = off;
+    size_t lora = 0;
+    const std::pair<const qimm_weight *, const qimm_adapters *> adapted[] = {
+        {blk->qkv, blk->ad_qkv}, {blk->q, blk->ad_q}, {blk->k, blk->ad_k}, {blk->v, blk->ad_v},
+        {blk->out, blk->ad_out}, {blk->gate_up, blk->ad_gate_up}, {blk->down, blk->ad_down}};
+    for (const auto &[w, ad] : adapted)
+        if (ad) lora = std::max(lora, adapters_scratch(w, ad, M));
+    if (lora) off += align_up((size_t)M * 4);
+    L.lora = off;
+    off += align_up(lora);
     L.total = off;
     L.part = 0;
     const qimm_weight *ws_list[] = {blk->qkv, blk->q, blk->k, blk->v, blk->out, blk->gate_up, blk->down};
@@ -278,6 +350,17 @@ int block_forward_impl(qimm_block *blk, const float *x, float *x_out, int64_t ba
     float *part_ws = part_need ? (float *)ctx->ws_part : nullptr;
     const size_t part_bytes = part_need ? ctx->ws_part_bytes : 0;
 
+    // a product with the batch entries' adapters where the block has any
+    int32_t *ids = (int32_t *)(ws + L.ids);
+    const bool adapted = blk->ad_ids && L.total > L.lora;
+    if (adapted) QIMM_HIP(ctx, qimm::launch_repeat_ids(blk->ad_ids, M, seq, ids, s));
+    auto product = [&](const qimm_weight *w, const qimm_adapters *ad, const uint16_t *a, int64_t k, int epi,
+                       const qimm::EpiParams &e) -> int {
+        if (adapted && ad) return adapted_product(ctx, w, ad, ids, a, M, k, epi, e, ws + L.lora, s);
+        QIMM_HIP(ctx, qimm::launch_qgemm(w->gw, a, M, k, epi, e, s));
+        return QIMM_OK;
+    };
+
 #define STAGE_MARK(i) \
     if (blk->profiling) QIMM_HIP(ctx, hipEventRecord(blk->ev[i], s))
     STAGE_MARK(0);
@@ -312,9 +395,10 @@ int block_forward_impl(qimm_block *blk, const float *x, float *x_out, int64_t ba
     ep.q_scale = (1.0f / sqrtf(128.0f)) * 1.4426950408889634f;
     if (blk->qkv_fused) {
         ep.n_offset = 0;
-        QIMM_HIP(ctx, qimm::launch_qgemm(blk->qkv->gw, xn, M, hid, qimm::EPI_QKV, ep, s));
+        if ((rc = product(blk->qkv, blk->ad_qkv, xn, hid, qimm::EPI_QKV, ep))) return rc;
     } else {
         const qimm_weight *parts[3] = {blk->q, blk->k, blk->v};
+        const qimm_adapters *part_ads[3] = {blk->ad_q, blk->ad_k, blk->ad_v};
         for (int i = 0; i < 3; i++) {
             ep.n_offset = i * hid;
             // q, k, v of different vec-dot types round the same norm1 output
@@ -323,7 +407,7 @@ int block_forward_impl(qimm_block *blk, const float *x, float *x_out, int64_t ba
                 QIMM_HIP(ctx, qimm::launch_ln_mod(x, M, hid, modp, 4 * hid, rows_per, xn, s, qb));
                 qb_norm1 = qb;
             }
-            QIMM_HIP(ctx, qimm::launch_qgemm(parts[i]->gw, xn, M, hid, qimm::EPI_QKV, ep, s));
+            if ((rc = product(parts[i], part_ads[i], xn, hid, qimm::EPI_QKV, ep))) return rc;
         }
     }
     STAGE_MARK(2);
@@ -365,7 +449,7 @@ int block_forward_impl(qimm_block *blk, const float *x, float *x_out, int64_t ba
     er.gvec = modp + hid;
     er.g_stride = 4 * hid;
     er.g_rows_per = rows_per;
-    QIMM_HIP(ctx, qimm::launch_qgemm(blk->out->gw, att, M, hid, qimm::EPI_RESID, er, s));
+    if ((rc = product(blk->out, blk->ad_out, att, hid, qimm::EPI_RESID, er))) return rc;
     STAGE_MARK(5);
     // norm2(x1) * (1 + scale2)                                 (:276-278)
     QIMM_HIP(ctx, qimm::launch_ln_mod(x_out, M, hid, modp + 2 * hid, 4 * hid, rows_per, xn, s,
@@ -386,7 +470,7 @@ int block_forward_impl(qimm_block *blk, const float *x, float *x_out, int64_t ba
     eg.hmid_q8_0 = qb_down == 32;
     eg.hmid_round_later = round_sep;
     const bool round_in_gemm = (eg.hmid_q8k || eg.hmid_q8_0) && !round_sep;
-    QIMM_HIP(ctx, qimm::launch_qgemm(blk->gate_up->gw, xn, M, hid, qimm::EPI_SWIGLU, eg, s));
+    if ((rc = product(blk->gate_up, blk->ad_gate_up, xn, hid, qimm::EPI_SWIGLU, eg))) return rc;
     STAGE_MARK(7);
     if (qb_down && !round_in_gemm) QIMM_HIP(ctx, qimm::launch_quant_rows(stage_f32, F, M, F, qb_down, hm, F, s));
     STAGE_MARK(8);
@@ -399,7 +483,7 @@ int block_forward_impl(qimm_block *blk, const float *x, float *x_out, int64_t ba
     ed.gvec = modp + 3 * hid;
     ed.g_stride = 4 * hid;
     ed.g_rows_per = rows_per;
-    QIMM_HIP(ctx, qimm::launch_qgemm(blk->down->gw, hm, M, F, qimm::EPI_RESID, ed, s));
+    if ((rc = product(blk->down, blk->ad_down, hm, F, qimm::EPI_RESID, ed))) return rc;
     STAGE_MARK(9);
 #undef STAGE_MARK
     if (blk->profiling) blk->profiled_once = true;
@@ -434,6 +518,66 @@ int qimm_block_reserve(qimm_block *blk, int64_t batch, int64_t seq, int64_t mod_
     for (const qimm_weight *wt : ws_list)
         if (wt) part = std::max(part, qimm::qgemm_workspace_up_to(wt->gw, batch * seq));
     return part ? ensure_part_workspace(ctx, part) : QIMM_OK;
+}
+
+int qimm_block_set_adapters(qimm_block *blk, const qimm_block_adapter *list, int64_t n) {
+    if (!blk || n < 0 || (n > 0 && !list)) return QIMM_ERR_ARG;
+    qimm_ctx *ctx = blk->ctx;
+    if (n > 65535) return set_err(ctx, QIMM_ERR_SHAPE, "block adapters: at most 65535 of them");
+    const int64_t hid = blk->cfg.hidden, F = blk->cfg.mlp;
+    qimm_block fresh;  // the new adapters; taken over only when all of them are there
+    int rc = QIMM_OK;
+    try {
+        std::vector<float> scale((size_t)n);
+        for (int64_t i = 0; i < n; i++) {
+            scale[(size_t)i] = list[i].scale;
+            if (list[i].gate_up.a.data && (list[i].proj.a.data || list[i].gate_layer.a.data))
+                return set_err(ctx, QIMM_ERR_ARG, "block adapters: gate_up, or proj and gate_layer");
+        }
+        auto build = [&](int64_t rows, int64_t cols, auto parts, qimm_adapters **out) {
+            if (rc) return;
+            std::vector<std::vector<AdapterPart>> all;
+            for (int64_t i = 0; i < n; i++) all.push_back(parts(list[i]));
+            rc = product_adapters(ctx, rows, cols, scale, all, out);
+        };
+        using Parts = std::vector<AdapterPart>;
+        using A = qimm_block_adapter;
+        if (blk->qkv_fused) {
+            build(3 * hid, hid, [&](const A &a) { return Parts{{&a.to_q, hid, rows_0}, {&a.to_k, hid, rows_1}, {&a.to_v, hid, rows_2}}; },
+                  &fresh.ad_qkv);
+        } else {
+            build(hid, hid, [&](const A &a) { return Parts{{&a.to_q, hid, rows_0}}; }, &fresh.ad_q);
+            build(hid, hid, [&](const A &a) { return Parts{{&a.to_k, hid, rows_0}}; }, &fresh.ad_k);
+            build(hid, hid, [&](const A &a) { return Parts{{&a.to_v, hid, rows_0}}; }, &fresh.ad_v);
+        }
+        build(hid, hid, [&](const A &a) { return Parts{{&a.to_out, hid, rows_0}}; }, &fresh.ad_out);
+        build(2 * F, hid, [&](const A &a) {
+            return Parts{{&a.gate_up, 2 * F, rows_gate_up}, {&a.gate_layer, F, rows_gate}, {&a.proj, F, rows_up}};
+        }, &fresh.ad_gate_up);
+        build(hid, F, [&](const A &a) { return Parts{{&a.mlp_out, hid, rows_0}}; }, &fresh.ad_down);
+    } catch (const std::bad_alloc &) {
+        rc = set_err(ctx, QIMM_ERR_OOM, "block adapters: host staging allocation failed");
+    }
+    if (rc) {
+        free_adapters(&fresh);
+        return rc;
+    }
+    free_adapters(blk);
+    blk->ad_qkv = fresh.ad_qkv;
+    blk->ad_q = fresh.ad_q;
+    blk->ad_k = fresh.ad_k;
+    blk->ad_v = fresh.ad_v;
+    blk->ad_out = fresh.ad_out;
+    blk->ad_gate_up = fresh.ad_gate_up;
+    blk->ad_down = fresh.ad_down;
+    return QIMM_OK;
+}
+
+int qimm_block_set_adapter_ids(qimm_block *blk, const int32_t *ids) {
+    if (!blk) return QIMM_ERR_ARG;
+    if ((uintptr_t)ids & 3) return set_err(blk->ctx, QIMM_ERR_ARG, "block adapters: ids must be 4-byte aligned");
+    blk->ad_ids = ids;
+    return QIMM_OK;
 }
 
 int qimm_block_set_act_mode(qimm_block *blk, int mode) {

@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include <string>
+#include <vector>
 
 #include "../kernels/kernels.h"
 #include "qimm.h"
@@ -84,6 +85,11 @@ struct qimm_block {
     // and the bf16 rounding
     float q_norm_bound = 0.f, k_norm_bound = 0.f;
     int act = QIMM_ACT_CANDLE;           // arithmetic at the quantized matmul inputs
+    // low-rank adapters of the products above (null: none has any) and the batch
+    // entries' ids (device, the caller's)
+    qimm_adapters *ad_qkv = nullptr, *ad_q = nullptr, *ad_k = nullptr, *ad_v = nullptr;
+    qimm_adapters *ad_out = nullptr, *ad_gate_up = nullptr, *ad_down = nullptr;
+    const int32_t *ad_ids = nullptr;
     // stage timing (qimm_block_profile): events around the stages of a forward
     bool profiling = false;
     bool profiled_once = false;
@@ -104,6 +110,22 @@ void to_bf16(int type, const uint8_t *src, int64_t n, uint16_t *dst);
 // the checks of a product's arguments
 int qmatmul_check(qimm_ctx *ctx, const qimm_weight *w, const void *x_bf16, int64_t m, int64_t lda, void *y, int out_type);
 int block_values(int type);
+
+// One adapter in host memory: a [rank][cols], b [rows][rank] bf16.
+struct HostAdapter {
+    int64_t rank;
+    float scale;
+    std::vector<uint16_t> a, b;
+};
+// the checks of one adapter's tensors; their values as bf16; the device copy (may throw bad_alloc)
+int adapter_tensors(qimm_ctx *ctx, const qimm_tensor &a, const qimm_tensor &b, int64_t rows, int64_t cols);
+std::vector<uint16_t> tensor_bf16(const qimm_tensor &t);
+int adapters_build(qimm_ctx *ctx, int64_t rows, int64_t cols, const std::vector<HostAdapter> &list, qimm_adapters **out);
+// launch_qgemm with the rows' adapters (ids int32 [m], device); ws: adapters_scratch bytes,
+// which serve any smaller m too; ep with its part_ws
+size_t adapters_scratch(const qimm_weight *w, const qimm_adapters *ad, int64_t m);
+int adapted_product(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapters *ad, const int32_t *ids, const uint16_t *x,
+                    int64_t m, int64_t lda, int epi, const qimm::EpiParams &ep, char *ws, hipStream_t s);
 
 // The key segment of cache layer `layer` for kernels launched on stream s. A
 // host cache stages the layer into a slot first (or waits for a prefetch);

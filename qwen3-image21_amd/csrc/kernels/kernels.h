@@ -281,6 +281,8 @@ struct AdapterDev {
     float scale;
     int32_t pad;
 };
+// out[row] = ids[row / per], rows of them
+hipError_t launch_repeat_ids(const int32_t *ids, int64_t rows, int64_t per, int32_t *out, hipStream_t stream);
 // Few rows (lora_few): t[row][0:rank) (f32, row stride ldt, the largest rank) = scale x A^T
 // with the adapter ids[row] of each row; x [m][k] bf16, row stride lda. Then y [m][n] = base
 // (f32) + t B^T, to y32 (f32, may be base) when set, else bf16 to y16.
@@ -308,8 +310,9 @@ hipError_t launch_lora_up(const float *part, LoraShares sh, int64_t m, int64_t r
 // the adapter's rank; rows without one are not written.
 hipError_t launch_lora_split(const float *part, LoraShares sh, int64_t m, int64_t kt, int parts, const AdapterDev *ad, int count,
                              const int32_t *ids, uint16_t *t16, hipStream_t stream);
-// The product over bf16 rows with the adapters' second product as further k steps
-// (launch_qgemm_bf16's plain outputs, `head` tiles of 256 tokens): y = A W^T + t B^T.
+// The product over bf16 rows with the adapters' second product as further k steps, in
+// launch_qgemm_bf16's epilogues without the rounding of the hidden state; `head` tiles of 256
+// tokens: epilogue(A W^T + t B^T).
 struct AdapterSteps {
     const uint16_t *t;     // t16
     int kb, steps;         // kt / 64; parts of them

@@ -297,10 +297,22 @@ __global__ __launch_bounds__(256) void lora_up_row_kernel(const float *__restric
         y16[row * N + n] = (uint16_t)(pack_bf16x2(s, 0.f) & 0xffffu);
 }
 
+__global__ __launch_bounds__(256) void repeat_ids_kernel(const int32_t *__restrict__ ids, int64_t rows, int64_t per,
+                                                        int32_t *__restrict__ out) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < rows) out[i] = ids[i / per];
+}
+
 // Up to this many rows each row is taken by itself.
 constexpr int64_t FEW_ROWS = 64;
 
 }  // namespace
+
+hipError_t launch_repeat_ids(const int32_t *ids, int64_t rows, int64_t per, int32_t *out, hipStream_t stream) {
+    if (rows <= 0) return hipSuccess;
+    repeat_ids_kernel<<<dim3((unsigned)((rows + 255) / 256)), dim3(256), 0, stream>>>(ids, rows, per, out);
+    return hipGetLastError();
+}
 
 bool lora_few(int64_t m) { return m <= FEW_ROWS; }
 

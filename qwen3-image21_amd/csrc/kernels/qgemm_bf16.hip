@@ -844,11 +844,16 @@ hipError_t launch_qgemm_bf16(const GemmWeight &w, const uint16_t *a, int64_t m, 
 
 hipError_t launch_qgemm_bf16_adapters(const GemmWeight &w, const uint16_t *a, int64_t m, int64_t lda, int epi,
                                       const EpiParams &ep, int64_t head, const AdapterSteps &x, hipStream_t stream) {
-    if (!qgemm_bf16_fits(w) || lda > ((int64_t)1 << 22) || (epi != EPI_F32 && epi != EPI_BF16) || head < 0 ||
-        x.kb < 1 || x.steps % x.kb)
-        return hipErrorInvalidValue;
-    return epi == EPI_F32 ? launch_one<EPI_F32, true>(w, a, m, lda, ep, head, 1, stream, x)
-                          : launch_one<EPI_BF16, true>(w, a, m, lda, ep, head, 1, stream, x);
+    if (!qgemm_bf16_fits(w) || lda > ((int64_t)1 << 22) || head < 0 || x.kb < 1 || x.steps % x.kb) return hipErrorInvalidValue;
+    switch (epi) {
+    case EPI_F32: return launch_one<EPI_F32, true>(w, a, m, lda, ep, head, 1, stream, x);
+    case EPI_BF16: return launch_one<EPI_BF16, true>(w, a, m, lda, ep, head, 1, stream, x);
+    case EPI_QKV: return launch_one<EPI_QKV, true>(w, a, m, lda, ep, head, 1, stream, x);
+    case EPI_RESID: return launch_one<EPI_RESID, true>(w, a, m, lda, ep, head, 1, stream, x);
+    case EPI_SWIGLU:
+        return ep.hmid_q8k || ep.hmid_q8_0 ? hipErrorInvalidValue : launch_one<EPI_SWIGLU, true>(w, a, m, lda, ep, head, 1, stream, x);
+    default: return hipErrorInvalidValue;
+    }
 }
 
 }  // namespace qimm

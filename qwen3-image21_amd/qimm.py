@@ -79,6 +79,8 @@ SIGNATURES = [
     ("qimm_block_reserve", _i32, [_vp, _i64, _i64, _i64]),
     ("qimm_block_set_act_mode", _i32, [_vp, _i32]),
     ("qimm_block_act_mode", _i32, [_vp]),
+    ("qimm_block_set_adapters", _i32, [_vp, _vp, _i64]),
+    ("qimm_block_set_adapter_ids", _i32, [_vp, _vp]),
     ("qimm_quantize_act", _i32, [_vp, _i32, _vp, _i64, _i64, _i64, _vp, _i64, _vp]),
     ("qimm_block_forward_masked", _i32, [_vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp,
                                          _vp]),
@@ -126,6 +128,17 @@ class Tensor(C.Structure):
 class Adapter(C.Structure):
     """qimm_adapter: scale, a [rank, cols], b [rows, rank]."""
     _fields_ = [("scale", _f32), ("a", Tensor), ("b", Tensor)]
+
+
+class AdapterPair(C.Structure):
+    """qimm_adapter_pair."""
+    _fields_ = [("a", Tensor), ("b", Tensor)]
+
+
+class BlockAdapter(C.Structure):
+    """qimm_block_adapter: one scale, a pair for each projection that has one."""
+    PROJECTIONS = ("to_q", "to_k", "to_v", "to_out", "gate_up", "proj", "gate_layer", "mlp_out")
+    _fields_ = [("scale", _f32)] + [(n, AdapterPair) for n in PROJECTIONS]
 
 
 class BlockTensors(C.Structure):
@@ -437,6 +450,19 @@ class Block:
     @property
     def act_mode(self) -> int:
         return self.ctx.lib.qimm_block_act_mode(self.h)
+
+    def set_adapters(self, adapters):
+        """adapters: (scale, {projection: (type, rows, cols, rank, a bytes, b bytes)}) each; replaces the block's."""
+        keep, arr = [], (BlockAdapter * max(1, len(adapters)))()
+        for slot, (scale, pairs) in zip(arr, adapters):
+            slot.scale = scale
+            for name, (t, rows, cols, rank, a, b) in pairs.items():
+                setattr(slot, name, AdapterPair(make_tensor(t, rank, cols, a, keep), make_tensor(t, rows, rank, b, keep)))
+        self.ctx.check(self.ctx.lib.qimm_block_set_adapters(self.h, C.byref(arr), len(adapters)), "qimm_block_set_adapters")
+
+    def set_adapter_ids(self, ids_dev: int | None):
+        """int32 [batch] on the device: the adapter of each batch entry in later forwards (None: no adapters)."""
+        self.ctx.check(self.ctx.lib.qimm_block_set_adapter_ids(self.h, ids_dev), "qimm_block_set_adapter_ids")
 
     def forward(self, x_dev, x_out_dev, batch, seq, mod_dev, pe_dev, kv=None, layer=0, k_out=None, v_out=None,
                 stream=0):

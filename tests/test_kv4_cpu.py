@@ -37,3 +37,15 @@ def test_null_arguments():
     assert lib.qimm_kv_create_q4(None, 1, 1, 1, 8, 128, C.byref(h)) == 1
     assert lib.qimm_kv_bits(None) == -1
     assert lib.qimm_kv_device_bytes(None) == -1
+
+
+def test_null_arguments_of_the_adapters():
+    lib = qimm.load()
+    h = C.c_void_p()
+    assert lib.qimm_adapters_create(None, 128, 64, None, 0, C.byref(h)) == 1
+    assert lib.qimm_adapters_destroy(None) == 1
+    assert lib.qimm_adapters_device_bytes(None) == -1
+    assert lib.qimm_qmatmul_adapters(None, None, None, None, None, 1, 64, None, 0, None) == 1
+    assert lib.qimm_qmatmul_adapters_reserve(None, None, None, 1, 0) == 1
+    assert lib.qimm_block_set_adapters(None, None, 0) == 1
+    assert lib.qimm_block_set_adapter_ids(None, None) == 1
