@@ -41,7 +41,7 @@ struct Route {
 Route route_of(const qimm_weight *w, const qimm_adapters *ad, int64_t m, int64_t lda, int epi) {
     Route r{};
     const bool plain = epi == qimm::EPI_F32 || epi == qimm::EPI_BF16;
-    r.few = qimm::lora_few(m);
+    r.few = qimm::lora_few(m, ad->max_rank, ad->count);
     r.parts = epi == qimm::EPI_F32 ? 3 : 2;
     r.head = m;
     qimm::EpiParams ep{};

@@ -286,7 +286,7 @@ hipError_t launch_repeat_ids(const int32_t *ids, int64_t rows, int64_t per, int3
 // Few rows (lora_few): t[row][0:rank) (f32, row stride ldt, the largest rank) = scale x A^T
 // with the adapter ids[row] of each row; x [m][k] bf16, row stride lda. Then y [m][n] = base
 // (f32) + t B^T, to y32 (f32, may be base) when set, else bf16 to y16.
-bool lora_few(int64_t m);
+bool lora_few(int64_t m, int64_t max_rank, int64_t count);
 hipError_t launch_lora_few_down(const uint16_t *x, int64_t lda, int64_t m, int64_t k, const AdapterDev *ad, int count,
                                 const int32_t *ids, float *t, int64_t ldt, hipStream_t stream);
 hipError_t launch_lora_few_up(const float *t, int64_t ldt, int64_t m, int64_t n, const AdapterDev *ad, int count,

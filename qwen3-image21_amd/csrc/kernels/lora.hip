@@ -303,8 +303,13 @@ __global__ __launch_bounds__(256) void repeat_ids_kernel(const int32_t *__restri
     if (i < rows) out[i] = ids[i / per];
 }
 
-// Up to this many rows each row is taken by itself.
-constexpr int64_t FEW_ROWS = 64;
+// Each row is taken by itself up to 64 rows, and up to 256 where that costs a batch of one
+// adapter nothing or, with many adapters, little: the tiles' time grows with the adapters among
+// their rows, of which the host knows only the bound. Q8_0 4096 x 4096, us by tiles with one
+// adapter / one per row -> by rows with one / one per row: rank 16, 128 rows 32 / 304 -> 30 / 32,
+// 256 rows 39 / 312 -> 40 / 45; rank 64, 128 rows 40 / 438 -> 39 / 75 (Q4_K 12288 x 4096 65 / 482
+// -> 93 / 157), 256 rows 47 / 458 -> 58 / 127.
+constexpr int64_t FEW_ROWS = 64, MORE_ROWS = 256;
 
 }  // namespace
 
@@ -314,12 +319,14 @@ hipError_t launch_repeat_ids(const int32_t *ids, int64_t rows, int64_t per, int3
     return hipGetLastError();
 }
 
-bool lora_few(int64_t m) { return m <= FEW_ROWS; }
+bool lora_few(int64_t m, int64_t max_rank, int64_t count) {
+    return m <= FEW_ROWS || (m <= MORE_ROWS && m * max_rank <= (count >= 8 ? 8192 : 4096));
+}
 
 hipError_t launch_lora_few_down(const uint16_t *x, int64_t lda, int64_t m, int64_t k, const AdapterDev *ad, int count,
                                 const int32_t *ids, float *t, int64_t ldt, hipStream_t stream) {
     if (m <= 0) return hipSuccess;
-    if (m > FEW_ROWS) return hipErrorInvalidValue;
+    if (m > MORE_ROWS) return hipErrorInvalidValue;
     lora_down_row_kernel<<<dim3((unsigned)((ldt + 3) / 4), (unsigned)m), dim3(256), 0, stream>>>(x, lda, k, ad, count, ids, t, ldt);
     return hipGetLastError();
 }
@@ -327,7 +334,7 @@ hipError_t launch_lora_few_down(const uint16_t *x, int64_t lda, int64_t m, int64
 hipError_t launch_lora_few_up(const float *t, int64_t ldt, int64_t m, int64_t n, const AdapterDev *ad, int count,
                               const int32_t *ids, const float *base, float *y32, uint16_t *y16, hipStream_t stream) {
     if (m <= 0) return hipSuccess;
-    if (m > FEW_ROWS) return hipErrorInvalidValue;
+    if (m > MORE_ROWS) return hipErrorInvalidValue;
     lora_up_row_kernel<<<dim3((unsigned)((n + 255) / 256), (unsigned)m), dim3(256), 0, stream>>>(t, ldt, n, ad, count, ids, base,
                                                                                                 y32, y16);
     return hipGetLastError();

@@ -120,6 +120,21 @@ def test_quantized_weights(torch_cuda, qctx, qctx_codes, t, m, codes_only):
     c.free()
 
 
+@pytest.mark.parametrize("m,ranks", [
+    (65, (64,) * 3), (100, (40, 41) * 60), (128, (64,) * 128), (129, (64,) * 8), (200, (16, 20) * 100), (256, (16,) * 256),
+    (256, (32,) * 300), (257, (16,) * 257)])
+def test_an_adapter_for_every_row(torch_cuda, qctx, m, ranks):
+    """By rows and by tiles, on both sides of the bounds between them."""
+    c = Case(torch_cuda, qctx, synth.BF16, 256, 256, ranks, seed=m)
+    rng = np.random.default_rng(m)
+    x_d, x = bf16_dev(torch_cuda, rng.standard_normal((m, 256)))
+    ids = rng.permutation(max(m, len(ranks)))[:m]
+    ids_d = dev(torch_cuda, ids.astype(np.int32))
+    for out_type in (qimm.F32, qimm.BF16):
+        c.check(host(c.call(x_d, m, ids_d, out_type).float()), x, ids, out_type)
+    c.free()
+
+
 @pytest.mark.parametrize("out_type", [qimm.F32, qimm.BF16])
 @pytest.mark.parametrize("m,n,k,ranks", [
     (4096, 4096, 256, (64,)), (700, 12288, 128, (16, 3)), (1030, 12288, 256, (8, 65, 130)), (4299, 4096, 256, (33, 16)),
