@@ -110,9 +110,11 @@ __global__ __launch_bounds__(256, 2) void attn4_kernel(const Attn4 a) {
         for (int j = 0; j < 2; j++) vs[j] = *(const int *)(t + (KV4_VS - KV4_V) + (j * 64 + lane) * 4);
     };
     // The running maximum over the N scores of a lane's query and its three other lanes',
-    // with the sums taken along; the scores become 2^8 exp(scale (s - max)), hidden ones 0.
-    // `seen` has a bit per score.
-    auto softmax = [&](float *s, auto count, bool some, uint32_t seen) __attribute__((always_inline)) {
+    // with the sums taken along; the scores become 2^(8 - e) exp(scale (s - max)), hidden ones 0,
+    // and e is returned: 0, or of a tile of the cache the power of two of its own largest (from
+    // -100 on), so that e4m3, which ends at 2^-23 of the largest with its lo, holds the keys of
+    // other tiles than that of a key that takes nearly all. `seen` has a bit per score.
+    auto softmax = [&](float *s, auto count, bool some, uint32_t seen) __attribute__((always_inline)) -> int {
         constexpr int N = decltype(count)::value;
         if (some)
 #pragma unroll
@@ -122,6 +124,7 @@ __global__ __launch_bounds__(256, 2) void attn4_kernel(const Attn4 a) {
         for (int e = 1; e < N; e++) mx = fmaxf(mx, s[e]);
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float top = mx;
         mx = fmaxf(mx, m);
         if (__ballot(mx > m)) {
             // a lane without a visible key so far has sums of 0
@@ -133,7 +136,9 @@ __global__ __launch_bounds__(256, 2) void attn4_kernel(const Attn4 a) {
 #pragma unroll
                 for (int r = 0; r < 4; r++) o[j][r] *= al;
         }
-        const float c = 8.f - (mx == -INFINITY ? 0.f : mx * a.sl2);
+        // (no visible key, or all of them infinite: -100, of no consequence)
+        const int e2 = N == 32 ? (int)fmaxf(__builtin_ceilf((top - mx) * a.sl2), -100.f) : 0;
+        const float c = (float)(8 - e2) - (mx == -INFINITY ? 0.f : mx * a.sl2);
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < N; e++) {
@@ -142,7 +147,8 @@ __global__ __launch_bounds__(256, 2) void attn4_kernel(const Attn4 a) {
             s[e] = p;
             sum += p;
         }
-        l += sum;
+        l += __builtin_amdgcn_ldexpf(sum, e2);
+        return e2;
     };
     // visible keys of 64 from key k0 of the P + So, the first `have` of them there (have >= 1)
     auto validity = [&](int64_t k0, int have) __attribute__((always_inline)) -> uint64_t {
@@ -231,7 +237,7 @@ __global__ __launch_bounds__(256, 2) void attn4_kernel(const Attn4 a) {
             float s[32];
 #pragma unroll
             for (int e = 0; e < 32; e++) s[e] = acc[e >> 2][e & 3];
-            softmax(s, std::integral_constant<int, 32>{}, some, seen);
+            const int e2 = softmax(s, std::integral_constant<int, 32>{}, some, seen);
             i32x8 ph, pl;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
@@ -240,7 +246,7 @@ __global__ __launch_bounds__(256, 2) void attn4_kernel(const Attn4 a) {
                 ph[i] = hi;
                 pl[i] = lo;
             }
-            constexpr int psc = 127 | 122 << 8;
+            const int psc = (127 | 122 << 8) + e2 * 257;  // scale bytes: hi, lo
 #define PV(j, p, sel) \
     o[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(widen(vc[j]), p, o[j], 4, 0, j & 3, vs[j >> 2], sel, psc);
             PV(0, ph, 0) PV(1, ph, 0) PV(2, ph, 0) PV(3, ph, 0) PV(4, ph, 0) PV(5, ph, 0) PV(6, ph, 0) PV(7, ph, 0)

@@ -7,7 +7,7 @@ Bar of the attention over codes, per output with A = sum p |v| (p the exact prob
   largest (error 2^-22 of it), so scores are off by f32 roundings: e^s by less than 2^-12;
 - a prefix key's probability is hi + lo, hi off by half a step 2^-4, lo by 2^-4 of that: 2^-8;
   an own key's is rounded to bf16: 2^-8; what falls below the e4m3 range of lo, 2^-23 of the
-  largest each: less than 2^-10 in all below 2^13 keys of equal values;
+  largest of its 128 keys each: less than 2^-16 in all of keys of equal values;
 - the output is rounded to bf16: 2^-8 of it.
 Together 2^-8 (A + |out|) + 2^-9 A.
 """
@@ -204,6 +204,32 @@ def test_a_row_without_a_visible_key_is_nan(torch_cuda, qctx, h, sq, so):
         assert_near(got[:1], want[:1], a[:1])
     else:
         kv_close(got[:1], want[:1])
+
+
+@pytest.mark.parametrize("sq,bits", [(8192, 24.0), (8192, 16.5), (2, 24.0), (2, 40.0)])
+def test_a_key_that_takes_nearly_all_leaves_the_others_their_precision(torch_cuda, qctx, sq, bits):
+    """A key of value 0 with 2^bits the probability of each other one, in one share or many. Its own
+    tile's probabilities are off by up to 2^-23 of its."""
+    torch = torch_cuda
+    p, at, rng = 1536, 40, np.random.default_rng(3)
+    q_d, q = bf16(torch, np.where(np.arange(128) == 0, 1.0, 0.0) * np.ones((1, 1, sq, 1)))
+    k = np.zeros((1, 1, p, 128))
+    k[0, 0, at, 0] = 6.0
+    v = np.abs(rng.standard_normal((1, 1, p, 128))) + 0.5
+    v[0, 0, at] = 0.0
+    (k_d, k), (v_d, v) = bf16(torch, k), bf16(torch, v)
+    pk, pv = kv4_ref.near_kv(k, v)
+    scale = bits * np.log(2.0) / 6.0
+    kv = stored(torch, qctx, k_d, v_d)
+    out = torch.empty(1, sq, 128, dtype=torch.bfloat16, device="cuda")
+    qctx.attention(q_d.data_ptr(), 1, 1, sq, kv, 0, None, None, 0, scale, out.data_ptr(), stream(torch))
+    kv.free()
+    got = host(out.float()).reshape(1, sq, 1, 128).astype(np.float64)
+    want, a = kv4_ref.attention(q[:, :, :1], pk, pv, scale, None)
+    extra = 2.0 ** -23 * np.abs(pv[0, 0, :128]).sum(0)
+    tol = 2.0 ** -8 * (a + np.abs(want)) + 2.0 ** -9 * a + extra
+    worst = np.max(np.abs(got - want) / tol)
+    assert np.isfinite(got).all() and worst <= 1.0, worst
 
 
 def test_attention_with_many_shares_and_few(torch_cuda, qctx):
