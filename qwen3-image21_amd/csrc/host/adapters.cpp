@@ -112,11 +112,13 @@ int run(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapters *ad, const int3
     es.ldo = N;
     es.part_ws = ep.part_ws;
     es.part_ws_bytes = ep.part_ws_bytes;
+    qimm::SplitSums base{sums, 1};
+    if (!qimm::qgemm_route(w->gw, m - row0, lda, qimm::EPI_F32, es).tail) es.left = &base;
     QIMM_HIP(ctx, qimm::launch_qgemm(w->gw, x + row0 * lda, m - row0, lda, qimm::EPI_F32, es, s));
     if (r.few)
-        QIMM_HIP(ctx, qimm::launch_lora_few_up(shares, ad->max_rank, m, N, table, n, ids, sums, y32, y16, s));
+        QIMM_HIP(ctx, qimm::launch_lora_few_up(shares, ad->max_rank, m, N, table, n, ids, base, y32, y16, s));
     else
-        QIMM_HIP(ctx, qimm::launch_lora_up(shares, sh, m, row0, m - row0, N, table, n, ids + row0, sums, y32, y16, s));
+        QIMM_HIP(ctx, qimm::launch_lora_up(shares, sh, m, row0, m - row0, N, table, n, ids + row0, base, y32, y16, s));
     if (epi != qimm::EPI_F32 && epi != qimm::EPI_BF16)
         QIMM_HIP(ctx, qimm::launch_split_epilogue(sums, 1, m, N, epi, ep, s));
     return QIMM_OK;

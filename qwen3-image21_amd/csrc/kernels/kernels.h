@@ -18,6 +18,12 @@ enum : int { WF_Q8_0 = 0, WF_Q4_K = 1, WF_Q6_K = 2, WF_BF16 = 3 };
 
 enum : int { EPI_F32 = 0, EPI_BF16 = 1, EPI_QKV = 2, EPI_RESID = 3, EPI_SWIGLU = 4 };
 
+// Sums of a product split over K: splits of [m][N] f32, one after the other.
+struct SplitSums {
+    const float *part;
+    int splits;
+};
+
 struct EpiParams {
     // EPI_F32 / EPI_BF16: out[m * ldo + n]
     void *out;
@@ -69,6 +75,9 @@ struct EpiParams {
     // without it short M takes the 128x128 kernel)
     float *part_ws = nullptr;
     size_t part_ws_bytes = 0;
+    // EPI_F32 of a product without a tail: where set and the product is split over K,
+    // its sums are left in part_ws, not added to `out`, and *left tells (host memory)
+    SplitSums *left = nullptr;
 };
 
 struct GemmWeight {
@@ -285,12 +294,13 @@ struct AdapterDev {
 hipError_t launch_repeat_ids(const int32_t *ids, int64_t rows, int64_t per, int32_t *out, hipStream_t stream);
 // Few rows (lora_few): t[row][0:rank) (f32, row stride ldt, the largest rank) = scale x A^T
 // with the adapter ids[row] of each row; x [m][k] bf16, row stride lda. Then y [m][n] = base
-// (f32) + t B^T, to y32 (f32, may be base) when set, else bf16 to y16.
+// (f32 sums, base.splits of them) + t B^T, to y32 (f32, may be base's one) when set, else bf16
+// to y16.
 bool lora_few(int64_t m, int64_t max_rank, int64_t count);
 hipError_t launch_lora_few_down(const uint16_t *x, int64_t lda, int64_t m, int64_t k, const AdapterDev *ad, int count,
                                 const int32_t *ids, float *t, int64_t ldt, hipStream_t stream);
 hipError_t launch_lora_few_up(const float *t, int64_t ldt, int64_t m, int64_t n, const AdapterDev *ad, int count,
-                              const int32_t *ids, const float *base, float *y32, uint16_t *y16, hipStream_t stream);
+                              const int32_t *ids, SplitSums base, float *y32, uint16_t *y16, hipStream_t stream);
 // Many rows: partial sums of t in scratch, lora_down_scratch bytes: [shares][m][ldp] f32 over
 // shares of K, without the scale; rows without an adapter are not written.
 struct LoraShares {
@@ -301,10 +311,10 @@ LoraShares lora_shares(int64_t m, int64_t k, int64_t max_rank);
 size_t lora_down_scratch(int64_t m, int64_t k, int64_t max_rank);
 hipError_t launch_lora_down(const uint16_t *x, int64_t lda, int64_t m, int64_t k, int64_t max_rank, const AdapterDev *ad, int count,
                             const int32_t *ids, float *part, hipStream_t stream);
-// y = base + t B^T of rows row0 .. row0 + rows (of part's m rows; ids, base and y are the rows'
-// own), to y32 (f32, may be base) when set, else bf16 to y16
+// y = base (of `rows` rows) + t B^T of rows row0 .. row0 + rows (of part's m rows; ids, base and
+// y are the rows' own), to y32 (f32, may be base) when set, else bf16 to y16
 hipError_t launch_lora_up(const float *part, LoraShares sh, int64_t m, int64_t row0, int64_t rows, int64_t n, const AdapterDev *ad,
-                          int count, const int32_t *ids, const float *base, float *y32, uint16_t *y16, hipStream_t stream);
+                          int count, const int32_t *ids, SplitSums base, float *y32, uint16_t *y16, hipStream_t stream);
 // t16[row][parts][kt] (kt the largest rank rounded up to 64) = t as a sum of bf16 numbers, each
 // the rounding of what the ones before leave: two parts keep 2^-16 of t, three 2^-24; zeros past
 // the adapter's rank; rows without one are not written.

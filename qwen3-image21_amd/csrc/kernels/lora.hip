@@ -175,12 +175,15 @@ __global__ __launch_bounds__(256) void lora_split_kernel(const float *__restrict
 }
 
 // y = base + t B^T for 16 rows x 256 columns, 64 columns per wave; t from the shares' sums,
-// in PARTS bf16 operands. A = B's rows, B = t's.
+// in PARTS bf16 operands. A = B's rows, B = t's. base: the product's sums, `splits` of them
+// (base_stride apart) where it is split over K, added here in their order instead of in a
+// launch of their own (514 rows x 4096 x 4096 BF16, rank 16: 48 -> 45 us; 200 x 4096
+// x 4096 Q8_0 35 -> 32).
 template <int PARTS>
 __global__ __launch_bounds__(256) void lora_up_kernel(const float *__restrict__ part, int shares, int64_t m, int64_t ldp,
                                                      int64_t rows, int64_t N, const AdapterDev *__restrict__ ad, int count,
-                                                     const int32_t *__restrict__ ids, const float *base,
-                                                     float *y32, uint16_t *y16) {
+                                                     const int32_t *__restrict__ ids, const float *base, int splits,
+                                                     int64_t base_stride, float *y32, uint16_t *y16) {
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
     const int64_t row = (int64_t)blockIdx.y * 16 + l16, n0 = (int64_t)blockIdx.x * 256 + 64 * wave;
     if (n0 >= N) return;  // N is a multiple of 128
@@ -188,6 +191,10 @@ __global__ __launch_bounds__(256) void lora_up_kernel(const float *__restrict__ 
     f32x4 acc[4] = {}, base4[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) base4[i] = *(const f32x4 *)(base + min(row, rows - 1) * N + n0 + 16 * i + 4 * lg);
+#pragma unroll 2
+    for (int s = 1; s < splits; s++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) base4[i] += *(const f32x4 *)(base + s * base_stride + min(row, rows - 1) * N + n0 + 16 * i + 4 * lg);
     uint64_t todo = __ballot(id >= 0) & 0xffffu;
     while (todo) {
         const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
@@ -271,12 +278,13 @@ __global__ __launch_bounds__(256) void lora_down_row_kernel(const uint16_t *__re
 // y of row blockIdx.y, one column per thread: a thread reads its row of B, 16 B at a time.
 __global__ __launch_bounds__(256) void lora_up_row_kernel(const float *__restrict__ t, int64_t ldt, int64_t N,
                                                          const AdapterDev *__restrict__ ad, int count,
-                                                         const int32_t *__restrict__ ids, const float *base, float *y32,
-                                                         uint16_t *y16) {
+                                                         const int32_t *__restrict__ ids, const float *base, int splits,
+                                                         int64_t base_stride, float *y32, uint16_t *y16) {
     const int64_t row = blockIdx.y, n = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int id = ids[row];
     if (n >= N) return;
-    const float b0 = base[row * N + n];
+    float b0 = base[row * N + n];
+    for (int s = 1; s < splits; s++) b0 += base[s * base_stride + row * N + n];
     float s = 0.f;
     if (id >= 0 && id < count) {
         const AdapterDev d = ad[id];
@@ -332,11 +340,11 @@ hipError_t launch_lora_few_down(const uint16_t *x, int64_t lda, int64_t m, int64
 }
 
 hipError_t launch_lora_few_up(const float *t, int64_t ldt, int64_t m, int64_t n, const AdapterDev *ad, int count,
-                              const int32_t *ids, const float *base, float *y32, uint16_t *y16, hipStream_t stream) {
+                              const int32_t *ids, SplitSums base, float *y32, uint16_t *y16, hipStream_t stream) {
     if (m <= 0) return hipSuccess;
     if (m > MORE_ROWS) return hipErrorInvalidValue;
-    lora_up_row_kernel<<<dim3((unsigned)((n + 255) / 256), (unsigned)m), dim3(256), 0, stream>>>(t, ldt, n, ad, count, ids, base,
-                                                                                                y32, y16);
+    lora_up_row_kernel<<<dim3((unsigned)((n + 255) / 256), (unsigned)m), dim3(256), 0, stream>>>(t, ldt, n, ad, count, ids, base.part,
+                                                                                                base.splits, m * n, y32, y16);
     return hipGetLastError();
 }
 
@@ -396,7 +404,7 @@ hipError_t launch_lora_split(const float *part, LoraShares sh, int64_t m, int64_
 }
 
 hipError_t launch_lora_up(const float *part, LoraShares sh, int64_t m, int64_t row0, int64_t rows, int64_t n, const AdapterDev *ad,
-                          int count, const int32_t *ids, const float *base, float *y32, uint16_t *y16, hipStream_t stream) {
+                          int count, const int32_t *ids, SplitSums base, float *y32, uint16_t *y16, hipStream_t stream) {
     if (n % 128) return hipErrorInvalidValue;
     constexpr int64_t MOST = 16 * 65535;  // rows of one grid
     for (int64_t r = 0; r < rows; r += MOST) {
@@ -404,11 +412,11 @@ hipError_t launch_lora_up(const float *part, LoraShares sh, int64_t m, int64_t r
         const dim3 grid((unsigned)((n + 255) / 256), (unsigned)((some + 15) / 16));
         const float *p = part + (row0 + r) * sh.ldp;
         if (y32)
-            lora_up_kernel<3><<<grid, dim3(256), 0, stream>>>(p, sh.shares, m, sh.ldp, some, n, ad, count, ids + r, base + r * n,
-                                                             y32 + r * n, nullptr);
+            lora_up_kernel<3><<<grid, dim3(256), 0, stream>>>(p, sh.shares, m, sh.ldp, some, n, ad, count, ids + r, base.part + r * n,
+                                                             base.splits, rows * n, y32 + r * n, nullptr);
         else
-            lora_up_kernel<2><<<grid, dim3(256), 0, stream>>>(p, sh.shares, m, sh.ldp, some, n, ad, count, ids + r, base + r * n,
-                                                             nullptr, y16 + r * n);
+            lora_up_kernel<2><<<grid, dim3(256), 0, stream>>>(p, sh.shares, m, sh.ldp, some, n, ad, count, ids + r, base.part + r * n,
+                                                             base.splits, rows * n, nullptr, y16 + r * n);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
     return hipSuccess;

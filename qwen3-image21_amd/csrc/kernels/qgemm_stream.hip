@@ -1816,6 +1816,10 @@ hipError_t launch_qgemm_stream(const GemmWeight &w, const uint16_t *a, int64_t m
 hipError_t launch_split_epilogue(const float *part, int splits, int64_t m, int64_t N, int epi, const EpiParams &ep,
                                  hipStream_t stream) {
     if (splits < 1 || splits > MAX_SPLITS || N % 4 || m * N >= (int64_t)1 << 31) return hipErrorInvalidValue;
+    if (ep.left && epi == EPI_F32) {
+        *ep.left = {part, splits};
+        return hipSuccess;
+    }
     const int64_t quads = (epi == EPI_SWIGLU ? m * N / 2 : m * N) / 4;
     const dim3 grid((unsigned)((quads + 255) / 256)), block(256);
     switch (epi) {
