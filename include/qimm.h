@@ -199,7 +199,8 @@ int64_t qimm_adapters_device_bytes(const qimm_adapters *ad);
 /* y[m] = x[m] W^T + scale_a (x[m] A_a^T) B_a^T with a = ids[m], int32 [m] on the device;
  * an id outside [0, n) is a row without an adapter. The rest as qimm_qmatmul (the same
  * checks, the same products of W); sums are f32, y is rounded once. Rows of one adapter
- * next to each other are fastest: a tile of rows is multiplied once per adapter in it.
+ * next to each other are fastest from 65 rows on (257 of ranks up to 16; up to 32 with
+ * eight adapters or more): a tile of rows is multiplied once per adapter in it.
  * Scratch is the context's and grows like qimm_qmatmul's; after a
  * qimm_qmatmul_adapters_reserve with the call's weight, adapters, m and out_type it neither
  * allocates nor synchronizes and can be captured (as for a captured block forward, no later

@@ -26,8 +26,8 @@ size_t align_up(size_t v) { return (v + 255) & ~(size_t)255; }
 // How a product of m rows is taken: each row by itself beside the product's f32 sums (few); or
 // t of all rows first, then the rows before the product's tail and the tail, each as k steps of
 // the product over bf16 rows (steps) or with a pass over its f32 sums. The pass is for what runs
-// over the codes or split over K: its sums are in memory for the reduction anyway (4096 x 12288
-// Q4_K at 128 / 512 rows 51 / 77 us, 63 / 84 as steps), while 1024 x 12288 x 4096 takes 106 as
+// over the codes or split over K: its sums are in memory for the reduction anyway, and the pass adds
+// them (4096 x 12288 Q4_K at 512 rows 73 us, 84 as steps), while 1024 x 12288 x 4096 takes 106 as
 // steps and 121 with it. Only plain outputs have a tail; the others take the pass up to
 // PASS_ROWS rows at most where there are bf16 rows, which bounds its sums.
 // Offsets into the scratch: t16 of the steps (or t of the few), t's shares, the f32 sums.
