@@ -177,17 +177,22 @@ __global__ __launch_bounds__(256) void lora_split_kernel(const float *__restrict
 // y = base + t B^T for 16 rows x 256 columns, 64 columns per wave; t from the shares' sums,
 // in PARTS bf16 operands. A = B's rows, B = t's. base: the product's sums, `splits` of them
 // (base_stride apart) where it is split over K, added here in their order instead of in a
-// launch of their own (514 rows x 4096 x 4096 BF16, rank 16: 48 -> 45 us; 200 x 4096
-// x 4096 Q8_0 35 -> 32).
+// launch of their own (514 rows x 4096 x 4096 BF16, rank 16: 48 -> 45 us in all). Bound by the
+// bytes of base and y; the shares of t are read once per workgroup and go through LDS (each
+// wave's own reads of up to 16 shares took 17 us at 1024 x 4096, now 12.7: 42 MB).
 template <int PARTS>
 __global__ __launch_bounds__(256) void lora_up_kernel(const float *__restrict__ part, int shares, int64_t m, int64_t ldp,
                                                      int64_t rows, int64_t N, const AdapterDev *__restrict__ ad, int count,
                                                      const int32_t *__restrict__ ids, const float *base, int splits,
                                                      int64_t base_stride, float *y32, uint16_t *y16) {
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
-    const int64_t row = (int64_t)blockIdx.y * 16 + l16, n0 = (int64_t)blockIdx.x * 256 + 64 * wave;
-    if (n0 >= N) return;  // N is a multiple of 128
-    const int id = row_id(ids, row, rows, count);
+    // t of 32 ranks, each half of the workgroup the sum of every other share
+    constexpr int PITCH = 36;
+    __shared__ __attribute__((aligned(16))) float ts[2][16 * PITCH];
+    const int half = tid >> 7, trow = (tid & 127) >> 3, tq = 4 * (tid & 7);
+    const int64_t row0 = (int64_t)blockIdx.y * 16, row = row0 + l16;
+    const int64_t n1 = (int64_t)blockIdx.x * 256 + 64 * wave, n0 = n1 < N ? n1 : 0;  // N is a multiple of 128
+    const int id = row_id(ids, row, rows, count), tid_of = row_id(ids, row0 + trow, rows, count);
     f32x4 acc[4] = {}, base4[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) base4[i] = *(const f32x4 *)(base + min(row, rows - 1) * N + n0 + 16 * i + 4 * lg);
@@ -202,11 +207,14 @@ __global__ __launch_bounds__(256) void lora_up_kernel(const float *__restrict__ 
         const AdapterDev d = ad[a];
         for (int r0 = 0; r0 < d.rank; r0 += 32) {
             const int r = r0 + 8 * lg;
-            f32x4 u{}, v{};
-            if (id == a && r < d.rank) {
-                u = add_shares(part + row * ldp + r, shares, m * ldp);
-                if (r + 4 < d.rank) v = add_shares(part + row * ldp + r + 4, shares, m * ldp);
-            }
+            f32x4 t4{};
+            if (tid_of == a && r0 + tq < d.rank)
+                t4 = add_shares(part + half * (m * ldp) + (row0 + trow) * ldp + r0 + tq, (shares - half + 1) / 2, 2 * m * ldp);
+            __syncthreads();
+            *(f32x4 *)&ts[half][trow * PITCH + tq] = t4;
+            __syncthreads();
+            const float *t0 = &ts[0][l16 * PITCH + 8 * lg], *t1 = &ts[1][l16 * PITCH + 8 * lg];
+            f32x4 u = *(const f32x4 *)t0 + *(const f32x4 *)t1, v = *(const f32x4 *)(t0 + 4) + *(const f32x4 *)(t1 + 4);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 u[e] = r + e < d.rank ? u[e] * d.scale : 0.f;
@@ -230,7 +238,7 @@ __global__ __launch_bounds__(256) void lora_up_kernel(const float *__restrict__ 
             }
         }
     }
-    if (row >= rows) return;
+    if (row >= rows || n1 >= N) return;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int64_t at = row * N + n0 + 16 * i + 4 * lg;
