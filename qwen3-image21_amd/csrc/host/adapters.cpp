@@ -16,7 +16,9 @@ struct qimm_adapters {
     size_t bytes = 0;
     const qimm::AdapterDev *table() const { return (const qimm::AdapterDev *)dev; }
     const uint16_t *zeros() const { return (const uint16_t *)dev + bytes / 2 - 128; }
-    int64_t kt() const { return (max_rank + 63) / 64 * 64; }
+    // a part of t, and the k steps of 64 over its parts
+    int64_t width() const { return (max_rank + 7) / 8 * 8; }
+    int64_t steps(int parts) const { return (parts * width() + 63) / 64; }
 };
 
 namespace {
@@ -60,7 +62,7 @@ Route route_of(const qimm_weight *w, const qimm_adapters *ad, int64_t m, int64_t
             r.tiles = qimm::qgemm_bf16_plan(w->gw, m, false).head;
         }
         if (r.steps) pass = m - r.head;
-        r.shares = r.steps ? align_up((size_t)(m * r.parts * ad->kt()) * 2) : 0;
+        r.shares = r.steps ? align_up((size_t)(m * 64 * ad->steps(r.parts)) * 2) : 0;
         r.sums = r.shares + align_up(qimm::lora_down_scratch(m, w->cols, ad->max_rank));
     } else {
         r.sums = align_up((size_t)(m * ad->max_rank) * 4);
@@ -85,7 +87,7 @@ int reserve(qimm_ctx *ctx, const qimm_weight *w, int64_t m, const Route &r) {
 
 int run(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapters *ad, const int32_t *ids, const uint16_t *x, int64_t m,
         int64_t lda, int epi, const qimm::EpiParams &ep, const Route &r, char *ws, hipStream_t s) {
-    const int64_t K = w->cols, N = w->rows, kt = ad->kt();
+    const int64_t K = w->cols, N = w->rows, steps = ad->steps(r.parts);
     const qimm::AdapterDev *table = ad->table();
     const int n = (int)ad->count;
     float *shares = (float *)(ws + r.shares);
@@ -97,8 +99,8 @@ int run(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapters *ad, const int3
     int64_t row0 = 0;
     if (r.steps) {
         uint16_t *t16 = (uint16_t *)ws;
-        QIMM_HIP(ctx, qimm::launch_lora_split(shares, sh, m, kt, r.parts, table, n, ids, t16, s));
-        const qimm::AdapterSteps st{t16, (int)(kt / 64), (int)(kt / 64) * r.parts, table, n, ids, ad->zeros()};
+        QIMM_HIP(ctx, qimm::launch_lora_split(shares, sh, m, ad->width(), r.parts, table, n, ids, t16, 64 * steps, s));
+        const qimm::AdapterSteps st{t16, (int)ad->width(), (int)steps, table, n, ids, ad->zeros()};
         QIMM_HIP(ctx, qimm::launch_qgemm_bf16_adapters(w->gw, x, r.head, lda, epi, ep, r.tiles, st, s));
         row0 = r.head;
     }
@@ -208,7 +210,7 @@ size_t adapters_scratch(const qimm_weight *w, const qimm_adapters *ad, int64_t m
     const qimm::LoraShares one = qimm::lora_shares(m, w->cols, ad->max_rank);
     // t16; the shares, two workgroups of 128 rows per CU or one share; the sums
     const int64_t pass = qimm::qgemm_bf16_fits(w->gw) ? std::min(m, PASS_ROWS) : m;
-    return align_up((size_t)(m * 2 * ad->kt()) * 2) + align_up((size_t)(std::max(m, 2 * cus * 128) * one.ldp) * 4) +
+    return align_up((size_t)(m * 64 * ad->steps(2)) * 2) + align_up((size_t)(std::max(m, 2 * cus * 128) * one.ldp) * 4) +
            (size_t)(pass * w->rows) * 4;
 }
 

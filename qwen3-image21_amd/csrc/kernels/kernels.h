@@ -315,17 +315,18 @@ hipError_t launch_lora_down(const uint16_t *x, int64_t lda, int64_t m, int64_t k
 // y are the rows' own), to y32 (f32, may be base) when set, else bf16 to y16
 hipError_t launch_lora_up(const float *part, LoraShares sh, int64_t m, int64_t row0, int64_t rows, int64_t n, const AdapterDev *ad,
                           int count, const int32_t *ids, SplitSums base, float *y32, uint16_t *y16, hipStream_t stream);
-// t16[row][parts][kt] (kt the largest rank rounded up to 64) = t as a sum of bf16 numbers, each
-// the rounding of what the ones before leave: two parts keep 2^-16 of t, three 2^-24; zeros past
-// the adapter's rank; rows without one are not written.
-hipError_t launch_lora_split(const float *part, LoraShares sh, int64_t m, int64_t kt, int parts, const AdapterDev *ad, int count,
-                             const int32_t *ids, uint16_t *t16, hipStream_t stream);
+// t16[row][ld], the first parts * width of each row: t as a sum of bf16 numbers, each the rounding
+// of what the ones before leave (two parts keep 2^-16 of t, three 2^-24), width the largest rank
+// rounded up to 8; zeros past the adapter's rank and past the parts; rows without an adapter are
+// not written.
+hipError_t launch_lora_split(const float *part, LoraShares sh, int64_t m, int64_t width, int parts, const AdapterDev *ad, int count,
+                             const int32_t *ids, uint16_t *t16, int64_t ld, hipStream_t stream);
 // The product over bf16 rows with the adapters' second product as further k steps, in
 // launch_qgemm_bf16's epilogues without the rounding of the hidden state; `head` tiles of 256
 // tokens: epilogue(A W^T + t B^T).
 struct AdapterSteps {
-    const uint16_t *t;     // t16
-    int kb, steps;         // kt / 64; parts of them
+    const uint16_t *t;     // t16, rows of 64 * steps
+    int width, steps;      // of a part of t; of 64 over all parts
     const AdapterDev *ad;
     int count;
     const int32_t *ids;    // [m]

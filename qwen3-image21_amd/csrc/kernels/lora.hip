@@ -149,13 +149,16 @@ __device__ __forceinline__ uint32_t take_bf16x2(float &a, float &b) {
     return w;
 }
 
-// The shares' sums times the scale as PARTS bf16 rows of kt, zeros past the rank; four ranks per
-// thread. Rows without an adapter are not written.
+// The shares' sums times the scale as PARTS bf16 rows of `width` one after the other, zeros past
+// the rank and up to ld; four ranks per thread. Rows without an adapter are not written. One
+// after the other at the width of the ranks, not each from a step of 64 on: a tile of two
+// adapters of rank 16 takes two k steps instead of four.
 template <int PARTS>
 __global__ __launch_bounds__(256) void lora_split_kernel(const float *__restrict__ part, int shares, int64_t m, int64_t ldp,
                                                         int64_t rows, const AdapterDev *__restrict__ ad, int count,
-                                                        const int32_t *__restrict__ ids, uint16_t *__restrict__ t16, int64_t kt) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = kt / 4, row = i / per;
+                                                        const int32_t *__restrict__ ids, uint16_t *__restrict__ t16, int64_t width,
+                                                        int64_t ld) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = width / 4, row = i / per;
     if (row >= rows) return;
     const int id = row_id(ids, row, rows, count), r = (int)(i % per) * 4;
     if (id < 0) return;
@@ -165,13 +168,14 @@ __global__ __launch_bounds__(256) void lora_split_kernel(const float *__restrict
     if (r < rank) s = add_shares(part + row * ldp + r, shares, m * ldp);  // written up to the rank's tile of 16
 #pragma unroll
     for (int e = 0; e < 4; e++) s[e] = r + e < rank ? s[e] * scale : 0.f;
-    uint16_t *dst = t16 + row * PARTS * kt + r;
+    uint16_t *dst = t16 + row * ld + r;
 #pragma unroll
     for (int p = 0; p < PARTS; p++) {
         float a = s[0], b = s[1], c = s[2], d = s[3];
-        *(u32x2 *)(dst + p * kt) = u32x2{take_bf16x2(a, b), take_bf16x2(c, d)};
+        *(u32x2 *)(dst + p * width) = u32x2{take_bf16x2(a, b), take_bf16x2(c, d)};
         s = f32x4{a, b, c, d};
     }
+    for (int64_t e = PARTS * width; e + r < ld; e += width) *(u32x2 *)(dst + e) = u32x2{0, 0};
 }
 
 // y = base + t B^T for 16 rows x 256 columns, 64 columns per wave; t from the shares' sums,
@@ -392,20 +396,20 @@ hipError_t launch_lora_down(const uint16_t *x, int64_t lda, int64_t m, int64_t k
     return hipGetLastError();
 }
 
-hipError_t launch_lora_split(const float *part, LoraShares sh, int64_t m, int64_t kt, int parts, const AdapterDev *ad, int count,
-                             const int32_t *ids, uint16_t *t16, hipStream_t stream) {
+hipError_t launch_lora_split(const float *part, LoraShares sh, int64_t m, int64_t width, int parts, const AdapterDev *ad, int count,
+                             const int32_t *ids, uint16_t *t16, int64_t ld, hipStream_t stream) {
     if (m <= 0) return hipSuccess;
-    if (parts != 2 && parts != 3) return hipErrorInvalidValue;
+    if ((parts != 2 && parts != 3) || width % 8 || ld % 8 || ld < parts * width) return hipErrorInvalidValue;
     constexpr int64_t MOST = 1 << 20;  // rows of one grid (2^28 threads at rank 1024)
     for (int64_t r = 0; r < m; r += MOST) {
         const int64_t rows = std::min(m - r, MOST);
-        const dim3 grid((unsigned)((rows * (kt / 4) + 255) / 256));
+        const dim3 grid((unsigned)((rows * (width / 4) + 255) / 256));
         const float *p = part + r * sh.ldp;
-        uint16_t *t = t16 + r * parts * kt;
+        uint16_t *t = t16 + r * ld;
         if (parts == 2)
-            lora_split_kernel<2><<<grid, dim3(256), 0, stream>>>(p, sh.shares, m, sh.ldp, rows, ad, count, ids + r, t, kt);
+            lora_split_kernel<2><<<grid, dim3(256), 0, stream>>>(p, sh.shares, m, sh.ldp, rows, ad, count, ids + r, t, width, ld);
         else
-            lora_split_kernel<3><<<grid, dim3(256), 0, stream>>>(p, sh.shares, m, sh.ldp, rows, ad, count, ids + r, t, kt);
+            lora_split_kernel<3><<<grid, dim3(256), 0, stream>>>(p, sh.shares, m, sh.ldp, rows, ad, count, ids + r, t, width, ld);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
     return hipSuccess;

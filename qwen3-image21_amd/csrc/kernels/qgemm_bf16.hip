@@ -32,8 +32,6 @@
 // tokens against the 128x128 kernel 4096 x 4096 95 -> 62, 4096 x 12288 (Q6_K)
 // 313 -> 172; bf16 weights 12288 x 4096 at 2050 tokens against the four-wave
 // kernel of qgemm_large.hip 219 -> 191.
-#include <stddef.h>
-
 #include <algorithm>
 #include <type_traits>
 
@@ -85,8 +83,8 @@ struct Shape {
 // AD: the rows' low-rank adapters as further k steps, so that their product is summed in
 // the same accumulators and costs no pass over the outputs. For each adapter among the
 // tile's ids (in ascending order, the list in LDS) x.steps of them: the token operand is
-// x.t's row, the parts of t one after the other, a zero row for tokens of other adapters;
-// the weight operand the adapter's B rows, zeros past the rank. Measured, with one adapter of
+// x.t's row, the parts of t one after the other, zero for tokens of other adapters; the
+// weight operand the adapter's B rows once per part, zeros past the rank. Measured, with one adapter of
 // rank 64 / without: 4096 tokens x 4096 x 12288 295 / 287 us; 16384 x 12288 x 4096 with three of
 // rank 32 1253 / 1226 (and 377 for the pass).
 template <int EPI, bool SMALL, bool AD>
@@ -96,8 +94,12 @@ __global__ __launch_bounds__(64 * NWAVE, 1) void qgemm_bf16_kernel(const uint16_
     constexpr int WN = waves_n<EPI>();
     constexpr int LDS_BYTES = Shape<WN, 4>::LDS > (SMALL ? Shape<WN, 2>::LDS : 0) ? Shape<WN, 4>::LDS : Shape<WN, 2>::LDS;
     constexpr int LIST = AD ? Shape<WN, 4>::BM : 0;  // adapters of a tile, at most one per token
-    __shared__ __attribute__((aligned(16))) uint8_t lds[LDS_BYTES + 4 * LIST];
-    int *list = (int *)(lds + LDS_BYTES);
+    struct Entry {
+        const uint16_t *b;
+        int id, ldb;
+    };
+    __shared__ __attribute__((aligned(16))) uint8_t lds[LDS_BYTES + sizeof(Entry) * LIST];
+    Entry *list = (Entry *)(lds + LDS_BYTES);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nt = (int)(N / (128 * WN));
     // a split product (EPI_F32): share blockIdx.y of the k steps, its sums to
@@ -172,19 +174,10 @@ __global__ __launch_bounds__(64 * NWAVE, 1) void qgemm_bf16_kernel(const uint16_
                 for (int h = 0; h < NTP; h++) tid_of[h][i] = x.ids[m0 + min(r + h * RT, mlast)];
             }
         }
-        // the current adapter and its B, in scalar registers: no load of them may be pending in
-        // the loop, whose waits count the direct loads (with one, every phase waited for all of
-        // them: 4096 x 12288 at 4096 tokens 290 -> 690 us)
-        [[maybe_unused]] auto take = [&](int a) __attribute__((always_inline)) {
-            const u32x4 e = *(const u32x4 *)(x.ad + a), f = *((const u32x4 *)(x.ad + a) + 1);
-            static_assert(offsetof(AdapterDev, b) == 8 && offsetof(AdapterDev, ldb) == 20, "as read here");
-            ad_at = a;
-            b_at = (const uint16_t *)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)e[2]) |
-                                      (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)e[3]) << 32);
-            ldb_at = __builtin_amdgcn_readfirstlane((int)f[1]);
-        };
-        // AD, with the first loads in flight: every wave lists the tile's adapters (the smallest id
-        // above the last one, until none is left); the first one's B is looked up here, ahead of its steps
+        // AD, with the first loads in flight: every wave finds the tile's adapters (the smallest id
+        // above the last one, until none is left), the first one lists them with their B. No load
+        // from memory but the direct ones may be pending in the loop, whose waits count those
+        // (with one, every phase waited for all of them: 4096 x 12288 at 4096 tokens 290 -> 690 us)
         auto list_adapters = [&]() __attribute__((always_inline)) {
             if constexpr (AD) {
 #pragma unroll
@@ -197,12 +190,14 @@ __global__ __launch_bounds__(64 * NWAVE, 1) void qgemm_bf16_kernel(const uint16_
                     for (int o = 32; o > 0; o >>= 1) next = min(next, __shfl_xor(next, o));
                     at = __builtin_amdgcn_readfirstlane(next);
                     if (at == 0x7fffffff) break;
-                    if (slots == 0) {
-                        slot_at = 0;
-                        take(at);
-                    }
-                    if (wave == 0 && lane == 0) list[slots] = at;
+                    if (wave == 0 && lane == 0) list[slots].id = at;
                 }
+                if (wave == 0)
+                    for (int i = lane; i < slots; i += 64) {
+                        const AdapterDev &d = x.ad[list[i].id];
+                        list[i].b = d.b;
+                        list[i].ldb = d.ldb;
+                    }
                 KT = KB + slots * x.steps;
                 if (TT == 4) KT += KT & 1;  // steps come in pairs there: one of zeros
 #pragma unroll
@@ -220,10 +215,14 @@ __global__ __launch_bounds__(64 * NWAVE, 1) void qgemm_bf16_kernel(const uint16_
             const int slot = e / x.steps;
             if (slot != slot_at) {
                 slot_at = slot;
-                if (slot < slots)
-                    take(__builtin_amdgcn_readfirstlane(list[slot]));
-                else
-                    ad_at = -2;  // no row's
+                ad_at = -2;  // no row's
+                if (slot < slots) {  // in scalar registers
+                    const u32x4 e = *(const u32x4 *)(list + slot);
+                    b_at = (const uint16_t *)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)e[0]) |
+                                              (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)e[1]) << 32);
+                    ad_at = __builtin_amdgcn_readfirstlane((int)e[2]);
+                    ldb_at = __builtin_amdgcn_readfirstlane((int)e[3]);
+                }
             }
             return slot < slots ? e - slot * x.steps : 0;
         };
@@ -254,11 +253,12 @@ __global__ __launch_bounds__(64 * NWAVE, 1) void qgemm_bf16_kernel(const uint16_
             if constexpr (decltype(ext)::value || !AD) kt = min(kt, KT - 1);
             if constexpr (AD && decltype(ext)::value)
                 if (kt >= KB) {
-                    const int blk = adapter_of(kt - KB) % x.kb;
+                    const int e0 = 64 * adapter_of(kt - KB);
 #pragma unroll
                     for (int i = 0; i < WI; i++) {
                         const int q = WI * wave + i, r = q / 8 * 128 + q % 8 * 8 + h * 64;
-                        const int rl = r + (lane >> 3), c = 8 * ((lane & 7) ^ swz_key(rl)), rank = 64 * blk + c;
+                        const int rl = r + (lane >> 3), c = 8 * ((lane & 7) ^ swz_key(rl)), e = e0 + c;
+                        const int rank = e - (e >= x.width ? x.width : 0) - (e >= 2 * x.width ? x.width : 0);
                         const uint16_t *src = rank < ldb_at ? b_at + (n0 + rl) * ldb_at + rank : x.zero + c;
                         __builtin_amdgcn_global_load_lds((const void *)src, (lds_ptr_t)(lds + NS * TB + s * WB + r * ROWB),
                                                          16, 0, 0);
@@ -844,7 +844,8 @@ hipError_t launch_qgemm_bf16(const GemmWeight &w, const uint16_t *a, int64_t m, 
 
 hipError_t launch_qgemm_bf16_adapters(const GemmWeight &w, const uint16_t *a, int64_t m, int64_t lda, int epi,
                                       const EpiParams &ep, int64_t head, const AdapterSteps &x, hipStream_t stream) {
-    if (!qgemm_bf16_fits(w) || lda > ((int64_t)1 << 22) || head < 0 || x.kb < 1 || x.steps % x.kb) return hipErrorInvalidValue;
+    if (!qgemm_bf16_fits(w) || lda > ((int64_t)1 << 22) || head < 0 || x.width < 8 || x.width % 8 || x.steps < 1)
+        return hipErrorInvalidValue;
     switch (epi) {
     case EPI_F32: return launch_one<EPI_F32, true>(w, a, m, lda, ep, head, 1, stream, x);
     case EPI_BF16: return launch_one<EPI_BF16, true>(w, a, m, lda, ep, head, 1, stream, x);
