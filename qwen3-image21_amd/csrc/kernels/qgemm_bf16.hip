@@ -84,9 +84,10 @@ struct Shape {
 // the same accumulators and costs no pass over the outputs. For each adapter among the
 // tile's ids (in ascending order, the list in LDS) x.steps of them: the token operand is
 // x.t's row, the parts of t one after the other, zero for tokens of other adapters; the
-// weight operand the adapter's B rows once per part, zeros past the rank. Measured, with one adapter of
-// rank 64 / without: 4096 tokens x 4096 x 12288 295 / 287 us; 16384 x 12288 x 4096 with three of
-// rank 32 1253 / 1226 (and 377 for the pass).
+// weight operand the adapter's B rows once per part, zeros past the rank. Measured, the whole
+// call with t / without adapters: 4096 tokens x 4096 x 12288, one of rank 64, 302 / 266 us; 16384
+// x 12288 x 4096, three of rank 32, 1220 / 1163 (t and its split 32; a pass over the sums
+// instead 377).
 template <int EPI, bool SMALL, bool AD>
 __global__ __launch_bounds__(64 * NWAVE, 1) void qgemm_bf16_kernel(const uint16_t *__restrict__ A, int64_t M, int64_t lda,
                                                                  const uint16_t *__restrict__ W, int64_t N, int64_t K,
@@ -199,7 +200,6 @@ __global__ __launch_bounds__(64 * NWAVE, 1) void qgemm_bf16_kernel(const uint16_
                         list[i].ldb = d.ldb;
                     }
                 KT = KB + slots * x.steps;
-                if (TT == 4) KT += KT & 1;  // steps come in pairs there: one of zeros
 #pragma unroll
                 for (int i = 0; i < TI; i++)
 #pragma unroll
@@ -215,16 +215,13 @@ __global__ __launch_bounds__(64 * NWAVE, 1) void qgemm_bf16_kernel(const uint16_
             const int slot = e / x.steps;
             if (slot != slot_at) {
                 slot_at = slot;
-                ad_at = -2;  // no row's
-                if (slot < slots) {  // in scalar registers
-                    const u32x4 e = *(const u32x4 *)(list + slot);
-                    b_at = (const uint16_t *)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)e[0]) |
-                                              (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)e[1]) << 32);
-                    ad_at = __builtin_amdgcn_readfirstlane((int)e[2]);
-                    ldb_at = __builtin_amdgcn_readfirstlane((int)e[3]);
-                }
+                const u32x4 e = *(const u32x4 *)(list + slot);  // to scalar registers
+                b_at = (const uint16_t *)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)e[0]) |
+                                          (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)e[1]) << 32);
+                ad_at = __builtin_amdgcn_readfirstlane((int)e[2]);
+                ldb_at = __builtin_amdgcn_readfirstlane((int)e[3]);
             }
-            return slot < slots ? e - slot * x.steps : 0;
+            return e - slot * x.steps;
         };
         // EXT: the step may be past K
         auto dma_t = [&](auto ext, int s, int h, int kt) __attribute__((always_inline)) {
@@ -362,10 +359,12 @@ __global__ __launch_bounds__(64 * NWAVE, 1) void qgemm_bf16_kernel(const uint16_
                     step(K0{}, kt, std::integral_constant<int, 0>{});
                     step(K0{}, kt + 1, std::integral_constant<int, 1>{});
                 }
-            for (; kt < KT; kt += 2) {  // KT is even
+            for (; kt + 2 <= KT; kt += 2) {  // KT is even without adapters
                 step(EXT{}, kt, std::integral_constant<int, 0>{});
                 step(EXT{}, kt + 1, std::integral_constant<int, 1>{});
             }
+            if constexpr (AD)
+                if (kt < KT) step(EXT{}, kt, std::integral_constant<int, 0>{});
         } else {
             dma_t(K0{}, 0, 0, 0);
             dma_w(K0{}, 0, 0, 0);
