@@ -201,7 +201,8 @@ int64_t qimm_adapters_device_bytes(const qimm_adapters *ad);
  * checks, the same products of W); sums are f32, y is rounded once. Rows of one adapter
  * next to each other are fastest from 65 rows on (257 of ranks up to 16; up to 32 with
  * eight adapters or more): a tile of rows is multiplied once per adapter in it.
- * Scratch is the context's and grows like qimm_qmatmul's; after a
+ * Scratch is the context's and grows like qimm_qmatmul's, by t of every row and, for bf16
+ * outputs of weights without bf16 rows, f32 sums of at most 512 MiB (rows up to 2^19); after a
  * qimm_qmatmul_adapters_reserve with the call's weight, adapters, m and out_type it neither
  * allocates nor synchronizes and can be captured (as for a captured block forward, no later
  * call may grow the scratch: reserve every size first). ids and x may change between replays. */
@@ -398,7 +399,8 @@ int qimm_block_act_mode(const qimm_block *blk);
  * b [out, rank]: F32, F16 or BF16, kept as bf16) for the projections it has, data NULL for the
  * others; gate_up [2 mlp] as in qimm_block_tensors, or proj and gate_layer. They replace the
  * block's earlier ones (n = 0: none); on an error those stay. Ranks of q, k and v together, and
- * of proj and gate_layer, at most QIMM_ADAPTER_MAX_RANK. Sizes the scratch of later forwards:
+ * of proj and gate_layer, at most QIMM_ADAPTER_MAX_RANK. Sizes the scratch of later forwards (t of
+ * every token and f32 sums, at most 512 MiB of them at any batch):
  * call it before qimm_block_reserve, and not while a captured forward may still be replayed.
  * ids: int32 [batch] on the device, the adapter of each batch entry in every later forward of
  * the block (also by a model's forward or prefix fill), an id outside [0, n) none; read by the

@@ -31,12 +31,19 @@ size_t align_up(size_t v) { return (v + 255) & ~(size_t)255; }
 // over the codes or split over K: its sums are in memory for the reduction anyway, and the pass adds
 // them (4096 x 12288 Q4_K at 512 rows 73 us, 84 as steps), while 1024 x 12288 x 4096 takes 106 as
 // steps and 121 with it. Only plain outputs have a tail; the others take the pass up to
-// PASS_ROWS rows at most where there are bf16 rows, which bounds its sums.
+// PASS_ROWS rows at most where there are bf16 rows, which bounds its sums. Without bf16 rows every
+// row has the pass: its sums are held of part_rows rows at a time (PART_SUMS of them, 512 MiB, and
+// PART_ROWS rows at most, which fill the card at any width), one part after the other.
 // Offsets into the scratch: t16 of the steps (or t of the few), t's shares, the f32 sums.
 constexpr int64_t PASS_ROWS = 1024;
+constexpr int64_t PART_SUMS = (int64_t)1 << 27, PART_ROWS = 16384;
+int64_t part_rows(int64_t n, int64_t rows) {
+    return std::min(rows, std::max<int64_t>(256, std::min(PART_ROWS, PART_SUMS / n / 256 * 256)));
+}
 struct Route {
     bool few, steps;
     int64_t head, tiles;  // rows before the tail; their tiles of 256
+    int64_t part;         // rows of a part of the pass
     int parts;
     size_t shares, sums, total;
 };
@@ -67,7 +74,8 @@ Route route_of(const qimm_weight *w, const qimm_adapters *ad, int64_t m, int64_t
     } else {
         r.sums = align_up((size_t)(m * ad->max_rank) * 4);
     }
-    r.total = r.sums + (epi == qimm::EPI_F32 ? 0 : (size_t)(pass * w->rows) * 4);
+    r.part = epi == qimm::EPI_F32 ? pass : part_rows(w->rows, pass);  // f32 outputs take the sums themselves
+    r.total = r.sums + (epi == qimm::EPI_F32 ? 0 : (size_t)(r.part * w->rows) * 4);
     return r;
 }
 
@@ -81,7 +89,7 @@ int check_pair(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapters *ad) {
 
 int reserve(qimm_ctx *ctx, const qimm_weight *w, int64_t m, const Route &r) {
     if (const int rc = ensure_workspace(ctx, r.total)) return rc;
-    const size_t part = qimm::qgemm_workspace(w->gw, m);
+    const size_t part = adapters_part_workspace(w, m);
     return part ? ensure_part_workspace(ctx, part) : QIMM_OK;
 }
 
@@ -105,24 +113,29 @@ int run(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapters *ad, const int3
         row0 = r.head;
     }
     if (row0 == m) return QIMM_OK;
-    // the rest's f32 sums, to the output where that is f32, and the pass
-    float *sums = epi == qimm::EPI_F32 ? (float *)ep.out + row0 * N : (float *)(ws + r.sums);
-    float *y32 = epi == qimm::EPI_BF16 ? nullptr : sums;
-    uint16_t *y16 = epi == qimm::EPI_BF16 ? (uint16_t *)ep.out + row0 * N : nullptr;
-    qimm::EpiParams es{};
-    es.out = sums;
-    es.ldo = N;
-    es.part_ws = ep.part_ws;
-    es.part_ws_bytes = ep.part_ws_bytes;
-    qimm::SplitSums base{sums, 1};
-    if (!qimm::qgemm_route(w->gw, m - row0, lda, qimm::EPI_F32, es).tail) es.left = &base;
-    QIMM_HIP(ctx, qimm::launch_qgemm(w->gw, x + row0 * lda, m - row0, lda, qimm::EPI_F32, es, s));
-    if (r.few)
-        QIMM_HIP(ctx, qimm::launch_lora_few_up(shares, ad->max_rank, m, N, table, n, ids, base, y32, y16, s));
-    else
-        QIMM_HIP(ctx, qimm::launch_lora_up(shares, sh, m, row0, m - row0, N, table, n, ids + row0, base, y32, y16, s));
-    if (epi != qimm::EPI_F32 && epi != qimm::EPI_BF16)
-        QIMM_HIP(ctx, qimm::launch_split_epilogue(sums, 1, m, N, epi, ep, s));
+    // the rest's f32 sums, to the output where that is f32, and the pass: in parts of whole
+    // sequences, or of one that is longer, where the epilogue asks for a row's place in its own
+    const int64_t seq = epi == qimm::EPI_QKV ? ep.seq : epi == qimm::EPI_RESID ? ep.g_rows_per : 1;
+    for (int64_t at = row0, rows; at < m; at += rows) {
+        rows = std::min(seq <= r.part ? r.part / seq * seq : std::min(r.part, seq - at % seq), m - at);
+        float *sums = epi == qimm::EPI_F32 ? (float *)ep.out + at * N : (float *)(ws + r.sums);
+        float *y32 = epi == qimm::EPI_BF16 ? nullptr : sums;
+        uint16_t *y16 = epi == qimm::EPI_BF16 ? (uint16_t *)ep.out + at * N : nullptr;
+        qimm::EpiParams es{};
+        es.out = sums;
+        es.ldo = N;
+        es.part_ws = ep.part_ws;
+        es.part_ws_bytes = ep.part_ws_bytes;
+        qimm::SplitSums base{sums, 1};
+        if (!qimm::qgemm_route(w->gw, rows, lda, qimm::EPI_F32, es).tail) es.left = &base;
+        QIMM_HIP(ctx, qimm::launch_qgemm(w->gw, x + at * lda, rows, lda, qimm::EPI_F32, es, s));
+        if (r.few)
+            QIMM_HIP(ctx, qimm::launch_lora_few_up(shares, ad->max_rank, rows, N, table, n, ids, base, y32, y16, s));
+        else
+            QIMM_HIP(ctx, qimm::launch_lora_up(shares, sh, m, at, rows, N, table, n, ids + at, base, y32, y16, s));
+        if (epi != qimm::EPI_F32 && epi != qimm::EPI_BF16)
+            QIMM_HIP(ctx, qimm::launch_split_epilogue(sums, 1, rows, N, epi, qimm::rows_from(ep, epi, w->gw, at), s));
+    }
     return QIMM_OK;
 }
 
@@ -209,9 +222,16 @@ size_t adapters_scratch(const qimm_weight *w, const qimm_adapters *ad, int64_t m
     const int64_t cus = std::max(qimm::device_cu_count(), 1);
     const qimm::LoraShares one = qimm::lora_shares(m, w->cols, ad->max_rank);
     // t16; the shares, two workgroups of 128 rows per CU or one share; the sums
-    const int64_t pass = qimm::qgemm_bf16_fits(w->gw) ? std::min(m, PASS_ROWS) : m;
+    const int64_t pass = part_rows(w->rows, qimm::qgemm_bf16_fits(w->gw) ? std::min(m, PASS_ROWS) : m);
     return align_up((size_t)(m * 64 * ad->steps(2)) * 2) + align_up((size_t)(std::max(m, 2 * cus * 128) * one.ldp) * 4) +
            (size_t)(pass * w->rows) * 4;
+}
+
+size_t adapters_part_workspace(const qimm_weight *w, int64_t m) {
+    const size_t whole = qimm::qgemm_workspace(w->gw, m);
+    // a pass in parts, the last of any size
+    const int64_t part = part_rows(w->rows, m);
+    return part == m ? whole : std::max(whole, qimm::qgemm_workspace_up_to(w->gw, part));
 }
 
 int adapted_product(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapters *ad, const int32_t *ids, const uint16_t *x,
@@ -221,8 +241,6 @@ int adapted_product(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapters *ad
     qimm::EpiParams e = ep;
     e.hmid_q8k = e.hmid_q8_0 = 0;
     const Route r = route_of(w, ad, m, lda, epi);
-    if (!r.steps && m * w->rows >= (int64_t)1 << 31)
-        return set_err(ctx, QIMM_ERR_SHAPE, "adapters: too many tokens without the weight's bf16 rows");
     if (const int rc = run(ctx, w, ad, ids, x, m, lda, epi, e, r, ws, s)) return rc;
     if (rounding && !ep.hmid_round_later)
         QIMM_HIP(ctx, qimm::launch_quant_rows(ep.hmid_f32, ep.ldh, m, w->rows / 2, rounding, ep.hmid, ep.ldh, s));
@@ -287,7 +305,7 @@ int qimm_qmatmul_adapters(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapte
     qimm::EpiParams ep{};
     ep.out = y;
     ep.ldo = w->rows;
-    if (qimm::qgemm_workspace(w->gw, m)) {
+    if (adapters_part_workspace(w, m)) {
         ep.part_ws = (float *)ctx->ws_part;
         ep.part_ws_bytes = ctx->ws_part_bytes;
     }

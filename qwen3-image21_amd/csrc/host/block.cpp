@@ -289,13 +289,16 @@ WsLayout ws_layout(const qimm_block *blk, int64_t batch, int64_t seq, int64_t mo
     const std::pair<const qimm_weight *, const qimm_adapters *> adapted[] = {
         {blk->qkv, blk->ad_qkv}, {blk->q, blk->ad_q}, {blk->k, blk->ad_k}, {blk->v, blk->ad_v},
         {blk->out, blk->ad_out}, {blk->gate_up, blk->ad_gate_up}, {blk->down, blk->ad_down}};
+    L.part = 0;
     for (const auto &[w, ad] : adapted)
-        if (ad) lora = std::max(lora, adapters_scratch(w, ad, M));
+        if (ad) {
+            lora = std::max(lora, adapters_scratch(w, ad, M));
+            L.part = std::max(L.part, adapters_part_workspace(w, M));
+        }
     if (lora) off += align_up((size_t)M * 4);
     L.lora = off;
     off += align_up(lora);
     L.total = off;
-    L.part = 0;
     const qimm_weight *ws_list[] = {blk->qkv, blk->q, blk->k, blk->v, blk->out, blk->gate_up, blk->down};
     for (const qimm_weight *wt : ws_list)
         if (wt) L.part = std::max(L.part, qimm::qgemm_workspace(wt->gw, M));

@@ -124,6 +124,8 @@ int adapters_build(qimm_ctx *ctx, int64_t rows, int64_t cols, const std::vector<
 // launch_qgemm with the rows' adapters (ids int32 [m], device); ws: adapters_scratch bytes,
 // which serve any smaller m too; ep with its part_ws
 size_t adapters_scratch(const qimm_weight *w, const qimm_adapters *ad, int64_t m);
+// the split-K scratch of that product of m rows (the part_ws of its ep)
+size_t adapters_part_workspace(const qimm_weight *w, int64_t m);
 int adapted_product(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapters *ad, const int32_t *ids, const uint16_t *x,
                     int64_t m, int64_t lda, int epi, const qimm::EpiParams &ep, char *ws, hipStream_t s);
 

@@ -99,6 +99,9 @@ struct GemmWeight {
 // the decoding 256x256 kernels.
 hipError_t launch_qgemm(const GemmWeight &w, const uint16_t *a, int64_t m, int64_t lda,
                         int epi, const EpiParams &ep, hipStream_t stream);
+// The epilogue of rows head .. of a product as that of a product of its own; the rows share
+// one gate row (EPI_RESID) or lie in one sequence (EPI_QKV), or head starts one.
+EpiParams rows_from(const EpiParams &ep, int epi, const GemmWeight &w, int64_t head);
 // How launch_qgemm takes a product: the kernel (qimm_gemm_kernel's values), its shares
 // of K, the token tiles of 256 of the kernel over bf16 rows, the last rows that run as
 // a product of their own first (0: none), and whether the kernel rounds the SwiGLU
@@ -163,7 +166,8 @@ hipError_t launch_qgemm_bf16(const GemmWeight &w, const uint16_t *a, int64_t m, 
 // out [N][K] = the bf16 values of a quantized weight
 hipError_t launch_weight_rows_bf16(const GemmWeight &w, uint16_t *out, hipStream_t stream);
 // Sum of split-K partials part[splits][m][N] (f32) in split order, with the
-// epilogue epi applied (the second kernel of the split paths).
+// epilogue epi applied (the second kernel of the split paths). q/k/v: whole sequences, or
+// the first m rows of one.
 hipError_t launch_split_epilogue(const float *part, int splits, int64_t m, int64_t N, int epi, const EpiParams &ep,
                                  hipStream_t stream);
 // K split of the 128x128 kernel (64 < M < 512) when its tiles alone leave CUs

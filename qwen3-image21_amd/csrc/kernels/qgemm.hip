@@ -690,7 +690,8 @@ int64_t tail_rows(const GemmWeight &w, int64_t m, int epi, const EpiParams &ep) 
     return 0;
 }
 
-// The epilogue of rows head .. of a product as that of a product of its own
+}  // namespace
+
 EpiParams rows_from(const EpiParams &ep, int epi, const GemmWeight &w, int64_t head) {
     EpiParams e = ep;
     if (epi == EPI_F32 || epi == EPI_BF16) {
@@ -714,6 +715,8 @@ EpiParams rows_from(const EpiParams &ep, int epi, const GemmWeight &w, int64_t h
     }
     return e;
 }
+
+namespace {
 
 // A product over bf16 rows (plan p of bf16_plan): the tail after full rounds as a
 // product of its own where that is faster and its epilogue's rows can be shifted,

@@ -1639,6 +1639,7 @@ __global__ __launch_bounds__(256) void stream_epi_kernel(const float *__restrict
 // whole), writes the [B,H,S,D] copy directly and goes through an LDS tile
 // [d][token] for vt [B,H,D,S], whose rows then take 32 consecutive tokens per
 // store run instead of one 2-byte store per value.
+// The rows are whole sequences, or the first of one (S: its stride in the outputs).
 constexpr int VT_T = 32;  // tokens per v workgroup
 constexpr int VT_P = 33;  // bf16 pitch of the transpose tile rows: the 32 rows 4 c of one write go to distinct banks
 template <int HG>
@@ -1647,9 +1648,9 @@ __global__ __launch_bounds__(256) void stream_qkv_kernel(const float *__restrict
                                                          int64_t heads_v) {
     __shared__ uint16_t tile[128 * VT_P];
     const int64_t MN = M * N;
-    const int64_t S = ep.seq, H = ep.heads;
+    const int64_t S = ep.seq, H = ep.heads, rows = min(S, M);  // rows of a sequence here
     if ((int64_t)blockIdx.x >= nqk) {
-        const int64_t sblocks = (S + VT_T - 1) / VT_T;
+        const int64_t sblocks = (rows + VT_T - 1) / VT_T;
         int64_t L = (int64_t)blockIdx.x - nqk;
         const int64_t hv = L % heads_v;
         L /= heads_v;
@@ -1660,11 +1661,11 @@ __global__ __launch_bounds__(256) void stream_qkv_kernel(const float *__restrict
 #pragma unroll
         for (int r = 0; r < VT_T / 8; r++) {
             const int i = (tid >> 5) + 8 * r;  // token s0 + i, columns 4 c .. 4 c + 3
-            const int64_t s = min(s0 + i, S - 1);
-            const int64_t m = b * S + s;
+            const int64_t s = min(s0 + i, rows - 1);
+            const int64_t m = b * rows + s;
             const f32x4 v = csum4(part, splits, MN, m * N + col + 4 * c);
             const u32x2 pk{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-            if (ep.v_bhsd && s0 + i < S) *(u32x2 *)(ep.v_bhsd + ((b * H + head) * S + s) * 128 + 4 * c) = pk;
+            if (ep.v_bhsd && s0 + i < rows) *(u32x2 *)(ep.v_bhsd + ((b * H + head) * S + s) * 128 + 4 * c) = pk;
             tile[(4 * c) * VT_P + i] = (uint16_t)(pk[0] & 0xffffu);
             tile[(4 * c + 1) * VT_P + i] = (uint16_t)(pk[0] >> 16);
             tile[(4 * c + 2) * VT_P + i] = (uint16_t)(pk[1] & 0xffffu);
@@ -1673,7 +1674,7 @@ __global__ __launch_bounds__(256) void stream_qkv_kernel(const float *__restrict
         __syncthreads();
         // row d = tid / 2, tokens 16 (tid % 2) .. + 16 of the block
         const int d = tid >> 1, t0 = (VT_T / 2) * (tid & 1);
-        const int nt = (int)min((int64_t)(VT_T / 2), S - s0 - t0);
+        const int nt = (int)min((int64_t)(VT_T / 2), rows - s0 - t0);
         if (nt <= 0) return;
         uint16_t *dst = ep.vt + ((b * H + head) * 128 + d) * ep.vt_ld + s0 + t0;
         const uint16_t *src = tile + d * VT_P + t0;
@@ -1700,7 +1701,7 @@ __global__ __launch_bounds__(256) void stream_qkv_kernel(const float *__restrict
     const int sec = (int)(nb / ep.hidden);      // a group stays in one section (heads per section % HG == 0)
     if (sec >= 2) return;                       // v heads: the workgroups after nqk
     const int64_t head = (nb % ep.hidden) / 128;
-    const int64_t b = m / S, s = m % S;
+    const int64_t b = m / rows, s = m % rows;
     const float *nw = sec == 0 ? ep.norm_q : ep.norm_k;
     const float2 w2 = *(const float2 *)(nw + 2 * lane);
     const float2 cs2 = *(const float2 *)(ep.pe + s * 128 + 2 * lane);  // (cos, sin) of pair lane
@@ -1830,7 +1831,7 @@ hipError_t launch_split_epilogue(const float *part, int splits, int64_t m, int64
     case EPI_QKV: {
         // q / k heads one wave each, then the v heads (fused columns [2 hidden,
         // 3 hidden)) by (batch, 32 tokens, head)
-        if (ep.seq <= 0 || m % ep.seq) return hipErrorInvalidValue;
+        if (ep.seq <= 0 || (m > ep.seq && m % ep.seq)) return hipErrorInvalidValue;
         // heads per q / k wave: groups never straddle a section boundary
         const int64_t hps = ep.hidden / 128, off = ep.n_offset / 128, nh = N / 128;
         const int hg = (hps % 4 == 0 && off % 4 == 0 && nh % 4 == 0) ? 4 : (hps % 2 == 0 && off % 2 == 0 && nh % 2 == 0) ? 2 : 1;
@@ -1838,7 +1839,8 @@ hipError_t launch_split_epilogue(const float *part, int splits, int64_t m, int64
         const int64_t v0 = std::max<int64_t>(0, 2 * ep.hidden - ep.n_offset);
         const int64_t v1 = std::min<int64_t>(N, 3 * ep.hidden - ep.n_offset);
         const int64_t heads_v = v1 > v0 ? (v1 - v0) / 128 : 0;
-        const int64_t nv = heads_v * (m / ep.seq) * ((ep.seq + VT_T - 1) / VT_T);
+        const int64_t rows = std::min(ep.seq, m);
+        const int64_t nv = heads_v * (m / rows) * ((rows + VT_T - 1) / VT_T);
         const dim3 grid((unsigned)(nqk + nv));
         const int64_t hv = std::max<int64_t>(heads_v, 1);
         if (hg == 4) stream_qkv_kernel<4><<<grid, dim3(256), 0, stream>>>(part, splits, m, N, ep, nqk, v0, hv);
