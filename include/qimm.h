@@ -182,9 +182,9 @@ int qimm_qmatmul_route(int ggml_type, int64_t rows, int64_t cols, int bf16_rows,
  * batch of requests, each row of the product takes its own request's adapter, or none. A
  * qimm_adapters holds the adapters of one projection [rows, cols]: a [rank, cols] and b
  * [rows, rank], F32, F16 or BF16 in host memory, kept as bf16 (nearest even) on the device;
- * scale multiplies their product (alpha / rank of the usual files). Ranks may differ, 1 to
- * QIMM_ADAPTER_MAX_RANK; rows a multiple of 128, cols of 64; 1 to 65535 adapters. No
- * counterpart in the reference. */
+ * scale, a finite number, multiplies their product (alpha / rank of the usual files). Ranks
+ * may differ, 1 to QIMM_ADAPTER_MAX_RANK; rows a multiple of 128, cols of 64; 1 to 65535
+ * adapters. No counterpart in the reference. */
 typedef struct qimm_adapters qimm_adapters;
 #define QIMM_ADAPTER_MAX_RANK 1024
 typedef struct {
@@ -395,13 +395,13 @@ int qimm_block_set_act_mode(qimm_block *blk, int mode);
 int qimm_block_act_mode(const qimm_block *blk);
 
 /* Low-rank adapters of a block's projections, for batches whose entries belong to requests
- * with adapters of their own. list: n adapters, each with one scale and a pair (a [rank, in],
+ * with adapters of their own. list: n adapters, each with one finite scale and a pair (a [rank, in],
  * b [out, rank]: F32, F16 or BF16, kept as bf16) for the projections it has, data NULL for the
  * others; gate_up [2 mlp] as in qimm_block_tensors, or proj and gate_layer. They replace the
  * block's earlier ones (n = 0: none); on an error those stay. Ranks of q, k and v together, and
- * of proj and gate_layer, at most QIMM_ADAPTER_MAX_RANK. Sizes the scratch of later forwards (t of
- * every token and f32 sums, at most 512 MiB of them at any batch):
- * call it before qimm_block_reserve, and not while a captured forward may still be replayed.
+ * of proj and gate_layer, at most QIMM_ADAPTER_MAX_RANK. Sizes the scratch of later forwards (t
+ * of every token, and f32 sums of at most 512 MiB at any batch): call it before
+ * qimm_block_reserve, and not while a captured forward may still be replayed.
  * ids: int32 [batch] on the device, the adapter of each batch entry in every later forward of
  * the block (also by a model's forward or prefix fill), an id outside [0, n) none; read by the
  * forwards, so it must stay; NULL, the default: no adapters. Each projection becomes

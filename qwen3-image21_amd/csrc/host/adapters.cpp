@@ -2,6 +2,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <cmath>
 #include <new>
 #include <vector>
 
@@ -258,8 +259,10 @@ int qimm_adapters_create(qimm_ctx *ctx, int64_t rows, int64_t cols, const qimm_a
     if (rows <= 0 || rows % 128 || cols <= 0 || cols % 64 || rows >= (int64_t)1 << 31 || cols >= (int64_t)1 << 31)
         return set_err(ctx, QIMM_ERR_SHAPE, "adapters: needs rows % 128 == 0 and cols % 64 == 0");
     if (n < 1 || n > 65535) return set_err(ctx, QIMM_ERR_SHAPE, "adapters: 1 to 65535 of them");
-    for (int64_t i = 0; i < n; i++)
+    for (int64_t i = 0; i < n; i++) {
+        if (!std::isfinite(list[i].scale)) return set_err(ctx, QIMM_ERR_ARG, "adapters: a scale must be a finite number");
         if (const int rc = adapter_tensors(ctx, list[i].a, list[i].b, rows, cols)) return rc;
+    }
     try {
         std::vector<HostAdapter> all((size_t)n);
         for (int64_t i = 0; i < n; i++)

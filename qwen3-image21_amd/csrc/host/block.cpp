@@ -5,6 +5,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <cmath>
 #include <new>
 #include <utility>
 #include <vector>
@@ -534,6 +535,9 @@ int qimm_block_set_adapters(qimm_block *blk, const qimm_block_adapter *list, int
         std::vector<float> scale((size_t)n);
         for (int64_t i = 0; i < n; i++) {
             scale[(size_t)i] = list[i].scale;
+            // it would reach the projections that the adapter leaves alone: their zeros times it
+            if (!std::isfinite(list[i].scale))
+                return set_err(ctx, QIMM_ERR_ARG, "block adapters: a scale must be a finite number");
             if (list[i].gate_up.a.data && (list[i].proj.a.data || list[i].gate_layer.a.data))
                 return set_err(ctx, QIMM_ERR_ARG, "block adapters: gate_up, or proj and gate_layer");
         }
