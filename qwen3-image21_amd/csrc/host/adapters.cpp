@@ -34,12 +34,15 @@ size_t align_up(size_t v) { return (v + 255) & ~(size_t)255; }
 // steps and 121 with it. Only plain outputs have a tail; the others take the pass up to
 // PASS_ROWS rows at most where there are bf16 rows, which bounds its sums. Without bf16 rows every
 // row has the pass: its sums are held of part_rows rows at a time (PART_SUMS of them, 512 MiB, and
-// PART_ROWS rows at most, which fill the card at any width), one part after the other.
+// PART_ROWS rows at most, which fill the card at any width), one part after the other, of one size
+// (Q4_K 12288 x 4096 at 16384 rows: all at once 1835 us, 10752 and the rest 1900, two halves 1840).
 // Offsets into the scratch: t16 of the steps (or t of the few), t's shares, the f32 sums.
 constexpr int64_t PASS_ROWS = 1024;
 constexpr int64_t PART_SUMS = (int64_t)1 << 27, PART_ROWS = 16384;
+int64_t most_rows(int64_t n) { return std::max<int64_t>(256, std::min(PART_ROWS, PART_SUMS / n / 256 * 256)); }
 int64_t part_rows(int64_t n, int64_t rows) {
-    return std::min(rows, std::max<int64_t>(256, std::min(PART_ROWS, PART_SUMS / n / 256 * 256)));
+    const int64_t parts = (rows + most_rows(n) - 1) / most_rows(n);
+    return parts <= 1 ? rows : ((rows + parts - 1) / parts + 255) / 256 * 256;
 }
 struct Route {
     bool few, steps;
@@ -223,7 +226,7 @@ size_t adapters_scratch(const qimm_weight *w, const qimm_adapters *ad, int64_t m
     const int64_t cus = std::max(qimm::device_cu_count(), 1);
     const qimm::LoraShares one = qimm::lora_shares(m, w->cols, ad->max_rank);
     // t16; the shares, two workgroups of 128 rows per CU or one share; the sums
-    const int64_t pass = part_rows(w->rows, qimm::qgemm_bf16_fits(w->gw) ? std::min(m, PASS_ROWS) : m);
+    const int64_t pass = std::min(most_rows(w->rows), qimm::qgemm_bf16_fits(w->gw) ? std::min(m, PASS_ROWS) : m);
     return align_up((size_t)(m * 64 * ad->steps(2)) * 2) + align_up((size_t)(std::max(m, 2 * cus * 128) * one.ldp) * 4) +
            (size_t)(pass * w->rows) * 4;
 }
@@ -231,8 +234,8 @@ size_t adapters_scratch(const qimm_weight *w, const qimm_adapters *ad, int64_t m
 size_t adapters_part_workspace(const qimm_weight *w, int64_t m) {
     const size_t whole = qimm::qgemm_workspace(w->gw, m);
     // a pass in parts, the last of any size
-    const int64_t part = part_rows(w->rows, m);
-    return part == m ? whole : std::max(whole, qimm::qgemm_workspace_up_to(w->gw, part));
+    const int64_t most = most_rows(w->rows);
+    return m <= most ? whole : std::max(whole, qimm::qgemm_workspace_up_to(w->gw, most));
 }
 
 int adapted_product(qimm_ctx *ctx, const qimm_weight *w, const qimm_adapters *ad, const int32_t *ids, const uint16_t *x,

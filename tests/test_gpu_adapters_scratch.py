@@ -84,7 +84,8 @@ def test_products_in_parts(torch_cuda, codes_ctx, m, n, k, t, out_type):
     x = torch.randn(m, k, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).to(torch.bfloat16)
     ids = (np.arange(m) * 7 // m) % 3 - 1
     got = c.call(x, m, dev(torch, ids.astype(np.int32)), out_type)
-    at = np.unique(np.r_[0:3, 10750:10755, 16382:16387, 21503:21506, 32766:32770, m - 3:m, np.arange(0, m, 977)])
+    # around the parts' ends (8448 and 13568 rows each) and in between
+    at = np.unique(np.r_[0:3, 8446:8450, 13566:13570, 16894:16898, 25342:25346, 27134:27138, m - 3:m, np.arange(0, m, 977)])
     at = at[at < m]
     rows = torch.from_numpy(at).cuda()
     c.check(host(got[rows].float()), host(x[rows].float()), ids[at], out_type)
@@ -137,7 +138,7 @@ def test_a_forward_in_parts_equals_its_entries(torch_cuda, codes_ctx, b, s, grou
 
 @pytest.mark.parametrize("mod_rows", ["one", "each"])
 def test_a_sequence_longer_than_a_part(torch_cuda, codes_ctx, mod_rows):
-    """Every projection of one sequence of 20008 tokens in two parts, its second at position 16384."""
+    """Every projection of one sequence of 20008 tokens in two parts, the second from position 13568 on."""
     torch = torch_cuda
     b, s, hid, mlp = 2, 20008, SMALL["hidden"], SMALL["mlp"]
     x, mod, pe, _ = inputs(torch, b, s, hid, 3)
