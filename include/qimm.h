@@ -550,7 +550,8 @@ int qimm_model_forward(qimm_model *m, const float *latents, int64_t batch, int64
  * pieces: npieces (kind, start, len) triples in layout order, kind 0 = text
  * rows, 1 = condition rows (JointLayout::assemble, src/joint_layout.rs:112-126;
  * qimm_joint_layout_pieces); image_ids int32 [P] and key_valid uint8
- * [batch][P] (or NULL) on the device; pe [P, 128] f32. P = kv's prefix_len. */
+ * [batch][P] (or NULL) on the device; pe [P, 128] f32. P = kv's prefix_len; kv has
+ * the blocks' heads. */
 int qimm_model_prefix_fill(qimm_model *m, const float *txt, int64_t text_len, const float *cond, int64_t cond_len,
                            int64_t batch, const int64_t *pieces, int64_t npieces, const int32_t *image_ids,
                            const uint8_t *key_valid, const float *pe, qimm_kv *kv, void *stream);

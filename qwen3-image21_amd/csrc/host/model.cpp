@@ -222,6 +222,8 @@ int qimm_model_prefix_fill(qimm_model *m, const float *txt, int64_t text_len, co
     const int64_t hid = m->cfg.hidden, ch = m->cfg.in_channels, jd = m->cfg.joint_dim, P = kv->prefix;
     if (kv->batch != batch || kv->layers < m->cfg.layers)
         return set_err(ctx, QIMM_ERR_SHAPE, "prefix fill: cache batch or layer count differs");
+    if (m->cfg.layers > 0 && kv->heads * 128 != hid)
+        return set_err(ctx, QIMM_ERR_SHAPE, "prefix fill: cache heads differ from the blocks'");
     // without txt_in the prompt rows are used as they are (:368-371), so they are hidden wide
     const int64_t tw = jd ? jd : hid;  // prompt row width before txt_in
     int64_t total = 0;
