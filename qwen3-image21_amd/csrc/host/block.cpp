@@ -86,7 +86,9 @@ int64_t rows_up(int64_t i, int64_t) { return i / 64 * 128 + 64 + i % 64; }
 int64_t rows_gate_up(int64_t i, int64_t n) { return i < n / 2 ? rows_gate(i, n) : rows_up(i - n / 2, n); }
 
 // The adapters of one product: A stacked over the parts that an adapter has, B with each
-// part's columns in its rows; an adapter without any is one of zeros. Null if none has any.
+// part's columns in its rows and zeros elsewhere, which are multiplied like the rest (rank 64 of
+// q, k and v: 6 steps of 64 for each tile, of which 2 hold anything); an adapter without any part is
+// one of zeros. Null if none has any.
 int product_adapters(qimm_ctx *ctx, int64_t rows, int64_t cols, const std::vector<float> &scale,
                      const std::vector<std::vector<AdapterPart>> &list, qimm_adapters **out) {
     std::vector<HostAdapter> all(list.size());

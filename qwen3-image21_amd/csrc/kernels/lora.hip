@@ -323,12 +323,15 @@ __global__ __launch_bounds__(256) void repeat_ids_kernel(const int32_t *__restri
     if (i < rows) out[i] = ids[i / per];
 }
 
-// Each row is taken by itself up to 64 rows, and up to 256 where that costs a batch of one
-// adapter nothing or, with many adapters, little: the tiles' time grows with the adapters among
-// their rows, of which the host knows only the bound. Q8_0 4096 x 4096, us by tiles with one
-// adapter / one per row -> by rows with one / one per row: rank 16, 128 rows 32 / 304 -> 30 / 32,
-// 256 rows 39 / 312 -> 40 / 45; rank 64, 128 rows 40 / 438 -> 39 / 75 (Q4_K 12288 x 4096 65 / 482
-// -> 93 / 157), 256 rows 47 / 458 -> 58 / 127.
+// Each row is taken by itself up to 64 rows, and up to 256 of small ranks: the tiles' time grows with
+// the adapters among their rows, of which the host knows only how many are held. us, by tiles with one
+// adapter / one per row -> by rows, the same: Q8_0 4096 x 4096, rank 16, 64 rows 24 / 155 -> 22 / 22,
+// 128 rows 29 / 277 -> 27 / 27, 256 rows 32 / 284 -> 32 / 38; rank 64, 64 rows 27 / 229 -> 26 / 43, 128
+// rows 31 / 389 -> 34 / 92, 256 rows 36 / 435 -> 50 / 165. Q4_K 12288 x 4096, rank 64, 64 rows 32 / 235 ->
+// 50 / 127, 128 rows 45 / 453 -> 80 / 242, 256 rows 52 / 494 -> 123 / 453; rank 1024 (16 adapters), 16 rows
+// 77 / 993 -> 115 / 163, 64 rows 87 / 999 -> 425 / 1239. So it gives away: large ranks of one adapter at up
+// to 64 rows, 128 rows of one of eight or more adapters held, and, by tiles, more than 128 rows of rank 64
+// with an adapter each.
 constexpr int64_t FEW_ROWS = 64, MORE_ROWS = 256;
 
 }  // namespace
