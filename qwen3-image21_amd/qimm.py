@@ -457,6 +457,8 @@ class Block:
         for slot, (scale, pairs) in zip(arr, adapters):
             slot.scale = scale
             for name, (t, rows, cols, rank, a, b) in pairs.items():
+                if name not in BlockAdapter.PROJECTIONS:  # a name that ctypes does not know would be dropped
+                    raise QimmError(f"set_adapters: no projection {name!r} in a block")
                 setattr(slot, name, AdapterPair(make_tensor(t, rank, cols, a, keep), make_tensor(t, rows, rank, b, keep)))
         self.ctx.check(self.ctx.lib.qimm_block_set_adapters(self.h, C.byref(arr), len(adapters)), "qimm_block_set_adapters")
 
