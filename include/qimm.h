@@ -292,6 +292,90 @@ int qimm_kv_create_q4(qimm_ctx *ctx, int64_t layers, int64_t batch, int64_t head
 int qimm_kv_bits(const qimm_kv *kv);
 int64_t qimm_kv_device_bytes(const qimm_kv *kv);
 
+/* ---------------- paged K/V cache ---------------- */
+
+/* For batches of requests of unequal lengths that come and go, where qimm_kv would pad every
+ * one to the longest: the cache is `pages` pages of page_size tokens, and a request holds those
+ * that its row of a block table names. Page tables, lengths and the queue of free pages are the
+ * caller's device arrays (int32); qimm_page_plan makes a step's out of the requests' lengths,
+ * qimm_pages_store writes the step's keys and values, qimm_attention_paged reads them.
+ * No counterpart in the reference. */
+
+/* One step of the page tables. Request r has lengths[r] tokens, in the pages tables[r * max_pages]
+ * ..., and adds added[r] of them (0: none this step), or gives its pages back (added[r] < 0).
+ * The rows of a step are the new tokens of all requests, one request after the other: request r's are
+ * starts[r] .. starts[r + 1] - 1. Its new pages come from the queue in order, requests in theirs,
+ * and are written to its table. A row's slot is page * page_size + position % page_size, its position
+ * the number of tokens before it in the request (the row of a RoPE table). Rows from starts[requests] to max_rows
+ * get slot -1 and position 0, so that a captured step may have a fixed number of rows.
+ * The queue is a ring of `pages` entries, state[0] the entry of the next free page and state[1]
+ * their number; pages given back go to its end, free from the next step on.
+ * A request is refused, and has its length left, its rows slot -1 and position 0, where its table or the
+ * rows have no room for it, its length is negative, or it needs pages and, with the pages that it and
+ * the requests before it ask for, more than are free. state_out: the two, the rows, the requests refused.
+ * lengths_out and state_out may be lengths and state; everything else is distinct. work:
+ * qimm_page_plan_work(requests) int32 of scratch; positions may be NULL. Entries of a table past a
+ * request's pages, and of the queue outside its free pages, are not looked at. Allocates nothing and
+ * can be captured. page_size: a multiple of 16 up to 512; up to 65536 requests; pages * page_size
+ * below 2^31. */
+typedef struct {
+    int64_t page_size, pages;
+    int64_t requests, max_pages, max_rows;
+    int32_t *tables;          /* [requests][max_pages] */
+    const int32_t *lengths;   /* [requests] */
+    const int32_t *added;     /* [requests] */
+    int32_t *queue;           /* [pages] */
+    const int32_t *state;     /* [2] */
+    int32_t *lengths_out;     /* [requests] */
+    int32_t *state_out;       /* [4] */
+    int32_t *starts;          /* [requests + 1] */
+    int32_t *slots;           /* [max_rows] */
+    int32_t *positions;       /* [max_rows] */
+    int32_t *work;
+} qimm_page_plan_args;
+int qimm_page_plan(qimm_ctx *ctx, const qimm_page_plan_args *p, void *stream);
+int64_t qimm_page_plan_work(int64_t requests);
+
+/* The pages of `layers` layers, bf16, in a layout of the library's own; head_dim 64 or 128. */
+typedef struct qimm_pages qimm_pages;
+int qimm_pages_create(qimm_ctx *ctx, int64_t layers, int64_t pages, int64_t page_size, int64_t kv_heads,
+                      int64_t head_dim, qimm_pages **out);
+int qimm_pages_destroy(qimm_pages *pg);
+int64_t qimm_pages_device_bytes(const qimm_pages *pg);
+/* Keys and values of `rows` rows, [kv_heads][head_dim] each, to their slots of a layer: F32, F16 or
+ * BF16, rounded to bf16 (nearest even). k_row, k_head, v_row, v_head: elements from one row, one head
+ * to the next (0: dense rows); k, v and the strides 16-byte aligned. A row whose slot is
+ * outside the pages is left out; of rows with the same slot one is stored, in parts maybe. */
+int qimm_pages_store(qimm_pages *pg, int64_t layer, const void *k, const void *v, int type, int64_t rows,
+                     int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, const int32_t *slots, void *stream);
+/* The rows of slots back, dense [rows][kv_heads][head_dim] bf16; zeros where a slot is outside the pages. */
+int qimm_pages_load(const qimm_pages *pg, int64_t layer, uint16_t *k, uint16_t *v, int64_t rows,
+                    const int32_t *slots, void *stream);
+
+/* Attention of a step's rows, q [rows][heads][head_dim] bf16 with element strides q_row, q_head (0:
+ * dense), over the pages of their requests; out [rows][heads * head_dim] bf16. Query heads h G .. h G
+ * + G - 1 share key head h, G = heads / kv_heads. lengths: the requests' tokens with this step's
+ * (qimm_page_plan's lengths_out); starts as qimm_page_plan's, or NULL where row r is request r's one.
+ * Row i of a request's n rows is its token p = length - n + i. It sees every key of its request, or
+ * (causal) keys j <= p; in a window (> 0) of them j > p - window, and the first `sinks` keys,
+ * j < sinks. A row that sees no key (p < 0) gives zeros; rows of no request are left as they were.
+ * What keys hold that a row does not see does not count, NaN and infinities either. A table entry
+ * outside the pages hides its keys. scale: positive. Rows of a refused request are of no use. q, its
+ * strides and out are 16-byte aligned; up to 65536 requests. Allocates nothing and can be captured. */
+typedef struct {
+    const uint16_t *q;
+    int64_t q_row, q_head;
+    int64_t rows, heads, requests, max_pages;
+    const int32_t *tables;    /* [requests][max_pages] */
+    const int32_t *lengths;   /* [requests] */
+    const int32_t *starts;    /* [requests + 1] or NULL */
+    int causal;
+    int64_t window, sinks;
+    float scale;
+    uint16_t *out;
+} qimm_paged_attention;
+int qimm_attention_paged(qimm_pages *pg, int64_t layer, const qimm_paged_attention *a, void *stream);
+
 /* ---------------- attention ---------------- */
 
 /* Per-head RmsNorm (eps 1e-6, weight norm_w[128] device f32) then RoPE with

@@ -361,6 +361,44 @@ hipError_t launch_attn4(const uint16_t *q, const uint8_t *tiles, int64_t p, cons
                         int64_t so, const uint8_t *kvalid, int64_t b, int64_t h, int64_t sq, float scale, float *scratch,
                         uint16_t *out, hipStream_t stream);
 
+// ---- the paged prefix cache (pages.hip, paged_attn.hip; the layout is in paged.h) ----
+struct PageDims {
+    int64_t pages;
+    int page_size, kv_heads, head_dim;
+    int64_t layer_bytes() const { return pages * page_size * kv_heads * head_dim * 4; }
+};
+// qimm_page_plan's arrays (device); work: page_plan_work(requests) int32.
+struct PagePlanArgs {
+    int64_t pages, requests, max_pages, max_rows;
+    int page_size;
+    int32_t *tables;
+    const int32_t *lengths, *added;
+    int32_t *queue;
+    const int32_t *state;
+    int32_t *lengths_out, *state_out, *starts, *slots, *positions, *work;
+};
+inline int64_t page_plan_work(int64_t requests) { return 4 * requests + 4; }
+hipError_t launch_page_plan(const PagePlanArgs &p, hipStream_t stream);
+// k and v, rows of `type` (F32, F16, BF16) with element strides (row, head), to the slots of a layer;
+// and back as dense bf16 [rows][kv_heads][head_dim], zeros where a row has no slot.
+hipError_t launch_pages_store(const PageDims &d, uint8_t *layer, const void *k, const void *v, int type, int64_t k_row,
+                              int64_t k_head, int64_t v_row, int64_t v_head, const int32_t *slots, int64_t rows,
+                              hipStream_t stream);
+hipError_t launch_pages_load(const PageDims &d, const uint8_t *layer, uint16_t *k, uint16_t *v, const int32_t *slots,
+                             int64_t rows, hipStream_t stream);
+struct PagedAttnArgs {
+    const uint16_t *q;  // element strides q_row, q_head
+    int64_t q_row, q_head, rows, heads;
+    const int32_t *tables;  // [requests][max_pages]
+    int64_t requests, max_pages;
+    const int32_t *lengths, *starts;  // starts may be null: row r is request r's
+    int causal;
+    int64_t window, sinks;
+    float scale;
+    uint16_t *out;  // [rows][heads * head_dim]
+};
+hipError_t launch_paged_attention(const PageDims &d, const uint8_t *layer, const PagedAttnArgs &a, hipStream_t stream);
+
 // ---- the denoising step around the blocks (step.hip), all f32 ----
 enum : int { ACT_NONE = 0, ACT_SILU = 1, ACT_GELU_TANH = 2 };
 // y[m][n] (row stride ldy) = act(sum_k x[m][k] * w[n][k]); x row stride ldx, w [n][k] dense.

@@ -1,0 +1,413 @@
+// Attention over the paged K/V cache (paged.h), gfx950: the rows of a step, any number per request,
+// over their requests' pages.
+//
+// O = softmax(scale Q K^T) V. Row i of a request's n, of which `len` tokens are in the cache, stands at
+// p = len - n + i and sees the keys j <= p (causal) or j < len; in a window of W only j > p - W, and
+// j < sinks. One pass over the keys with the running maximum and sum; f32 scores, sums and output,
+// rounded to bf16 once; probabilities are rounded to bf16 (2^-9 each) as the operand of P V.
+//
+// The query heads of one key head share its keys: a tile is 32 of a request's (row, head of
+// the group) pairs, in row order. Each wave computes S^T = K Q^T with v_mfma_f32_32x32x16_bf16, so a
+// lane owns one pair and its maximum and sum need one lane more.
+//
+// Few pairs are bound by the cache's bytes: HBM gives a CU about 9 B a clock, 16 KB of a 32-key
+// tile of 128 dims take it 1900 clocks, its 16 matrix instructions a SIMD 512 and the softmax about as
+// many, so the columns of a tile that are empty cost nothing. Four waves take tiles of 32 keys in
+// turn straight into registers (two operands of 8 KB in flight each: no LDS, no barrier) and join their
+// sums through LDS.
+#include <algorithm>
+
+#include "device_common.h"
+#include "paged.h"
+
+namespace qimm {
+namespace {
+
+constexpr int KT = 32;  // keys of a wave's tile
+
+struct Attn {
+    const uint16_t *q;
+    int64_t q_row, q_head;
+    const uint8_t *cache;  // the layer
+    int64_t pages;
+    const int32_t *tables;
+    int64_t max_pages;
+    const int32_t *lengths, *starts;
+    int32_t R, T;          // requests, rows
+    int32_t Hkv, G;        // key heads, query heads of each
+    int32_t ps16;          // granules of a page
+    uint32_t ps16_magic;   // ceil(2^32 / ps16): x / ps16 = x magic >> 32 for x < 2^27, ps16 <= 32
+    int32_t cap;           // keys that a table row has room for
+    int32_t causal, window, sinks;  // window 0: none
+    float sl2;             // scale * log2 e
+    uint16_t *out;
+};
+
+// a request's rows and tokens
+struct Req {
+    int start, n, len;
+};
+__device__ __forceinline__ Req req_of(const Attn &a, int r) {
+    const int s = a.starts ? min(max(a.starts[r], 0), a.T) : r;
+    const int e = a.starts ? min(max(a.starts[r + 1], s), a.T) : min(r + 1, a.T);
+    return {s, e - s, min(max(a.lengths[r], 0), a.cap)};
+}
+
+// The keys that some pair of tile `tile` (TM pairs) sees: first .. [0, sk) and lo .. hi - 1, as tiles of
+// `keys`: ns of the first ones, then from w0 on; pos0, pos1: the positions of its first and last row.
+struct Range {
+    int pos0, pos1, lo, hi, sk, ns, w0, tiles;
+};
+template <int TM, int KEYS>
+__device__ __forceinline__ Range range_of(const Attn &a, const Req &q, int tile) {
+    Range g;
+    const int i0 = tile * TM / a.G, i1 = min(q.n - 1, (tile * TM + TM - 1) / a.G);
+    g.pos0 = a.causal ? q.len - q.n + i0 : q.len - 1;
+    g.pos1 = a.causal ? q.len - q.n + i1 : q.len - 1;
+    g.hi = max(g.pos1 + 1, 0);
+    g.lo = a.window ? max(g.pos0 - a.window + 1, 0) : 0;
+    g.sk = a.window ? min(a.sinks, g.hi) : 0;
+    g.ns = (g.sk + KEYS - 1) / KEYS;
+    g.w0 = g.lo / KEYS;
+    if (g.w0 <= g.ns) g.ns = g.w0 = 0;
+    g.tiles = g.ns + (g.hi + KEYS - 1) / KEYS - g.w0;
+    return g;
+}
+__device__ __forceinline__ int tile_at(const Range &g, int v) { return v < g.ns ? v : v - g.ns + g.w0; }
+
+// What a workgroup takes: tile `tile` of request r's pairs for key head h.
+struct Piece {
+    int r, h, tile;
+};
+
+// exclusive sums over 256 threads
+__device__ __forceinline__ int scan256(int v, int *part, int &total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int s = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(s, o);
+        if (lane >= o) s += x;
+    }
+    __syncthreads();
+    if (lane == 63) part[wave] = s;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        if (w < wave) before += part[w];
+        total += part[w];
+    }
+    return before + s - v;
+}
+
+// The piece of workgroup `item`, in request order (tiles before heads); false: there is none. Every
+// thread counts the pieces of its share of the requests, the one whose share has it looks which.
+template <int TM>
+__device__ __forceinline__ bool piece_of(const Attn &a, int item, Piece &out) {
+    __shared__ int part[4], found[3];
+    const int c = (a.R + 255) / 256, r0 = min((int)threadIdx.x * c, a.R), r1 = min(r0 + c, a.R);
+    auto items = [&](int r) __attribute__((always_inline)) { return (req_of(a, r).n * a.G + TM - 1) / TM * a.Hkv; };
+    int mine = 0, total;
+    for (int r = r0; r < r1; r++) mine += items(r);
+    int at = scan256(mine, part, total);
+    if (item >= total) return false;
+    if (item >= at && item < at + mine) {
+        int r = r0;
+        for (;; r++) {
+            const int n = items(r);
+            if (item < at + n) break;
+            at += n;
+        }
+        found[0] = r;
+        found[1] = (item - at) % a.Hkv;
+        found[2] = (item - at) / a.Hkv;
+    }
+    __syncthreads();
+    out = {found[0], found[1], found[2]};
+    return true;
+}
+
+__device__ __forceinline__ bool not_finite2(uint32_t w) {
+    return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+}
+
+// The values of a 32-key tile that are no numbers, taken out of it (v: an A operand per granule and 32
+// dims) and added to the sums o of those pairs whose probability of the key is not 0. p: the tile's
+// probabilities as B operands; through `lds`, 128 (32 + D / 2) B of the wave's own.
+template <int D>
+__device__ __forceinline__ void add_not_finite(u32x4 (&v)[2][D / 32], const uint32_t (&p)[8], f32x16 (&o)[D / 32], uint8_t *lds, int lane) {
+    const int l32 = lane & 31, hi = lane >> 5;
+    float *pl = (float *)lds;                    // [key][pair]
+    uint16_t *vl = (uint16_t *)(lds + 4096);     // [key][dim]
+    uint32_t keys = 0;
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const int key = 16 * j + 8 * (w >> 1) + 4 * hi + 2 * (w & 1);
+            pl[key * 32 + l32] = __uint_as_float(p[4 * j + w] << 16);
+            pl[(key + 1) * 32 + l32] = __uint_as_float(p[4 * j + w] & 0xffff0000u);
+#pragma unroll
+            for (int dt = 0; dt < D / 32; dt++) {
+                const uint32_t x = v[j][dt][w];
+                vl[key * D + 32 * dt + l32] = (uint16_t)x;
+                vl[(key + 1) * D + 32 * dt + l32] = (uint16_t)(x >> 16);
+                const bool a = (x & 0x7f80u) == 0x7f80u, b = (x & 0x7f800000u) == 0x7f800000u;
+                keys |= (a ? 1u << key : 0u) | (b ? 2u << key : 0u);
+                v[j][dt][w] = x & ((a ? 0u : 0xffffu) | (b ? 0u : 0xffff0000u));
+            }
+        }
+#pragma unroll
+    for (int i = 32; i > 0; i >>= 1) keys |= (uint32_t)__shfl_xor((int)keys, i);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll 1
+    for (keys = __builtin_amdgcn_readfirstlane(keys); keys; keys &= keys - 1) {
+        const int key = __builtin_ctz(keys);
+        const bool sees = pl[key * 32 + l32] > 0.f;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; dt++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const u32x2 x = *(const u32x2 *)(vl + key * D + 32 * dt + 8 * e + 4 * hi);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t u = i & 1 ? x[i >> 1] & 0xffff0000u : x[i >> 1] << 16;
+                    if (sees && (u & 0x7f800000u) == 0x7f800000u) o[dt][4 * e + i] += __uint_as_float(u);
+                }
+            }
+    }
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <int D>
+__global__ __launch_bounds__(256, 2) void paged_attn_kernel(const Attn a) {
+    constexpr int KK = D / 16, DT = D / 32, PITCH = D + 4;
+    __shared__ __attribute__((aligned(16))) float so[4 * 32 * PITCH];
+    __shared__ float sm[4][32], sl[4][32];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int l32 = lane & 31, hi = lane >> 5;
+
+    Piece pc;
+    if (!piece_of<32>(a, blockIdx.x, pc)) return;
+    const int r = __builtin_amdgcn_readfirstlane(pc.r), h = __builtin_amdgcn_readfirstlane(pc.h);
+    const int tile = __builtin_amdgcn_readfirstlane(pc.tile);
+    const Req rq = req_of(a, r);
+    const Range g = range_of<32, KT>(a, rq, tile);
+
+    // the lane's pair: row i of the request, head h G + hd
+    const int f = tile * 32 + l32, row = f / a.G, hd = f - row * a.G;
+    const bool there = row < rq.n;
+    const int pos = !there ? -1 : a.causal ? rq.len - rq.n + row : rq.len - 1;
+    const int low = a.window ? pos - a.window : -1;  // sees key j <= pos if j > low or j < g.sk
+    const int low0 = a.window ? g.pos0 - a.window : -1;
+    const int pmin = tile * 32 + 31 < rq.n * a.G ? g.pos0 : -1;  // every pair sees up to it
+
+    // ---- queries: dims 16 kk + 8 hi .. + 7 of the lane's pair ----
+    bf16x8 qf[KK];
+    {
+        const uint16_t *src = a.q + (int64_t)(rq.start + (there ? row : 0)) * a.q_row + (int64_t)(h * a.G + (there ? hd : 0)) * a.q_head + 8 * hi;
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) {
+            u32x4 v = *(const u32x4 *)(src + 16 * kk);
+            if (!there) v = u32x4{};
+            qf[kk] = __builtin_bit_cast(bf16x8, v);
+        }
+    }
+
+    // ---- the granules of the wave's next 32 tiles, lane 2 k + j: granule j of tile k (-1: no page) ----
+    const int32_t *table = a.tables + (int64_t)r * a.max_pages;
+    int gran = 0;
+    auto load_granules = [&](int v) __attribute__((always_inline)) {
+        const int mine = v + (lane >> 1) * 4;
+        gran = -1;
+        if (mine < g.tiles) {
+            const uint32_t x = 2 * tile_at(g, mine) + (lane & 1);
+            const uint32_t k = __umulhi(x, a.ps16_magic) + (a.ps16 == 1 ? x : 0);
+            if ((int64_t)k < a.max_pages) {
+                const int page = table[k];
+                if (page >= 0 && page < a.pages) gran = (page * a.Hkv + h) * a.ps16 + (int)(x - k * a.ps16);
+            }
+        }
+    };
+    u32x4 kc[KK], vc[2][DT];
+    auto base_of = [&](int gn) __attribute__((always_inline)) { return a.cache + (int64_t)max(gn, 0) * granule_bytes(D); };
+    auto load_k = [&](int g0, int g1) __attribute__((always_inline)) {
+        const uint8_t *p = (l32 < 16 ? base_of(g0) : base_of(g1)) + hi * 256 + (l32 & 15) * 16;
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) kc[kk] = *(const u32x4 *)(p + kk * 512);
+    };
+    auto load_v = [&](int g0, int g1) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const uint8_t *p = base_of(j ? g1 : g0) + D * 32 + hi * (D * 16) + l32 * 16;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) vc[j][dt] = *(const u32x4 *)(p + dt * 512);
+        }
+    };
+
+    f32x16 o[DT] = {};
+    float m = -INFINITY, l = 0.f;
+    int g0 = -1, g1 = -1, n0 = -1, n1 = -1, k = 0;
+    int v = wave;
+    if (v < g.tiles) {
+        load_granules(v);
+        g0 = __builtin_amdgcn_readlane(gran, 0);
+        g1 = __builtin_amdgcn_readlane(gran, 1);
+        load_k(g0, g1);
+        load_v(g0, g1);
+    }
+    for (; v < g.tiles; v += 4) {
+        const int key0 = tile_at(g, v) * KT;
+        f32x16 s = {};
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++)
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kc[kk]), qf[kk], s, 0, 0, 0);
+        const bool more = v + 4 < g.tiles;
+        if (more) {
+            if (++k == 32) {
+                k = 0;
+                load_granules(v + 4);
+            }
+            n0 = __builtin_amdgcn_readlane(gran, 2 * k);
+            n1 = __builtin_amdgcn_readlane(gran, 2 * k + 1);
+            load_k(n0, n1);
+        }
+
+        // every pair of the tile sees all of it, or some do not
+        const bool some = !(key0 + KT - 1 <= pmin && (g0 | g1) >= 0 &&
+                            (a.window == 0 || key0 > g.pos1 - a.window || key0 + KT <= g.sk));
+        if (some) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int key = key0 + 8 * (e >> 2) + 4 * hi + (e & 3);
+                const bool ok = key <= pos && (key > low || key < g.sk) && (e < 8 ? g0 : g1) >= 0;
+                s[e] = ok ? s[e] : -INFINITY;
+            }
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int e = 1; e < 16; e++) mx = fmaxf(mx, s[e]);
+        mx = fmaxf(fmaxf(mx, __shfl_xor(mx, 32)), m);
+        if (__ballot(mx > m)) {
+            // a pair without a visible key so far has sums of 0
+            const float al = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - mx) * a.sl2);
+            m = mx;
+            l *= al;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[dt][e] *= al;
+        }
+        const float c = mx == -INFINITY ? 0.f : -mx * a.sl2;
+        float sum = 0.f;
+        uint32_t p[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * e], a.sl2, c));
+            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * e + 1], a.sl2, c));
+            sum += x;
+            sum += y;
+            p[e] = pack_bf16x2(x, y);
+        }
+        l += sum;
+
+        bf16x8 pf[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) pf[j] = __builtin_bit_cast(bf16x8, u32x4{p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]});
+        // what a key holds that no pair sees does not count, a NaN or an infinity either (0 times them
+        // is NaN); where only some pairs see one, it goes to those by itself
+        if (some) {
+            bool odd = false;
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    const int key = key0 + 16 * j + 8 * (w >> 1) + 4 * hi + 2 * (w & 1);
+                    uint32_t seen = (key <= g.pos1 && (key > low0 || key < g.sk) ? 0xffffu : 0u) |
+                                    (key + 1 <= g.pos1 && (key + 1 > low0 || key + 1 < g.sk) ? 0xffff0000u : 0u);
+                    if ((j ? g1 : g0) < 0) seen = 0;
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++) {
+                        vc[j][dt][w] &= seen;
+                        odd = odd || not_finite2(vc[j][dt][w]);
+                    }
+                }
+            }
+            if (g.pos0 != g.pos1 && __ballot(odd)) add_not_finite<D>(vc, p, o, (uint8_t *)(so + wave * 32 * PITCH), lane);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vc[j][dt]), pf[j], o[dt], 0, 0, 0);
+        if (more) load_v(n0, n1);
+        g0 = n0;
+        g1 = n1;
+    }
+
+    // ---- the four waves' sums ----
+    l += __shfl_xor(l, 32);
+    if (hi == 0) {
+        sm[wave][l32] = m;
+        sl[wave][l32] = l;
+    }
+    float *mine = so + (wave * 32 + l32) * PITCH + 4 * hi;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            *(f32x4 *)(mine + 32 * dt + 8 * e) = f32x4{o[dt][4 * e], o[dt][4 * e + 1], o[dt][4 * e + 2], o[dt][4 * e + 3]};
+    __syncthreads();
+    const int pr = tid / 8, pf = tile * 32 + pr;  // eight threads a pair
+    if (pf >= rq.n * a.G) return;
+    const int prow = pf / a.G, phd = pf - prow * a.G;
+    const float mm = fmaxf(fmaxf(sm[0][pr], sm[1][pr]), fmaxf(sm[2][pr], sm[3][pr]));
+    float ll = 0.f, fac[4];
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        fac[w] = sm[w][pr] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((sm[w][pr] - mm) * a.sl2);
+        ll += sl[w][pr] * fac[w];
+    }
+    const float inv = ll == 0.f ? 0.f : 1.0f / ll;  // a pair that sees no key gives zeros
+    uint16_t *dst = a.out + ((int64_t)(rq.start + prow) * a.Hkv * a.G + h * a.G + phd) * D;
+#pragma unroll
+    for (int e = 0; e < D / 32; e++) {
+        const int d = (tid & 7) * 4 + 32 * e;
+        f32x4 x{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const f32x4 y = *(const f32x4 *)(so + (w * 32 + pr) * PITCH + d);
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] += y[i] * fac[w];
+        }
+        *(u32x2 *)(dst + d) = u32x2{pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv)};
+    }
+}
+
+}  // namespace
+
+hipError_t launch_paged_attention(const PageDims &d, const uint8_t *layer, const PagedAttnArgs &x, hipStream_t stream) {
+    if (x.rows <= 0 || x.requests <= 0) return hipSuccess;
+    const int64_t g = x.heads / d.kv_heads, cap = std::min<int64_t>(x.max_pages * d.page_size, 0x7fffffff - 64);
+    const int ps16 = d.page_size / 16;
+    const Attn a{x.q, x.q_row, x.q_head, layer, d.pages, x.tables, x.max_pages, x.lengths, x.starts, (int32_t)x.requests,
+                 (int32_t)x.rows, d.kv_heads, (int32_t)g, ps16, (uint32_t)(((1ull << 32) + ps16 - 1) / ps16),
+                 (int32_t)cap, x.causal, (int32_t)std::min<int64_t>(x.window, 0x7fffffff),
+                 (int32_t)std::min<int64_t>(x.sinks, 0x7fffffff), x.scale * 1.4426950408889634f, x.out};
+    // at most one tile more than the pairs fill for each request
+    const int64_t most = (x.rows * g / 32 + x.requests) * d.kv_heads;
+    if (most >= (int64_t)1 << 24) return hipErrorInvalidValue;
+    if (d.head_dim == 128)
+        paged_attn_kernel<128><<<(unsigned)most, 256, 0, stream>>>(a);
+    else if (d.head_dim == 64)
+        paged_attn_kernel<64><<<(unsigned)most, 256, 0, stream>>>(a);
+    else
+        return hipErrorInvalidValue;
+    return hipGetLastError();
+}
+
+}  // namespace qimm

@@ -69,6 +69,14 @@ SIGNATURES = [
     ("qimm_kv_bits", _i32, [_vp]),
     ("qimm_kv_device_bytes", _i64, [_vp]),
     ("qimm_kv_prefetch", _i32, [_vp, _i64, _vp]),
+    ("qimm_page_plan", _i32, [_vp, _vp, _vp]),
+    ("qimm_page_plan_work", _i64, [_i64]),
+    ("qimm_pages_create", _i32, [_vp, _i64, _i64, _i64, _i64, _i64, C.POINTER(_vp)]),
+    ("qimm_pages_destroy", _i32, [_vp]),
+    ("qimm_pages_device_bytes", _i64, [_vp]),
+    ("qimm_pages_store", _i32, [_vp, _i64, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _vp]),
+    ("qimm_pages_load", _i32, [_vp, _i64, _vp, _vp, _i64, _vp, _vp]),
+    ("qimm_attention_paged", _i32, [_vp, _i64, _vp, _vp]),
     ("qimm_qk_norm_rope", _i32, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
     ("qimm_v_transpose", _i32, [_vp, _vp, _i64, _i64, _i64, _vp, _vp]),
     ("qimm_attention", _i32, [_vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _f32, _vp, _vp]),
@@ -160,6 +168,20 @@ class AttnMask(C.Structure):
     _fields_ = [("image_ids", _vp), ("key_valid", _vp)]
 
 
+class PagePlan(C.Structure):
+    """qimm_page_plan_args: one step of the page tables; arrays are device addresses (int32)."""
+    _fields_ = [("page_size", _i64), ("pages", _i64), ("requests", _i64), ("max_pages", _i64), ("max_rows", _i64),
+                ("tables", _vp), ("lengths", _vp), ("added", _vp), ("queue", _vp), ("state", _vp), ("lengths_out", _vp),
+                ("state_out", _vp), ("starts", _vp), ("slots", _vp), ("positions", _vp), ("work", _vp)]
+
+
+class PagedAttention(C.Structure):
+    """qimm_paged_attention: a step's rows over the pages of their requests (device addresses)."""
+    _fields_ = [("q", _vp), ("q_row", _i64), ("q_head", _i64), ("rows", _i64), ("heads", _i64), ("requests", _i64),
+                ("max_pages", _i64), ("tables", _vp), ("lengths", _vp), ("starts", _vp), ("causal", _i32),
+                ("window", _i64), ("sinks", _i64), ("scale", _f32), ("out", _vp)]
+
+
 class GgufTensorInfo(C.Structure):
     """qimm_gguf_tensor_info."""
     _fields_ = [("name", C.c_char_p), ("ggml_type", _i32), ("n_dims", C.c_int32), ("ne", _i64 * 4),
@@ -218,6 +240,14 @@ def qmatmul_route(ggml_type: int, rows: int, cols: int, m: int, cus: int, bf16_r
     if rc:
         raise QimmError(f"qimm_qmatmul_route: {status_name(rc)}", rc)
     return r
+
+
+def page_plan_work(requests: int) -> int:
+    """int32 values of a page plan's work array (qimm_page_plan_work)."""
+    n = int(load().qimm_page_plan_work(requests))
+    if n < 0:
+        raise QimmError(f"qimm_page_plan_work({requests})", 2)
+    return n
 
 
 class Context:
@@ -348,6 +378,18 @@ class Context:
                    "qimm_kv_create_q4")
         return KvCache(self, h, layers, batch, heads, prefix_len)
 
+    # -- paged cache --
+    def page_plan(self, plan: PagePlan, stream: int = 0):
+        """The page tables, slots and row offsets of a step from the requests' lengths (qimm_page_plan)."""
+        self.check(self.lib.qimm_page_plan(self.h, C.byref(plan), stream), "qimm_page_plan")
+
+    def pages_create(self, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int = 128) -> "Pages":
+        """A paged K/V cache for requests of unequal lengths (qimm_pages_create)."""
+        h = C.c_void_p()
+        self.check(self.lib.qimm_pages_create(self.h, layers, pages, page_size, kv_heads, head_dim, C.byref(h)),
+                   "qimm_pages_create")
+        return Pages(self, h, layers, pages, page_size, kv_heads, head_dim)
+
     # -- attention --
     def qk_norm_rope(self, x_dev, batch, seq, heads, norm_w_dev, pe_dev, out_dev, stream=0):
         self.check(self.lib.qimm_qk_norm_rope(self.h, x_dev, batch, seq, heads, norm_w_dev, pe_dev, out_dev,
@@ -432,6 +474,35 @@ class KvCache:
     def free(self):
         if self.h:
             self.ctx.lib.qimm_kv_destroy(self.h)
+            self.h = None
+
+
+class Pages:
+    """A paged K/V cache (qimm_pages)."""
+
+    def __init__(self, ctx, h, layers, pages, page_size, kv_heads, head_dim):
+        self.ctx, self.h = ctx, h
+        self.layers, self.pages, self.page_size, self.kv_heads, self.head_dim = layers, pages, page_size, kv_heads, head_dim
+
+    def store(self, layer, k_dev, v_dev, row_type, rows, slots_dev, k_row=0, k_head=0, v_row=0, v_head=0, stream=0):
+        """Rows of F32, F16 or BF16 keys and values to their slots; element strides, 0 for dense rows."""
+        self.ctx.check(self.ctx.lib.qimm_pages_store(self.h, layer, k_dev, v_dev, row_type, rows, k_row, k_head, v_row,
+                                                     v_head, slots_dev, stream), "qimm_pages_store")
+
+    def load(self, layer, k_dev, v_dev, rows, slots_dev, stream=0):
+        self.ctx.check(self.ctx.lib.qimm_pages_load(self.h, layer, k_dev, v_dev, rows, slots_dev, stream),
+                       "qimm_pages_load")
+
+    def attention(self, layer, call: PagedAttention, stream=0):
+        """A step's rows over the pages of their requests (qimm_attention_paged)."""
+        self.ctx.check(self.ctx.lib.qimm_attention_paged(self.h, layer, C.byref(call), stream), "qimm_attention_paged")
+
+    def device_bytes(self) -> int:
+        return int(self.ctx.lib.qimm_pages_device_bytes(self.h))
+
+    def free(self):
+        if self.h:
+            self.ctx.lib.qimm_pages_destroy(self.h)
             self.h = None
 
 
