@@ -12,8 +12,10 @@ struct qimm_pages {
     int64_t layers = 0;
     qimm::PageDims dims{};
     uint8_t *mem = nullptr;
+    void *scratch = nullptr;  // of the attention: its shares' sums
     uint8_t *layer(int64_t i) const { return mem + i * dims.layer_bytes(); }
-    int64_t bytes() const { return layers * dims.layer_bytes(); }
+    int64_t cache_bytes() const { return layers * dims.layer_bytes(); }
+    int64_t scratch_bytes() const { return (int64_t)qimm::paged_attention_scratch(dims.head_dim); }
 };
 
 namespace {
@@ -78,8 +80,14 @@ int qimm_pages_create(qimm_ctx *ctx, int64_t layers, int64_t pages, int64_t page
         return set_err(ctx, QIMM_ERR_OOM, "pages: too large");
     }
     hipError_t e = hipSetDevice(ctx->device);
-    if (e == hipSuccess) e = hipMalloc((void **)&pg->mem, (size_t)pg->bytes());
+    if (e == hipSuccess) e = hipMalloc((void **)&pg->mem, (size_t)pg->cache_bytes());
+    if (e == hipSuccess) e = hipMalloc(&pg->scratch, (size_t)pg->scratch_bytes());
+    // the null stream does not order a later call on a non-blocking stream: wait for the fill
+    if (e == hipSuccess) e = hipMemset(pg->scratch, 0, qimm::PAGED_COUNTER_BYTES);
+    if (e == hipSuccess) e = hipDeviceSynchronize();
     if (e != hipSuccess) {
+        if (pg->mem) (void)hipFree(pg->mem);
+        if (pg->scratch) (void)hipFree(pg->scratch);
         delete pg;
         return hip_err(ctx, e, "hipMalloc(pages)");
     }
@@ -90,11 +98,12 @@ int qimm_pages_create(qimm_ctx *ctx, int64_t layers, int64_t pages, int64_t page
 int qimm_pages_destroy(qimm_pages *pg) {
     if (!pg) return QIMM_ERR_ARG;
     if (pg->mem) (void)hipFree(pg->mem);
+    if (pg->scratch) (void)hipFree(pg->scratch);
     delete pg;
     return QIMM_OK;
 }
 
-int64_t qimm_pages_device_bytes(const qimm_pages *pg) { return pg ? pg->bytes() : -1; }
+int64_t qimm_pages_device_bytes(const qimm_pages *pg) { return pg ? pg->cache_bytes() + pg->scratch_bytes() : -1; }
 
 int qimm_pages_store(qimm_pages *pg, int64_t layer, const void *k, const void *v, int type, int64_t rows, int64_t k_row,
                      int64_t k_head, int64_t v_row, int64_t v_head, const int32_t *slots, void *stream) {
@@ -152,7 +161,7 @@ int qimm_attention_paged(qimm_pages *pg, int64_t layer, const qimm_paged_attenti
     const qimm::PagedAttnArgs a{x->q, x->q_row ? x->q_row : x->heads * d, x->q_head ? x->q_head : d, x->rows, x->heads,
                                 x->tables, x->requests, x->max_pages, x->lengths, x->starts, x->causal, x->window,
                                 x->sinks, x->scale, x->out};
-    QIMM_HIP(ctx, qimm::launch_paged_attention(pg->dims, pg->layer(layer), a, (hipStream_t)stream));
+    QIMM_HIP(ctx, qimm::launch_paged_attention(pg->dims, pg->layer(layer), a, pg->scratch, (hipStream_t)stream));
     return QIMM_OK;
 }
 

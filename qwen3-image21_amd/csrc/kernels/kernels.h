@@ -397,7 +397,12 @@ struct PagedAttnArgs {
     float scale;
     uint16_t *out;  // [rows][heads * head_dim]
 };
-hipError_t launch_paged_attention(const PageDims &d, const uint8_t *layer, const PagedAttnArgs &a, hipStream_t stream);
+// scratch: paged_attention_scratch bytes, of which the first PAGED_COUNTER_BYTES are zero before the
+// first call; every call leaves them zero
+size_t paged_attention_scratch(int head_dim);
+constexpr size_t PAGED_COUNTER_BYTES = 8192;
+hipError_t launch_paged_attention(const PageDims &d, const uint8_t *layer, const PagedAttnArgs &a, void *scratch,
+                                  hipStream_t stream);
 
 // ---- the denoising step around the blocks (step.hip), all f32 ----
 enum : int { ACT_NONE = 0, ACT_SILU = 1, ACT_GELU_TANH = 2 };

@@ -15,6 +15,11 @@
 // many, so the columns of a tile that are empty cost nothing. Four waves take tiles of 32 keys in
 // turn straight into registers (two operands of 8 KB in flight each: no LDS, no barrier) and join their
 // sums through LDS.
+//
+// Long requests in few workgroups are split over their keys. The host does not know the lengths, so
+// every workgroup counts the rounds of 128 keys of all requests, which gives the rounds of a share and
+// with that which share of which request it is itself: two sums over the requests, one load each up
+// to 256 of them. The shares' sums go through memory; the last one to arrive joins them, in order.
 #include <algorithm>
 
 #include "device_common.h"
@@ -23,7 +28,13 @@
 namespace qimm {
 namespace {
 
-constexpr int KT = 32;  // keys of a wave's tile
+constexpr int KT = 32;      // keys of a wave's tile
+constexpr int ROUND = 128;  // keys of a workgroup's four tiles
+// Shares: as many as make WANT workgroups of all requests, at least GRAIN rounds each, at most MOST of a
+// tile; a request is split in at most twice its part of WANT.
+constexpr int WANT = 1024, GRAIN = 4, MOST = 128;
+constexpr int SLOTS = 2 * WANT;
+static_assert(SLOTS * 4 <= PAGED_COUNTER_BYTES, "a counter per slot");
 
 struct Attn {
     const uint16_t *q;
@@ -41,6 +52,8 @@ struct Attn {
     int32_t causal, window, sinks;  // window 0: none
     float sl2;             // scale * log2 e
     uint16_t *out;
+    uint32_t *count;       // arrivals, zero between calls; null: no request is long enough to be split
+    float *part;           // per slot O [TM][D], then (m, l) [TM]
 };
 
 // a request's rows and tokens
@@ -75,24 +88,33 @@ __device__ __forceinline__ Range range_of(const Attn &a, const Req &q, int tile)
 }
 __device__ __forceinline__ int tile_at(const Range &g, int v) { return v < g.ns ? v : v - g.ns + g.w0; }
 
-// What a workgroup takes: tile `tile` of request r's pairs for key head h.
+// Rounds of the keys that any tile of a request sees, at most.
+template <int TM>
+__device__ __forceinline__ int rounds_of(const Attn &a, const Req &q) {
+    int64_t keys = q.len;
+    if (a.window) keys = min(keys, (int64_t)a.sinks + a.window + TM / a.G + 3 * KT);
+    return (int)((keys + ROUND - 1) / ROUND);
+}
+
+// What a workgroup takes: share `share` of `shares` of tile `tile` of request r's pairs for key head h; slot:
+// the tile's first of the shares' slots.
 struct Piece {
-    int r, h, tile;
+    int r, h, tile, share, shares, slot;
 };
 
-// exclusive sums over 256 threads
-__device__ __forceinline__ int scan256(int v, int *part, int &total) {
+// sums over 256 threads: those before this one
+__device__ __forceinline__ int64_t scan256(int64_t v, int64_t *part, int64_t &total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int s = v;
+    int64_t s = v;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const int x = __shfl_up(s, o);
+        const int64_t x = __shfl_up(s, o);
         if (lane >= o) s += x;
     }
     __syncthreads();
     if (lane == 63) part[wave] = s;
     __syncthreads();
-    int before = 0;
+    int64_t before = 0;
     total = 0;
 #pragma unroll
     for (int w = 0; w < 4; w++) {
@@ -102,35 +124,178 @@ __device__ __forceinline__ int scan256(int v, int *part, int &total) {
     return before + s - v;
 }
 
-// The piece of workgroup `item`, in request order (tiles before heads); false: there is none. Every
-// thread counts the pieces of its share of the requests, the one whose share has it looks which.
+// The piece of workgroup `item`, in request order (the last tiles first: under causal rows they see the
+// most keys; heads fastest); false: there is none. Every thread counts its share of the requests, and the one
+// whose share has the piece looks which.
 template <int TM>
 __device__ __forceinline__ bool piece_of(const Attn &a, int item, Piece &out) {
-    __shared__ int part[4], found[3];
+    __shared__ int64_t part[4];
+    __shared__ Piece found;
     const int c = (a.R + 255) / 256, r0 = min((int)threadIdx.x * c, a.R), r1 = min(r0 + c, a.R);
-    auto items = [&](int r) __attribute__((always_inline)) { return (req_of(a, r).n * a.G + TM - 1) / TM * a.Hkv; };
-    int mine = 0, total;
-    for (int r = r0; r < r1; r++) mine += items(r);
-    int at = scan256(mine, part, total);
-    if (item >= total) return false;
-    if (item >= at && item < at + mine) {
+    int64_t chunk = 0, all;
+    if (a.count) {
+        int64_t rounds = 0;
+        for (int r = r0; r < r1; r++) {
+            const Req q = req_of(a, r);
+            rounds += (int64_t)((q.n * a.G + TM - 1) / TM) * rounds_of<TM>(a, q);
+        }
+        scan256(rounds, part, all);
+        chunk = max((int64_t)GRAIN, (all * a.Hkv + WANT - 1) / WANT);
+    }
+    // tiles and shares of request r; its pieces in the low bits of the sums, the slots of a split one above
+    auto split = [&](int r, int &tiles, int &shares) __attribute__((always_inline)) {
+        const Req q = req_of(a, r);
+        tiles = (q.n * a.G + TM - 1) / TM;
+        shares = 1;
+        if (chunk && tiles) shares = max((int)min((rounds_of<TM>(a, q) + chunk - 1) / chunk, (int64_t)MOST), 1);
+    };
+    constexpr int HIGH = 44;
+    constexpr int64_t LOW = ((int64_t)1 << HIGH) - 1;
+    auto pieces = [&](int tiles, int shares) __attribute__((always_inline)) {
+        const int64_t n = min((int64_t)tiles * shares * a.Hkv, (int64_t)1 << 27);
+        return n + (shares > 1 ? n << HIGH : 0);
+    };
+    int64_t mine, at;
+    int tiles, shares;
+    for (;;) {
+        mine = 0;
+        for (int r = r0; r < r1; r++) {
+            split(r, tiles, shares);
+            mine += pieces(tiles, shares);
+        }
+        at = scan256(mine, part, all);
+        // more than there can be: `starts` that overlap. Every share has to arrive, so nothing is split.
+        if (!chunk || ((all & LOW) <= gridDim.x && (all >> HIGH) <= SLOTS)) break;
+        chunk = 0;
+    }
+    if (item >= (all & LOW)) return false;
+    if (item >= (at & LOW) && item < (at & LOW) + (mine & LOW)) {
         int r = r0;
         for (;; r++) {
-            const int n = items(r);
-            if (item < at + n) break;
+            split(r, tiles, shares);
+            const int64_t n = pieces(tiles, shares);
+            if (item < ((at + n) & LOW)) break;
             at += n;
         }
-        found[0] = r;
-        found[1] = (item - at) % a.Hkv;
-        found[2] = (item - at) / a.Hkv;
+        const int i = (int)(item - (at & LOW)), x = i / a.Hkv;
+        found.r = r;
+        found.h = i - x * a.Hkv;
+        found.tile = tiles - 1 - x / shares;
+        found.share = x % shares;
+        found.shares = shares;
+        found.slot = (int)(at >> HIGH) + (found.tile * a.Hkv + found.h) * shares;
     }
     __syncthreads();
-    out = {found[0], found[1], found[2]};
+    out.r = __builtin_amdgcn_readfirstlane(found.r);
+    out.h = __builtin_amdgcn_readfirstlane(found.h);
+    out.tile = __builtin_amdgcn_readfirstlane(found.tile);
+    out.share = __builtin_amdgcn_readfirstlane(found.share);
+    out.shares = __builtin_amdgcn_readfirstlane(found.shares);
+    out.slot = __builtin_amdgcn_readfirstlane(found.slot);
     return true;
 }
 
 __device__ __forceinline__ bool not_finite2(uint32_t w) {
     return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+}
+
+// The shares' sums cross the XCDs: stored through to and loaded from memory (sc0 sc1), so that a
+// share's are there once its stores are done, without a fence that writes back all of an L2.
+struct Part {
+    __amdgpu_buffer_rsrc_t r;
+    static constexpr int SYS = 1 | 16;
+    __device__ __forceinline__ Part(const float *base, uint32_t floats)
+        : r(__builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)(floats * 4), 0x00020000)) {}
+    __device__ __forceinline__ void put4(uint32_t i, f32x4 v) const {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, i * 4u, 0, SYS);
+    }
+    __device__ __forceinline__ f32x4 get4(uint32_t i) const {
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, i * 4u, 0, SYS));
+    }
+    __device__ __forceinline__ void put2(uint32_t i, float x, float y) const {
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(x), __float_as_uint(y)}, r, i * 4u, 0, SYS);
+    }
+    __device__ __forceinline__ u32x2 get2(uint32_t i) const {
+        return __builtin_amdgcn_raw_buffer_load_b64(r, i * 4u, 0, SYS);
+    }
+};
+template <int TM, int D>
+__device__ __forceinline__ constexpr uint32_t slot_floats() {
+    return TM * (D + 2);
+}
+
+// After the last of a tile's shares has stored its sums: the join, by 256 threads. pairs: those of the
+// tile that there are; `lds` MOST * pairs + 8 * D floats; row(p) the output of pair p.
+template <int TM, int D, typename Row>
+__device__ __forceinline__ void join_shares(const Attn &a, const Piece &pc, int pairs, float *lds, Row row) {
+    constexpr uint32_t SF = slot_floats<TM, D>();
+    const Part pb(a.part + (int64_t)pc.slot * SF, (uint32_t)pc.shares * SF);
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    // a share's factor for each pair: exp2 of its maximum relative to the largest, over the sum
+    for (int p = wave; p < pairs; p += 4) {
+        float m[MOST / 64], l[MOST / 64], mm = -INFINITY, ll = 0.f;
+#pragma unroll
+        for (int i = 0; i < MOST / 64; i++) {
+            const int s = lane + 64 * i;
+            m[i] = -INFINITY;
+            l[i] = 0.f;
+            if (s < pc.shares) {
+                const u32x2 x = pb.get2((uint32_t)s * SF + TM * D + 2 * p);
+                m[i] = __uint_as_float(x[0]);
+                l[i] = __uint_as_float(x[1]);
+            }
+            mm = fmaxf(mm, m[i]);
+        }
+        mm = max_wave(mm);
+#pragma unroll
+        for (int i = 0; i < MOST / 64; i++) {
+            m[i] = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[i] - mm) * a.sl2);
+            ll += l[i] * m[i];
+        }
+        ll = wave_sum(ll);
+        const float inv = ll == 0.f ? 0.f : 1.0f / ll;
+#pragma unroll
+        for (int i = 0; i < MOST / 64; i++)
+            if (lane + 64 * i < pc.shares) lds[p * MOST + lane + 64 * i] = m[i] * inv;
+    }
+    __syncthreads();
+    // D / 4 threads a pair; where they are more than the pairs need, each takes some of the shares
+    constexpr int COLS = D / 4, TEAMS = 256 / COLS;
+    const int team = tid / COLS, d = tid % COLS * 4;
+    int per = 1;  // teams a pair
+    while (per * 2 * pairs <= TEAMS) per *= 2;
+    float *sums = lds + MOST * pairs;
+    for (int p0 = 0; p0 < pairs; p0 += TEAMS / per) {
+        const int p = p0 + team / per, part = team % per;
+        f32x4 x{0.f, 0.f, 0.f, 0.f};
+        if (p < pairs) {
+            constexpr int AT = 8;
+            for (int s0 = part; s0 < pc.shares; s0 += AT * per) {
+                f32x4 y[AT];
+#pragma unroll
+                for (int i = 0; i < AT; i++) y[i] = pb.get4((uint32_t)min(s0 + i * per, pc.shares - 1) * SF + p * D + d);
+#pragma unroll
+                for (int i = 0; i < AT; i++) {
+                    const float f = s0 + i * per < pc.shares ? lds[p * MOST + s0 + i * per] : 0.f;
+                    if (f != 0.f)  // (an infinity of a share that does not count would be NaN)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) x[e] += y[i][e] * f;
+                }
+            }
+        }
+        if (per > 1) {
+            __syncthreads();
+            *(f32x4 *)(sums + team * D + d) = x;
+            __syncthreads();
+            if (part == 0)
+                for (int i = 1; i < per; i++) {
+                    const f32x4 y = *(const f32x4 *)(sums + (team + i) * D + d);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[e] += y[e];
+                }
+        }
+        if (p < pairs && part == 0) *(u32x2 *)(row(p) + d) = u32x2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+    }
 }
 
 // The values of a 32-key tile that are no numbers, taken out of it (v: an A operand per granule and 32
@@ -193,10 +358,13 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(const Attn a) {
 
     Piece pc;
     if (!piece_of<32>(a, blockIdx.x, pc)) return;
-    const int r = __builtin_amdgcn_readfirstlane(pc.r), h = __builtin_amdgcn_readfirstlane(pc.h);
-    const int tile = __builtin_amdgcn_readfirstlane(pc.tile);
+    const int r = pc.r, h = pc.h, tile = pc.tile;
     const Req rq = req_of(a, r);
     const Range g = range_of<32, KT>(a, rq, tile);
+    // the share's tiles: whole rounds
+    const int rounds = (g.tiles + 3) / 4;
+    const int first = (int)((int64_t)rounds * pc.share / pc.shares) * 4;
+    const int last = min((int)((int64_t)rounds * (pc.share + 1) / pc.shares) * 4, g.tiles);
 
     // the lane's pair: row i of the request, head h G + hd
     const int f = tile * 32 + l32, row = f / a.G, hd = f - row * a.G;
@@ -224,7 +392,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(const Attn a) {
     auto load_granules = [&](int v) __attribute__((always_inline)) {
         const int mine = v + (lane >> 1) * 4;
         gran = -1;
-        if (mine < g.tiles) {
+        if (mine < last) {
             const uint32_t x = 2 * tile_at(g, mine) + (lane & 1);
             const uint32_t k = __umulhi(x, a.ps16_magic) + (a.ps16 == 1 ? x : 0);
             if ((int64_t)k < a.max_pages) {
@@ -252,21 +420,21 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(const Attn a) {
     f32x16 o[DT] = {};
     float m = -INFINITY, l = 0.f;
     int g0 = -1, g1 = -1, n0 = -1, n1 = -1, k = 0;
-    int v = wave;
-    if (v < g.tiles) {
+    int v = first + wave;
+    if (v < last) {
         load_granules(v);
         g0 = __builtin_amdgcn_readlane(gran, 0);
         g1 = __builtin_amdgcn_readlane(gran, 1);
         load_k(g0, g1);
         load_v(g0, g1);
     }
-    for (; v < g.tiles; v += 4) {
+    for (; v < last; v += 4) {
         const int key0 = tile_at(g, v) * KT;
         f32x16 s = {};
 #pragma unroll
         for (int kk = 0; kk < KK; kk++)
             s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kc[kk]), qf[kk], s, 0, 0, 0);
-        const bool more = v + 4 < g.tiles;
+        const bool more = v + 4 < last;
         if (more) {
             if (++k == 32) {
                 k = 0;
@@ -362,44 +530,71 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(const Attn a) {
         for (int e = 0; e < 4; e++)
             *(f32x4 *)(mine + 32 * dt + 8 * e) = f32x4{o[dt][4 * e], o[dt][4 * e + 1], o[dt][4 * e + 2], o[dt][4 * e + 3]};
     __syncthreads();
-    const int pr = tid / 8, pf = tile * 32 + pr;  // eight threads a pair
-    if (pf >= rq.n * a.G) return;
-    const int prow = pf / a.G, phd = pf - prow * a.G;
-    const float mm = fmaxf(fmaxf(sm[0][pr], sm[1][pr]), fmaxf(sm[2][pr], sm[3][pr]));
-    float ll = 0.f, fac[4];
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-        fac[w] = sm[w][pr] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((sm[w][pr] - mm) * a.sl2);
-        ll += sl[w][pr] * fac[w];
-    }
-    const float inv = ll == 0.f ? 0.f : 1.0f / ll;  // a pair that sees no key gives zeros
-    uint16_t *dst = a.out + ((int64_t)(rq.start + prow) * a.Hkv * a.G + h * a.G + phd) * D;
-#pragma unroll
-    for (int e = 0; e < D / 32; e++) {
-        const int d = (tid & 7) * 4 + 32 * e;
-        f32x4 x{0.f, 0.f, 0.f, 0.f};
+    const int pairs = min(rq.n * a.G - tile * 32, 32), pr = tid / 8;  // eight threads a pair
+    auto row_of = [&](int p) __attribute__((always_inline)) {
+        const int at = (tile * 32 + p) / a.G, hd = tile * 32 + p - at * a.G;
+        return a.out + ((int64_t)(rq.start + at) * a.Hkv * a.G + h * a.G + hd) * D;
+    };
+    const Part pb(a.part + (int64_t)(pc.slot + pc.share) * slot_floats<32, D>(), slot_floats<32, D>());
+    if (pr < pairs) {
+        const float mm = fmaxf(fmaxf(sm[0][pr], sm[1][pr]), fmaxf(sm[2][pr], sm[3][pr]));
+        float ll = 0.f, fac[4];
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-            const f32x4 y = *(const f32x4 *)(so + (w * 32 + pr) * PITCH + d);
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[i] += y[i] * fac[w];
+            fac[w] = sm[w][pr] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((sm[w][pr] - mm) * a.sl2);
+            ll += sl[w][pr] * fac[w];
         }
-        *(u32x2 *)(dst + d) = u32x2{pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv)};
+        const float inv = ll == 0.f ? 0.f : 1.0f / ll;  // a pair that sees no key gives zeros
+        if (pc.shares > 1 && (tid & 7) == 0) pb.put2(32 * D + 2 * pr, mm, ll);
+        uint16_t *dst = row_of(pr);
+#pragma unroll
+        for (int e = 0; e < D / 32; e++) {
+            const int d = (tid & 7) * 4 + 32 * e;
+            f32x4 x{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const f32x4 y = *(const f32x4 *)(so + (w * 32 + pr) * PITCH + d);
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] += y[i] * fac[w];
+            }
+            if (pc.shares > 1)
+                pb.put4(pr * D + d, x);
+            else
+                *(u32x2 *)(dst + d) = u32x2{pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv)};
+        }
     }
+    if (pc.shares == 1) return;
+    __shared__ uint32_t arrived;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();  // (also: nobody reads so any more)
+    if (tid == 0) {
+        arrived = atomicAdd(&a.count[pc.slot], 1u);
+        if (arrived == (uint32_t)pc.shares - 1) __hip_atomic_store(&a.count[pc.slot], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (arrived == (uint32_t)pc.shares - 1) join_shares<32, D>(a, pc, pairs, so, row_of);
 }
 
 }  // namespace
 
-hipError_t launch_paged_attention(const PageDims &d, const uint8_t *layer, const PagedAttnArgs &x, hipStream_t stream) {
+size_t paged_attention_scratch(int d) { return PAGED_COUNTER_BYTES + (size_t)SLOTS * 32 * (d + 2) * 4; }
+
+hipError_t launch_paged_attention(const PageDims &d, const uint8_t *layer, const PagedAttnArgs &x, void *scratch,
+                                  hipStream_t stream) {
     if (x.rows <= 0 || x.requests <= 0) return hipSuccess;
     const int64_t g = x.heads / d.kv_heads, cap = std::min<int64_t>(x.max_pages * d.page_size, 0x7fffffff - 64);
     const int ps16 = d.page_size / 16;
-    const Attn a{x.q, x.q_row, x.q_head, layer, d.pages, x.tables, x.max_pages, x.lengths, x.starts, (int32_t)x.requests,
-                 (int32_t)x.rows, d.kv_heads, (int32_t)g, ps16, (uint32_t)(((1ull << 32) + ps16 - 1) / ps16),
-                 (int32_t)cap, x.causal, (int32_t)std::min<int64_t>(x.window, 0x7fffffff),
-                 (int32_t)std::min<int64_t>(x.sinks, 0x7fffffff), x.scale * 1.4426950408889634f, x.out};
-    // at most one tile more than the pairs fill for each request
-    const int64_t most = (x.rows * g / 32 + x.requests) * d.kv_heads;
+    Attn a{x.q, x.q_row, x.q_head, layer, d.pages, x.tables, x.max_pages, x.lengths, x.starts, (int32_t)x.requests,
+           (int32_t)x.rows, d.kv_heads, (int32_t)g, ps16, (uint32_t)(((1ull << 32) + ps16 - 1) / ps16),
+           (int32_t)cap, x.causal, (int32_t)std::min<int64_t>(x.window, 0x7fffffff),
+           (int32_t)std::min<int64_t>(x.sinks, 0x7fffffff), x.scale * 1.4426950408889634f, x.out, nullptr, nullptr};
+    // at most one tile more than the pairs fill for each request, and the shares
+    int64_t most = (x.rows * g / 32 + x.requests) * d.kv_heads;
+    if (cap > GRAIN * ROUND) {
+        a.count = (uint32_t *)scratch;
+        a.part = (float *)((char *)scratch + PAGED_COUNTER_BYTES);
+        most += WANT;
+    }
     if (most >= (int64_t)1 << 24) return hipErrorInvalidValue;
     if (d.head_dim == 128)
         paged_attn_kernel<128><<<(unsigned)most, 256, 0, stream>>>(a);
