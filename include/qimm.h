@@ -337,7 +337,7 @@ int qimm_page_plan(qimm_ctx *ctx, const qimm_page_plan_args *p, void *stream);
 int64_t qimm_page_plan_work(int64_t requests);
 
 /* The pages of `layers` layers, bf16, in a layout of the library's own; head_dim 64 or 128. The
- * attention's scratch (17 to 35 MB) belongs to them: attention calls with one qimm_pages must not
+ * attention's scratch (33 or 64 MB) belongs to them: attention calls with one qimm_pages must not
  * overlap on the device, two replayed graphs neither. */
 typedef struct qimm_pages qimm_pages;
 int qimm_pages_create(qimm_ctx *ctx, int64_t layers, int64_t pages, int64_t page_size, int64_t kv_heads,

@@ -28,13 +28,19 @@
 namespace qimm {
 namespace {
 
-constexpr int KT = 32;      // keys of a wave's tile
-constexpr int ROUND = 128;  // keys of a workgroup's four tiles
-// Shares: as many as make WANT workgroups of all requests, at least GRAIN rounds each, at most MOST of a
-// tile; a request is split in at most twice its part of WANT.
-constexpr int WANT = 1024, GRAIN = 4, MOST = 128;
-constexpr int SLOTS = 2 * WANT;
-static_assert(SLOTS * 4 <= PAGED_COUNTER_BYTES, "a counter per slot");
+// The two forms: pairs of a tile, keys of a round, and the shares: as many as make WANT workgroups of all
+// requests, at least GRAIN rounds each, at most MOST of a tile; fewer where they are more than SLOTS.
+struct Few {
+    static constexpr bool ROWS = false;
+    static constexpr int TM = 32, ROUND = 128, WANT = 1024, GRAIN = 4, MOST = 128, SLOTS = WANT / 4 * 5;
+};
+struct Rows {
+    static constexpr bool ROWS = true;
+    static constexpr int TM = 128, ROUND = 64, WANT = 512, GRAIN = 8, MOST = 64, SLOTS = WANT / 4 * 5;
+};
+constexpr int KT = 32;          // keys of a wave's tile, few pairs
+constexpr int FEW_PAIRS = 32;   // more pairs of a request and key head are rows
+static_assert((Few::SLOTS + Rows::SLOTS) * 4 <= PAGED_COUNTER_BYTES, "a counter per slot");
 
 struct Attn {
     const uint16_t *q;
@@ -52,8 +58,10 @@ struct Attn {
     int32_t causal, window, sinks;  // window 0: none
     float sl2;             // scale * log2 e
     uint16_t *out;
-    uint32_t *count;       // arrivals, zero between calls; null: no request is long enough to be split
+    uint32_t *count;       // arrivals per slot, the few's and the rows', zero between calls; null: no request
+                           // is long enough to be split
     float *part;           // per slot O [TM][D], then (m, l) [TM]
+    int32_t row_pieces;    // workgroups for rows, before those for few
 };
 
 // a request's rows and tokens
@@ -66,15 +74,15 @@ __device__ __forceinline__ Req req_of(const Attn &a, int r) {
     return {s, e - s, min(max(a.lengths[r], 0), a.cap)};
 }
 
-// The keys that some pair of tile `tile` (TM pairs) sees: first .. [0, sk) and lo .. hi - 1, as tiles of
-// `keys`: ns of the first ones, then from w0 on; pos0, pos1: the positions of its first and last row.
+// The keys that some pair of `pairs` from `first` on sees: [0, sk) and lo .. hi - 1, as tiles of KEYS: ns of
+// the first ones, then from w0 on; pos0, pos1: the positions of the first and last row.
 struct Range {
     int pos0, pos1, lo, hi, sk, ns, w0, tiles;
 };
-template <int TM, int KEYS>
-__device__ __forceinline__ Range range_of(const Attn &a, const Req &q, int tile) {
+template <int KEYS>
+__device__ __forceinline__ Range range_of(const Attn &a, const Req &q, int first, int pairs) {
     Range g;
-    const int i0 = tile * TM / a.G, i1 = min(q.n - 1, (tile * TM + TM - 1) / a.G);
+    const int i0 = min(first / a.G, q.n - 1), i1 = min(q.n - 1, (first + pairs - 1) / a.G);
     g.pos0 = a.causal ? q.len - q.n + i0 : q.len - 1;
     g.pos1 = a.causal ? q.len - q.n + i1 : q.len - 1;
     g.hi = max(g.pos1 + 1, 0);
@@ -88,12 +96,17 @@ __device__ __forceinline__ Range range_of(const Attn &a, const Req &q, int tile)
 }
 __device__ __forceinline__ int tile_at(const Range &g, int v) { return v < g.ns ? v : v - g.ns + g.w0; }
 
-// Rounds of the keys that any tile of a request sees, at most.
-template <int TM>
+// A request's tiles of the form's, and the rounds of the keys that any of them sees, at most.
+template <typename F>
+__device__ __forceinline__ int tiles_of(const Attn &a, const Req &q) {
+    const int pairs = q.n * a.G;
+    return (pairs > FEW_PAIRS) == F::ROWS ? (pairs + F::TM - 1) / F::TM : 0;
+}
+template <typename F>
 __device__ __forceinline__ int rounds_of(const Attn &a, const Req &q) {
     int64_t keys = q.len;
-    if (a.window) keys = min(keys, (int64_t)a.sinks + a.window + TM / a.G + 3 * KT);
-    return (int)((keys + ROUND - 1) / ROUND);
+    if (a.window) keys = min(keys, (int64_t)a.sinks + a.window + F::TM / a.G + 2 * F::ROUND);
+    return (int)((keys + F::ROUND - 1) / F::ROUND);
 }
 
 // What a workgroup takes: share `share` of `shares` of tile `tile` of request r's pairs for key head h; slot:
@@ -127,8 +140,8 @@ __device__ __forceinline__ int64_t scan256(int64_t v, int64_t *part, int64_t &to
 // The piece of workgroup `item`, in request order (the last tiles first: under causal rows they see the
 // most keys; heads fastest); false: there is none. Every thread counts its share of the requests, and the one
 // whose share has the piece looks which.
-template <int TM>
-__device__ __forceinline__ bool piece_of(const Attn &a, int item, Piece &out) {
+template <typename F>
+__device__ __forceinline__ bool piece_of(const Attn &a, int item, int most, Piece &out) {
     __shared__ int64_t part[4];
     __shared__ Piece found;
     const int c = (a.R + 255) / 256, r0 = min((int)threadIdx.x * c, a.R), r1 = min(r0 + c, a.R);
@@ -137,17 +150,17 @@ __device__ __forceinline__ bool piece_of(const Attn &a, int item, Piece &out) {
         int64_t rounds = 0;
         for (int r = r0; r < r1; r++) {
             const Req q = req_of(a, r);
-            rounds += (int64_t)((q.n * a.G + TM - 1) / TM) * rounds_of<TM>(a, q);
+            rounds += (int64_t)tiles_of<F>(a, q) * rounds_of<F>(a, q);
         }
         scan256(rounds, part, all);
-        chunk = max((int64_t)GRAIN, (all * a.Hkv + WANT - 1) / WANT);
+        chunk = max((int64_t)F::GRAIN, (all * a.Hkv + F::WANT - 1) / F::WANT);
     }
     // tiles and shares of request r; its pieces in the low bits of the sums, the slots of a split one above
     auto split = [&](int r, int &tiles, int &shares) __attribute__((always_inline)) {
         const Req q = req_of(a, r);
-        tiles = (q.n * a.G + TM - 1) / TM;
+        tiles = tiles_of<F>(a, q);
         shares = 1;
-        if (chunk && tiles) shares = max((int)min((rounds_of<TM>(a, q) + chunk - 1) / chunk, (int64_t)MOST), 1);
+        if (chunk && tiles) shares = max((int)min((rounds_of<F>(a, q) + chunk - 1) / chunk, (int64_t)F::MOST), 1);
     };
     constexpr int HIGH = 44;
     constexpr int64_t LOW = ((int64_t)1 << HIGH) - 1;
@@ -164,9 +177,9 @@ __device__ __forceinline__ bool piece_of(const Attn &a, int item, Piece &out) {
             mine += pieces(tiles, shares);
         }
         at = scan256(mine, part, all);
-        // more than there can be: `starts` that overlap. Every share has to arrive, so nothing is split.
-        if (!chunk || ((all & LOW) <= gridDim.x && (all >> HIGH) <= SLOTS)) break;
-        chunk = 0;
+        if (!chunk || ((all & LOW) <= most && (all >> HIGH) <= F::SLOTS)) break;
+        // more pieces than there can be: `starts` that overlap. Every share has to arrive, so nothing is split.
+        chunk = (all & LOW) <= most ? 2 * chunk : 0;
     }
     if (item >= (all & LOW)) return false;
     if (item >= (at & LOW) && item < (at & LOW) + (mine & LOW)) {
@@ -183,7 +196,7 @@ __device__ __forceinline__ bool piece_of(const Attn &a, int item, Piece &out) {
         found.tile = tiles - 1 - x / shares;
         found.share = x % shares;
         found.shares = shares;
-        found.slot = (int)(at >> HIGH) + (found.tile * a.Hkv + found.h) * shares;
+        found.slot = (F::ROWS ? Few::SLOTS : 0) + (int)(at >> HIGH) + (found.tile * a.Hkv + found.h) * shares;
     }
     __syncthreads();
     out.r = __builtin_amdgcn_readfirstlane(found.r);
@@ -219,17 +232,24 @@ struct Part {
         return __builtin_amdgcn_raw_buffer_load_b64(r, i * 4u, 0, SYS);
     }
 };
-template <int TM, int D>
+// floats of a slot, and where slot `slot` starts
+template <typename F, int D>
 __device__ __forceinline__ constexpr uint32_t slot_floats() {
-    return TM * (D + 2);
+    return F::TM * (D + 2);
+}
+template <typename F, int D>
+__device__ __forceinline__ const float *slot_at(const Attn &a, int slot) {
+    const int64_t few = (int64_t)Few::SLOTS * slot_floats<Few, D>();
+    return F::ROWS ? a.part + few + (int64_t)(slot - Few::SLOTS) * slot_floats<F, D>() : a.part + (int64_t)slot * slot_floats<F, D>();
 }
 
 // After the last of a tile's shares has stored its sums: the join, by 256 threads. pairs: those of the
 // tile that there are; `lds` MOST * pairs + 8 * D floats; row(p) the output of pair p.
-template <int TM, int D, typename Row>
+template <typename F, int D, typename Row>
 __device__ __forceinline__ void join_shares(const Attn &a, const Piece &pc, int pairs, float *lds, Row row) {
-    constexpr uint32_t SF = slot_floats<TM, D>();
-    const Part pb(a.part + (int64_t)pc.slot * SF, (uint32_t)pc.shares * SF);
+    constexpr int TM = F::TM, MOST = F::MOST;
+    constexpr uint32_t SF = slot_floats<F, D>();
+    const Part pb(slot_at<F, D>(a, pc.slot), (uint32_t)pc.shares * SF);
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     // a share's factor for each pair: exp2 of its maximum relative to the largest, over the sum
     for (int p = wave; p < pairs; p += 4) {
@@ -299,21 +319,18 @@ __device__ __forceinline__ void join_shares(const Attn &a, const Piece &pc, int 
 }
 
 // The values of a 32-key tile that are no numbers, taken out of it (v: an A operand per granule and 32
-// dims) and added to the sums o of those pairs whose probability of the key is not 0. p: the tile's
-// probabilities as B operands; through `lds`, 128 (32 + D / 2) B of the wave's own.
-template <int D>
-__device__ __forceinline__ void add_not_finite(u32x4 (&v)[2][D / 32], const uint32_t (&p)[8], f32x16 (&o)[D / 32], uint8_t *lds, int lane) {
+// dims) and added to the sums o of those pairs that see the key, `sees` of its index in the tile; through
+// `lds`, 64 D B of the wave's own.
+template <int D, typename Sees>
+__device__ __forceinline__ void add_not_finite(u32x4 (&v)[2][D / 32], f32x16 (&o)[D / 32], uint8_t *lds, int lane, Sees sees) {
     const int l32 = lane & 31, hi = lane >> 5;
-    float *pl = (float *)lds;                    // [key][pair]
-    uint16_t *vl = (uint16_t *)(lds + 4096);     // [key][dim]
+    uint16_t *vl = (uint16_t *)lds;  // [key][dim]
     uint32_t keys = 0;
 #pragma unroll
     for (int j = 0; j < 2; j++)
 #pragma unroll
         for (int w = 0; w < 4; w++) {
             const int key = 16 * j + 8 * (w >> 1) + 4 * hi + 2 * (w & 1);
-            pl[key * 32 + l32] = __uint_as_float(p[4 * j + w] << 16);
-            pl[(key + 1) * 32 + l32] = __uint_as_float(p[4 * j + w] & 0xffff0000u);
 #pragma unroll
             for (int dt = 0; dt < D / 32; dt++) {
                 const uint32_t x = v[j][dt][w];
@@ -332,7 +349,7 @@ __device__ __forceinline__ void add_not_finite(u32x4 (&v)[2][D / 32], const uint
 #pragma unroll 1
     for (keys = __builtin_amdgcn_readfirstlane(keys); keys; keys &= keys - 1) {
         const int key = __builtin_ctz(keys);
-        const bool sees = pl[key * 32 + l32] > 0.f;
+        const bool mine = sees(key);
 #pragma unroll
         for (int dt = 0; dt < D / 32; dt++)
 #pragma unroll
@@ -341,26 +358,43 @@ __device__ __forceinline__ void add_not_finite(u32x4 (&v)[2][D / 32], const uint
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const uint32_t u = i & 1 ? x[i >> 1] & 0xffff0000u : x[i >> 1] << 16;
-                    if (sees && (u & 0x7f800000u) == 0x7f800000u) o[dt][4 * e + i] += __uint_as_float(u);
+                    if (mine && (u & 0x7f800000u) == 0x7f800000u) o[dt][4 * e + i] += __uint_as_float(u);
                 }
             }
     }
     __builtin_amdgcn_wave_barrier();
 }
 
+// A share's sums are stored; the last share of its tile joins them.
+template <typename F, int D, typename Row>
+__device__ __forceinline__ void arrive(const Attn &a, const Piece &pc, int pairs, float *lds, Row row) {
+    __shared__ uint32_t arrived;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();  // (also: nobody reads the workgroup's own sums in `lds` any more)
+    if (threadIdx.x == 0) {
+        arrived = atomicAdd(&a.count[pc.slot], 1u);
+        if (arrived == (uint32_t)pc.shares - 1) __hip_atomic_store(&a.count[pc.slot], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (arrived == (uint32_t)pc.shares - 1) join_shares<F, D>(a, pc, pairs, lds, row);
+}
+
+constexpr int few_lds(int d) { return 4 * 32 * (d + 4) * 4; }
+
+// A tile of few pairs.
 template <int D>
-__global__ __launch_bounds__(256, 2) void paged_attn_kernel(const Attn a) {
+__device__ __forceinline__ void few_pairs(const Attn &a, int item, uint8_t *lds) {
     constexpr int KK = D / 16, DT = D / 32, PITCH = D + 4;
-    __shared__ __attribute__((aligned(16))) float so[4 * 32 * PITCH];
+    float *so = (float *)lds;
     __shared__ float sm[4][32], sl[4][32];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int l32 = lane & 31, hi = lane >> 5;
 
     Piece pc;
-    if (!piece_of<32>(a, blockIdx.x, pc)) return;
+    if (!piece_of<Few>(a, item, (int)gridDim.x - a.row_pieces, pc)) return;
     const int r = pc.r, h = pc.h, tile = pc.tile;
     const Req rq = req_of(a, r);
-    const Range g = range_of<32, KT>(a, rq, tile);
+    const Range g = range_of<KT>(a, rq, tile * 32, 32);
     // the share's tiles: whole rounds
     const int rounds = (g.tiles + 3) / 4;
     const int first = (int)((int64_t)rounds * pc.share / pc.shares) * 4;
@@ -505,7 +539,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(const Attn a) {
                     }
                 }
             }
-            if (g.pos0 != g.pos1 && __ballot(odd)) add_not_finite<D>(vc, p, o, (uint8_t *)(so + wave * 32 * PITCH), lane);
+            if (g.pos0 != g.pos1 && __ballot(odd))
+                add_not_finite<D>(vc, o, (uint8_t *)(so + wave * 32 * PITCH), lane,
+                                  [&](int key) { return key0 + key <= pos && (key0 + key > low || key0 + key < g.sk); });
         }
 #pragma unroll
         for (int j = 0; j < 2; j++)
@@ -535,7 +571,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(const Attn a) {
         const int at = (tile * 32 + p) / a.G, hd = tile * 32 + p - at * a.G;
         return a.out + ((int64_t)(rq.start + at) * a.Hkv * a.G + h * a.G + hd) * D;
     };
-    const Part pb(a.part + (int64_t)(pc.slot + pc.share) * slot_floats<32, D>(), slot_floats<32, D>());
+    const Part pb(slot_at<Few, D>(a, pc.slot + pc.share), slot_floats<Few, D>());
     if (pr < pairs) {
         const float mm = fmaxf(fmaxf(sm[0][pr], sm[1][pr]), fmaxf(sm[2][pr], sm[3][pr]));
         float ll = 0.f, fac[4];
@@ -563,21 +599,263 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(const Attn a) {
                 *(u32x2 *)(dst + d) = u32x2{pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv)};
         }
     }
-    if (pc.shares == 1) return;
-    __shared__ uint32_t arrived;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();  // (also: nobody reads so any more)
-    if (tid == 0) {
-        arrived = atomicAdd(&a.count[pc.slot], 1u);
-        if (arrived == (uint32_t)pc.shares - 1) __hip_atomic_store(&a.count[pc.slot], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (pc.shares > 1) arrive<Few, D>(a, pc, pairs, so, row_of);
+}
+
+// ---- many pairs ----
+
+constexpr int rows_lds(int d) { return 8 * (int)granule_bytes(d); }
+
+// A tile of 128 pairs, a wave 32 of them: 64-key tiles go straight from the pages into LDS, a granule a
+// wave, the next one while this one is multiplied. K operands are read there conflict-free (paged.h).
+// The reference point of a pair's exponentials follows its maximum where that grew by more than 2^8.
+template <int D>
+__device__ __forceinline__ void many_pairs(const Attn &a, int item, uint8_t *lds) {
+    constexpr int KK = D / 16, DT = D / 32, KEYS = 64;
+    constexpr int GB = (int)granule_bytes(D), STAGE = 4 * GB;
+    constexpr float LAG = 8.f;
+    __shared__ int none[2][4];  // granules of a stage without a page
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int l32 = lane & 31, hi = lane >> 5;
+
+    Piece pc;
+    if (!piece_of<Rows>(a, item, a.row_pieces, pc)) return;
+    const int r = pc.r, h = pc.h, f0 = pc.tile * Rows::TM;
+    const Req rq = req_of(a, r);
+    const Range g = range_of<KEYS>(a, rq, f0, Rows::TM);
+    const int first = (int)((int64_t)g.tiles * pc.share / pc.shares);
+    const int last = (int)((int64_t)g.tiles * (pc.share + 1) / pc.shares);
+
+    // the wave's pairs
+    const int pairs = min(rq.n * a.G - f0, Rows::TM);
+    const Range w = range_of<KEYS>(a, rq, f0 + 32 * wave, 32);
+    const bool any = 32 * wave < pairs;
+    const int f = f0 + 32 * wave + l32, row = f / a.G, hd = f - row * a.G;
+    const bool there = row < rq.n;
+    const int pos = !there ? -1 : a.causal ? rq.len - rq.n + row : rq.len - 1;
+    const int low = a.window ? pos - a.window : -1;      // sees key j <= pos if j > low or j < sk
+    const int low0 = a.window ? w.pos0 - a.window : -1, sk = a.window ? a.sinks : 0;
+    const int pmin = 32 * wave + 31 < pairs ? w.pos0 : -1;  // every pair sees up to it
+
+    // ---- tiles from the pages: the wave's granule of the next 64 tiles, a lane each ----
+    const int32_t *table = a.tables + (int64_t)r * a.max_pages;
+    int gran = -1;
+    auto load_granules = [&](int v) __attribute__((always_inline)) {
+        gran = -1;
+        if (v + lane < last) {
+            const uint32_t x = 4 * tile_at(g, v + lane) + wave;
+            const uint32_t k = __umulhi(x, a.ps16_magic) + (a.ps16 == 1 ? x : 0);
+            if ((int64_t)k < a.max_pages) {
+                const int page = table[k];
+                if (page >= 0 && page < a.pages) gran = (page * a.Hkv + h) * a.ps16 + (int)(x - k * a.ps16);
+            }
+        }
+    };
+    int k = 0;
+    auto load_tile = [&](int v, int stage) __attribute__((always_inline)) {
+        if (k == 64) {
+            k = 0;
+            load_granules(v);
+        }
+        const int gn = __builtin_amdgcn_readlane(gran, k++);
+        const uint8_t *src = a.cache + (int64_t)max(gn, 0) * GB + lane * 16;
+        uint8_t *dst = lds + stage * STAGE + wave * GB;
+#pragma unroll
+        for (int i = 0; i < GB / 1024; i++)
+            __builtin_amdgcn_global_load_lds((const void *)(src + i * 1024), (lds_ptr_t)(dst + i * 1024), 16, 0, 0);
+        if (lane == 0) none[stage][wave] = gn < 0;
+    };
+    if (first < last) {
+        load_granules(first);
+        load_tile(first, 0);
     }
-    __syncthreads();
-    if (arrived == (uint32_t)pc.shares - 1) join_shares<32, D>(a, pc, pairs, so, row_of);
+
+    bf16x8 qf[KK];
+    {
+        const uint16_t *src = a.q + (int64_t)(rq.start + (there ? row : 0)) * a.q_row + (int64_t)(h * a.G + (there ? hd : 0)) * a.q_head + 8 * hi;
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) {
+            u32x4 x = *(const u32x4 *)(src + 16 * kk);
+            if (!there) x = u32x4{};
+            qf[kk] = __builtin_bit_cast(bf16x8, x);
+        }
+    }
+
+    f32x16 o[DT] = {};
+    float m = -INFINITY, l = 0.f;
+    const uint8_t *kl = lds + (l32 >> 4) * GB + hi * 256 + (l32 & 15) * 16;  // + half, dims
+    const uint8_t *vl = lds + D * 32 + hi * (D * 16) + l32 * 16;             // + granule, dims
+
+    for (int v = first; v < last; v++) {
+        const int stage = (v - first) & 1;
+        __builtin_amdgcn_s_waitcnt(WAIT_VM0_LGKM0);
+        __syncthreads();
+        const int key0 = tile_at(g, v) * KEYS;
+        uint32_t gone = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) gone |= none[stage][i] ? 1u << i : 0u;
+        gone = __builtin_amdgcn_readfirstlane(gone);
+        if (v + 1 < last) load_tile(v + 1, stage ^ 1);
+        // no pair of the wave sees any of it
+        if (!any || key0 > w.pos1 || (a.window && key0 + KEYS - 1 <= low0 && key0 >= sk)) continue;
+        // every pair sees all of it, or some do not
+        const bool some = !(key0 + KEYS - 1 <= pmin && gone == 0 && (a.window == 0 || key0 > w.pos1 - a.window || key0 + KEYS <= sk));
+
+        f32x16 s[2] = {};
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++)
+                s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8 *)(kl + stage * STAGE + b * 2 * GB + kk * 512), qf[kk],
+                                                               s[b], 0, 0, 0);
+        if (some) {
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int key = key0 + 32 * b + 8 * (e >> 2) + 4 * hi + (e & 3);
+                    const bool ok = key <= pos && (key > low || key < sk) && !((gone >> (2 * b + (e >> 3))) & 1u);
+                    s[b][e] = ok ? s[b][e] : -INFINITY;
+                }
+        }
+        float m0 = s[0][0], m1 = s[1][0];
+#pragma unroll
+        for (int e = 1; e < 16; e++) {
+            m0 = fmaxf(m0, s[0][e]);
+            m1 = fmaxf(m1, s[1][e]);
+        }
+        float mx = fmaxf(m0, m1);
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        if (__ballot((mx - m) * a.sl2 > LAG)) {  // (a pair without a visible key yet: NaN or infinity)
+            const float top = fmaxf(mx, m);
+            const float al = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * a.sl2);
+            m = top;
+            l *= al;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[dt][e] *= al;
+        }
+        const float c = m == -INFINITY ? 0.f : -m * a.sl2;
+        bf16x8 pf[4];
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            uint32_t p[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][2 * e], a.sl2, c));
+                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][2 * e + 1], a.sl2, c));
+                l += x;
+                l += y;
+                p[e] = pack_bf16x2(x, y);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                pf[2 * b + j] = __builtin_bit_cast(bf16x8, u32x4{p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]});
+        }
+        const uint8_t *vs = vl + stage * STAGE;
+        if (some) {
+            // what a key holds that no pair sees does not count; where only some see a value that is no
+            // number, it goes to those by itself
+            auto seen = [&](int j, int i) __attribute__((always_inline)) {
+                const int key = key0 + 16 * j + 8 * (i >> 1) + 4 * hi + 2 * (i & 1);
+                const uint32_t x = (key <= w.pos1 && (key > low0 || key < sk) ? 0xffffu : 0u) |
+                                   (key + 1 <= w.pos1 && (key + 1 > low0 || key + 1 < sk) ? 0xffff0000u : 0u);
+                return (gone >> j) & 1u ? 0u : x;
+            };
+            uint32_t odd = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                u32x4 keep;
+#pragma unroll
+                for (int i = 0; i < 4; i++) keep[i] = seen(j, i);
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) {
+                    u32x4 x = *(const u32x4 *)(vs + j * GB + dt * 512) & keep;
+                    if (w.pos0 != w.pos1) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const uint32_t bad = ((x[i] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((x[i] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+                            odd |= bad;
+                            x[i] &= ~bad;
+                        }
+                    }
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), pf[j], o[dt], 0, 0, 0);
+                }
+            }
+            if (__builtin_expect(__ballot(odd != 0) != 0, 0)) {
+#pragma unroll 1
+                for (int key = 0; key < KEYS; key++) {
+                    const bool sees = key0 + key <= pos && (key0 + key > low || key0 + key < sk) && !((gone >> (key >> 4)) & 1u);
+                    const uint8_t *src = lds + stage * STAGE + (key >> 4) * GB + granule_v(D, key & 15, 4 * hi);
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            const uint32_t u = (uint32_t)*(const uint16_t *)(src + (32 * dt + 8 * (e >> 2) + (e & 3)) * 16) << 16;
+                            if (sees && (u & 0x7f800000u) == 0x7f800000u) o[dt][e] += __uint_as_float(u);
+                        }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++)
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8 *)(vs + j * GB + dt * 512), pf[j], o[dt], 0, 0, 0);
+        }
+    }
+
+    l += __shfl_xor(l, 32);
+    auto row_of = [&](int p) __attribute__((always_inline)) {
+        const int at = (f0 + p) / a.G, head = f0 + p - at * a.G;
+        return a.out + ((int64_t)(rq.start + at) * a.Hkv * a.G + h * a.G + head) * D;
+    };
+    const int p = 32 * wave + l32;
+    if (pc.shares == 1) {
+        if (!there) return;
+        const float inv = l == 0.f ? 0.f : 1.0f / l;  // a pair that sees no key gives zeros
+        uint16_t *dst = row_of(p) + 4 * hi;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                *(u32x2 *)(dst + 32 * dt + 8 * e) = u32x2{pack_bf16x2(o[dt][4 * e] * inv, o[dt][4 * e + 1] * inv),
+                                                          pack_bf16x2(o[dt][4 * e + 2] * inv, o[dt][4 * e + 3] * inv)};
+        return;
+    }
+    if (there) {
+        const Part pb(slot_at<Rows, D>(a, pc.slot + pc.share), slot_floats<Rows, D>());
+        if (hi == 0) pb.put2(Rows::TM * D + 2 * p, m, l);
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                pb.put4(p * D + 32 * dt + 8 * e + 4 * hi, f32x4{o[dt][4 * e], o[dt][4 * e + 1], o[dt][4 * e + 2], o[dt][4 * e + 3]});
+    }
+    arrive<Rows, D>(a, pc, pairs, (float *)lds, row_of);
+}
+
+template <int D>
+__global__ __launch_bounds__(256, 2) void paged_tokens_kernel(const Attn a) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[few_lds(D)];
+    few_pairs<D>(a, blockIdx.x, lds);
+}
+// the pieces of requests with many pairs first, they take longer
+template <int D>
+__global__ __launch_bounds__(256, 2) void paged_rows_kernel(const Attn a) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[few_lds(D) > rows_lds(D) ? few_lds(D) : rows_lds(D)];
+    if ((int)blockIdx.x < a.row_pieces)
+        many_pairs<D>(a, blockIdx.x, lds);
+    else
+        few_pairs<D>(a, (int)blockIdx.x - a.row_pieces, lds);
 }
 
 }  // namespace
 
-size_t paged_attention_scratch(int d) { return PAGED_COUNTER_BYTES + (size_t)SLOTS * 32 * (d + 2) * 4; }
+size_t paged_attention_scratch(int d) {
+    return PAGED_COUNTER_BYTES + ((size_t)Few::SLOTS * Few::TM + (size_t)Rows::SLOTS * Rows::TM) * (d + 2) * 4;
+}
 
 hipError_t launch_paged_attention(const PageDims &d, const uint8_t *layer, const PagedAttnArgs &x, void *scratch,
                                   hipStream_t stream) {
@@ -587,21 +865,34 @@ hipError_t launch_paged_attention(const PageDims &d, const uint8_t *layer, const
     Attn a{x.q, x.q_row, x.q_head, layer, d.pages, x.tables, x.max_pages, x.lengths, x.starts, (int32_t)x.requests,
            (int32_t)x.rows, d.kv_heads, (int32_t)g, ps16, (uint32_t)(((1ull << 32) + ps16 - 1) / ps16),
            (int32_t)cap, x.causal, (int32_t)std::min<int64_t>(x.window, 0x7fffffff),
-           (int32_t)std::min<int64_t>(x.sinks, 0x7fffffff), x.scale * 1.4426950408889634f, x.out, nullptr, nullptr};
-    // at most one tile more than the pairs fill for each request, and the shares
-    int64_t most = (x.rows * g / 32 + x.requests) * d.kv_heads;
-    if (cap > GRAIN * ROUND) {
+           (int32_t)std::min<int64_t>(x.sinks, 0x7fffffff), x.scale * 1.4426950408889634f, x.out, nullptr, nullptr, 0};
+    // Workgroups: of a request with few pairs one for each key head, of one with many at most a tile more
+    // than its pairs fill, and the shares. Without starts every request has g pairs.
+    const bool rows = x.starts ? x.rows * g > FEW_PAIRS : g > FEW_PAIRS, few = g <= FEW_PAIRS;
+    int64_t many = rows ? (x.rows * g / Rows::TM + std::min(x.requests, x.rows)) * d.kv_heads : 0;
+    int64_t tokens = few ? std::min(x.requests, x.rows) * d.kv_heads : 0;
+    if (cap > std::min(Few::GRAIN * Few::ROUND, Rows::GRAIN * Rows::ROUND)) {
         a.count = (uint32_t *)scratch;
         a.part = (float *)((char *)scratch + PAGED_COUNTER_BYTES);
-        most += WANT;
+        if (many) many += Rows::WANT;
+        if (tokens) tokens += Few::WANT;
     }
-    if (most >= (int64_t)1 << 24) return hipErrorInvalidValue;
-    if (d.head_dim == 128)
-        paged_attn_kernel<128><<<(unsigned)most, 256, 0, stream>>>(a);
-    else if (d.head_dim == 64)
-        paged_attn_kernel<64><<<(unsigned)most, 256, 0, stream>>>(a);
-    else
+    if (many + tokens >= (int64_t)1 << 24) return hipErrorInvalidValue;
+    a.row_pieces = (int32_t)many;
+    const unsigned grid = (unsigned)(many + tokens);
+    if (d.head_dim == 128) {
+        if (many)
+            paged_rows_kernel<128><<<grid, 256, 0, stream>>>(a);
+        else
+            paged_tokens_kernel<128><<<grid, 256, 0, stream>>>(a);
+    } else if (d.head_dim == 64) {
+        if (many)
+            paged_rows_kernel<64><<<grid, 256, 0, stream>>>(a);
+        else
+            paged_tokens_kernel<64><<<grid, 256, 0, stream>>>(a);
+    } else {
         return hipErrorInvalidValue;
+    }
     return hipGetLastError();
 }
 
