@@ -68,8 +68,8 @@ int qimm_pages_create(qimm_ctx *ctx, int64_t layers, int64_t pages, int64_t page
     if (!page_size_fits(page_size)) return set_err(ctx, QIMM_ERR_SHAPE, "pages: the page size must be a multiple of 16 up to 512");
     if (layers <= 0 || pages <= 0 || kv_heads <= 0 || kv_heads > 65535)
         return set_err(ctx, QIMM_ERR_SHAPE, "pages: layers and pages must be positive, 1 to 65535 heads");
-    if (pages >= MAX_TOKENS / page_size || pages >= MAX_TOKENS / (kv_heads * (page_size / 16)))
-        return set_err(ctx, QIMM_ERR_SHAPE, "pages: pages * page_size and pages * kv_heads * page_size / 16 must be below 2^31");
+    if (pages >= MAX_TOKENS / page_size || pages >= MAX_TOKENS / 2 / (kv_heads * (page_size / 16)))
+        return set_err(ctx, QIMM_ERR_SHAPE, "pages: pages * page_size must be below 2^31, pages * kv_heads * page_size / 16 below 2^30");
     qimm_pages *pg = new (std::nothrow) qimm_pages();
     if (!pg) return set_err(ctx, QIMM_ERR_OOM, "pages: host allocation failed");
     pg->ctx = ctx;

@@ -21,6 +21,7 @@
 // with that which share of which request it is itself: two sums over the requests, one load each up
 // to 256 of them. The shares' sums go through memory; the last one to arrive joins them, in order.
 #include <algorithm>
+#include <type_traits>
 
 #include "device_common.h"
 #include "paged.h"
@@ -604,6 +605,27 @@ __device__ __forceinline__ void few_pairs(const Attn &a, int item, uint8_t *lds)
 
 // ---- many pairs ----
 
+// 4 KB of consecutive memory, 64 lanes of 16 B four times, into LDS (from `dst`, uniform, on) without
+// registers. The caller waits (lds_wait). In assembly, where the compiler does not see that LDS is
+// written: it would have every later read of LDS wait for these loads, those of the other stage too.
+__device__ __forceinline__ void load_lds_4k(const uint8_t *src, uint8_t *dst) {
+    const uint32_t at = (uint32_t)(uintptr_t)(lds_ptr_t)dst;
+    uint32_t m0;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %1\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %2, off\n\t"
+        "global_load_lds_dwordx4 %2, off offset:1024\n\t"
+        "global_load_lds_dwordx4 %2, off offset:2048\n\t"
+        "global_load_lds_dwordx4 %2, off offset:3072\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(m0)
+        : "s"(__builtin_amdgcn_readfirstlane(at)), "v"(src)
+        : "memory");
+}
+__device__ __forceinline__ void lds_wait() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+
 constexpr int rows_lds(int d) { return 8 * (int)granule_bytes(d); }
 
 // A tile of 128 pairs, a wave 32 of them: 64-key tiles go straight from the pages into LDS, a granule a
@@ -614,7 +636,8 @@ __device__ __forceinline__ void many_pairs(const Attn &a, int item, uint8_t *lds
     constexpr int KK = D / 16, DT = D / 32, KEYS = 64;
     constexpr int GB = (int)granule_bytes(D), STAGE = 4 * GB;
     constexpr float LAG = 8.f;
-    __shared__ int none[2][4];  // granules of a stage without a page
+    constexpr int ODD = 1 << 30;
+    __shared__ int info[2][4];  // a stage's granules: -1 without a page, ODD where values were taken out
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int l32 = lane & 31, hi = lane >> 5;
 
@@ -639,7 +662,7 @@ __device__ __forceinline__ void many_pairs(const Attn &a, int item, uint8_t *lds
 
     // ---- tiles from the pages: the wave's granule of the next 64 tiles, a lane each ----
     const int32_t *table = a.tables + (int64_t)r * a.max_pages;
-    int gran = -1;
+    int gran = -1, k = 0, here = -1;
     auto load_granules = [&](int v) __attribute__((always_inline)) {
         gran = -1;
         if (v + lane < last) {
@@ -651,23 +674,50 @@ __device__ __forceinline__ void many_pairs(const Attn &a, int item, uint8_t *lds
             }
         }
     };
-    int k = 0;
-    auto load_tile = [&](int v, int stage) __attribute__((always_inline)) {
+    auto load_tile = [&](int v, auto stage) __attribute__((always_inline)) {
+        constexpr int ST = decltype(stage)::value;
         if (k == 64) {
             k = 0;
             load_granules(v);
         }
-        const int gn = __builtin_amdgcn_readlane(gran, k++);
-        const uint8_t *src = a.cache + (int64_t)max(gn, 0) * GB + lane * 16;
-        uint8_t *dst = lds + stage * STAGE + wave * GB;
+        here = __builtin_amdgcn_readlane(gran, k++);
+        const uint8_t *src = a.cache + (int64_t)max(here, 0) * GB + lane * 16;
 #pragma unroll
-        for (int i = 0; i < GB / 1024; i++)
-            __builtin_amdgcn_global_load_lds((const void *)(src + i * 1024), (lds_ptr_t)(dst + i * 1024), 16, 0, 0);
-        if (lane == 0) none[stage][wave] = gn < 0;
+        for (int i = 0; i < GB / 4096; i++) load_lds_4k(src + i * 4096, lds + ST * STAGE + wave * GB + i * 4096);
+        info[ST][wave] = here;
+    };
+    // The wave's granule of tile v is there. Where not every pair of the workgroup sees all of the tile: what
+    // a key holds that none sees does not count, a NaN or an infinity either (0 times them is NaN); values
+    // that are no numbers and only some see are taken out, and go to those by themselves below.
+    auto clean = [&](int key0, auto stage) __attribute__((always_inline)) {
+        constexpr int ST = decltype(stage)::value;
+        if (here >= 0 && key0 + KEYS - 1 <= g.pos0 && (a.window == 0 || key0 > g.pos1 - a.window || key0 + KEYS <= sk)) return;
+        const int above = a.window ? g.pos0 - a.window : -1;
+        bool odd = false;
+#pragma unroll 1
+        for (int i = 0; i < D / 32; i++) {
+            // 64 lanes: a half's keys of 64 dims
+            u32x4 *at = (u32x4 *)(lds + ST * STAGE + wave * GB + D * 32 + i * 1024 + lane * 16);
+            const int half = i / (D / 64);
+            u32x4 x = *at;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int key = key0 + 16 * wave + 8 * (j >> 1) + 4 * half + 2 * (j & 1) + e;
+                    const bool seen = here >= 0 && key <= g.pos1 && (key > above || key < sk);
+                    const uint32_t bits = e ? 0xffff0000u : 0xffffu, big = e ? 0x7f800000u : 0x7f80u;
+                    const bool bad = (x[j] & big) == big;
+                    odd = odd || (seen && bad);
+                    if (!seen || bad) x[j] &= ~bits;
+                }
+            *at = x;
+        }
+        if (__ballot(odd)) info[ST][wave] = here | ODD;
     };
     if (first < last) {
         load_granules(first);
-        load_tile(first, 0);
+        load_tile(first, std::integral_constant<int, 0>{});
     }
 
     bf16x8 qf[KK];
@@ -682,40 +732,37 @@ __device__ __forceinline__ void many_pairs(const Attn &a, int item, uint8_t *lds
     }
 
     f32x16 o[DT] = {};
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, mc = 0.f, l[4] = {};
     const uint8_t *kl = lds + (l32 >> 4) * GB + hi * 256 + (l32 & 15) * 16;  // + half, dims
     const uint8_t *vl = lds + D * 32 + hi * (D * 16) + l32 * 16;             // + granule, dims
 
-    for (int v = first; v < last; v++) {
-        const int stage = (v - first) & 1;
-        __builtin_amdgcn_s_waitcnt(WAIT_VM0_LGKM0);
-        __syncthreads();
+    auto step = [&](int v, auto stage) __attribute__((always_inline)) {
+        constexpr int ST = decltype(stage)::value;
         const int key0 = tile_at(g, v) * KEYS;
-        uint32_t gone = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) gone |= none[stage][i] ? 1u << i : 0u;
-        gone = __builtin_amdgcn_readfirstlane(gone);
-        if (v + 1 < last) load_tile(v + 1, stage ^ 1);
+        lds_wait();
+        clean(key0, stage);
+        __syncthreads();
+        if (v + 1 < last) load_tile(v + 1, std::integral_constant<int, ST ^ 1>{});
         // no pair of the wave sees any of it
-        if (!any || key0 > w.pos1 || (a.window && key0 + KEYS - 1 <= low0 && key0 >= sk)) continue;
-        // every pair sees all of it, or some do not
-        const bool some = !(key0 + KEYS - 1 <= pmin && gone == 0 && (a.window == 0 || key0 > w.pos1 - a.window || key0 + KEYS <= sk));
+        if (!any || key0 > w.pos1 || (a.window && key0 + KEYS - 1 <= low0 && key0 >= sk)) return;
+        const int about = info[ST][lane & 3];
 
         f32x16 s[2] = {};
 #pragma unroll
         for (int b = 0; b < 2; b++)
 #pragma unroll
             for (int kk = 0; kk < KK; kk++)
-                s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8 *)(kl + stage * STAGE + b * 2 * GB + kk * 512), qf[kk],
-                                                               s[b], 0, 0, 0);
-        if (some) {
+                s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8 *)(kl + ST * STAGE + b * 2 * GB + kk * 512), qf[kk], s[b], 0, 0, 0);
+        // every pair sees all of it, or some do not
+        const uint32_t gone = (uint32_t)__ballot(about < 0) & 15u;
+        if (key0 + KEYS - 1 > pmin || gone || (a.window && key0 <= w.pos1 - a.window && key0 + KEYS > sk)) {
 #pragma unroll
             for (int b = 0; b < 2; b++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     const int key = key0 + 32 * b + 8 * (e >> 2) + 4 * hi + (e & 3);
-                    const bool ok = key <= pos && (key > low || key < sk) && !((gone >> (2 * b + (e >> 3))) & 1u);
-                    s[b][e] = ok ? s[b][e] : -INFINITY;
+                    const int ok = (int)(key <= pos) & ((int)(key > low) | (int)(key < sk)) & (int)(~gone >> (2 * b + (e >> 3)));
+                    s[b][e] = ok & 1 ? s[b][e] : -INFINITY;
                 }
         }
         float m0 = s[0][0], m1 = s[1][0];
@@ -730,83 +777,57 @@ __device__ __forceinline__ void many_pairs(const Attn &a, int item, uint8_t *lds
             const float top = fmaxf(mx, m);
             const float al = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * a.sl2);
             m = top;
-            l *= al;
+            mc = m == -INFINITY ? 0.f : -m * a.sl2;
+#pragma unroll
+            for (int i = 0; i < 4; i++) l[i] *= al;
 #pragma unroll
             for (int dt = 0; dt < DT; dt++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) o[dt][e] *= al;
         }
-        const float c = m == -INFINITY ? 0.f : -m * a.sl2;
-        bf16x8 pf[4];
 #pragma unroll
         for (int b = 0; b < 2; b++) {
             uint32_t p[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][2 * e], a.sl2, c));
-                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][2 * e + 1], a.sl2, c));
-                l += x;
-                l += y;
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][2 * e], a.sl2, mc));
+                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][2 * e + 1], a.sl2, mc));
+                l[2 * b] += x;
+                l[2 * b + 1] += y;
                 p[e] = pack_bf16x2(x, y);
             }
 #pragma unroll
-            for (int j = 0; j < 2; j++)
-                pf[2 * b + j] = __builtin_bit_cast(bf16x8, u32x4{p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]});
-        }
-        const uint8_t *vs = vl + stage * STAGE;
-        if (some) {
-            // what a key holds that no pair sees does not count; where only some see a value that is no
-            // number, it goes to those by itself
-            auto seen = [&](int j, int i) __attribute__((always_inline)) {
-                const int key = key0 + 16 * j + 8 * (i >> 1) + 4 * hi + 2 * (i & 1);
-                const uint32_t x = (key <= w.pos1 && (key > low0 || key < sk) ? 0xffffu : 0u) |
-                                   (key + 1 <= w.pos1 && (key + 1 > low0 || key + 1 < sk) ? 0xffff0000u : 0u);
-                return (gone >> j) & 1u ? 0u : x;
-            };
-            uint32_t odd = 0;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                u32x4 keep;
-#pragma unroll
-                for (int i = 0; i < 4; i++) keep[i] = seen(j, i);
-#pragma unroll
-                for (int dt = 0; dt < DT; dt++) {
-                    u32x4 x = *(const u32x4 *)(vs + j * GB + dt * 512) & keep;
-                    if (w.pos0 != w.pos1) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const uint32_t bad = ((x[i] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((x[i] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
-                            odd |= bad;
-                            x[i] &= ~bad;
-                        }
-                    }
-                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), pf[j], o[dt], 0, 0, 0);
-                }
-            }
-            if (__builtin_expect(__ballot(odd != 0) != 0, 0)) {
-#pragma unroll 1
-                for (int key = 0; key < KEYS; key++) {
-                    const bool sees = key0 + key <= pos && (key0 + key > low || key0 + key < sk) && !((gone >> (key >> 4)) & 1u);
-                    const uint8_t *src = lds + stage * STAGE + (key >> 4) * GB + granule_v(D, key & 15, 4 * hi);
-#pragma unroll
-                    for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-                        for (int e = 0; e < 16; e++) {
-                            const uint32_t u = (uint32_t)*(const uint16_t *)(src + (32 * dt + 8 * (e >> 2) + (e & 3)) * 16) << 16;
-                            if (sees && (u & 0x7f800000u) == 0x7f800000u) o[dt][e] += __uint_as_float(u);
-                        }
-                }
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
+            for (int j = 0; j < 2; j++) {
+                const bf16x8 pf = __builtin_bit_cast(bf16x8, u32x4{p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]});
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++)
-                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8 *)(vs + j * GB + dt * 512), pf[j], o[dt], 0, 0, 0);
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8 *)(vl + ST * STAGE + (2 * b + j) * GB + dt * 512), pf, o[dt], 0, 0, 0);
+            }
         }
+        if (__builtin_expect(__ballot(about >= ODD) != 0, 0)) {
+#pragma unroll 1
+            for (int i = 0; i < KEYS; i++) {
+                const int key = key0 + i, from = __builtin_amdgcn_readlane(about, i >> 4);
+                if (from < ODD) continue;
+                const bool sees = key <= pos && (key > low || key < sk);
+                const uint8_t *src = a.cache + (int64_t)(from - ODD) * GB + granule_v(D, i & 15, 0);
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const uint32_t u = (uint32_t)*(const uint16_t *)(src + (32 * dt + 8 * (e >> 2) + 4 * hi + (e & 3)) * 16) << 16;
+                        if (sees && (u & 0x7f800000u) == 0x7f800000u) o[dt][e] += __uint_as_float(u);
+                    }
+            }
+        }
+    };
+    for (int v = first; v < last; v += 2) {
+        step(v, std::integral_constant<int, 0>{});
+        if (v + 1 < last) step(v + 1, std::integral_constant<int, 1>{});
     }
 
-    l += __shfl_xor(l, 32);
+    float lsum = l[0] + l[1] + l[2] + l[3];
+    lsum += __shfl_xor(lsum, 32);
     auto row_of = [&](int p) __attribute__((always_inline)) {
         const int at = (f0 + p) / a.G, head = f0 + p - at * a.G;
         return a.out + ((int64_t)(rq.start + at) * a.Hkv * a.G + h * a.G + head) * D;
@@ -814,7 +835,7 @@ __device__ __forceinline__ void many_pairs(const Attn &a, int item, uint8_t *lds
     const int p = 32 * wave + l32;
     if (pc.shares == 1) {
         if (!there) return;
-        const float inv = l == 0.f ? 0.f : 1.0f / l;  // a pair that sees no key gives zeros
+        const float inv = lsum == 0.f ? 0.f : 1.0f / lsum;  // a pair that sees no key gives zeros
         uint16_t *dst = row_of(p) + 4 * hi;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
@@ -826,7 +847,7 @@ __device__ __forceinline__ void many_pairs(const Attn &a, int item, uint8_t *lds
     }
     if (there) {
         const Part pb(slot_at<Rows, D>(a, pc.slot + pc.share), slot_floats<Rows, D>());
-        if (hi == 0) pb.put2(Rows::TM * D + 2 * p, m, l);
+        if (hi == 0) pb.put2(Rows::TM * D + 2 * p, m, lsum);
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
