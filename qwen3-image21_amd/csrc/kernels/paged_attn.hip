@@ -111,9 +111,10 @@ __device__ __forceinline__ int rounds_of(const Attn &a, const Req &q) {
 }
 
 // What a workgroup takes: share `share` of `shares` of tile `tile` of request r's pairs for key head h; slot:
-// the tile's first of the shares' slots.
+// the tile's first of the shares' slots. rq: the request.
 struct Piece {
     int r, h, tile, share, shares, slot;
+    Req rq;
 };
 
 // sums over 256 threads: those before this one
@@ -138,11 +139,86 @@ __device__ __forceinline__ int64_t scan256(int64_t v, int64_t *part, int64_t &to
     return before + s - v;
 }
 
-// The piece of workgroup `item`, in request order (the last tiles first: under causal rows they see the
-// most keys; heads fastest); false: there is none. Every thread counts its share of the requests, and the one
-// whose share has the piece looks which.
+// A request's tiles and shares with `chunk` rounds a share (0: nothing is split); its pieces in the low
+// bits of the sums, the slots of a split one above.
+constexpr int HIGH = 44;
+constexpr int64_t LOW = ((int64_t)1 << HIGH) - 1;
+struct Split {
+    int tiles, shares;
+    int64_t pieces;
+};
+template <typename F>
+__device__ __forceinline__ Split split_of(const Attn &a, const Req &q, int64_t chunk) {
+    Split s;
+    s.tiles = tiles_of<F>(a, q);
+    s.shares = 1;
+    if (chunk && s.tiles) s.shares = max((int)min((rounds_of<F>(a, q) + chunk - 1) / chunk, (int64_t)F::MOST), 1);
+    const int64_t n = min((int64_t)s.tiles * s.shares * a.Hkv, (int64_t)1 << 27);
+    s.pieces = n + (s.shares > 1 ? n << HIGH : 0);
+    return s;
+}
+// rounds of a share, of `rounds` of all tiles for one head
+template <typename F>
+__device__ __forceinline__ int64_t chunk_of(const Attn &a, int64_t rounds) {
+    return max((int64_t)F::GRAIN, (rounds * a.Hkv + F::WANT - 1) / F::WANT);
+}
+// Piece `i` of a request whose sums start at `at`: heads fastest, the last tiles first (under causal rows
+// they see the most keys).
+template <typename F>
+__device__ __forceinline__ Piece piece_in(const Attn &a, int r, const Req &q, const Split &s, int i, int64_t at) {
+    Piece p;
+    const int x = i / a.Hkv;
+    p.r = r;
+    p.h = i - x * a.Hkv;
+    p.tile = s.tiles - 1 - x / s.shares;
+    p.share = x % s.shares;
+    p.shares = s.shares;
+    p.slot = (F::ROWS ? Few::SLOTS : 0) + (int)(at >> HIGH) + (p.tile * a.Hkv + p.h) * s.shares;
+    p.rq = q;
+    return p;
+}
+__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+// The piece of workgroup `item` of at most `most`, in request order; false: there is none. Up to 64
+// requests every wave counts them by itself, a lane each; of more, every thread counts its share and the one whose
+// share has the piece looks which.
 template <typename F>
 __device__ __forceinline__ bool piece_of(const Attn &a, int item, int most, Piece &out) {
+    if (a.R <= 64) {
+        const int lane = threadIdx.x & 63;
+        const Req q = lane < a.R ? req_of(a, lane) : Req{0, 0, 0};
+        int64_t chunk = 0, sum, all;
+        if (a.count) chunk = chunk_of<F>(a, wave_sum64((int64_t)tiles_of<F>(a, q) * rounds_of<F>(a, q)));
+        Split s;
+        for (;;) {
+            s = split_of<F>(a, q, chunk);
+            sum = s.pieces;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int64_t x = __shfl_up(sum, o);
+                if (lane >= o) sum += x;
+            }
+            all = __shfl(sum, 63);
+            if (!chunk || ((all & LOW) <= most && (all >> HIGH) <= F::SLOTS)) break;
+            // more pieces than there can be: `starts` that overlap. Every share has to arrive, so nothing is split.
+            chunk = (all & LOW) <= most ? 2 * chunk : 0;
+        }
+        const uint64_t behind = __ballot((sum & LOW) > item);
+        if (!behind) return false;
+        const int r = __builtin_ctzll(behind);
+        const int64_t at = __shfl(sum - s.pieces, r);
+        s.tiles = __builtin_amdgcn_readlane(s.tiles, r);
+        s.shares = __builtin_amdgcn_readlane(s.shares, r);
+        out = piece_in<F>(a, r,
+                          Req{__builtin_amdgcn_readlane(q.start, r), __builtin_amdgcn_readlane(q.n, r), __builtin_amdgcn_readlane(q.len, r)},
+                          s, item - __builtin_amdgcn_readfirstlane((int)(at & LOW)), at);
+        out.slot = __builtin_amdgcn_readfirstlane(out.slot);
+        return true;
+    }
     __shared__ int64_t part[4];
     __shared__ Piece found;
     const int c = (a.R + 255) / 256, r0 = min((int)threadIdx.x * c, a.R), r1 = min(r0 + c, a.R);
@@ -154,58 +230,32 @@ __device__ __forceinline__ bool piece_of(const Attn &a, int item, int most, Piec
             rounds += (int64_t)tiles_of<F>(a, q) * rounds_of<F>(a, q);
         }
         scan256(rounds, part, all);
-        chunk = max((int64_t)F::GRAIN, (all * a.Hkv + F::WANT - 1) / F::WANT);
+        chunk = chunk_of<F>(a, all);
     }
-    // tiles and shares of request r; its pieces in the low bits of the sums, the slots of a split one above
-    auto split = [&](int r, int &tiles, int &shares) __attribute__((always_inline)) {
-        const Req q = req_of(a, r);
-        tiles = tiles_of<F>(a, q);
-        shares = 1;
-        if (chunk && tiles) shares = max((int)min((rounds_of<F>(a, q) + chunk - 1) / chunk, (int64_t)F::MOST), 1);
-    };
-    constexpr int HIGH = 44;
-    constexpr int64_t LOW = ((int64_t)1 << HIGH) - 1;
-    auto pieces = [&](int tiles, int shares) __attribute__((always_inline)) {
-        const int64_t n = min((int64_t)tiles * shares * a.Hkv, (int64_t)1 << 27);
-        return n + (shares > 1 ? n << HIGH : 0);
-    };
     int64_t mine, at;
-    int tiles, shares;
     for (;;) {
         mine = 0;
-        for (int r = r0; r < r1; r++) {
-            split(r, tiles, shares);
-            mine += pieces(tiles, shares);
-        }
+        for (int r = r0; r < r1; r++) mine += split_of<F>(a, req_of(a, r), chunk).pieces;
         at = scan256(mine, part, all);
         if (!chunk || ((all & LOW) <= most && (all >> HIGH) <= F::SLOTS)) break;
-        // more pieces than there can be: `starts` that overlap. Every share has to arrive, so nothing is split.
         chunk = (all & LOW) <= most ? 2 * chunk : 0;
     }
     if (item >= (all & LOW)) return false;
-    if (item >= (at & LOW) && item < (at & LOW) + (mine & LOW)) {
-        int r = r0;
-        for (;; r++) {
-            split(r, tiles, shares);
-            const int64_t n = pieces(tiles, shares);
-            if (item < ((at + n) & LOW)) break;
-            at += n;
+    if (item >= (at & LOW) && item < (at & LOW) + (mine & LOW))
+        for (int r = r0;; r++) {
+            const Req q = req_of(a, r);
+            const Split s = split_of<F>(a, q, chunk);
+            if (item < ((at + s.pieces) & LOW)) {
+                found = piece_in<F>(a, r, q, s, (int)(item - (at & LOW)), at);
+                break;
+            }
+            at += s.pieces;
         }
-        const int i = (int)(item - (at & LOW)), x = i / a.Hkv;
-        found.r = r;
-        found.h = i - x * a.Hkv;
-        found.tile = tiles - 1 - x / shares;
-        found.share = x % shares;
-        found.shares = shares;
-        found.slot = (F::ROWS ? Few::SLOTS : 0) + (int)(at >> HIGH) + (found.tile * a.Hkv + found.h) * shares;
-    }
     __syncthreads();
-    out.r = __builtin_amdgcn_readfirstlane(found.r);
-    out.h = __builtin_amdgcn_readfirstlane(found.h);
-    out.tile = __builtin_amdgcn_readfirstlane(found.tile);
-    out.share = __builtin_amdgcn_readfirstlane(found.share);
-    out.shares = __builtin_amdgcn_readfirstlane(found.shares);
-    out.slot = __builtin_amdgcn_readfirstlane(found.slot);
+    const int *src = (const int *)&found;
+    int *dst = (int *)&out;
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(Piece) / 4); i++) dst[i] = __builtin_amdgcn_readfirstlane(src[i]);
     return true;
 }
 
@@ -394,7 +444,7 @@ __device__ __forceinline__ void few_pairs(const Attn &a, int item, uint8_t *lds)
     Piece pc;
     if (!piece_of<Few>(a, item, (int)gridDim.x - a.row_pieces, pc)) return;
     const int r = pc.r, h = pc.h, tile = pc.tile;
-    const Req rq = req_of(a, r);
+    const Req rq = pc.rq;
     const Range g = range_of<KT>(a, rq, tile * 32, 32);
     // the share's tiles: whole rounds
     const int rounds = (g.tiles + 3) / 4;
@@ -644,7 +694,7 @@ __device__ __forceinline__ void many_pairs(const Attn &a, int item, uint8_t *lds
     Piece pc;
     if (!piece_of<Rows>(a, item, a.row_pieces, pc)) return;
     const int r = pc.r, h = pc.h, f0 = pc.tile * Rows::TM;
-    const Req rq = req_of(a, r);
+    const Req rq = pc.rq;
     const Range g = range_of<KEYS>(a, rq, f0, Rows::TM);
     const int first = (int)((int64_t)g.tiles * pc.share / pc.shares);
     const int last = (int)((int64_t)g.tiles * (pc.share + 1) / pc.shares);
