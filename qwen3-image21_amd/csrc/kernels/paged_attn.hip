@@ -29,15 +29,15 @@
 namespace qimm {
 namespace {
 
-// The two forms: pairs of a tile, keys of a round, and the shares: as many as make WANT workgroups of all
-// requests, at least GRAIN rounds each, at most MOST of a tile; fewer where they are more than SLOTS.
+// The two forms: pairs of a tile, keys of a round, and the shares: at least GRAIN rounds each, at most MOST of
+// a tile, SLOTS in all; `want` workgroups are the aim (Attn).
 struct Few {
     static constexpr bool ROWS = false;
-    static constexpr int TM = 32, ROUND = 128, WANT = 1024, GRAIN = 4, MOST = 128, SLOTS = WANT / 4 * 5;
+    static constexpr int TM = 32, ROUND = 128, GRAIN = 4, MOST = 128, SLOTS = 1280;
 };
 struct Rows {
     static constexpr bool ROWS = true;
-    static constexpr int TM = 128, ROUND = 64, WANT = 512, GRAIN = 8, MOST = 64, SLOTS = WANT / 4 * 5;
+    static constexpr int TM = 128, ROUND = 64, GRAIN = 8, MOST = 64, SLOTS = 640;
 };
 constexpr int KT = 32;          // keys of a wave's tile, few pairs
 constexpr int FEW_PAIRS = 32;   // more pairs of a request and key head are rows
@@ -63,6 +63,7 @@ struct Attn {
                            // is long enough to be split
     float *part;           // per slot O [TM][D], then (m, l) [TM]
     int32_t row_pieces;    // workgroups for rows, before those for few
+    int32_t want[2];       // workgroups that few pairs, rows are divided into at least, where they are long enough
 };
 
 // a request's rows and tokens
@@ -157,10 +158,20 @@ __device__ __forceinline__ Split split_of(const Attn &a, const Req &q, int64_t c
     s.pieces = n + (s.shares > 1 ? n << HIGH : 0);
     return s;
 }
-// rounds of a share, of `rounds` of all tiles for one head
+// Rounds of a share, of `rounds` of all tiles for one head and `tiles` of them, and whether `all` pieces and
+// slots of it will do (else a little longer shares are tried, at the end nothing is split). Rows that one round of
+// workgroups takes are divided into no more than that, those of not much more than one into shares half as
+// long: 136 tiles of 100 rounds in 544 shares took 139 us, in 408 87.
 template <typename F>
-__device__ __forceinline__ int64_t chunk_of(const Attn &a, int64_t rounds) {
-    return max((int64_t)F::GRAIN, (rounds * a.Hkv + F::WANT - 1) / F::WANT);
+__device__ __forceinline__ int64_t chunk_of(const Attn &a, int64_t rounds, int64_t tiles) {
+    const int64_t want = a.want[F::ROWS], c = (rounds * a.Hkv + want - 1) / want;
+    return max((int64_t)F::GRAIN, F::ROWS && tiles * a.Hkv > want && tiles * a.Hkv < 2 * want ? (c + 1) / 2 : c);
+}
+template <typename F>
+__device__ __forceinline__ bool will_do(const Attn &a, int64_t all, int64_t tiles, int most) {
+    const int64_t slots = all >> HIGH, n = all & LOW;
+    if (slots == 0) return true;
+    return slots <= F::SLOTS && n <= most && !(F::ROWS && tiles * a.Hkv <= a.want[1] && n > a.want[1]);
 }
 // Piece `i` of a request whose sums start at `at`: heads fastest, the last tiles first (under causal rows
 // they see the most keys).
@@ -190,22 +201,40 @@ template <typename F>
 __device__ __forceinline__ bool piece_of(const Attn &a, int item, int most, Piece &out) {
     if (a.R <= 64) {
         const int lane = threadIdx.x & 63;
-        const Req q = lane < a.R ? req_of(a, lane) : Req{0, 0, 0};
-        int64_t chunk = 0, sum, all;
-        if (a.count) chunk = chunk_of<F>(a, wave_sum64((int64_t)tiles_of<F>(a, q) * rounds_of<F>(a, q)));
+        Req q = lane < a.R ? req_of(a, lane) : Req{0, 0, 0};
+        int64_t chunk = 0, tiles = 0, sum, all;
+        if (a.count) {
+            const int t = tiles_of<F>(a, q);
+            tiles = wave_sum64(t);
+            chunk = chunk_of<F>(a, wave_sum64((int64_t)t * rounds_of<F>(a, q)), tiles);
+        }
         Split s;
-        for (;;) {
+        for (;; chunk += (chunk + 7) / 8) {
             s = split_of<F>(a, q, chunk);
-            sum = s.pieces;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int64_t x = __shfl_up(sum, o);
-                if (lane >= o) sum += x;
+            all = wave_sum64(s.pieces);
+            if (!chunk || will_do<F>(a, all, tiles, most)) break;
+        }
+        int at_r = lane;
+        if (F::ROWS && a.R > 1) {
+            // the longest shares first: lane i takes the request of rank i
+            const int w = s.tiles ? (rounds_of<F>(a, q) + s.shares - 1) / s.shares : -1;
+            int rank = 0;
+            for (int i = 0; i < a.R; i++) {
+                const int x = __builtin_amdgcn_readlane(w, i);
+                rank += x > w || (x == w && i < lane);
             }
-            all = __shfl(sum, 63);
-            if (!chunk || ((all & LOW) <= most && (all >> HIGH) <= F::SLOTS)) break;
-            // more pieces than there can be: `starts` that overlap. Every share has to arrive, so nothing is split.
-            chunk = (all & LOW) <= most ? 2 * chunk : 0;
+            rank = (lane < a.R ? rank : lane) * 4;
+            q.start = __builtin_amdgcn_ds_permute(rank, q.start);
+            q.n = __builtin_amdgcn_ds_permute(rank, q.n);
+            q.len = __builtin_amdgcn_ds_permute(rank, q.len);
+            at_r = __builtin_amdgcn_ds_permute(rank, lane);
+            s = split_of<F>(a, q, chunk);
+        }
+        sum = s.pieces;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int64_t x = __shfl_up(sum, o);
+            if (lane >= o) sum += x;
         }
         const uint64_t behind = __ballot((sum & LOW) > item);
         if (!behind) return false;
@@ -213,7 +242,7 @@ __device__ __forceinline__ bool piece_of(const Attn &a, int item, int most, Piec
         const int64_t at = __shfl(sum - s.pieces, r);
         s.tiles = __builtin_amdgcn_readlane(s.tiles, r);
         s.shares = __builtin_amdgcn_readlane(s.shares, r);
-        out = piece_in<F>(a, r,
+        out = piece_in<F>(a, __builtin_amdgcn_readlane(at_r, r),
                           Req{__builtin_amdgcn_readlane(q.start, r), __builtin_amdgcn_readlane(q.n, r), __builtin_amdgcn_readlane(q.len, r)},
                           s, item - __builtin_amdgcn_readfirstlane((int)(at & LOW)), at);
         out.slot = __builtin_amdgcn_readfirstlane(out.slot);
@@ -222,23 +251,25 @@ __device__ __forceinline__ bool piece_of(const Attn &a, int item, int most, Piec
     __shared__ int64_t part[4];
     __shared__ Piece found;
     const int c = (a.R + 255) / 256, r0 = min((int)threadIdx.x * c, a.R), r1 = min(r0 + c, a.R);
-    int64_t chunk = 0, all;
+    int64_t chunk = 0, tiles = 0, all;
     if (a.count) {
-        int64_t rounds = 0;
+        int64_t t = 0, rounds = 0;
         for (int r = r0; r < r1; r++) {
             const Req q = req_of(a, r);
-            rounds += (int64_t)tiles_of<F>(a, q) * rounds_of<F>(a, q);
+            const int n = tiles_of<F>(a, q);
+            t += n;
+            rounds += (int64_t)n * rounds_of<F>(a, q);
         }
+        scan256(t, part, tiles);
         scan256(rounds, part, all);
-        chunk = chunk_of<F>(a, all);
+        chunk = chunk_of<F>(a, all, tiles);
     }
     int64_t mine, at;
-    for (;;) {
+    for (;; chunk += (chunk + 7) / 8) {
         mine = 0;
         for (int r = r0; r < r1; r++) mine += split_of<F>(a, req_of(a, r), chunk).pieces;
         at = scan256(mine, part, all);
-        if (!chunk || ((all & LOW) <= most && (all >> HIGH) <= F::SLOTS)) break;
-        chunk = (all & LOW) <= most ? 2 * chunk : 0;
+        if (!chunk || will_do<F>(a, all, tiles, most)) break;
     }
     if (item >= (all & LOW)) return false;
     if (item >= (at & LOW) && item < (at & LOW) + (mine & LOW))
@@ -259,6 +290,12 @@ __device__ __forceinline__ bool piece_of(const Attn &a, int item, int most, Piec
     return true;
 }
 
+// the larger magnitudes of two pairs of bf16 values, as bits
+__device__ __forceinline__ uint32_t magnitude2(uint32_t m, uint32_t w) {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m), __builtin_bit_cast(u16x2, w & 0x7fff7fffu)));
+}
+// (of values or their magnitudes)
 __device__ __forceinline__ bool not_finite2(uint32_t w) {
     return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
@@ -456,7 +493,6 @@ __device__ __forceinline__ void few_pairs(const Attn &a, int item, uint8_t *lds)
     const bool there = row < rq.n;
     const int pos = !there ? -1 : a.causal ? rq.len - rq.n + row : rq.len - 1;
     const int low = a.window ? pos - a.window : -1;  // sees key j <= pos if j > low or j < g.sk
-    const int low0 = a.window ? g.pos0 - a.window : -1;
     const int pmin = tile * 32 + 31 < rq.n * a.G ? g.pos0 : -1;  // every pair sees up to it
 
     // ---- queries: dims 16 kk + 8 hi .. + 7 of the lane's pair ----
@@ -571,28 +607,21 @@ __device__ __forceinline__ void few_pairs(const Attn &a, int item, uint8_t *lds)
         bf16x8 pf[2];
 #pragma unroll
         for (int j = 0; j < 2; j++) pf[j] = __builtin_bit_cast(bf16x8, u32x4{p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]});
-        // what a key holds that no pair sees does not count, a NaN or an infinity either (0 times them
-        // is NaN); where only some pairs see one, it goes to those by itself
+        // where not every pair sees all of it, values that are no numbers (0 times them is NaN) go to
+        // those that see them by themselves
         if (some) {
-            bool odd = false;
+            uint32_t mag = 0;
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
+            for (int j = 0; j < 2; j++)
 #pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    const int key = key0 + 16 * j + 8 * (w >> 1) + 4 * hi + 2 * (w & 1);
-                    uint32_t seen = (key <= g.pos1 && (key > low0 || key < g.sk) ? 0xffffu : 0u) |
-                                    (key + 1 <= g.pos1 && (key + 1 > low0 || key + 1 < g.sk) ? 0xffff0000u : 0u);
-                    if ((j ? g1 : g0) < 0) seen = 0;
+                for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-                    for (int dt = 0; dt < DT; dt++) {
-                        vc[j][dt][w] &= seen;
-                        odd = odd || not_finite2(vc[j][dt][w]);
-                    }
-                }
-            }
-            if (g.pos0 != g.pos1 && __ballot(odd))
-                add_not_finite<D>(vc, o, (uint8_t *)(so + wave * 32 * PITCH), lane,
-                                  [&](int key) { return key0 + key <= pos && (key0 + key > low || key0 + key < g.sk); });
+                    for (int w = 0; w < 4; w++) mag = magnitude2(mag, vc[j][dt][w]);
+            if (__builtin_expect(__ballot(not_finite2(mag)) != 0, 0))
+                add_not_finite<D>(vc, o, (uint8_t *)(so + wave * 32 * PITCH), lane, [&](int i) {
+                    const int key = key0 + i;
+                    return key <= pos && (key > low || key < g.sk) && (i < 16 ? g0 : g1) >= 0;
+                });
         }
 #pragma unroll
         for (int j = 0; j < 2; j++)
@@ -736,32 +765,37 @@ __device__ __forceinline__ void many_pairs(const Attn &a, int item, uint8_t *lds
         for (int i = 0; i < GB / 4096; i++) load_lds_4k(src + i * 4096, lds + ST * STAGE + wave * GB + i * 4096);
         info[ST][wave] = here;
     };
-    // The wave's granule of tile v is there. Where not every pair of the workgroup sees all of the tile: what
-    // a key holds that none sees does not count, a NaN or an infinity either (0 times them is NaN); values
-    // that are no numbers and only some see are taken out, and go to those by themselves below.
+    // The wave's granule of tile v is there. Where not every pair of the workgroup sees all of the tile, values
+    // that are no numbers are taken out (0 times them is NaN); those that some pairs see go to these by
+    // themselves below.
     auto clean = [&](int key0, auto stage) __attribute__((always_inline)) {
         constexpr int ST = decltype(stage)::value;
         if (here >= 0 && key0 + KEYS - 1 <= g.pos0 && (a.window == 0 || key0 > g.pos1 - a.window || key0 + KEYS <= sk)) return;
+        u32x4 *const mine = (u32x4 *)(lds + ST * STAGE + wave * GB + D * 32 + lane * 16);
+        uint32_t mag = 0;
+#pragma unroll
+        for (int i = 0; i < D / 32; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) mag = magnitude2(mag, mine[64 * i][j]);
+        if (__builtin_expect(__ballot(not_finite2(mag)) == 0, 1)) return;
         const int above = a.window ? g.pos0 - a.window : -1;
         bool odd = false;
 #pragma unroll 1
         for (int i = 0; i < D / 32; i++) {
             // 64 lanes: a half's keys of 64 dims
-            u32x4 *at = (u32x4 *)(lds + ST * STAGE + wave * GB + D * 32 + i * 1024 + lane * 16);
             const int half = i / (D / 64);
-            u32x4 x = *at;
+            u32x4 x = mine[64 * i];
 #pragma unroll
             for (int j = 0; j < 4; j++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     const int key = key0 + 16 * wave + 8 * (j >> 1) + 4 * half + 2 * (j & 1) + e;
-                    const bool seen = here >= 0 && key <= g.pos1 && (key > above || key < sk);
-                    const uint32_t bits = e ? 0xffff0000u : 0xffffu, big = e ? 0x7f800000u : 0x7f80u;
-                    const bool bad = (x[j] & big) == big;
-                    odd = odd || (seen && bad);
-                    if (!seen || bad) x[j] &= ~bits;
+                    const uint32_t big = e ? 0x7f800000u : 0x7f80u;
+                    if ((x[j] & big) != big) continue;
+                    odd = odd || (here >= 0 && key <= g.pos1 && (key > above || key < sk));
+                    x[j] &= e ? 0xffffu : 0xffff0000u;
                 }
-            *at = x;
+            mine[64 * i] = x;
         }
         if (__ballot(odd)) info[ST][wave] = here | ODD;
     };
@@ -936,7 +970,10 @@ hipError_t launch_paged_attention(const PageDims &d, const uint8_t *layer, const
     Attn a{x.q, x.q_row, x.q_head, layer, d.pages, x.tables, x.max_pages, x.lengths, x.starts, (int32_t)x.requests,
            (int32_t)x.rows, d.kv_heads, (int32_t)g, ps16, (uint32_t)(((1ull << 32) + ps16 - 1) / ps16),
            (int32_t)cap, x.causal, (int32_t)std::min<int64_t>(x.window, 0x7fffffff),
-           (int32_t)std::min<int64_t>(x.sinks, 0x7fffffff), x.scale * 1.4426950408889634f, x.out, nullptr, nullptr, 0};
+           (int32_t)std::min<int64_t>(x.sinks, 0x7fffffff), x.scale * 1.4426950408889634f, x.out, nullptr, nullptr, 0, {}};
+    const int cus = std::max(device_cu_count(), 1);
+    a.want[0] = std::min(4 * cus, Few::SLOTS);
+    a.want[1] = std::min(2 * cus, Rows::SLOTS);  // two workgroups a CU
     // Workgroups: of a request with few pairs one for each key head, of one with many at most a tile more
     // than its pairs fill, and the shares. Without starts every request has g pairs.
     const bool rows = x.starts ? x.rows * g > FEW_PAIRS : g > FEW_PAIRS, few = g <= FEW_PAIRS;
@@ -945,8 +982,8 @@ hipError_t launch_paged_attention(const PageDims &d, const uint8_t *layer, const
     if (cap > std::min(Few::GRAIN * Few::ROUND, Rows::GRAIN * Rows::ROUND)) {
         a.count = (uint32_t *)scratch;
         a.part = (float *)((char *)scratch + PAGED_COUNTER_BYTES);
-        if (many) many += Rows::WANT;
-        if (tokens) tokens += Few::WANT;
+        if (many) many += 2 * a.want[1];
+        if (tokens) tokens += a.want[0];
     }
     if (many + tokens >= (int64_t)1 << 24) return hipErrorInvalidValue;
     a.row_pieces = (int32_t)many;
