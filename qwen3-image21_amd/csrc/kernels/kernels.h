@@ -400,7 +400,7 @@ struct PagedAttnArgs {
 // scratch: paged_attention_scratch bytes, of which the first PAGED_COUNTER_BYTES are zero before the
 // first call; every call leaves them zero
 size_t paged_attention_scratch(int head_dim);
-constexpr size_t PAGED_COUNTER_BYTES = 8192;
+constexpr size_t PAGED_COUNTER_BYTES = 16384;
 hipError_t launch_paged_attention(const PageDims &d, const uint8_t *layer, const PagedAttnArgs &a, void *scratch,
                                   hipStream_t stream);
 

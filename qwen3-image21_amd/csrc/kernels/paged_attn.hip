@@ -41,7 +41,7 @@ struct Rows {
 };
 constexpr int KT = 32;          // keys of a wave's tile, few pairs
 constexpr int FEW_PAIRS = 32;   // more pairs of a request and key head are rows
-static_assert((Few::SLOTS + Rows::SLOTS) * 4 <= PAGED_COUNTER_BYTES, "a counter per slot");
+static_assert(2 * (Few::SLOTS + Rows::SLOTS) * 4 <= PAGED_COUNTER_BYTES, "two counters per slot");
 
 struct Attn {
     const uint16_t *q;
@@ -59,8 +59,8 @@ struct Attn {
     int32_t causal, window, sinks;  // window 0: none
     float sl2;             // scale * log2 e
     uint16_t *out;
-    uint32_t *count;       // arrivals per slot, the few's and the rows', zero between calls; null: no request
-                           // is long enough to be split
+    uint32_t *count;       // arrivals per slot, the few's and the rows', of shares and of teams, zero between
+                           // calls; null: no request is long enough to be split
     float *part;           // per slot O [TM][D], then (m, l) [TM]
     int32_t row_pieces;    // workgroups for rows, before those for few
     int32_t want[2];       // workgroups that few pairs, rows are divided into at least, where they are long enough
@@ -331,79 +331,122 @@ __device__ __forceinline__ const float *slot_at(const Attn &a, int slot) {
     return F::ROWS ? a.part + few + (int64_t)(slot - Few::SLOTS) * slot_floats<F, D>() : a.part + (int64_t)slot * slot_floats<F, D>();
 }
 
-// After the last of a tile's shares has stored its sums: the join, by 256 threads. pairs: those of the
-// tile that there are; `lds` MOST * pairs + 8 * D floats; row(p) the output of pair p.
-template <typename F, int D, typename Row>
-__device__ __forceinline__ void join_shares(const Attn &a, const Piece &pc, int pairs, float *lds, Row row) {
-    constexpr int TM = F::TM, MOST = F::MOST;
-    constexpr uint32_t SF = slot_floats<F, D>();
-    const Part pb(slot_at<F, D>(a, pc.slot), (uint32_t)pc.shares * SF);
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    // a share's factor for each pair: exp2 of its maximum relative to the largest, over the sum
-    for (int p = wave; p < pairs; p += 4) {
-        float m[MOST / 64], l[MOST / 64], mm = -INFINITY, ll = 0.f;
+// Where a thread's vectors of four sums lie in a slot, i < TM D / 1024 of them a thread: rows of D for few pairs,
+// for rows as the waves hold them (a wave's stores are 1 KB in a row).
+template <typename F, int D>
+__device__ __forceinline__ void vector_at(int i, uint32_t &at, int &pair, int &dim) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    if (F::ROWS) {
+        at = (uint32_t)(tid >> 6) * (32 * D) + i * 256 + lane * 4;
+        pair = (tid >> 6) * 32 + (lane & 31);
+        dim = 8 * i + 4 * (lane >> 5);
+    } else {
+        at = (uint32_t)(tid + 256 * i) * 4;
+        pair = (tid + 256 * i) / (D / 4);
+        dim = at % D;
+    }
+}
+
+// Joins the sums in n (up to TEAM) slots, `stride` apart from `first` on, by 256 threads: into the output, row(p)
+// that of pair p, or into the first of them. fac: TEAM * TM floats of LDS.
+constexpr int TEAM = 16;
+template <typename F, int D, int I0, int NV, int AT, typename Row>
+__device__ __forceinline__ void join_vectors(const Part &pb, int n, uint32_t step, int pairs, const float *fac, bool last, Row row) {
+    f32x4 x[NV] = {};
+    for (int s0 = 0; s0 < n; s0 += AT) {
+        f32x4 y[AT][NV];
 #pragma unroll
-        for (int i = 0; i < MOST / 64; i++) {
-            const int s = lane + 64 * i;
-            m[i] = -INFINITY;
-            l[i] = 0.f;
-            if (s < pc.shares) {
-                const u32x2 x = pb.get2((uint32_t)s * SF + TM * D + 2 * p);
-                m[i] = __uint_as_float(x[0]);
-                l[i] = __uint_as_float(x[1]);
+        for (int s = 0; s < AT; s++)
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                uint32_t at;
+                int p, d;
+                vector_at<F, D>(I0 + i, at, p, d);
+                y[s][i] = pb.get4((uint32_t)min(s0 + s, n - 1) * step + at);
             }
-            mm = fmaxf(mm, m[i]);
-        }
-        mm = max_wave(mm);
 #pragma unroll
-        for (int i = 0; i < MOST / 64; i++) {
-            m[i] = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[i] - mm) * a.sl2);
-            ll += l[i] * m[i];
-        }
-        ll = wave_sum(ll);
-        const float inv = ll == 0.f ? 0.f : 1.0f / ll;
+        for (int s = 0; s < AT; s++)
 #pragma unroll
-        for (int i = 0; i < MOST / 64; i++)
-            if (lane + 64 * i < pc.shares) lds[p * MOST + lane + 64 * i] = m[i] * inv;
+            for (int i = 0; i < NV; i++) {
+                uint32_t at;
+                int p, d;
+                vector_at<F, D>(I0 + i, at, p, d);
+                const float f = s0 + s < n && p < pairs ? fac[(s0 + s) * F::TM + p] : 0.f;
+                if (f != 0.f)  // (an infinity of a share that does not count would be NaN)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[i][e] += y[s][i][e] * f;
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        uint32_t at;
+        int p, d;
+        vector_at<F, D>(I0 + i, at, p, d);
+        if (p >= pairs) continue;
+        if (last)
+            *(u32x2 *)(row(p) + d) = u32x2{pack_bf16x2(x[i][0], x[i][1]), pack_bf16x2(x[i][2], x[i][3])};
+        else
+            pb.put4(at, x[i]);
+    }
+}
+template <typename F, int D, typename Row>
+__device__ __forceinline__ void join_shares(const Attn &a, int first, int n, int stride, int pairs, float *fac, bool last, Row row) {
+    const uint32_t step = (uint32_t)stride * slot_floats<F, D>();
+    const Part pb(slot_at<F, D>(a, first), (uint32_t)(n - 1) * step + slot_floats<F, D>());
+    // a share's factor for each pair: exp2 of its maximum relative to the largest, over the sum at last
+    const int p = threadIdx.x;
+    if (p < pairs) {
+        float m[TEAM], mm = -INFINITY, ll = 0.f;
+        u32x2 ml[TEAM];
+#pragma unroll
+        for (int s = 0; s < TEAM; s++) ml[s] = pb.get2((uint32_t)min(s, n - 1) * step + F::TM * D + 2 * p);
+#pragma unroll
+        for (int s = 0; s < TEAM; s++) {
+            m[s] = s < n ? __uint_as_float(ml[s][0]) : -INFINITY;
+            mm = fmaxf(mm, m[s]);
+        }
+#pragma unroll
+        for (int s = 0; s < TEAM; s++) {
+            m[s] = m[s] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m[s] - mm) * a.sl2);
+            ll += __uint_as_float(ml[s][1]) * m[s];
+        }
+        const float inv = !last ? 1.f : ll == 0.f ? 0.f : 1.0f / ll;
+#pragma unroll
+        for (int s = 0; s < TEAM; s++) fac[s * F::TM + p] = m[s] * inv;
+        if (!last) pb.put2(F::TM * D + 2 * p, mm, ll);
     }
     __syncthreads();
-    // D / 4 threads a pair; where they are more than the pairs need, each takes some of the shares
-    constexpr int COLS = D / 4, TEAMS = 256 / COLS;
-    const int team = tid / COLS, d = tid % COLS * 4;
-    int per = 1;  // teams a pair
-    while (per * 2 * pairs <= TEAMS) per *= 2;
-    float *sums = lds + MOST * pairs;
-    for (int p0 = 0; p0 < pairs; p0 += TEAMS / per) {
-        const int p = p0 + team / per, part = team % per;
-        f32x4 x{0.f, 0.f, 0.f, 0.f};
-        if (p < pairs) {
-            constexpr int AT = 8;
-            for (int s0 = part; s0 < pc.shares; s0 += AT * per) {
-                f32x4 y[AT];
-#pragma unroll
-                for (int i = 0; i < AT; i++) y[i] = pb.get4((uint32_t)min(s0 + i * per, pc.shares - 1) * SF + p * D + d);
-#pragma unroll
-                for (int i = 0; i < AT; i++) {
-                    const float f = s0 + i * per < pc.shares ? lds[p * MOST + s0 + i * per] : 0.f;
-                    if (f != 0.f)  // (an infinity of a share that does not count would be NaN)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) x[e] += y[i][e] * f;
-                }
-            }
-        }
-        if (per > 1) {
-            __syncthreads();
-            *(f32x4 *)(sums + team * D + d) = x;
-            __syncthreads();
-            if (part == 0)
-                for (int i = 1; i < per; i++) {
-                    const f32x4 y = *(const f32x4 *)(sums + (team + i) * D + d);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) x[e] += y[e];
-                }
-        }
-        if (p < pairs && part == 0) *(u32x2 *)(row(p) + d) = u32x2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+    if constexpr (!F::ROWS) {
+        if (pairs * (D / 4) <= 256)
+            join_vectors<F, D, 0, 1, TEAM>(pb, n, step, pairs, fac, last, row);
+        else
+            join_vectors<F, D, 0, D / 32, 4>(pb, n, step, pairs, fac, last, row);
+    } else {
+        join_vectors<F, D, 0, D / 16, 3>(pb, n, step, pairs, fac, last, row);
+        join_vectors<F, D, D / 16, D / 16, 3>(pb, n, step, pairs, fac, last, row);
     }
+}
+
+// Whether the workgroup, whose sums are stored, is the last of n to arrive at a counter, which it leaves zero.
+__device__ __forceinline__ bool last_of(uint32_t *counter, int n) {
+    __shared__ uint32_t arrived;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        arrived = atomicAdd(counter, 1u);
+        if (arrived == (uint32_t)n - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    return arrived == (uint32_t)n - 1;
+}
+// A share's sums are stored: the last of every TEAM shares joins them, the last of the teams those.
+template <typename F, int D, typename Row>
+__device__ __forceinline__ void arrive(const Attn &a, const Piece &pc, int pairs, float *lds, Row row) {
+    const int teams = (pc.shares + TEAM - 1) / TEAM, first = pc.share / TEAM * TEAM, n = min(TEAM, pc.shares - first);
+    if (!last_of(&a.count[pc.slot + first], n)) return;
+    join_shares<F, D>(a, pc.slot + first, n, 1, pairs, lds, teams == 1, row);
+    if (teams == 1 || !last_of(&a.count[Few::SLOTS + Rows::SLOTS + pc.slot], teams)) return;
+    join_shares<F, D>(a, pc.slot, teams, TEAM, pairs, lds, true, row);
 }
 
 // The values of a 32-key tile that are no numbers, taken out of it (v: an A operand per granule and 32
@@ -451,20 +494,6 @@ __device__ __forceinline__ void add_not_finite(u32x4 (&v)[2][D / 32], f32x16 (&o
             }
     }
     __builtin_amdgcn_wave_barrier();
-}
-
-// A share's sums are stored; the last share of its tile joins them.
-template <typename F, int D, typename Row>
-__device__ __forceinline__ void arrive(const Attn &a, const Piece &pc, int pairs, float *lds, Row row) {
-    __shared__ uint32_t arrived;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();  // (also: nobody reads the workgroup's own sums in `lds` any more)
-    if (threadIdx.x == 0) {
-        arrived = atomicAdd(&a.count[pc.slot], 1u);
-        if (arrived == (uint32_t)pc.shares - 1) __hip_atomic_store(&a.count[pc.slot], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (arrived == (uint32_t)pc.shares - 1) join_shares<F, D>(a, pc, pairs, lds, row);
 }
 
 constexpr int few_lds(int d) { return 4 * 32 * (d + 4) * 4; }
@@ -936,19 +965,19 @@ __device__ __forceinline__ void many_pairs(const Attn &a, int item, uint8_t *lds
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                pb.put4(p * D + 32 * dt + 8 * e + 4 * hi, f32x4{o[dt][4 * e], o[dt][4 * e + 1], o[dt][4 * e + 2], o[dt][4 * e + 3]});
+                pb.put4(wave * (32 * D) + (4 * dt + e) * 256 + lane * 4, f32x4{o[dt][4 * e], o[dt][4 * e + 1], o[dt][4 * e + 2], o[dt][4 * e + 3]});
     }
     arrive<Rows, D>(a, pc, pairs, (float *)lds, row_of);
 }
 
 template <int D>
-__global__ __launch_bounds__(256, 2) void paged_tokens_kernel(const Attn a) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tokens_kernel(const Attn a) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[few_lds(D)];
     few_pairs<D>(a, blockIdx.x, lds);
 }
 // the pieces of requests with many pairs first, they take longer
 template <int D>
-__global__ __launch_bounds__(256, 2) void paged_rows_kernel(const Attn a) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_rows_kernel(const Attn a) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[few_lds(D) > rows_lds(D) ? few_lds(D) : rows_lds(D)];
     if ((int)blockIdx.x < a.row_pieces)
         many_pairs<D>(a, blockIdx.x, lds);

@@ -117,6 +117,20 @@ def test_long_requests(torch_cuda, qctx, heads, kv, d):
     c.free()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads,kv,rows", [(4, 1, 1), (1, 1, 1), (32, 1, 1), (16, 2, 12), (1, 1, 33), (5, 1, 129)])
+def test_one_request_in_as_many_shares_as_there_may_be(torch_cuda, qctx, heads, kv, rows, d):
+    """Shares joined in teams and the teams' sums after them, call after call."""
+    c = Case(torch_cuda, qctx, [70001], [rows], heads, kv, d, 128)
+    for _ in range(3):
+        c.check()
+    first = c.out.clone()
+    c.check()
+    assert torch_cuda.equal(first, c.out)  # the order of the sums does not depend on that of the arrivals
+    c.check(causal=False)
+    c.free()
+
+
 def test_many_requests(torch_cuda, qctx):
     rng = np.random.default_rng(5)
     lengths = rng.integers(1, 90, 3000)
