@@ -63,8 +63,16 @@ struct Attn {
                            // calls; null: no request is long enough to be split
     float *part;           // per slot O [TM][D], then (m, l) [TM]
     int32_t row_pieces;    // workgroups for rows, before those for few
+    uint64_t g_magic;      // floor(2^64 / G) + 1: f / G = f g_magic >> 64 for f < 2^32, G > 1
     int32_t want[2];       // workgroups that few pairs, rows are divided into at least, where they are long enough
 };
+
+// pair f's row
+__device__ __forceinline__ int row_of_pair(const Attn &a, int f) {
+    const uint64_t lo = (uint64_t)(uint32_t)f * (uint32_t)a.g_magic >> 32;
+    const int x = (int)(((uint64_t)(uint32_t)f * (uint32_t)(a.g_magic >> 32) + lo) >> 32);
+    return a.G == 1 ? f : x;
+}
 
 // a request's rows and tokens
 struct Req {
@@ -84,7 +92,7 @@ struct Range {
 template <int KEYS>
 __device__ __forceinline__ Range range_of(const Attn &a, const Req &q, int first, int pairs) {
     Range g;
-    const int i0 = min(first / a.G, q.n - 1), i1 = min(q.n - 1, (first + pairs - 1) / a.G);
+    const int i0 = min(row_of_pair(a, first), q.n - 1), i1 = min(q.n - 1, row_of_pair(a, first + pairs - 1));
     g.pos0 = a.causal ? q.len - q.n + i0 : q.len - 1;
     g.pos1 = a.causal ? q.len - q.n + i1 : q.len - 1;
     g.hi = max(g.pos1 + 1, 0);
@@ -140,43 +148,39 @@ __device__ __forceinline__ int64_t scan256(int64_t v, int64_t *part, int64_t &to
     return before + s - v;
 }
 
-// A request's tiles and shares with `chunk` rounds a share (0: nothing is split); its pieces in the low
-// bits of the sums, the slots of a split one above.
-constexpr int HIGH = 44;
-constexpr int64_t LOW = ((int64_t)1 << HIGH) - 1;
+// A request's tiles and shares with `chunk` rounds a share (0: nothing is split), its pieces and, of a split
+// one, their slots.
 struct Split {
-    int tiles, shares;
-    int64_t pieces;
+    int tiles, shares, pieces, slots;
 };
 template <typename F>
-__device__ __forceinline__ Split split_of(const Attn &a, const Req &q, int64_t chunk) {
+__device__ __forceinline__ Split split_of(const Attn &a, const Req &q, int chunk) {
     Split s;
     s.tiles = tiles_of<F>(a, q);
     s.shares = 1;
-    if (chunk && s.tiles) s.shares = max((int)min((rounds_of<F>(a, q) + chunk - 1) / chunk, (int64_t)F::MOST), 1);
-    const int64_t n = min((int64_t)s.tiles * s.shares * a.Hkv, (int64_t)1 << 27);
-    s.pieces = n + (s.shares > 1 ? n << HIGH : 0);
+    if (chunk && s.tiles) s.shares = max(min((rounds_of<F>(a, q) + chunk - 1) / chunk, F::MOST), 1);
+    s.pieces = (int)min((int64_t)s.tiles * s.shares * a.Hkv, (int64_t)1 << 24);
+    s.slots = s.shares > 1 ? s.pieces : 0;
     return s;
 }
-// Rounds of a share, of `rounds` of all tiles for one head and `tiles` of them, and whether `all` pieces and
+// Rounds of a share, of `rounds` of all tiles for one head and `tiles` of them, and whether so many pieces and
 // slots of it will do (else a little longer shares are tried, at the end nothing is split). Rows that one round of
 // workgroups takes are divided into no more than that, those of not much more than one into shares half as
-// long: 136 tiles of 100 rounds in 544 shares took 139 us, in 408 87.
+// long: 136 tiles of 100 rounds in 544 shares took 139 us, in 408 112 (with their join as it was then).
 template <typename F>
-__device__ __forceinline__ int64_t chunk_of(const Attn &a, int64_t rounds, int64_t tiles) {
-    const int64_t want = a.want[F::ROWS], c = (rounds * a.Hkv + want - 1) / want;
-    return max((int64_t)F::GRAIN, F::ROWS && tiles * a.Hkv > want && tiles * a.Hkv < 2 * want ? (c + 1) / 2 : c);
+__device__ __forceinline__ int chunk_of(const Attn &a, float rounds, int64_t tiles) {
+    const int want = a.want[F::ROWS], c = (int)(rounds * (float)a.Hkv / (float)want) + 1;
+    return max(F::GRAIN, F::ROWS && tiles * a.Hkv > want && tiles * a.Hkv < 2 * want ? (c + 1) / 2 : c);
 }
 template <typename F>
-__device__ __forceinline__ bool will_do(const Attn &a, int64_t all, int64_t tiles, int most) {
-    const int64_t slots = all >> HIGH, n = all & LOW;
+__device__ __forceinline__ bool will_do(const Attn &a, int64_t pieces, int64_t slots, int64_t tiles, int most) {
     if (slots == 0) return true;
-    return slots <= F::SLOTS && n <= most && !(F::ROWS && tiles * a.Hkv <= a.want[1] && n > a.want[1]);
+    return slots <= F::SLOTS && pieces <= most && !(F::ROWS && tiles * a.Hkv <= a.want[1] && pieces > a.want[1]);
 }
-// Piece `i` of a request whose sums start at `at`: heads fastest, the last tiles first (under causal rows
+// Piece `i` of a request: heads fastest, the last tiles first (under causal rows
 // they see the most keys).
 template <typename F>
-__device__ __forceinline__ Piece piece_in(const Attn &a, int r, const Req &q, const Split &s, int i, int64_t at) {
+__device__ __forceinline__ Piece piece_in(const Attn &a, int r, const Req &q, const Split &s, int i, int slots_before) {
     Piece p;
     const int x = i / a.Hkv;
     p.r = r;
@@ -184,14 +188,28 @@ __device__ __forceinline__ Piece piece_in(const Attn &a, int r, const Req &q, co
     p.tile = s.tiles - 1 - x / s.shares;
     p.share = x % s.shares;
     p.shares = s.shares;
-    p.slot = (F::ROWS ? Few::SLOTS : 0) + (int)(at >> HIGH) + (p.tile * a.Hkv + p.h) * s.shares;
+    p.slot = (F::ROWS ? Few::SLOTS : 0) + slots_before + (p.tile * a.Hkv + p.h) * s.shares;
     p.rq = q;
     return p;
 }
-__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+// sums over the lanes up to this one
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+    const auto from = [](T x, auto ctrl, auto rows) __attribute__((always_inline)) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value,
+                                                                 decltype(rows)::value, 0xf, false));
+    };
+    v += from(v, std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});  // row_shr 1, 2, 4, 8
+    v += from(v, std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
+    v += from(v, std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
+    v += from(v, std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
+    v += from(v, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // row_bcast 15, 31
+    v += from(v, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
     return v;
+}
+template <typename T>
+__device__ __forceinline__ T lane_of(T v, int lane) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
 
 // The piece of workgroup `item` of at most `most`, in request order; false: there is none. Up to 64
@@ -202,19 +220,17 @@ __device__ __forceinline__ bool piece_of(const Attn &a, int item, int most, Piec
     if (a.R <= 64) {
         const int lane = threadIdx.x & 63;
         Req q = lane < a.R ? req_of(a, lane) : Req{0, 0, 0};
-        int64_t chunk = 0, tiles = 0, sum, all;
+        int chunk = 0, tiles = 0, r = lane;
         if (a.count) {
             const int t = tiles_of<F>(a, q);
-            tiles = wave_sum64(t);
-            chunk = chunk_of<F>(a, wave_sum64((int64_t)t * rounds_of<F>(a, q)), tiles);
+            tiles = lane_of(wave_scan(t), 63);
+            chunk = chunk_of<F>(a, lane_of(wave_scan((float)t * (float)rounds_of<F>(a, q)), 63), tiles);
         }
         Split s;
         for (;; chunk += (chunk + 7) / 8) {
             s = split_of<F>(a, q, chunk);
-            all = wave_sum64(s.pieces);
-            if (!chunk || will_do<F>(a, all, tiles, most)) break;
+            if (!chunk || will_do<F>(a, lane_of(wave_scan(s.pieces), 63), lane_of(wave_scan(s.slots), 63), tiles, most)) break;
         }
-        int at_r = lane;
         if (F::ROWS && a.R > 1) {
             // the longest shares first: lane i takes the request of rank i
             const int w = s.tiles ? (rounds_of<F>(a, q) + s.shares - 1) / s.shares : -1;
@@ -227,31 +243,23 @@ __device__ __forceinline__ bool piece_of(const Attn &a, int item, int most, Piec
             q.start = __builtin_amdgcn_ds_permute(rank, q.start);
             q.n = __builtin_amdgcn_ds_permute(rank, q.n);
             q.len = __builtin_amdgcn_ds_permute(rank, q.len);
-            at_r = __builtin_amdgcn_ds_permute(rank, lane);
+            r = __builtin_amdgcn_ds_permute(rank, lane);
             s = split_of<F>(a, q, chunk);
         }
-        sum = s.pieces;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int64_t x = __shfl_up(sum, o);
-            if (lane >= o) sum += x;
-        }
-        const uint64_t behind = __ballot((sum & LOW) > item);
+        const int pieces = wave_scan(s.pieces), slots = wave_scan(s.slots);
+        const uint64_t behind = __ballot(pieces > item);
         if (!behind) return false;
-        const int r = __builtin_ctzll(behind);
-        const int64_t at = __shfl(sum - s.pieces, r);
-        s.tiles = __builtin_amdgcn_readlane(s.tiles, r);
-        s.shares = __builtin_amdgcn_readlane(s.shares, r);
-        out = piece_in<F>(a, __builtin_amdgcn_readlane(at_r, r),
-                          Req{__builtin_amdgcn_readlane(q.start, r), __builtin_amdgcn_readlane(q.n, r), __builtin_amdgcn_readlane(q.len, r)},
-                          s, item - __builtin_amdgcn_readfirstlane((int)(at & LOW)), at);
-        out.slot = __builtin_amdgcn_readfirstlane(out.slot);
+        const int at = __builtin_ctzll(behind);
+        const Split mine{lane_of(s.tiles, at), lane_of(s.shares, at), 0, 0};
+        out = piece_in<F>(a, lane_of(r, at), Req{lane_of(q.start, at), lane_of(q.n, at), lane_of(q.len, at)}, mine,
+                          item - lane_of(pieces - s.pieces, at), lane_of(slots - s.slots, at));
         return true;
     }
     __shared__ int64_t part[4];
     __shared__ Piece found;
     const int c = (a.R + 255) / 256, r0 = min((int)threadIdx.x * c, a.R), r1 = min(r0 + c, a.R);
-    int64_t chunk = 0, tiles = 0, all;
+    int chunk = 0;
+    int64_t tiles = 0, all, slots_all;
     if (a.count) {
         int64_t t = 0, rounds = 0;
         for (int r = r0; r < r1; r++) {
@@ -262,25 +270,31 @@ __device__ __forceinline__ bool piece_of(const Attn &a, int item, int most, Piec
         }
         scan256(t, part, tiles);
         scan256(rounds, part, all);
-        chunk = chunk_of<F>(a, all, tiles);
+        chunk = chunk_of<F>(a, (float)all, tiles);
     }
-    int64_t mine, at;
+    int64_t mine, at, slots_mine, slots_at;
     for (;; chunk += (chunk + 7) / 8) {
-        mine = 0;
-        for (int r = r0; r < r1; r++) mine += split_of<F>(a, req_of(a, r), chunk).pieces;
+        mine = slots_mine = 0;
+        for (int r = r0; r < r1; r++) {
+            const Split s = split_of<F>(a, req_of(a, r), chunk);
+            mine += s.pieces;
+            slots_mine += s.slots;
+        }
         at = scan256(mine, part, all);
-        if (!chunk || will_do<F>(a, all, tiles, most)) break;
+        slots_at = scan256(slots_mine, part, slots_all);
+        if (!chunk || will_do<F>(a, all, slots_all, tiles, most)) break;
     }
-    if (item >= (all & LOW)) return false;
-    if (item >= (at & LOW) && item < (at & LOW) + (mine & LOW))
+    if (item >= all) return false;
+    if (item >= at && item < at + mine)
         for (int r = r0;; r++) {
             const Req q = req_of(a, r);
             const Split s = split_of<F>(a, q, chunk);
-            if (item < ((at + s.pieces) & LOW)) {
-                found = piece_in<F>(a, r, q, s, (int)(item - (at & LOW)), at);
+            if (item < at + s.pieces) {
+                found = piece_in<F>(a, r, q, s, (int)(item - at), (int)slots_at);
                 break;
             }
             at += s.pieces;
+            slots_at += s.slots;
         }
     __syncthreads();
     const int *src = (const int *)&found;
@@ -518,7 +532,7 @@ __device__ __forceinline__ void few_pairs(const Attn &a, int item, uint8_t *lds)
     const int last = min((int)((int64_t)rounds * (pc.share + 1) / pc.shares) * 4, g.tiles);
 
     // the lane's pair: row i of the request, head h G + hd
-    const int f = tile * 32 + l32, row = f / a.G, hd = f - row * a.G;
+    const int f = tile * 32 + l32, row = row_of_pair(a, f), hd = f - row * a.G;
     const bool there = row < rq.n;
     const int pos = !there ? -1 : a.causal ? rq.len - rq.n + row : rq.len - 1;
     const int low = a.window ? pos - a.window : -1;  // sees key j <= pos if j > low or j < g.sk
@@ -677,7 +691,7 @@ __device__ __forceinline__ void few_pairs(const Attn &a, int item, uint8_t *lds)
     __syncthreads();
     const int pairs = min(rq.n * a.G - tile * 32, 32), pr = tid / 8;  // eight threads a pair
     auto row_of = [&](int p) __attribute__((always_inline)) {
-        const int at = (tile * 32 + p) / a.G, hd = tile * 32 + p - at * a.G;
+        const int at = row_of_pair(a, tile * 32 + p), hd = tile * 32 + p - at * a.G;
         return a.out + ((int64_t)(rq.start + at) * a.Hkv * a.G + h * a.G + hd) * D;
     };
     const Part pb(slot_at<Few, D>(a, pc.slot + pc.share), slot_floats<Few, D>());
@@ -761,7 +775,7 @@ __device__ __forceinline__ void many_pairs(const Attn &a, int item, uint8_t *lds
     const int pairs = min(rq.n * a.G - f0, Rows::TM);
     const Range w = range_of<KEYS>(a, rq, f0 + 32 * wave, 32);
     const bool any = 32 * wave < pairs;
-    const int f = f0 + 32 * wave + l32, row = f / a.G, hd = f - row * a.G;
+    const int f = f0 + 32 * wave + l32, row = row_of_pair(a, f), hd = f - row * a.G;
     const bool there = row < rq.n;
     const int pos = !there ? -1 : a.causal ? rq.len - rq.n + row : rq.len - 1;
     const int low = a.window ? pos - a.window : -1;      // sees key j <= pos if j > low or j < sk
@@ -942,20 +956,32 @@ __device__ __forceinline__ void many_pairs(const Attn &a, int item, uint8_t *lds
     float lsum = l[0] + l[1] + l[2] + l[3];
     lsum += __shfl_xor(lsum, 32);
     auto row_of = [&](int p) __attribute__((always_inline)) {
-        const int at = (f0 + p) / a.G, head = f0 + p - at * a.G;
+        const int at = row_of_pair(a, f0 + p), head = f0 + p - at * a.G;
         return a.out + ((int64_t)(rq.start + at) * a.Hkv * a.G + h * a.G + head) * D;
     };
     const int p = 32 * wave + l32;
     if (pc.shares == 1) {
-        if (!there) return;
+        // through LDS, the wave's 32 rows of D in a pitch of D + 8, so that a store covers whole rows
+        __syncthreads();
+        constexpr int PITCH = 2 * D + 16;
+        uint8_t *mine = lds + wave * 32 * PITCH;
         const float inv = lsum == 0.f ? 0.f : 1.0f / lsum;  // a pair that sees no key gives zeros
-        uint16_t *dst = row_of(p) + 4 * hi;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                *(u32x2 *)(dst + 32 * dt + 8 * e) = u32x2{pack_bf16x2(o[dt][4 * e] * inv, o[dt][4 * e + 1] * inv),
-                                                          pack_bf16x2(o[dt][4 * e + 2] * inv, o[dt][4 * e + 3] * inv)};
+                *(u32x2 *)(mine + l32 * PITCH + (32 * dt + 8 * e + 4 * hi) * 2) =
+                    u32x2{pack_bf16x2(o[dt][4 * e] * inv, o[dt][4 * e + 1] * inv), pack_bf16x2(o[dt][4 * e + 2] * inv, o[dt][4 * e + 3] * inv)};
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        constexpr int LPR = D / 8;  // lanes a row
+#pragma unroll
+        for (int i = 0; i < 32 * LPR / 64; i++) {
+            const int q = i * (64 / LPR) + lane / LPR;
+            if (32 * wave + q < pairs)
+                *(u32x4 *)(row_of(32 * wave + q) + lane % LPR * 8) = *(const u32x4 *)(mine + q * PITCH + lane % LPR * 16);
+        }
         return;
     }
     if (there) {
@@ -999,7 +1025,8 @@ hipError_t launch_paged_attention(const PageDims &d, const uint8_t *layer, const
     Attn a{x.q, x.q_row, x.q_head, layer, d.pages, x.tables, x.max_pages, x.lengths, x.starts, (int32_t)x.requests,
            (int32_t)x.rows, d.kv_heads, (int32_t)g, ps16, (uint32_t)(((1ull << 32) + ps16 - 1) / ps16),
            (int32_t)cap, x.causal, (int32_t)std::min<int64_t>(x.window, 0x7fffffff),
-           (int32_t)std::min<int64_t>(x.sinks, 0x7fffffff), x.scale * 1.4426950408889634f, x.out, nullptr, nullptr, 0, {}};
+           (int32_t)std::min<int64_t>(x.sinks, 0x7fffffff), x.scale * 1.4426950408889634f, x.out, nullptr, nullptr, 0,
+           g > 1 ? ~0ull / (uint64_t)g + 1 : 0, {}};
     const int cus = std::max(device_cu_count(), 1);
     a.want[0] = std::min(4 * cus, Few::SLOTS);
     a.want[1] = std::min(2 * cus, Rows::SLOTS);  // two workgroups a CU
