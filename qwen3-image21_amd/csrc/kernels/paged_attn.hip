@@ -158,7 +158,8 @@ __device__ __forceinline__ Split split_of(const Attn &a, const Req &q, int chunk
     Split s;
     s.tiles = tiles_of<F>(a, q);
     s.shares = 1;
-    if (chunk && s.tiles) s.shares = max(min((rounds_of<F>(a, q) + chunk - 1) / chunk, F::MOST), 1);
+    const int rounds = rounds_of<F>(a, q);
+    if (chunk && s.tiles && rounds > F::GRAIN) s.shares = max(min((rounds + chunk - 1) / chunk, F::MOST), 1);
     s.pieces = (int)min((int64_t)s.tiles * s.shares * a.Hkv, (int64_t)1 << 24);
     s.slots = s.shares > 1 ? s.pieces : 0;
     return s;
@@ -166,11 +167,15 @@ __device__ __forceinline__ Split split_of(const Attn &a, const Req &q, int chunk
 // Rounds of a share, of `rounds` of all tiles for one head and `tiles` of them, and whether so many pieces and
 // slots of it will do (else a little longer shares are tried, at the end nothing is split). Rows that one round of
 // workgroups takes are divided into no more than that, those of not much more than one into shares half as
-// long: 136 tiles of 100 rounds in 544 shares took 139 us, in 408 112 (with their join as it was then).
+// long: 136 tiles of 100 rounds in 544 shares took 139 us, in 408 112 (with their join as it was then). Of few
+// pairs shares may be of half a GRAIN as long as each has a CU of its own: one token over 4000 keys of 8 heads
+// 14.5 us in 64 shares, 11.7 in 128, but 8 of them over 2000 18.4 in 256 and 19.5 in 512. Requests of up to a
+// GRAIN are not split: 333 keys of 32 heads 8.4 us, 10.2 in two shares.
 template <typename F>
 __device__ __forceinline__ int chunk_of(const Attn &a, float rounds, int64_t tiles) {
     const int want = a.want[F::ROWS], c = (int)(rounds * (float)a.Hkv / (float)want) + 1;
-    return max(F::GRAIN, F::ROWS && tiles * a.Hkv > want && tiles * a.Hkv < 2 * want ? (c + 1) / 2 : c);
+    if (F::ROWS) return max(F::GRAIN, tiles * a.Hkv > want && tiles * a.Hkv < 2 * want ? (c + 1) / 2 : c);
+    return max(rounds * (float)a.Hkv <= (float)(want / 2) ? F::GRAIN / 2 : F::GRAIN, c);
 }
 template <typename F>
 __device__ __forceinline__ bool will_do(const Attn &a, int64_t pieces, int64_t slots, int64_t tiles, int most) {

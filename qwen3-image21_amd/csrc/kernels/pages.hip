@@ -3,12 +3,13 @@
 // The plan. Request r has old_r tokens and adds a_r; with the sums over the requests before it,
 // start_r of rows and base_r of new pages, its page k from ceil(old_r / ps) on is entry base_r + ... of
 // the queue of free pages, and the slot of a token at position p is table[p / ps] ps + p % ps. Bound by
-// latency: a few bytes a request and 8 a row. One workgroup makes the sums in registers and LDS.
+// latency: a few bytes a request and 8 a row. One workgroup makes the sums in registers; where requests and
+// rows are few it writes the rows too, from LDS, else a second launch does.
 //
-// The store. Bound by bytes: a key's 8 dims are 16 B of its granule, four keys' values of one dim 8 B
-// (paged.h), so a thread takes 8 dims of four rows and turns their values over in registers where
-// the four rows are four consecutive slots; rows that are not (the ends of a request) write
-// their values one by one.
+// The store. Bound by bytes. Where 16 rows are the 16 slots of a granule, in order, a wave takes them: keys as
+// they are read are written 1 KB in a row, values are turned over in registers, four rows and eight dims a
+// lane, and gathered in LDS (paged.h). Other rows, the ends of a request and single tokens, are
+// written 16 B of a key and 2 B of a value at a time.
 #include <type_traits>
 
 #include "device_common.h"
@@ -17,47 +18,63 @@
 namespace qimm {
 namespace {
 
-constexpr int PLAN_THREADS = 1024;
+constexpr int PLAN_REQUESTS = 1024, PLAN_ROWS = 2048;  // what one launch takes
 
-// exclusive sums of v over the workgroup's threads, and the total; `part` takes a value per wave
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *part, int64_t &total) {
+// A step's sums over the requests, in 32 bits that stop at the largest number: rows up to max_rows, pages up
+// to those that are free and back to the queue are all that counts.
+struct Sums {
+    uint32_t rows, need, freed;
+};
+__device__ __forceinline__ Sums add(Sums a, Sums b) {
+    return {__builtin_elementwise_add_sat(a.rows, b.rows), __builtin_elementwise_add_sat(a.need, b.need),
+            __builtin_elementwise_add_sat(a.freed, b.freed)};
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ Sums scan_step(Sums s) {
+    const auto from = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false); };
+    return add(s, {from(s.rows), from(s.need), from(s.freed)});
+}
+// those of the threads before this one, and of all; `part` takes a value per wave
+template <int THREADS>
+__device__ __forceinline__ Sums block_scan(Sums v, Sums *part, Sums &total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int64_t s = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t x = __shfl_up(s, o);
-        if (lane >= o) s += x;
-    }
-    __syncthreads();  // part may still be read by an earlier call
+    Sums s = v;
+    s = scan_step<0x111, 0xf>(s);  // row_shr 1, 2, 4, 8
+    s = scan_step<0x112, 0xf>(s);
+    s = scan_step<0x114, 0xf>(s);
+    s = scan_step<0x118, 0xf>(s);
+    s = scan_step<0x142, 0xa>(s);  // row_bcast 15, 31
+    s = scan_step<0x143, 0xc>(s);
     if (lane == 63) part[wave] = s;
     __syncthreads();
-    int64_t before = 0;
-    total = 0;
-    for (int w = 0; w < (int)(blockDim.x >> 6); w++) {
-        if (w < wave) before += part[w];
-        total += part[w];
+    Sums before{0, 0, 0};
+    total = before;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; w++) {
+        if (w == wave) before = total;
+        total = add(total, part[w]);
     }
-    return before + s - v;
+    const Sums up{(uint32_t)__shfl_up((int)s.rows, 1), (uint32_t)__shfl_up((int)s.need, 1), (uint32_t)__shfl_up((int)s.freed, 1)};
+    return lane ? add(before, up) : before;
 }
 
-// A request's step. fits: it adds tokens, and its table and the rows have room for them.
+// A request's step. fits: it adds tokens and its table has room for them.
 struct Step {
     int old, add, have;  // tokens, tokens added (negative: given back), pages held
-    int64_t end;         // rows up to and with it
     bool fits;
     int need;            // new pages, 0 where it does not fit
     int freed;           // pages given back
+    __device__ Sums sums() const { return {(uint32_t)max(add, 0), (uint32_t)need, (uint32_t)freed}; }
 };
 
-__device__ __forceinline__ Step step_of(const PagePlanArgs &p, int64_t r, int64_t rows_before) {
+__device__ __forceinline__ Step step_of(const PagePlanArgs &p, int64_t r) {
     Step s;
     s.old = p.lengths[r];
     s.add = p.added[r];
     const int ps = p.page_size;
     const int64_t room = p.max_pages * ps, after = (int64_t)s.old + s.add;
     s.have = s.old > 0 ? (int)min(((int64_t)s.old + ps - 1) / ps, p.max_pages) : 0;
-    s.end = rows_before + max(s.add, 0);
-    s.fits = s.add > 0 && s.old >= 0 && after <= room && s.end <= p.max_rows;
+    s.fits = s.add > 0 && s.old >= 0 && after <= room;
     s.need = s.fits ? (int)((after + ps - 1) / ps) - s.have : 0;
     s.freed = s.add < 0 ? s.have : 0;
     return s;
@@ -86,94 +103,153 @@ __device__ __forceinline__ void fill_row(const PagePlanArgs &p, int64_t t, int64
     if (p.positions) p.positions[t] = pos;
 }
 
-// The sums of a step by one workgroup: starts, lengths_out, state_out, and per request in work
-// {start, old, base, entries before its first page given back (-1: none)}, then {head, free}.
-__global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(const PagePlanArgs p) {
-    __shared__ int64_t part[PLAN_THREADS / 64];
+// The pages of a request given back, `lane` of 64: `back` entries of the queue come before its first.
+__device__ __forceinline__ void give_back(const PagePlanArgs &p, int64_t r, int old, int64_t back, int head, int free, int lane) {
+    const int have = (int)min(((int64_t)old + p.page_size - 1) / p.page_size, p.max_pages);
+    // (entries past the queue's size would be pages given back twice)
+    for (int k = lane; k < have && free + back + k < 2 * p.pages; k += 64)
+        *queue_at(p, head, free + back + k) = p.tables[r * p.max_pages + k];
+}
+
+// The sums of a step by one workgroup: starts, lengths_out, state_out, and of every request {start, old,
+// base, entries before its first page given back (-1: none)}: in LDS (FILL: up to PLAN_REQUESTS), for
+// the rows, which it then writes; or in work, then {head, free}. A request that fits within the rows has
+// only such before it, so the sums need not ask for it.
+template <int THREADS, bool FILL>
+__global__ __launch_bounds__(THREADS) void page_plan_kernel(const PagePlanArgs p) {
+    __shared__ Sums part[THREADS / 64];
+    __shared__ int taken, refused;
+    __shared__ int4 of[FILL ? THREADS : 1];
+    __shared__ int starts[FILL ? THREADS + 1 : 1];
     const int tid = threadIdx.x;
-    const int64_t R = p.requests, c = (R + PLAN_THREADS - 1) / PLAN_THREADS;
+    const int64_t R = p.requests, c = FILL ? 1 : (R + THREADS - 1) / THREADS;
     const int64_t r0 = min(tid * c, R), r1 = min(r0 + c, R);
+    if (tid == 0) taken = refused = 0;
     const int free = (int)min((int64_t)max(p.state[1], 0), p.pages);
     int head = (int)(p.state[0] % p.pages);
     if (head < 0) head += (int)p.pages;
 
-    int64_t rows = 0, rows_all, need = 0, need_all, freed = 0, freed_all;
-    for (int64_t r = r0; r < r1; r++) rows += max(p.added[r], 0);
-    const int64_t rows0 = block_scan(rows, part, rows_all);
-    int64_t end = rows0;
+    Sums mine{0, 0, 0}, all;
+    Step s;
     for (int64_t r = r0; r < r1; r++) {
-        const Step s = step_of(p, r, end);
-        end = s.end;
-        need += s.need;
-        freed += s.freed;
+        s = step_of(p, r);
+        mine = add(mine, s.sums());
     }
-    int64_t cum = block_scan(need, part, need_all);
-    int64_t back = block_scan(freed, part, freed_all);
-    int64_t taken = 0, refused = 0;
-    end = rows0;
+    Sums at = block_scan<THREADS>(mine, part, all);
+    const uint32_t most = (uint32_t)p.max_rows;
+    int used = 0, no = 0;
     for (int64_t r = r0; r < r1; r++) {
-        const Step s = step_of(p, r, end);
-        const bool served = s.fits && (s.need == 0 || cum + s.need <= free);
-        const int start = (int)min(end, p.max_rows);
+        if (!FILL) s = step_of(p, r);
+        const Sums end = add(at, s.sums());
+        const bool served = s.fits && end.rows <= most && (s.need == 0 || end.need <= (uint32_t)free);
+        const int start = (int)min(at.rows, most);
+        const int4 w = make_int4(start, s.old, served ? (s.need ? (int)at.need : 0) : -1, s.freed ? (int)min(at.freed, 0x7fffffffu) : -1);
+        if (FILL) {
+            of[tid] = w;
+            starts[tid] = start;
+        } else {
+            *(int4 *)(p.work + 4 * r) = w;
+        }
         p.starts[r] = start;
-        int32_t *w = p.work + 4 * r;
-        w[0] = start;
-        w[1] = s.old;
-        w[2] = served ? (s.need ? (int)cum : 0) : -1;
-        w[3] = s.freed ? (int)min(back, (int64_t)0x7fffffff) : -1;
         p.lengths_out[r] = s.add < 0 ? 0 : served ? s.old + s.add : s.old;
-        taken += served ? s.need : 0;
-        refused += s.add > 0 && !served;
-        end = s.end;
-        cum += s.need;
-        back += s.freed;
+        if (served && s.need) used = (int)end.need;
+        no += s.add > 0 && !served;
+        at = end;
     }
-    int64_t taken_all, refused_all;
-    block_scan(taken, part, taken_all);
-    block_scan(refused, part, refused_all);
-    const int all = (int)min(rows_all, p.max_rows);
+    if (used) atomicMax(&taken, used);
+    if (no) atomicAdd(&refused, no);
+    __syncthreads();
+    const int rows = (int)min(all.rows, most);
     if (tid == 0) {
-        p.starts[R] = all;
-        int64_t at = head + taken_all;
-        if (at >= p.pages) at -= p.pages;
-        p.state_out[0] = (int)at;
-        p.state_out[1] = (int)min(free - taken_all + freed_all, p.pages);
-        p.state_out[2] = all;
-        p.state_out[3] = (int)refused_all;
-        p.work[4 * R] = head;
-        p.work[4 * R + 1] = free;
+        p.starts[R] = rows;
+        int64_t to = (int64_t)head + taken;
+        if (to >= p.pages) to -= p.pages;
+        p.state_out[0] = (int)to;
+        p.state_out[1] = (int)min((int64_t)free - taken + all.freed, p.pages);
+        p.state_out[2] = rows;
+        p.state_out[3] = refused;
+        if (!FILL) {
+            p.work[4 * R] = head;
+            p.work[4 * R + 1] = free;
+        }
     }
+    if constexpr (FILL) {
+        for (int64_t t = tid; t < p.max_rows; t += THREADS) {
+            if (t >= rows) {
+                p.slots[t] = -1;
+                if (p.positions) p.positions[t] = 0;
+                continue;
+            }
+            int lo = 0, hi = (int)R;  // starts[lo] <= t < starts[hi]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (starts[mid] <= t)
+                    lo = mid;
+                else
+                    hi = mid;
+            }
+            const int4 w = of[lo];
+            fill_row(p, t, lo, w.x, w.y, w.z, head);
+        }
+        if (all.freed)
+            for (int64_t r = tid >> 6; r < R; r += THREADS / 64)
+                if (of[r].w >= 0) give_back(p, r, of[r].y, of[r].w, head, free, tid & 63);
+    }
+}
+
+// The largest of `n` requests whose rows start at or before t (starts[0] is 0), by a wave: 64 at a time.
+__device__ __forceinline__ int64_t request_of(const int32_t *starts, int64_t n, int64_t t) {
+    const int lane = threadIdx.x & 63;
+    int64_t lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int64_t step = (hi - lo + 63) / 64, at = lo + lane * step;
+        const int k = __popcll(__ballot(at < hi && starts[min(at, hi - 1)] <= t));
+        lo += max(k - 1, 0) * step;
+        hi = min(lo + step, hi);
+    }
+    return lo;
 }
 
 // Slots, positions and table entries of the rows, then the queue entries of the pages given back.
 __global__ __launch_bounds__(256) void page_fill_kernel(const PagePlanArgs p) {
+    constexpr int HELD = 1024;
+    __shared__ int starts[HELD];
+    __shared__ int64_t ends[2];
     const int64_t R = p.requests;
     const int head = p.work[4 * R], free = p.work[4 * R + 1], all = p.starts[R];
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (t < all) {
-        int64_t lo = 0, hi = R;  // starts[lo] <= t < starts[hi]
-        while (hi - lo > 1) {
-            const int64_t mid = (lo + hi) >> 1;
-            if (p.starts[mid] <= t)
-                lo = mid;
-            else
-                hi = mid;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int64_t t0 = (int64_t)blockIdx.x * 256, t = t0 + tid;
+    if (t0 < all) {
+        // the requests of the workgroup's first and last row, their starts into LDS
+        if (tid < 128) {
+            const int64_t r = request_of(p.starts, R, tid < 64 ? t0 : min(t0 + 255, (int64_t)all - 1));
+            if (lane == 0) ends[tid >> 6] = r;
         }
-        const int32_t *w = p.work + 4 * lo;
-        fill_row(p, t, lo, w[0], w[1], w[2], head);
-    } else if (t < p.max_rows) {
+        __syncthreads();
+        const int64_t r0 = ends[0], n = ends[1] - r0 + 1;
+        for (int64_t i = tid; i < min(n, (int64_t)HELD); i += 256) starts[i] = p.starts[r0 + i];
+        __syncthreads();
+        if (t < all) {
+            int64_t lo = 0, hi = n;
+            while (hi - lo > 1) {
+                const int64_t mid = (lo + hi) >> 1;
+                if ((mid < HELD ? starts[mid] : p.starts[r0 + mid]) <= t)
+                    lo = mid;
+                else
+                    hi = mid;
+            }
+            const int4 w = *(const int4 *)(p.work + 4 * (r0 + lo));
+            fill_row(p, t, r0 + lo, w.x, w.y, w.z, head);
+        }
+    }
+    if (t >= all && t < p.max_rows) {
         p.slots[t] = -1;
         if (p.positions) p.positions[t] = 0;
     }
-    const int lane = threadIdx.x & 63;
     const int64_t waves = (int64_t)gridDim.x * 4;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < R; r += waves) {
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (tid >> 6); r < R; r += waves) {
         const int back = p.work[4 * r + 3];
-        if (back < 0) continue;
-        const int have = (int)min(((int64_t)p.work[4 * r + 1] + p.page_size - 1) / p.page_size, p.max_pages);
-        // (entries past the queue's size would be pages given back twice)
-        for (int k = lane; k < have && (int64_t)free + back + k < 2 * p.pages; k += 64)
-            *queue_at(p, head, (int64_t)free + back + k) = p.tables[r * p.max_pages + k];
+        if (back >= 0) give_back(p, r, p.work[4 * r + 1], back, head, free, lane);
     }
 }
 
@@ -205,90 +281,151 @@ __device__ __forceinline__ u32x2 column(const u32x4 (&x)[4], int e) {
     return u32x2{__builtin_amdgcn_perm(x[1][e >> 1], x[0][e >> 1], sel), __builtin_amdgcn_perm(x[3][e >> 1], x[2][e >> 1], sel)};
 }
 
-// T: the rows' type; STORE: into the pages, else out of them (bf16)
+// A wave takes rows t0 .. t0 + 15 of 128 / D heads. T: the rows' type; STORE: into the pages, else out of them
+// (bf16).
 template <typename T, bool STORE, int D>
 __global__ __launch_bounds__(256) void pages_rows_kernel(PageDims d, uint8_t *layer, T *k, T *v, int64_t k_row, int64_t k_head,
                                                          int64_t v_row, int64_t v_head, const int32_t *__restrict__ slots,
                                                          int64_t rows) {
-    constexpr int OCT = D / 8, GROUPS = 256 / OCT;
-    const int o = threadIdx.x % OCT, h = blockIdx.y;
-    const int64_t t0 = ((int64_t)blockIdx.x * GROUPS + threadIdx.x / OCT) * 4;
-    if (t0 >= rows) return;
+    constexpr int OCT = D / 8, HEADS = 128 / D;      // lanes a row; heads of a wave
+    __shared__ __attribute__((aligned(16))) uint8_t lds[4][4096];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int h = (blockIdx.y * 4 + wave) * HEADS + lane / (64 / HEADS);
+    const int64_t t0 = (int64_t)blockIdx.x * 16;
     const int64_t most = d.pages * d.page_size;
-    // the slots of rows t0 - 3 .. t0 + 6
-    int s[10];
-#pragma unroll
-    for (int i = 0; i < 10; i++) {
-        const int64_t t = t0 + i - 3;
-        const int x = t >= 0 && t < rows ? slots[t] : -1;
-        s[i] = x >= 0 && x < most ? x : -1;
-    }
-    auto granule = [&](int slot) __attribute__((always_inline)) {
-        const int page = slot / d.page_size, in = slot - page * d.page_size;
-        return layer + (((int64_t)page * d.kv_heads + h) * (d.page_size >> 4) + (in >> 4)) * granule_bytes(D);
+    // lane i: the slot of row t0 - 15 + i, and whether it leads 16 rows with the slots of a granule
+    const int64_t mine = t0 - 15 + lane;
+    int slot = -1;
+    if (lane < 46 && mine >= 0 && mine < rows) slot = slots[mine];
+    if (slot < 0 || slot >= most) slot = -1;
+    const uint64_t next = __ballot(slot >= 0 && __shfl_down(slot, 1) == slot + 1 && lane < 45);
+    const uint64_t leads = __ballot(lane < 31 && slot >= 0 && (slot & 15) == 0 && ((next >> lane) & 0x7fffu) == 0x7fffu);
+    const bool there = h < d.kv_heads;
+    const int hs = there ? h : 0;
+    auto granule = [&](int s) __attribute__((always_inline)) {
+        const int page = s / d.page_size, in = s - page * d.page_size;
+        return layer + (((int64_t)page * d.kv_heads + hs) * (d.page_size >> 4) + (in >> 4)) * granule_bytes(D);
     };
-    // whether row t0 + j (j = -3 .. 3) leads four rows with the four slots of a quad
-    auto leads = [&](int j) __attribute__((always_inline)) {
-        const int x = s[j + 3];
-        return x >= 0 && (x & 3) == 0 && s[j + 4] == x + 1 && s[j + 5] == x + 2 && s[j + 6] == x + 3;
-    };
+
+    const uint32_t here = (uint32_t)(leads >> 15) & 0xffffu;  // of rows t0 ..: at most one
+    if (here) {
+        const int lead = __builtin_ctz(here);
+        const int64_t t = t0 + lead;
+        uint8_t *g = granule(__builtin_amdgcn_readlane(slot, 15 + lead));
+        // keys: 16 rows of four 16 B chunks a time (of each head 16 lanes a chunk)
+        constexpr int CH = 4 / HEADS;
+        const int l = lane % (64 / HEADS), key = l & 15;
+        u32x4 y[OCT / CH];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int64_t t = t0 + j;
-        const int x = s[j + 3];
-        if (t >= rows) break;
-        T *kp = k + t * k_row + h * k_head + o * 8;
-        if (x < 0) {
-            if constexpr (!STORE) {
-                *(u32x4 *)kp = u32x4{};
-                *(u32x4 *)(v + t * v_row + h * v_head + o * 8) = u32x4{};
-            }
-            continue;
+        for (int i = 0; i < OCT / CH; i++) {
+            const int c = i * CH + (l >> 4);
+            T *src = k + (t + key) * k_row + hs * k_head + c * 8;
+            if constexpr (STORE)
+                y[i] = load8_bf16(src);
+            else
+                y[i] = *(const u32x4 *)(g + c * 256 + key * 16);
         }
-        uint8_t *g = granule(x);
-        u32x4 *kc = (u32x4 *)(g + granule_k(x & 15, o * 8));
-        if constexpr (STORE)
-            *kc = load8_bf16(kp);
-        else
-            *(u32x4 *)kp = *kc;
-        if (leads(j)) {
-            u32x4 y[4];
-            if constexpr (STORE) {
+        // values: four rows (a quad of keys) and eight dims a lane
+        const int o = l % OCT, quad = l / OCT;
+        uint8_t *const at = lds[wave] + lane / (64 / HEADS) * (4096 / HEADS);  // a head's granule half
+        auto swap = [&](int dim) { return dim ^ ((dim >> 3) & 7); };            // (spreads the eight dims over the banks)
+        u32x4 x[4];
+        T *vp = v + (t + 4 * quad) * v_row + hs * v_head + o * 8;
+        if constexpr (STORE) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) y[i] = load8_bf16(v + (t + i) * v_row + h * v_head + o * 8);
+            for (int i = 0; i < 4; i++) x[i] = load8_bf16(vp + i * v_row);
+        } else {
 #pragma unroll
-                for (int e = 0; e < 8; e++) *(u32x2 *)(g + granule_v(D, x & 15, o * 8 + e)) = column(y, e);
-            } else {
-                u32x2 c[8];
+            for (int i = 0; i < 4; i++) {
+                const int n = i * (64 / HEADS) + l, half = n / D, dim = n % D;
+                *(u32x4 *)(at + half * (D * 16) + swap(dim) * 16) = *(const u32x4 *)(g + D * 32 + n * 16);
+            }
+        }
+        if (there)
 #pragma unroll
-                for (int e = 0; e < 8; e++) c[e] = *(const u32x2 *)(g + granule_v(D, x & 15, o * 8 + e));
+            for (int i = 0; i < OCT / CH; i++) {
+                const int c = i * CH + (l >> 4);
+                if constexpr (STORE)
+                    *(u32x4 *)(g + c * 256 + key * 16) = y[i];
+                else
+                    *(u32x4 *)(k + (t + key) * k_row + hs * k_head + c * 8) = y[i];
+            }
+        uint8_t *const cell = at + (quad & 1) * (D * 16) + (quad >> 1) * 8;
+        auto wait = [] {
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        };
+        if constexpr (STORE) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) *(u32x2 *)(cell + swap(o * 8 + e) * 16) = column(x, e);
+            wait();
+            if (there)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int n = i * (64 / HEADS) + l, half = n / D, dim = n % D;
+                    *(u32x4 *)(g + D * 32 + n * 16) = *(const u32x4 *)(at + half * (D * 16) + swap(dim) * 16);
+                }
+        } else {
+            wait();
+            u32x2 c[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) c[e] = *(const u32x2 *)(cell + swap(o * 8 + e) * 16);
+            if (there)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const uint32_t sel = i & 1 ? 0x07060302u : 0x05040100u;
 #pragma unroll
-                    for (int w = 0; w < 4; w++) y[i][w] = __builtin_amdgcn_perm(c[2 * w + 1][i >> 1], c[2 * w][i >> 1], sel);
-                    *(u32x4 *)(v + (t + i) * v_row + h * v_head + o * 8) = y[i];
+                    for (int w = 0; w < 4; w++) x[i][w] = __builtin_amdgcn_perm(c[2 * w + 1][i >> 1], c[2 * w][i >> 1], sel);
+                    *(u32x4 *)(vp + i * v_row) = x[i];
                 }
-            }
-            continue;
         }
-        // rows t - (x & 3) .. of one quad are their leader's
-        bool led = false;
+    }
+
+    // the rows of no such 16, four at a time
+    uint32_t rest = 0xffffu;
+    for (uint64_t m = leads; m; m &= m - 1) {
+        const int a = __builtin_ctzll(m) - 15;  // leads rows t0 + a .. a + 15
+        rest &= ~(uint32_t)((a < 0 ? 0xffffull >> -a : 0xffffull << a));
+    }
+    if (rows - t0 < 16) rest &= (1u << (rows - t0)) - 1;
+    if (!rest) return;
+    const int o = lane % OCT, sub = lane % (64 / HEADS) / OCT;
+    int at[4];
+    u32x4 x[4], y[4];
 #pragma unroll
-        for (int i = 1; i < 4; i++) led = led || ((x & 3) == i && leads(j - i));
-        if (led) continue;
-        u32x4 y;
-        T *vp = v + t * v_row + h * v_head + o * 8;
-        if constexpr (STORE) y = load8_bf16(vp);
+    for (int i = 0; i < 4; i++) {
+        const int r = 4 * i + sub;
+        at[i] = __shfl(slot, 15 + r);
+        if (!there || !((rest >> r) & 1u)) at[i] = -2;
+        x[i] = y[i] = u32x4{};
+        if (at[i] < 0) continue;
+        if constexpr (STORE) {
+            x[i] = load8_bf16(k + (t0 + r) * k_row + h * k_head + o * 8);
+            y[i] = load8_bf16(v + (t0 + r) * v_row + h * v_head + o * 8);
+        } else {
+            const uint8_t *g = granule(at[i]);
+            x[i] = *(const u32x4 *)(g + granule_k(at[i] & 15, o * 8));
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            uint16_t *c = (uint16_t *)(g + granule_v(D, x & 15, o * 8 + e));
-            if constexpr (STORE)
-                *c = (uint16_t)(y[e >> 1] >> (16 * (e & 1)));
-            else
-                y[e >> 1] = e & 1 ? y[e >> 1] | (uint32_t)*c << 16 : (uint32_t)*c;
+            for (int e = 0; e < 8; e++)
+                y[i][e >> 1] |= (uint32_t)*(const uint16_t *)(g + granule_v(D, at[i] & 15, o * 8 + e)) << (16 * (e & 1));
         }
-        if constexpr (!STORE) *(u32x4 *)vp = y;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int r = 4 * i + sub;
+        if constexpr (STORE) {
+            if (at[i] < 0) continue;
+            uint8_t *g = granule(at[i]);
+            *(u32x4 *)(g + granule_k(at[i] & 15, o * 8)) = x[i];
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                *(uint16_t *)(g + granule_v(D, at[i] & 15, o * 8 + e)) = (uint16_t)(y[i][e >> 1] >> (16 * (e & 1)));
+        } else {
+            if (at[i] < -1) continue;
+            *(u32x4 *)(k + (t0 + r) * k_row + h * k_head + o * 8) = x[i];
+            *(u32x4 *)(v + (t0 + r) * v_row + h * v_head + o * 8) = y[i];
+        }
     }
 }
 
@@ -296,10 +433,10 @@ template <typename T, bool STORE>
 hipError_t launch_rows(const PageDims &d, uint8_t *layer, T *k, T *v, int64_t k_row, int64_t k_head, int64_t v_row,
                        int64_t v_head, const int32_t *slots, int64_t rows, hipStream_t stream) {
     if (rows <= 0) return hipSuccess;
-    const int per = 256 / (d.head_dim / 8) * 4;
-    const int64_t blocks = (rows + per - 1) / per;
+    const int per = 4 * 128 / d.head_dim;  // heads of a workgroup
+    const int64_t blocks = (rows + 15) / 16;
     if (blocks >= (int64_t)1 << 24 || d.kv_heads > 65535) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)blocks, (unsigned)d.kv_heads);
+    const dim3 grid((unsigned)blocks, (unsigned)((d.kv_heads + per - 1) / per));
     if (d.head_dim == 128)
         pages_rows_kernel<T, STORE, 128><<<grid, 256, 0, stream>>>(d, layer, k, v, k_row, k_head, v_row, v_head, slots, rows);
     else if (d.head_dim == 64)
@@ -314,7 +451,14 @@ hipError_t launch_rows(const PageDims &d, uint8_t *layer, T *k, T *v, int64_t k_
 hipError_t launch_page_plan(const PagePlanArgs &p, hipStream_t stream) {
     const int64_t blocks = (p.max_rows + 255) / 256;
     if (p.requests <= 0 || p.pages <= 0 || blocks >= (int64_t)1 << 24) return hipErrorInvalidValue;
-    page_plan_kernel<<<1, PLAN_THREADS, 0, stream>>>(p);
+    if (p.requests <= PLAN_REQUESTS && p.max_rows <= PLAN_ROWS) {
+        if (p.requests <= 256 && p.max_rows <= 512)
+            page_plan_kernel<256, true><<<1, 256, 0, stream>>>(p);
+        else
+            page_plan_kernel<PLAN_REQUESTS, true><<<1, PLAN_REQUESTS, 0, stream>>>(p);
+        return hipGetLastError();
+    }
+    page_plan_kernel<1024, false><<<1, 1024, 0, stream>>>(p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     page_fill_kernel<<<(unsigned)(blocks > 0 ? blocks : 1), 256, 0, stream>>>(p);
