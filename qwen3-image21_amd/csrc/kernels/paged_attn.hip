@@ -62,7 +62,8 @@ struct Attn {
     uint32_t *count;       // arrivals per slot, the few's and the rows', of shares and of teams, zero between
                            // calls; null: no request is long enough to be split
     float *part;           // per slot O [TM][D], then (m, l) [TM]
-    int32_t row_pieces;    // workgroups for rows, before those for few
+    int32_t row_pieces;    // workgroups for rows; the others are for few
+    int32_t turn;          // of which so many take turns, a multiple of the XCDs
     uint64_t g_magic;      // floor(2^64 / G) + 1: f / G = f g_magic >> 64 for f < 2^32, G > 1
     int32_t want[2];       // workgroups that few pairs, rows are divided into at least, where they are long enough
 };
@@ -1006,14 +1007,19 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_tokens_kernel(cons
     __shared__ __attribute__((aligned(16))) uint8_t lds[few_lds(D)];
     few_pairs<D>(a, blockIdx.x, lds);
 }
-// the pieces of requests with many pairs first, they take longer
+// Pieces of requests with many pairs and with few in turn, as many of each as there are CUs, as long as there are
+// both: the first are bound by the matrix pipe, the others by memory, and a CU has one of each (two chunks
+// of 517 rows and 30 single tokens, 59 and 81 us by themselves: 143 one after the other, 135 in turn).
 template <int D>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void paged_rows_kernel(const Attn a) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[few_lds(D) > rows_lds(D) ? few_lds(D) : rows_lds(D)];
-    if ((int)blockIdx.x < a.row_pieces)
-        many_pairs<D>(a, blockIdx.x, lds);
+    const int turn = a.turn, at = blockIdx.x / turn, rows = a.row_pieces / turn, both = min(rows, (int)(gridDim.x / turn) - rows);
+    const bool many = at < 2 * both ? !(at & 1) : rows > both;
+    const int item = (at < 2 * both ? at >> 1 : at - both) * turn + blockIdx.x % turn;
+    if (many)
+        many_pairs<D>(a, item, lds);
     else
-        few_pairs<D>(a, (int)blockIdx.x - a.row_pieces, lds);
+        few_pairs<D>(a, item, lds);
 }
 
 }  // namespace
@@ -1030,7 +1036,7 @@ hipError_t launch_paged_attention(const PageDims &d, const uint8_t *layer, const
     Attn a{x.q, x.q_row, x.q_head, layer, d.pages, x.tables, x.max_pages, x.lengths, x.starts, (int32_t)x.requests,
            (int32_t)x.rows, d.kv_heads, (int32_t)g, ps16, (uint32_t)(((1ull << 32) + ps16 - 1) / ps16),
            (int32_t)cap, x.causal, (int32_t)std::min<int64_t>(x.window, 0x7fffffff),
-           (int32_t)std::min<int64_t>(x.sinks, 0x7fffffff), x.scale * 1.4426950408889634f, x.out, nullptr, nullptr, 0,
+           (int32_t)std::min<int64_t>(x.sinks, 0x7fffffff), x.scale * 1.4426950408889634f, x.out, nullptr, nullptr, 0, 0,
            g > 1 ? ~0ull / (uint64_t)g + 1 : 0, {}};
     const int cus = std::max(device_cu_count(), 1);
     a.want[0] = std::min(4 * cus, Few::SLOTS);
@@ -1043,9 +1049,13 @@ hipError_t launch_paged_attention(const PageDims &d, const uint8_t *layer, const
     if (cap > std::min(Few::GRAIN * Few::ROUND, Rows::GRAIN * Rows::ROUND)) {
         a.count = (uint32_t *)scratch;
         a.part = (float *)((char *)scratch + PAGED_COUNTER_BYTES);
-        if (many) many += 2 * a.want[1];
-        if (tokens) tokens += a.want[0];
+        const int64_t keys = x.window ? std::min<int64_t>(cap, std::min<int64_t>(x.sinks, cap) + std::min<int64_t>(x.window, cap) + 512) : cap;
+        many = std::min(many * (1 + keys / (Rows::GRAIN * Rows::ROUND)), many + 2 * a.want[1]);
+        tokens = std::min(tokens * (1 + keys / (Few::GRAIN / 2 * Few::ROUND)), tokens + a.want[0]);
     }
+    a.turn = (cus + 7) / 8 * 8;
+    many = (many + a.turn - 1) / a.turn * a.turn;
+    if (many) tokens = (tokens + a.turn - 1) / a.turn * a.turn;
     if (many + tokens >= (int64_t)1 << 24) return hipErrorInvalidValue;
     a.row_pieces = (int32_t)many;
     const unsigned grid = (unsigned)(many + tokens);
