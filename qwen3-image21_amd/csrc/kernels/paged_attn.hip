@@ -542,7 +542,6 @@ __device__ __forceinline__ void few_pairs(const Attn &a, int item, uint8_t *lds)
     const bool there = row < rq.n;
     const int pos = !there ? -1 : a.causal ? rq.len - rq.n + row : rq.len - 1;
     const int low = a.window ? pos - a.window : -1;  // sees key j <= pos if j > low or j < g.sk
-    const int pmin = tile * 32 + 31 < rq.n * a.G ? g.pos0 : -1;  // every pair sees up to it
 
     // ---- queries: dims 16 kk + 8 hi .. + 7 of the lane's pair ----
     bf16x8 qf[KK];
@@ -615,8 +614,8 @@ __device__ __forceinline__ void few_pairs(const Attn &a, int item, uint8_t *lds)
             load_k(n0, n1);
         }
 
-        // every pair of the tile sees all of it, or some do not
-        const bool some = !(key0 + KT - 1 <= pmin && (g0 | g1) >= 0 &&
+        // every pair that there is sees all of the tile, or some do not (those that are not have queries of 0)
+        const bool some = !(key0 + KT - 1 <= g.pos0 && (g0 | g1) >= 0 &&
                             (a.window == 0 || key0 > g.pos1 - a.window || key0 + KT <= g.sk));
         if (some) {
 #pragma unroll
@@ -786,7 +785,6 @@ __device__ __forceinline__ void many_pairs(const Attn &a, int item, uint8_t *lds
     const int pos = !there ? -1 : a.causal ? rq.len - rq.n + row : rq.len - 1;
     const int low = a.window ? pos - a.window : -1;      // sees key j <= pos if j > low or j < sk
     const int low0 = a.window ? w.pos0 - a.window : -1, sk = a.window ? a.sinks : 0;
-    const int pmin = 32 * wave + 31 < pairs ? w.pos0 : -1;  // every pair sees up to it
 
     // ---- tiles from the pages: the wave's granule of the next 64 tiles, a lane each ----
     const int32_t *table = a.tables + (int64_t)r * a.max_pages;
@@ -888,7 +886,7 @@ __device__ __forceinline__ void many_pairs(const Attn &a, int item, uint8_t *lds
                 s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf16x8 *)(kl + ST * STAGE + b * 2 * GB + kk * 512), qf[kk], s[b], 0, 0, 0);
         // every pair sees all of it, or some do not
         const uint32_t gone = (uint32_t)__ballot(about < 0) & 15u;
-        if (key0 + KEYS - 1 > pmin || gone || (a.window && key0 <= w.pos1 - a.window && key0 + KEYS > sk)) {
+        if (key0 + KEYS - 1 > w.pos0 || gone || (a.window && key0 <= w.pos1 - a.window && key0 + KEYS > sk)) {
 #pragma unroll
             for (int b = 0; b < 2; b++)
 #pragma unroll
