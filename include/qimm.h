@@ -347,7 +347,8 @@ int64_t qimm_pages_device_bytes(const qimm_pages *pg);
 /* Keys and values of `rows` rows, [kv_heads][head_dim] each, to their slots of a layer: F32, F16 or
  * BF16, rounded to bf16 (nearest even). k_row, k_head, v_row, v_head: elements from one row, one head
  * to the next (0: dense rows); k, v and the strides 16-byte aligned. A row whose slot is
- * outside the pages is left out; of rows with the same slot one is stored, in parts maybe. */
+ * outside the pages is left out; of rows with the same slot one is stored, in parts maybe. Fewer than
+ * 2^28 rows. */
 int qimm_pages_store(qimm_pages *pg, int64_t layer, const void *k, const void *v, int type, int64_t rows,
                      int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head, const int32_t *slots, void *stream);
 /* The rows of slots back, dense [rows][kv_heads][head_dim] bf16; zeros where a slot is outside the pages. */
@@ -362,7 +363,8 @@ int qimm_pages_load(const qimm_pages *pg, int64_t layer, uint16_t *k, uint16_t *
  * (causal) keys j <= p; in a window (> 0) of them j > p - window, and the first `sinks` keys,
  * j < sinks. A row that sees no key (p < 0) gives zeros; rows of no request are left as they were.
  * What keys hold that a row does not see does not count, NaN and infinities either. A table entry
- * outside the pages hides its keys. scale: positive. Rows of a refused request are of no use. q, its
+ * outside the pages hides its keys. Lengths past the table are cut to it. scale: positive. Rows of
+ * a refused request are of no use. Requests may have pages in common. q, its
  * strides and out are 16-byte aligned; up to 65536 requests. Allocates nothing and can be captured. */
 typedef struct {
     const uint16_t *q;

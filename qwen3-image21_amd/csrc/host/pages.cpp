@@ -1,6 +1,7 @@
 // The paged K/V cache: page tables of a step, rows into pages and back, attention over them.
 #include <math.h>
 
+#include <algorithm>
 #include <new>
 
 #include "internal.h"
@@ -22,6 +23,7 @@ namespace {
 
 constexpr int64_t MAX_TOKENS = (int64_t)1 << 31;  // slots and granules are int32
 constexpr int64_t MAX_REQUESTS = 65536;
+constexpr int64_t MAX_ROWS = (int64_t)1 << 28;     // of a store, 16 a workgroup
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -117,7 +119,7 @@ int qimm_pages_store(qimm_pages *pg, int64_t layer, const void *k, const void *v
     if (k_row < 0 || k_head < 0 || v_row < 0 || v_head < 0 || (k_row | k_head | v_row | v_head) % unit || !aligned16(k) ||
         !aligned16(v))
         return set_err(ctx, QIMM_ERR_ARG, "pages store: k, v and their strides must be 16-byte aligned");
-    if (rows >= MAX_TOKENS) return set_err(ctx, QIMM_ERR_SHAPE, "pages store: too many rows");
+    if (rows >= MAX_ROWS) return set_err(ctx, QIMM_ERR_SHAPE, "pages store: rows must be below 2^28");
     QIMM_HIP(ctx, hipSetDevice(ctx->device));
     const int64_t dense = pg->dims.kv_heads * d;
     QIMM_HIP(ctx, qimm::launch_pages_store(pg->dims, pg->layer(layer), k, v, type, k_row ? k_row : dense, k_head ? k_head : d,
@@ -132,7 +134,7 @@ int qimm_pages_load(const qimm_pages *pg, int64_t layer, uint16_t *k, uint16_t *
     const int rc = check_layer(pg, layer, "pages load");
     if (rc) return rc;
     if (!aligned16(k) || !aligned16(v)) return set_err(ctx, QIMM_ERR_ARG, "pages load: k and v must be 16-byte aligned");
-    if (rows >= MAX_TOKENS) return set_err(ctx, QIMM_ERR_SHAPE, "pages load: too many rows");
+    if (rows >= MAX_ROWS) return set_err(ctx, QIMM_ERR_SHAPE, "pages load: rows must be below 2^28");
     QIMM_HIP(ctx, hipSetDevice(ctx->device));
     QIMM_HIP(ctx, qimm::launch_pages_load(pg->dims, pg->layer(layer), k, v, slots, rows, (hipStream_t)stream));
     return QIMM_OK;
@@ -150,6 +152,9 @@ int qimm_attention_paged(qimm_pages *pg, int64_t layer, const qimm_paged_attenti
     if (!x->starts && x->rows != x->requests)
         return set_err(ctx, QIMM_ERR_SHAPE, "paged attention: without starts every request has one row");
     if (x->rows >= (MAX_TOKENS - 64) / x->heads) return set_err(ctx, QIMM_ERR_SHAPE, "paged attention: rows * heads must be below 2^31 - 64");
+    // the grid of the attention: tiles of 128 rows and heads, one more a request, and the shares
+    if (x->rows * x->heads / 128 + std::min(x->requests, x->rows) * pg->dims.kv_heads * 2 >= ((int64_t)1 << 24) - 8192)
+        return set_err(ctx, QIMM_ERR_SHAPE, "paged attention: too many rows and requests for one call");
     if (x->window < 0 || x->sinks < 0 || (x->window && !x->causal) || (x->sinks && !x->window))
         return set_err(ctx, QIMM_ERR_ARG, "paged attention: a window needs causal rows, sinks a window");
     if (!isfinite(x->scale) || x->scale <= 0.f) return set_err(ctx, QIMM_ERR_ARG, "paged attention: the scale must be positive and finite");

@@ -86,7 +86,7 @@ __device__ __forceinline__ Req req_of(const Attn &a, int r) {
 }
 
 // The keys that some pair of `pairs` from `first` on sees: [0, sk) and lo .. hi - 1, as tiles of KEYS: ns of
-// the first ones, then from w0 on; pos0, pos1: the positions of the first and last row.
+// the first ones, then from w0 on; pos0, pos1: the positions of the first and last row (-1 before token 0).
 struct Range {
     int pos0, pos1, lo, hi, sk, ns, w0, tiles;
 };
@@ -94,9 +94,9 @@ template <int KEYS>
 __device__ __forceinline__ Range range_of(const Attn &a, const Req &q, int first, int pairs) {
     Range g;
     const int i0 = min(row_of_pair(a, first), q.n - 1), i1 = min(q.n - 1, row_of_pair(a, first + pairs - 1));
-    g.pos0 = a.causal ? q.len - q.n + i0 : q.len - 1;
-    g.pos1 = a.causal ? q.len - q.n + i1 : q.len - 1;
-    g.hi = max(g.pos1 + 1, 0);
+    g.pos0 = max(a.causal ? q.len - q.n + i0 : q.len - 1, -1);
+    g.pos1 = max(a.causal ? q.len - q.n + i1 : q.len - 1, -1);
+    g.hi = g.pos1 + 1;
     g.lo = a.window ? max(g.pos0 - a.window + 1, 0) : 0;
     g.sk = a.window ? min(a.sinks, g.hi) : 0;
     g.ns = (g.sk + KEYS - 1) / KEYS;
@@ -540,7 +540,7 @@ __device__ __forceinline__ void few_pairs(const Attn &a, int item, uint8_t *lds)
     // the lane's pair: row i of the request, head h G + hd
     const int f = tile * 32 + l32, row = row_of_pair(a, f), hd = f - row * a.G;
     const bool there = row < rq.n;
-    const int pos = !there ? -1 : a.causal ? rq.len - rq.n + row : rq.len - 1;
+    const int pos = !there ? -1 : max(a.causal ? rq.len - rq.n + row : rq.len - 1, -1);
     const int low = a.window ? pos - a.window : -1;  // sees key j <= pos if j > low or j < g.sk
 
     // ---- queries: dims 16 kk + 8 hi .. + 7 of the lane's pair ----
@@ -782,7 +782,7 @@ __device__ __forceinline__ void many_pairs(const Attn &a, int item, uint8_t *lds
     const bool any = 32 * wave < pairs;
     const int f = f0 + 32 * wave + l32, row = row_of_pair(a, f), hd = f - row * a.G;
     const bool there = row < rq.n;
-    const int pos = !there ? -1 : a.causal ? rq.len - rq.n + row : rq.len - 1;
+    const int pos = !there ? -1 : max(a.causal ? rq.len - rq.n + row : rq.len - 1, -1);
     const int low = a.window ? pos - a.window : -1;      // sees key j <= pos if j > low or j < sk
     const int low0 = a.window ? w.pos0 - a.window : -1, sk = a.window ? a.sinks : 0;
 

@@ -283,14 +283,14 @@ __device__ __forceinline__ u32x2 column(const u32x4 (&x)[4], int e) {
 
 // A wave takes rows t0 .. t0 + 15 of 128 / D heads. T: the rows' type; STORE: into the pages, else out of them
 // (bf16).
-template <typename T, bool STORE, int D>
-__global__ __launch_bounds__(256) void pages_rows_kernel(PageDims d, uint8_t *layer, T *k, T *v, int64_t k_row, int64_t k_head,
+template <typename T, bool STORE, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void pages_rows_kernel(PageDims d, uint8_t *layer, T *k, T *v, int64_t k_row, int64_t k_head,
                                                          int64_t v_row, int64_t v_head, const int32_t *__restrict__ slots,
                                                          int64_t rows) {
     constexpr int OCT = D / 8, HEADS = 128 / D;      // lanes a row; heads of a wave
-    __shared__ __attribute__((aligned(16))) uint8_t lds[4][4096];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[WAVES][4096];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int h = (blockIdx.y * 4 + wave) * HEADS + lane / (64 / HEADS);
+    const int h = (blockIdx.y * WAVES + wave) * HEADS + lane / (64 / HEADS);
     const int64_t t0 = (int64_t)blockIdx.x * 16;
     const int64_t most = d.pages * d.page_size;
     // lane i: the slot of row t0 - 15 + i, and whether it leads 16 rows with the slots of a granule
@@ -429,21 +429,28 @@ __global__ __launch_bounds__(256) void pages_rows_kernel(PageDims d, uint8_t *la
     }
 }
 
+template <typename T, bool STORE, int D>
+hipError_t launch_heads(const PageDims &d, uint8_t *layer, T *k, T *v, int64_t k_row, int64_t k_head, int64_t v_row,
+                        int64_t v_head, const int32_t *slots, int64_t rows, hipStream_t stream) {
+    const int64_t blocks = (rows + 15) / 16, heads = (d.kv_heads + 128 / D - 1) / (128 / D);
+    if (blocks >= (int64_t)1 << 24 || d.kv_heads > 65535) return hipErrorInvalidValue;
+    // Workgroups of one wave as long as they do not fill the CUs: single tokens are a store of 64 lines after the
+    // other (48 rows of 8 heads 5.0 us, 8.6 in fours).
+    if (blocks * heads <= 4 * (int64_t)device_cu_count())
+        pages_rows_kernel<T, STORE, D, 1><<<dim3((unsigned)blocks, (unsigned)heads), 64, 0, stream>>>(
+            d, layer, k, v, k_row, k_head, v_row, v_head, slots, rows);
+    else
+        pages_rows_kernel<T, STORE, D, 4><<<dim3((unsigned)blocks, (unsigned)((heads + 3) / 4)), 256, 0, stream>>>(
+            d, layer, k, v, k_row, k_head, v_row, v_head, slots, rows);
+    return hipGetLastError();
+}
 template <typename T, bool STORE>
 hipError_t launch_rows(const PageDims &d, uint8_t *layer, T *k, T *v, int64_t k_row, int64_t k_head, int64_t v_row,
                        int64_t v_head, const int32_t *slots, int64_t rows, hipStream_t stream) {
     if (rows <= 0) return hipSuccess;
-    const int per = 4 * 128 / d.head_dim;  // heads of a workgroup
-    const int64_t blocks = (rows + 15) / 16;
-    if (blocks >= (int64_t)1 << 24 || d.kv_heads > 65535) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)blocks, (unsigned)((d.kv_heads + per - 1) / per));
-    if (d.head_dim == 128)
-        pages_rows_kernel<T, STORE, 128><<<grid, 256, 0, stream>>>(d, layer, k, v, k_row, k_head, v_row, v_head, slots, rows);
-    else if (d.head_dim == 64)
-        pages_rows_kernel<T, STORE, 64><<<grid, 256, 0, stream>>>(d, layer, k, v, k_row, k_head, v_row, v_head, slots, rows);
-    else
-        return hipErrorInvalidValue;
-    return hipGetLastError();
+    if (d.head_dim == 128) return launch_heads<T, STORE, 128>(d, layer, k, v, k_row, k_head, v_row, v_head, slots, rows, stream);
+    if (d.head_dim == 64) return launch_heads<T, STORE, 64>(d, layer, k, v, k_row, k_head, v_row, v_head, slots, rows, stream);
+    return hipErrorInvalidValue;
 }
 
 }  // namespace

@@ -160,7 +160,11 @@ def test_rows_that_see_nothing(torch_cuda, qctx):
     of no request stay as they were."""
     torch = torch_cuda
     c = Case(torch, qctx, [0, 5, 0, 40], [1, 9, 3, 2], 4, 2, 128, 16)
-    for kw in (dict(), dict(window=3, sinks=1), dict(causal=False)):
+    d = Case(torch, qctx, [30], [300], 4, 2, 64, 32)
+    for kw in (dict(), dict(window=5), dict(window=2 ** 31 - 1)):
+        d.check(**kw)
+    d.free()
+    for kw in (dict(), dict(window=3, sinks=1), dict(window=10 ** 10), dict(window=2 ** 31 - 1, sinks=2), dict(causal=False)):
         c.pg.attention(0, c.call(rows=c.t + 3, out=torch.full((c.t + 3, 4 * 128), 7.0, dtype=torch.bfloat16, device="cuda"), **kw),
                        stream(torch))
         assert_near(torch, c.out[:c.t], *c.want(**kw))
@@ -234,6 +238,22 @@ def test_tables_and_lengths_out_of_range(torch_cuda, qctx):
     c.free()
 
 
+def test_starts_that_overlap_leave_the_next_call_alone(torch_cuda, qctx):
+    """Rows that several requests claim: more pieces than the rows can have; whatever is computed for them, a
+    later call finds its counters as they should be."""
+    torch = torch_cuda
+    c = Case(torch, qctx, [9000, 70, 9000, 8000], [60, 50, 3, 40], 8, 2, 64, 16)
+    c.check()
+    for starts in ([0, 153, 0, 153, 153], [153, 0, 153, 0, 153], [-5, 400, -7, 2 ** 31 - 1, 3], [0, 153, 153, 0, 153]):
+        a = c.call()
+        c.starts_d.copy_(dev(torch, np.array(starts, np.int32)))
+        for _ in range(2):
+            c.pg.attention(0, a, stream(torch))
+        torch.cuda.synchronize()
+        c.check()
+    c.free()
+
+
 def test_strided_queries_and_scales(torch_cuda, qctx):
     """Queries inside a fused projection, and head-major as qk_norm_rope leaves them."""
     torch = torch_cuda
@@ -302,7 +322,7 @@ def test_attention_refuses(torch_cuda, qctx):
     for layer in (-1, 1):
         assert lib.qimm_attention_paged(c.pg.h, layer, qimm.C.byref(c.call()), None) == 2
     for field, value, status in [("rows", -1, 2), ("requests", -1, 2), ("requests", 65537, 2), ("max_pages", -1, 2), ("heads", 0, 2), ("heads", 3, 2),
-                                 ("rows", 2 ** 30, 2), ("starts", None, 2), ("window", -1, 1), ("sinks", -1, 1), ("sinks", 2, 1), ("scale", 0.0, 1),
+                                 ("rows", 2 ** 30, 2), ("rows", 2 ** 29 - 64, 2), ("starts", None, 2), ("window", -1, 1), ("sinks", -1, 1), ("sinks", 2, 1), ("scale", 0.0, 1),
                                  ("scale", -1.0, 1), ("scale", float("nan"), 1), ("scale", float("inf"), 1), ("q", None, 1), ("out", None, 1),
                                  ("tables", None, 1), ("lengths", None, 1), ("q", c.q.data_ptr() + 2, 1), ("q_row", 260, 1), ("q_head", -64, 1)]:
         a = c.call()
