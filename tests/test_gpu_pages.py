@@ -84,6 +84,17 @@ def test_plan_of_the_largest_chunk(torch_cuda, qctx):
     p.check(paged_ref.plan(page, pages, *case))
 
 
+@pytest.mark.parametrize("n", [3, 3000])
+def test_plan_without_positions(torch_cuda, qctx, n):
+    torch = torch_cuda
+    case = a_case(np.random.default_rng(n), n, 16, 60, 9)
+    p = Plan(torch, 16, *case)
+    p.call.positions = None
+    qctx.page_plan(p.call, stream(torch))
+    want = paged_ref.plan(16, len(case[3]), *case)
+    assert np.array_equal(host(p.slots), want["slots"]) and (p.positions == -99).all()
+
+
 def test_plan_of_lengths_that_make_no_sense(torch_cuda, qctx):
     """Negative lengths, lengths past the table, sums past 32 bits, a state outside the queue: refused
     or cut, and nothing outside the arrays is touched."""
