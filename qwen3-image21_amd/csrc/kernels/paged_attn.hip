@@ -229,6 +229,13 @@ __device__ __forceinline__ T lane_of(T v, int lane) {
 // share has the piece looks which.
 template <typename F>
 __device__ __forceinline__ bool piece_of(const Attn &a, int item, int most, Piece &out) {
+    if (!F::ROWS && !a.starts && !a.count) {
+        // one tile of every request and key head
+        const int r = item / a.Hkv;
+        if (r >= a.R) return false;
+        out = {r, item - r * a.Hkv, 0, 0, 1, 0, req_of(a, r)};
+        return true;
+    }
     if (a.R <= 64) {
         const int lane = threadIdx.x & 63;
         Req q = lane < a.R ? req_of(a, lane) : Req{0, 0, 0};
@@ -537,19 +544,23 @@ __device__ __forceinline__ void few_pairs(const Attn &a, int item, uint8_t *lds)
     if (!piece_of<Few>(a, item, (int)gridDim.x - a.row_pieces, pc)) return;
     const int r = pc.r, h = pc.h, tile = pc.tile;
     const Req rq = pc.rq;
-    const Range g = range_of<KT>(a, rq, tile * 32, 32);
-    // the share's tiles: whole rounds
-    const int rounds = (g.tiles + 3) / 4;
-    const int first = (int)((int64_t)rounds * pc.share / pc.shares) * 4;
-    const int last = min((int)((int64_t)rounds * (pc.share + 1) / pc.shares) * 4, g.tiles);
 
-    // the lane's pair: row i of the request, head h G + hd
+    // ---- the granules of the wave's next 32 tiles, lane 2 k + j: granule j of tile k (-1: no page) ----
+    const int32_t *table = a.tables + (int64_t)r * a.max_pages;
+    auto page_at = [&](uint32_t x, uint32_t &k) __attribute__((always_inline)) {
+        k = __umulhi(x, a.ps16_magic) + (a.ps16 == 1 ? x : 0);
+        return (int64_t)k < a.max_pages ? table[k] : -1;
+    };
+    // without a window and shares the first ones do not depend on the length: one read less before the keys'
+    uint32_t k0 = 0;
+    const uint32_t x0 = 2 * (wave + (lane >> 1) * 4) + (lane & 1);
+    const bool ahead = !a.window && pc.shares == 1;
+    int page0 = -1;
+    if (ahead) page0 = page_at(x0, k0);
+
+    // the lane's pair: row i of the request, head h G + hd; its queries' dims 16 kk + 8 hi .. + 7
     const int f = tile * 32 + l32, row = row_of_pair(a, f), hd = f - row * a.G;
     const bool there = row < rq.n;
-    const int pos = !there ? -1 : max(a.causal ? rq.len - rq.n + row : rq.len - 1, -1);
-    const int low = a.window ? pos - a.window : -1;  // sees key j <= pos if j > low or j < g.sk
-
-    // ---- queries: dims 16 kk + 8 hi .. + 7 of the lane's pair ----
     bf16x8 qf[KK];
     {
         const uint16_t *src = a.q + (int64_t)(rq.start + (there ? row : 0)) * a.q_row + (int64_t)(h * a.G + (there ? hd : 0)) * a.q_head + 8 * hi;
@@ -561,19 +572,26 @@ __device__ __forceinline__ void few_pairs(const Attn &a, int item, uint8_t *lds)
         }
     }
 
-    // ---- the granules of the wave's next 32 tiles, lane 2 k + j: granule j of tile k (-1: no page) ----
-    const int32_t *table = a.tables + (int64_t)r * a.max_pages;
+    const Range g = range_of<KT>(a, rq, tile * 32, 32);
+    // the share's tiles: whole rounds
+    const int rounds = (g.tiles + 3) / 4;
+    const int first = (int)((int64_t)rounds * pc.share / pc.shares) * 4;
+    const int last = min((int)((int64_t)rounds * (pc.share + 1) / pc.shares) * 4, g.tiles);
+    const int pos = !there ? -1 : max(a.causal ? rq.len - rq.n + row : rq.len - 1, -1);
+    const int low = a.window ? pos - a.window : -1;  // sees key j <= pos if j > low or j < g.sk
+
     int gran = 0;
+    auto granule_of = [&](int page, uint32_t x, uint32_t k) __attribute__((always_inline)) {
+        return page >= 0 && page < a.pages ? (page * a.Hkv + h) * a.ps16 + (int)(x - k * a.ps16) : -1;
+    };
     auto load_granules = [&](int v) __attribute__((always_inline)) {
         const int mine = v + (lane >> 1) * 4;
         gran = -1;
         if (mine < last) {
             const uint32_t x = 2 * tile_at(g, mine) + (lane & 1);
-            const uint32_t k = __umulhi(x, a.ps16_magic) + (a.ps16 == 1 ? x : 0);
-            if ((int64_t)k < a.max_pages) {
-                const int page = table[k];
-                if (page >= 0 && page < a.pages) gran = (page * a.Hkv + h) * a.ps16 + (int)(x - k * a.ps16);
-            }
+            uint32_t k;
+            const int page = page_at(x, k);
+            gran = granule_of(page, x, k);
         }
     };
     u32x4 kc[KK], vc[2][DT];
@@ -597,7 +615,10 @@ __device__ __forceinline__ void few_pairs(const Attn &a, int item, uint8_t *lds)
     int g0 = -1, g1 = -1, n0 = -1, n1 = -1, k = 0;
     int v = first + wave;
     if (v < last) {
-        load_granules(v);
+        if (ahead)
+            gran = (int)(x0 >> 1) < last ? granule_of(page0, x0, k0) : -1;
+        else
+            load_granules(v);
         g0 = __builtin_amdgcn_readlane(gran, 0);
         g1 = __builtin_amdgcn_readlane(gran, 1);
         load_k(g0, g1);
