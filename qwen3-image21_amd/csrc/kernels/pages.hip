@@ -115,7 +115,8 @@ __device__ __forceinline__ void give_back(const PagePlanArgs &p, int64_t r, int 
 // base, entries before its first page given back (-1: none)}: in LDS (FILL: up to PLAN_REQUESTS), for
 // the rows, which it then writes; or in work, then {head, free}. A request that fits within the rows has
 // only such before it, so the sums need not ask for it.
-template <int THREADS, bool FILL>
+// HELD: the requests of a thread, in registers (their lengths are read together); 0: any number, read twice.
+template <int THREADS, bool FILL, int HELD>
 __global__ __launch_bounds__(THREADS) void page_plan_kernel(const PagePlanArgs p) {
     __shared__ Sums part[THREADS / 64];
     __shared__ int taken, refused;
@@ -130,16 +131,21 @@ __global__ __launch_bounds__(THREADS) void page_plan_kernel(const PagePlanArgs p
     if (head < 0) head += (int)p.pages;
 
     Sums mine{0, 0, 0}, all;
-    Step s;
-    for (int64_t r = r0; r < r1; r++) {
-        s = step_of(p, r);
-        mine = add(mine, s.sums());
+    Step held[HELD ? HELD : 1];
+    if constexpr (HELD > 0) {
+#pragma unroll
+        for (int i = 0; i < HELD; i++)
+            if (r0 + i < r1) held[i] = step_of(p, r0 + i);
+#pragma unroll
+        for (int i = 0; i < HELD; i++)
+            if (r0 + i < r1) mine = add(mine, held[i].sums());
+    } else {
+        for (int64_t r = r0; r < r1; r++) mine = add(mine, step_of(p, r).sums());
     }
     Sums at = block_scan<THREADS>(mine, part, all);
     const uint32_t most = (uint32_t)p.max_rows;
     int used = 0, no = 0;
-    for (int64_t r = r0; r < r1; r++) {
-        if (!FILL) s = step_of(p, r);
+    auto settle = [&](int64_t r, const Step &s) __attribute__((always_inline)) {
         const Sums end = add(at, s.sums());
         const bool served = s.fits && end.rows <= most && (s.need == 0 || end.need <= (uint32_t)free);
         const int start = (int)min(at.rows, most);
@@ -155,6 +161,13 @@ __global__ __launch_bounds__(THREADS) void page_plan_kernel(const PagePlanArgs p
         if (served && s.need) used = (int)end.need;
         no += s.add > 0 && !served;
         at = end;
+    };
+    if constexpr (HELD > 0) {
+#pragma unroll
+        for (int i = 0; i < HELD; i++)
+            if (r0 + i < r1) settle(r0 + i, held[i]);
+    } else {
+        for (int64_t r = r0; r < r1; r++) settle(r, step_of(p, r));
     }
     if (used) atomicMax(&taken, used);
     if (no) atomicAdd(&refused, no);
@@ -210,37 +223,40 @@ __device__ __forceinline__ int64_t request_of(const int32_t *starts, int64_t n, 
     return lo;
 }
 
-// Slots, positions and table entries of the rows, then the queue entries of the pages given back.
+// Slots, positions and table entries of the rows, then the queue entries of the pages given back. Starts of up to
+// HELD requests are all read into LDS, of more those of the workgroup's rows.
 __global__ __launch_bounds__(256) void page_fill_kernel(const PagePlanArgs p) {
-    constexpr int HELD = 1024;
+    constexpr int HELD = 4096;
     __shared__ int starts[HELD];
     __shared__ int64_t ends[2];
     const int64_t R = p.requests;
     const int head = p.work[4 * R], free = p.work[4 * R + 1], all = p.starts[R];
     const int tid = threadIdx.x, lane = tid & 63;
     const int64_t t0 = (int64_t)blockIdx.x * 256, t = t0 + tid;
-    if (t0 < all) {
-        // the requests of the workgroup's first and last row, their starts into LDS
+    int64_t r0 = 0, n = R;  // the requests that may have the workgroup's rows
+    if (R > HELD && t0 < all) {
         if (tid < 128) {
             const int64_t r = request_of(p.starts, R, tid < 64 ? t0 : min(t0 + 255, (int64_t)all - 1));
             if (lane == 0) ends[tid >> 6] = r;
         }
         __syncthreads();
-        const int64_t r0 = ends[0], n = ends[1] - r0 + 1;
-        for (int64_t i = tid; i < min(n, (int64_t)HELD); i += 256) starts[i] = p.starts[r0 + i];
-        __syncthreads();
-        if (t < all) {
-            int64_t lo = 0, hi = n;
-            while (hi - lo > 1) {
-                const int64_t mid = (lo + hi) >> 1;
-                if ((mid < HELD ? starts[mid] : p.starts[r0 + mid]) <= t)
-                    lo = mid;
-                else
-                    hi = mid;
-            }
-            const int4 w = *(const int4 *)(p.work + 4 * (r0 + lo));
-            fill_row(p, t, r0 + lo, w.x, w.y, w.z, head);
+        r0 = ends[0];
+        n = ends[1] - r0 + 1;
+    }
+#pragma unroll 8
+    for (int64_t i = tid; i < min(n, (int64_t)HELD); i += 256) starts[i] = p.starts[r0 + i];
+    __syncthreads();
+    if (t < all) {
+        int64_t lo = 0, hi = n;
+        while (hi - lo > 1) {
+            const int64_t mid = (lo + hi) >> 1;
+            if ((mid < HELD ? starts[mid] : p.starts[r0 + mid]) <= t)
+                lo = mid;
+            else
+                hi = mid;
         }
+        const int4 w = *(const int4 *)(p.work + 4 * (r0 + lo));
+        fill_row(p, t, r0 + lo, w.x, w.y, w.z, head);
     }
     if (t >= all && t < p.max_rows) {
         p.slots[t] = -1;
@@ -460,12 +476,15 @@ hipError_t launch_page_plan(const PagePlanArgs &p, hipStream_t stream) {
     if (p.requests <= 0 || p.pages <= 0 || blocks >= (int64_t)1 << 24) return hipErrorInvalidValue;
     if (p.requests <= PLAN_REQUESTS && p.max_rows <= PLAN_ROWS) {
         if (p.requests <= 256 && p.max_rows <= 512)
-            page_plan_kernel<256, true><<<1, 256, 0, stream>>>(p);
+            page_plan_kernel<256, true, 1><<<1, 256, 0, stream>>>(p);
         else
-            page_plan_kernel<PLAN_REQUESTS, true><<<1, PLAN_REQUESTS, 0, stream>>>(p);
+            page_plan_kernel<PLAN_REQUESTS, true, 1><<<1, PLAN_REQUESTS, 0, stream>>>(p);
         return hipGetLastError();
     }
-    page_plan_kernel<1024, false><<<1, 1024, 0, stream>>>(p);
+    if (p.requests <= 4096)
+        page_plan_kernel<1024, false, 4><<<1, 1024, 0, stream>>>(p);
+    else
+        page_plan_kernel<1024, false, 0><<<1, 1024, 0, stream>>>(p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     page_fill_kernel<<<(unsigned)(blocks > 0 ? blocks : 1), 256, 0, stream>>>(p);

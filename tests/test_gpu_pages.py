@@ -73,6 +73,17 @@ def test_plan(torch_cuda, qctx, n, page, longest, most_new, short, rows_short, s
         p.check(want)
 
 
+@pytest.mark.parametrize("n,every", [(4096, 1), (4096, 300), (4097, 1), (4097, 300), (20000, 150)])
+def test_plan_of_many_that_add_nothing(torch_cuda, qctx, n, every):
+    """One request in `every` has a step: few rows lie thousands of requests apart."""
+    torch = torch_cuda
+    case = list(a_case(np.random.default_rng(n + every), n, 16, 40, 7))
+    case[2][np.arange(n) % every != every - 1] = 0
+    p = Plan(torch, 16, *case)
+    qctx.page_plan(p.call, stream(torch))
+    p.check(paged_ref.plan(16, len(case[3]), *case))
+
+
 def test_plan_of_the_largest_chunk(torch_cuda, qctx):
     torch = torch_cuda
     page, new = 16, 300001
