@@ -15,10 +15,10 @@
 // clock, 16 KB of a 32-key tile of 128 dims take it 1900 clocks, its 16 matrix instructions a SIMD 512 and
 // the softmax about as many, so the columns of a tile that are empty cost nothing. Four waves take
 // tiles of 32 keys in turn straight into registers (two operands of 8 KB in flight each: no LDS, no barrier) and
-// join their sums through LDS. One token over 131001 keys of 8 heads: 105 us, 5.1 TB/s.
+// join their sums through LDS. One token over 131001 keys of 8 heads: 103 us, 5.2 TB/s.
 //
 // More (many_pairs) are bound by the matrix pipe and the softmax beside it: four waves share 64-key tiles in
-// LDS, where each key is read by 128 pairs. A prompt of 8395 tokens, 32 heads over 8, causal: 593 us, 0.98
+// LDS, where each key is read by 128 pairs. A prompt of 8395 tokens, 32 heads over 8, causal: 582 us, 0.99
 // PFLOP/s (two such workgroups on a CU take 2.1 us a tile each, one alone 1.7).
 //
 // Long requests in few workgroups are split over their keys. The host does not know the lengths, so
@@ -177,7 +177,7 @@ __device__ __forceinline__ Split split_of(const Attn &a, const Req &q, int chunk
 // long: 136 tiles of 100 rounds in 544 shares took 139 us, in 408 112 (with their join as it was then). Of few
 // pairs shares may be of half a GRAIN as long as each has a CU of its own: one token over 4000 keys of 8 heads
 // 14.5 us in 64 shares, 11.7 in 128, but 8 of them over 2000 18.4 in 256 and 19.5 in 512. Requests of up to a
-// GRAIN are not split: 333 keys of 32 heads 8.4 us, 10.2 in two shares.
+// GRAIN are not split: 333 keys of 32 heads took 8.4 us whole (6.6 since) and 10.2 in two shares.
 template <typename F>
 __device__ __forceinline__ int chunk_of(const Attn &a, float rounds, int64_t tiles) {
     const int want = a.want[F::ROWS], c = (int)(rounds * (float)a.Hkv / (float)want) + 1;

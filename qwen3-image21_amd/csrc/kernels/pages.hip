@@ -3,8 +3,9 @@
 // The plan. Request r has old_r tokens and adds a_r; with the sums over the requests before it,
 // start_r of rows and base_r of new pages, its page k from ceil(old_r / ps) on is entry base_r + ... of
 // the queue of free pages, and the slot of a token at position p is table[p / ps] ps + p % ps. Bound by
-// latency: a few bytes a request and 8 a row. One workgroup makes the sums in registers; where requests and
-// rows are few it writes the rows too, from LDS, else a second launch does.
+// latency: a few bytes a request and 8 a row, so reads that do not depend on each other are made together. One workgroup
+// makes the sums in registers; where requests and rows are few it writes the rows too, from LDS, else a second
+// launch does. 48 requests of a token: 3.0 us; 2048 requests, 128 of them of 509 tokens: 5.3 and 6.7.
 //
 // The store. Bound by bytes. Where 16 rows are the 16 slots of a granule, in order, a wave takes them: keys as
 // they are read are written 1 KB in a row, values are turned over in registers, four rows and eight dims a
@@ -115,7 +116,8 @@ __device__ __forceinline__ void give_back(const PagePlanArgs &p, int64_t r, int 
 // base, entries before its first page given back (-1: none)}: in LDS (FILL: up to PLAN_REQUESTS), for
 // the rows, which it then writes; or in work, then {head, free}. A request that fits within the rows has
 // only such before it, so the sums need not ask for it.
-// HELD: the requests of a thread, in registers (their lengths are read together); 0: any number, read twice.
+// HELD: the requests of a thread, in registers (their lengths are read together, which took the launch for 2048
+// requests from 6.3 to 5.3 us); 0: any number, read twice.
 template <int THREADS, bool FILL, int HELD>
 __global__ __launch_bounds__(THREADS) void page_plan_kernel(const PagePlanArgs p) {
     __shared__ Sums part[THREADS / 64];
