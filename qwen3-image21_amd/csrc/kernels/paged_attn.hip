@@ -770,12 +770,12 @@ __device__ __forceinline__ void load_lds_4k(const uint8_t *src, uint8_t *dst) {
         "s_mov_b32 m0, %1\n\t"
         "s_nop 0\n\t"
         "global_load_lds_dwordx4 %2, off\n\t"
-        "global_load_lds_dwordx4 %2, off offset:1024\n\t"
-        "global_load_lds_dwordx4 %2, off offset:2048\n\t"
-        "global_load_lds_dwordx4 %2, off offset:3072\n\t"
+        "global_load_lds_dwordx4 %2, off offset:%3\n\t"
+        "global_load_lds_dwordx4 %2, off offset:%4\n\t"
+        "global_load_lds_dwordx4 %2, off offset:%5\n\t"
         "s_mov_b32 m0, %0"
         : "=&s"(m0)
-        : "s"(__builtin_amdgcn_readfirstlane(at)), "v"(src)
+        : "s"(__builtin_amdgcn_readfirstlane(at)), "v"(src), "i"(1 << 10), "i"(2 << 10), "i"(3 << 10)
         : "memory");
 }
 __device__ __forceinline__ void lds_wait() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
