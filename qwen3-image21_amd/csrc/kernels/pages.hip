@@ -11,6 +11,7 @@
 // they are read are written 1 KB in a row, values are turned over in registers, four rows and eight dims a
 // lane, and gathered in LDS (paged.h). Other rows, the ends of a request and single tokens, are
 // written 16 B of a key and 2 B of a value at a time.
+#include <algorithm>
 #include <type_traits>
 
 #include "device_common.h"
@@ -112,6 +113,21 @@ __device__ __forceinline__ void give_back(const PagePlanArgs &p, int64_t r, int 
         *queue_at(p, head, free + back + k) = p.tables[r * p.max_pages + k];
 }
 
+// The pages of all requests given back, wave `wave` of `waves`: of its requests, every `waves`-th, a lane each
+// looks whether it is one. of(r): {, old, , entries before its first page (-1: not given back)}.
+template <typename OF>
+__device__ __forceinline__ void give_back_all(const PagePlanArgs &p, int64_t wave, int64_t waves, int head, int free, OF of) {
+    const int lane = threadIdx.x & 63;
+    for (int64_t r0 = wave; r0 < p.requests; r0 += 64 * waves) {
+        const int64_t r = r0 + lane * waves;
+        const int4 w = r < p.requests ? of(r) : make_int4(0, 0, 0, -1);
+        for (uint64_t some = __ballot(w.w >= 0); some; some &= some - 1) {
+            const int i = __builtin_ctzll(some);
+            give_back(p, r0 + i * waves, __builtin_amdgcn_readlane(w.y, i), __builtin_amdgcn_readlane(w.w, i), head, free, lane);
+        }
+    }
+}
+
 // The sums of a step by one workgroup: starts, lengths_out, state_out, and of every request {start, old,
 // base, entries before its first page given back (-1: none)}: in LDS (FILL: up to PLAN_REQUESTS), for
 // the rows, which it then writes; or in work, then {head, free}. A request that fits within the rows has
@@ -207,8 +223,7 @@ __global__ __launch_bounds__(THREADS) void page_plan_kernel(const PagePlanArgs p
             fill_row(p, t, lo, w.x, w.y, w.z, head);
         }
         if (all.freed)
-            for (int64_t r = tid >> 6; r < R; r += THREADS / 64)
-                if (of[r].w >= 0) give_back(p, r, of[r].y, of[r].w, head, free, tid & 63);
+            give_back_all(p, tid >> 6, THREADS / 64, head, free, [&](int64_t r) { return of[r]; });
     }
 }
 
@@ -226,7 +241,8 @@ __device__ __forceinline__ int64_t request_of(const int32_t *starts, int64_t n, 
 }
 
 // Slots, positions and table entries of the rows, then the queue entries of the pages given back. Starts of up to
-// HELD requests are all read into LDS, of more those of the workgroup's rows.
+// HELD requests are all read into LDS, of more those of the workgroup's rows. Workgroups behind the rows only give
+// pages back.
 __global__ __launch_bounds__(256) void page_fill_kernel(const PagePlanArgs p) {
     constexpr int HELD = 4096;
     __shared__ int starts[HELD];
@@ -245,9 +261,11 @@ __global__ __launch_bounds__(256) void page_fill_kernel(const PagePlanArgs p) {
         r0 = ends[0];
         n = ends[1] - r0 + 1;
     }
+    if (t0 < p.max_rows) {
 #pragma unroll 8
-    for (int64_t i = tid; i < min(n, (int64_t)HELD); i += 256) starts[i] = p.starts[r0 + i];
-    __syncthreads();
+        for (int64_t i = tid; i < min(n, (int64_t)HELD); i += 256) starts[i] = p.starts[r0 + i];
+        __syncthreads();
+    }
     if (t < all) {
         int64_t lo = 0, hi = n;
         while (hi - lo > 1) {
@@ -264,11 +282,8 @@ __global__ __launch_bounds__(256) void page_fill_kernel(const PagePlanArgs p) {
         p.slots[t] = -1;
         if (p.positions) p.positions[t] = 0;
     }
-    const int64_t waves = (int64_t)gridDim.x * 4;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + (tid >> 6); r < R; r += waves) {
-        const int back = p.work[4 * r + 3];
-        if (back >= 0) give_back(p, r, p.work[4 * r + 1], back, head, free, lane);
-    }
+    give_back_all(p, (int64_t)blockIdx.x * 4 + (tid >> 6), (int64_t)gridDim.x * 4, head, free,
+                  [&](int64_t r) { return *(const int4 *)(p.work + 4 * r); });
 }
 
 // ---- rows to slots and back ----
@@ -489,7 +504,8 @@ hipError_t launch_page_plan(const PagePlanArgs &p, hipStream_t stream) {
         page_plan_kernel<1024, false, 0><<<1, 1024, 0, stream>>>(p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    page_fill_kernel<<<(unsigned)(blocks > 0 ? blocks : 1), 256, 0, stream>>>(p);
+    // (a wave for every two requests, up to 4096 waves: all of those may be given back)
+    page_fill_kernel<<<(unsigned)std::max(blocks, std::min((p.requests + 7) / 8, (int64_t)1024)), 256, 0, stream>>>(p);
     return hipGetLastError();
 }
 

@@ -84,6 +84,19 @@ def test_plan_of_many_that_add_nothing(torch_cuda, qctx, n, every):
     p.check(paged_ref.plan(16, len(case[3]), *case))
 
 
+@pytest.mark.parametrize("n,rows", [(200, 0), (1000, 0), (1500, 7), (9000, 700), (65536, 0), (65536, 40)])
+def test_plan_of_many_given_back(torch_cuda, qctx, n, rows):
+    """Most requests give their pages back, up to a few that add a token."""
+    torch = torch_cuda
+    case = list(a_case(np.random.default_rng(n + rows), n, 16, 60, 0))
+    case[2][:] = np.where(np.arange(n) % 11 == 3, 0, -1)
+    case[2][np.random.default_rng(n).permutation(n)[:rows]] = 1
+    case[5] = rows + 3 if rows else 0
+    p = Plan(torch, 16, *case)
+    qctx.page_plan(p.call, stream(torch))
+    p.check(paged_ref.plan(16, len(case[3]), *case))
+
+
 def test_plan_of_the_largest_chunk(torch_cuda, qctx):
     torch = torch_cuda
     page, new = 16, 300001
