@@ -35,14 +35,14 @@ namespace qimm {
 namespace {
 
 // The two forms: pairs of a tile, keys of a round, and the shares: at least GRAIN rounds each, at most MOST of
-// a tile, SLOTS in all; `want` workgroups are the aim (Attn).
+// a tile, SLOTS in all; `want` workgroups are the aim (Attn), ON_CU a CU.
 struct Few {
     static constexpr bool ROWS = false;
-    static constexpr int TM = 32, ROUND = 128, GRAIN = 4, MOST = 128, SLOTS = 1280;
+    static constexpr int TM = 32, ROUND = 128, GRAIN = 4, MOST = 128, SLOTS = 1280, ON_CU = 4;
 };
 struct Rows {
     static constexpr bool ROWS = true;
-    static constexpr int TM = 128, ROUND = 64, GRAIN = 8, MOST = 64, SLOTS = 640;
+    static constexpr int TM = 128, ROUND = 64, GRAIN = 8, MOST = 64, SLOTS = 640, ON_CU = 2;
 };
 constexpr int KT = 32;          // keys of a wave's tile, few pairs
 constexpr int FEW_PAIRS = 32;   // more pairs of a request and key head are rows
@@ -174,15 +174,15 @@ __device__ __forceinline__ Split split_of(const Attn &a, const Req &q, int chunk
 // Rounds of a share, of `rounds` of all tiles for one head and `tiles` of them, and whether so many pieces and
 // slots of it will do (else a little longer shares are tried, at the end nothing is split). Rows that one round of
 // workgroups takes are divided into no more than that, those of not much more than one into shares half as
-// long: 136 tiles of 100 rounds in 544 shares took 139 us, in 408 112 (with their join as it was then). Of few
-// pairs shares may be of half a GRAIN as long as each has a CU of its own: one token over 4000 keys of 8 heads
-// 14.5 us in 64 shares, 11.7 in 128, but 8 of them over 2000 18.4 in 256 and 19.5 in 512. Requests of up to a
-// GRAIN are not split: 333 keys of 32 heads took 8.4 us whole (6.6 since) and 10.2 in two shares.
+// long: 136 tiles of 100 rounds in 544 shares took 139 us, in 408 112 (with their join as it was then). Shares may
+// be of half a GRAIN as long as each has a CU of its own: one token over 4000 keys of 8 heads 14.5 us in 64
+// shares, 11.7 in 128, but 8 of them over 2000 18.4 in 256 and 19.5 in 512; 221 rows of 3 heads over 10114 keys of
+// one 41.0 in 120 shares, 32.7 in 240 (with smaller teams of the join). Requests of up to a GRAIN are not split: 333 keys of 32 heads took 8.4 us whole (6.6 since) and 10.2 in two shares.
 template <typename F>
 __device__ __forceinline__ int chunk_of(const Attn &a, float rounds, int64_t tiles) {
     const int want = a.want[F::ROWS], c = (int)(rounds * (float)a.Hkv / (float)want) + 1;
-    if (F::ROWS) return max(F::GRAIN, tiles * a.Hkv > want && tiles * a.Hkv < 2 * want ? (c + 1) / 2 : c);
-    return max(rounds * (float)a.Hkv <= (float)(want / 2) ? F::GRAIN / 2 : F::GRAIN, c);
+    const int least = rounds * (float)a.Hkv <= (float)(want / F::ON_CU * (F::GRAIN / 2)) ? F::GRAIN / 2 : F::GRAIN;
+    return max(least, F::ROWS && tiles * a.Hkv > want && tiles * a.Hkv < 2 * want ? (c + 1) / 2 : c);
 }
 template <typename F>
 __device__ __forceinline__ bool will_do(const Attn &a, int64_t pieces, int64_t slots, int64_t tiles, int most) {
@@ -455,8 +455,9 @@ __device__ __forceinline__ void join_shares(const Attn &a, int first, int n, int
         else
             join_vectors<F, D, 0, D / 32, 4>(pb, n, step, pairs, fac, last, row);
     } else {
-        join_vectors<F, D, 0, D / 16, 3>(pb, n, step, pairs, fac, last, row);
-        join_vectors<F, D, D / 16, D / 16, 3>(pb, n, step, pairs, fac, last, row);
+        // (two shares in flight: with three, teams of 4 read two for nothing, 28.8 us for 27.0 below)
+        join_vectors<F, D, 0, D / 16, 2>(pb, n, step, pairs, fac, last, row);
+        join_vectors<F, D, D / 16, D / 16, 2>(pb, n, step, pairs, fac, last, row);
     }
 }
 
@@ -472,14 +473,18 @@ __device__ __forceinline__ bool last_of(uint32_t *counter, int n) {
     __syncthreads();
     return arrived == (uint32_t)n - 1;
 }
-// A share's sums are stored: the last of every TEAM shares joins them, the last of the teams those.
+// A share's sums are stored: the last of every team of shares joins them, the last of the teams those. A slot of rows
+// is 66 KB at D = 128, so their teams are small and join at the same time: 16 rows of 32 heads over 8000 keys
+// 34.5 us in teams of 16, 30.5 of 8, 28.5 of 4 (27.0 with two shares read at a time).
 template <typename F, int D, typename Row>
 __device__ __forceinline__ void arrive(const Attn &a, const Piece &pc, int pairs, float *lds, Row row) {
-    const int teams = (pc.shares + TEAM - 1) / TEAM, first = pc.share / TEAM * TEAM, n = min(TEAM, pc.shares - first);
+    constexpr int OF = F::ROWS ? 4 : TEAM;
+    static_assert(F::MOST <= OF * TEAM);
+    const int teams = (pc.shares + OF - 1) / OF, first = pc.share / OF * OF, n = min(OF, pc.shares - first);
     if (!last_of(&a.count[pc.slot + first], n)) return;
     join_shares<F, D>(a, pc.slot + first, n, 1, pairs, lds, teams == 1, row);
     if (teams == 1 || !last_of(&a.count[Few::SLOTS + Rows::SLOTS + pc.slot], teams)) return;
-    join_shares<F, D>(a, pc.slot, teams, TEAM, pairs, lds, true, row);
+    join_shares<F, D>(a, pc.slot, teams, OF, pairs, lds, true, row);
 }
 
 // The values of a 32-key tile that are no numbers, taken out of it (v: an A operand per granule and 32
@@ -1064,8 +1069,8 @@ hipError_t launch_paged_attention(const PageDims &d, const uint8_t *layer, const
            (int32_t)std::min<int64_t>(x.sinks, 0x7fffffff), x.scale * 1.4426950408889634f, x.out, nullptr, nullptr, 0, 0,
            g > 1 ? ~0ull / (uint64_t)g + 1 : 0, {}};
     const int cus = std::max(device_cu_count(), 1);
-    a.want[0] = std::min(4 * cus, Few::SLOTS);
-    a.want[1] = std::min(2 * cus, Rows::SLOTS);  // two workgroups a CU
+    a.want[0] = std::min(Few::ON_CU * cus, Few::SLOTS);
+    a.want[1] = std::min(Rows::ON_CU * cus, Rows::SLOTS);
     // Workgroups: of a request with few pairs one for each key head, of one with many at most a tile more
     // than its pairs fill, and the shares. Without starts every request has g pairs.
     const bool rows = x.starts ? x.rows * g > FEW_PAIRS : g > FEW_PAIRS, few = g <= FEW_PAIRS;
@@ -1075,7 +1080,7 @@ hipError_t launch_paged_attention(const PageDims &d, const uint8_t *layer, const
         a.count = (uint32_t *)scratch;
         a.part = (float *)((char *)scratch + PAGED_COUNTER_BYTES);
         const int64_t keys = x.window ? std::min<int64_t>(cap, std::min<int64_t>(x.sinks, cap) + std::min<int64_t>(x.window, cap) + 512) : cap;
-        many = std::min(many * (1 + keys / (Rows::GRAIN * Rows::ROUND)), many + 2 * a.want[1]);
+        many = std::min(many * (1 + keys / (Rows::GRAIN / 2 * Rows::ROUND)), many + 2 * a.want[1]);
         tokens = std::min(tokens * (1 + keys / (Few::GRAIN / 2 * Few::ROUND)), tokens + a.want[0]);
     }
     a.turn = (cus + 7) / 8 * 8;

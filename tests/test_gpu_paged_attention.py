@@ -131,6 +131,21 @@ def test_one_request_in_as_many_shares_as_there_may_be(torch_cuda, qctx, heads, 
     c.free()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("keys", [512, 513, 700, 1030, 1280, 1285, 2100, 4097, 4200, 16000])
+def test_rows_in_few_and_many_shares(torch_cuda, qctx, keys, d):
+    """Two to 64 shares of a tile of rows: teams of them that are whole, of one share, and one alone; the same
+    outputs each time."""
+    c = Case(torch_cuda, qctx, [keys], [40], 2, 1, d, 64, seed=keys)
+    c.check()
+    before = c.out.clone()
+    for _ in range(3):
+        c.check()
+        assert torch_cuda.equal(before, c.out)
+    c.check(window=keys // 2 + 3, sinks=2)
+    c.free()
+
+
 def test_many_requests(torch_cuda, qctx):
     rng = np.random.default_rng(5)
     lengths = rng.integers(1, 90, 3000)
