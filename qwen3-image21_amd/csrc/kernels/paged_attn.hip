@@ -18,7 +18,7 @@
 // join their sums through LDS. One token over 131001 keys of 8 heads: 103 us, 5.2 TB/s.
 //
 // More (many_pairs) are bound by the matrix pipe and the softmax beside it: four waves share 64-key tiles in
-// LDS, where each key is read by 128 pairs. A prompt of 8395 tokens, 32 heads over 8, causal: 582 us, 0.99
+// LDS, where each key is read by 128 pairs. A prompt of 8395 tokens, 32 heads over 8, causal: 585 us, 0.99
 // PFLOP/s (two such workgroups on a CU take 2.1 us a tile each, one alone 1.7).
 //
 // Long requests in few workgroups are split over their keys. The host does not know the lengths, so
