@@ -311,8 +311,9 @@ int64_t qimm_kv_device_bytes(const qimm_kv *kv);
  * The queue is a ring of `pages` entries, state[0] the entry of the next free page and state[1]
  * their number; pages given back go to its end, free from the next step on.
  * A request is refused, and has its length left, its rows slot -1 and position 0, where its table or the
- * rows have no room for it, its length is negative, or it needs pages and, with the pages that it and
- * the requests before it ask for, more than are free. state_out: the two, the rows, the requests refused.
+ * rows have no room for it, it would have 2^31 tokens or more, its length is negative, or it needs pages and,
+ * with the pages that it and the requests before it ask for, more than are free. state_out: the two, the rows,
+ * the requests refused.
  * lengths_out and state_out may be lengths and state; everything else is distinct. work:
  * qimm_page_plan_work(requests) int32 of scratch; positions may be NULL. Entries of a table past a
  * request's pages, and of the queue outside its free pages, are not looked at. Allocates nothing and

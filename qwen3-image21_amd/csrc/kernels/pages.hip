@@ -74,7 +74,8 @@ __device__ __forceinline__ Step step_of(const PagePlanArgs &p, int64_t r) {
     s.old = p.lengths[r];
     s.add = p.added[r];
     const int ps = p.page_size;
-    const int64_t room = p.max_pages * ps, after = (int64_t)s.old + s.add;
+    // (lengths and positions are 32 bits, a table may be wider)
+    const int64_t room = min(p.max_pages * ps, (int64_t)0x7fffffff), after = (int64_t)s.old + s.add;
     s.have = s.old > 0 ? (int)min(((int64_t)s.old + ps - 1) / ps, p.max_pages) : 0;
     s.fits = s.add > 0 && s.old >= 0 && after <= room;
     s.need = s.fits ? (int)((after + ps - 1) / ps) - s.have : 0;
