@@ -309,7 +309,10 @@ int64_t qimm_kv_device_bytes(const qimm_kv *kv);
  * the number of tokens before it in the request (the row of a RoPE table). Rows from starts[requests] to max_rows
  * get slot -1 and position 0, so that a captured step may have a fixed number of rows.
  * The queue is a ring of `pages` entries, state[0] the entry of the next free page and state[1]
- * their number; pages given back go to its end, free from the next step on.
+ * their number; pages given back go to its end, free from the next step on, as many as the ring has
+ * room for. A page that several requests hold is the caller's to look after: given back with each of them
+ * it is in the queue as often, and later two requests get it; a request that goes on in the
+ * free part of such a page writes there for the others too.
  * A request is refused, and has its length left, its rows slot -1 and position 0, where its table or the
  * rows have no room for it, it would have 2^31 tokens or more, its length is negative, or it needs pages and,
  * with the pages that it and the requests before it ask for, more than are free. state_out: the two, the rows,

@@ -83,10 +83,10 @@ __device__ __forceinline__ Step step_of(const PagePlanArgs &p, int64_t r) {
     return s;
 }
 
-// entry i of the queue after its head, i < 2 * pages
+// entry i of the queue after its head, i < pages
 __device__ __forceinline__ int32_t *queue_at(const PagePlanArgs &p, int head, int64_t i) {
     int64_t at = head + i;
-    while (at >= p.pages) at -= p.pages;
+    if (at >= p.pages) at -= p.pages;
     return p.queue + at;
 }
 
@@ -109,8 +109,8 @@ __device__ __forceinline__ void fill_row(const PagePlanArgs &p, int64_t t, int64
 // The pages of a request given back, `lane` of 64: `back` entries of the queue come before its first.
 __device__ __forceinline__ void give_back(const PagePlanArgs &p, int64_t r, int old, int64_t back, int head, int free, int lane) {
     const int have = (int)min(((int64_t)old + p.page_size - 1) / p.page_size, p.max_pages);
-    // (entries past the queue's size would be pages given back twice)
-    for (int k = lane; k < have && free + back + k < 2 * p.pages; k += 64)
+    // (more pages than the queue has room for are pages given back twice: those that are free stay)
+    for (int k = lane; k < have && free + back + k < p.pages; k += 64)
         *queue_at(p, head, free + back + k) = p.tables[r * p.max_pages + k];
 }
 
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(THREADS) void page_plan_kernel(const PagePlanArgs p
         int64_t to = (int64_t)head + taken;
         if (to >= p.pages) to -= p.pages;
         p.state_out[0] = (int)to;
-        p.state_out[1] = (int)min((int64_t)free - taken + all.freed, p.pages);
+        p.state_out[1] = free - taken + (int)min((int64_t)all.freed, p.pages - free);
         p.state_out[2] = rows;
         p.state_out[3] = refused;
         if (!FILL) {
