@@ -22,6 +22,9 @@ namespace {
 
 constexpr int PLAN_REQUESTS = 1024, PLAN_ROWS = 2048;  // what one launch takes
 
+// four int32 of the plan's work, which is aligned as its caller's int32 are
+typedef int work4 __attribute__((ext_vector_type(4), aligned(4)));
+
 // A step's sums over the requests, in 32 bits that stop at the largest number: rows up to max_rows, pages up
 // to those that are free and back to the queue are all that counts.
 struct Sums {
@@ -173,7 +176,7 @@ __global__ __launch_bounds__(THREADS) void page_plan_kernel(const PagePlanArgs p
             of[tid] = w;
             starts[tid] = start;
         } else {
-            *(int4 *)(p.work + 4 * r) = w;
+            *(work4 *)(p.work + 4 * r) = work4{w.x, w.y, w.z, w.w};
         }
         p.starts[r] = start;
         p.lengths_out[r] = s.add < 0 ? 0 : served ? s.old + s.add : s.old;
@@ -276,7 +279,7 @@ __global__ __launch_bounds__(256) void page_fill_kernel(const PagePlanArgs p) {
             else
                 hi = mid;
         }
-        const int4 w = *(const int4 *)(p.work + 4 * (r0 + lo));
+        const work4 w = *(const work4 *)(p.work + 4 * (r0 + lo));
         fill_row(p, t, r0 + lo, w.x, w.y, w.z, head);
     }
     if (t >= all && t < p.max_rows) {
@@ -284,7 +287,10 @@ __global__ __launch_bounds__(256) void page_fill_kernel(const PagePlanArgs p) {
         if (p.positions) p.positions[t] = 0;
     }
     give_back_all(p, (int64_t)blockIdx.x * 4 + (tid >> 6), (int64_t)gridDim.x * 4, head, free,
-                  [&](int64_t r) { return *(const int4 *)(p.work + 4 * r); });
+                  [&](int64_t r) {
+                      const work4 w = *(const work4 *)(p.work + 4 * r);
+                      return make_int4(w.x, w.y, w.z, w.w);
+                  });
 }
 
 // ---- rows to slots and back ----

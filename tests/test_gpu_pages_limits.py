@@ -1,10 +1,11 @@
-"""Steps of the page tables at the limits of their numbers: tokens past 31 bits."""
+"""Steps of the page tables at the limits of their numbers and arrays: tokens past 31 bits, scratch anywhere."""
 import numpy as np
 import pytest
 
+import paged_ref
 import qimm
 from gpu_util import host, stream
-from test_gpu_pages import Plan
+from test_gpu_pages import Plan, a_case
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +31,18 @@ def test_a_table_wider_than_a_length_can_be(torch_cuda, qctx, max_rows):
     tables[4, 0] = 3
     p.check(dict(tables=tables, lengths=np.array([most - 2, most - 5, most, most, 2]), queue=queue, state=np.array([1, 3, 17, 2]),
                  starts=np.array([0, 3, 13, 14, 15, 17]), slots=slots, positions=positions))
+
+
+@pytest.mark.parametrize("at", [1, 2, 3])
+@pytest.mark.parametrize("n", [60, 1025, 5000])
+def test_scratch_on_any_int32(torch_cuda, qctx, n, at):
+    """work begins 4, 8 and 12 bytes behind a multiple of 16; what lies around it stays."""
+    torch = torch_cuda
+    case = a_case(np.random.default_rng(n), n, 16, 60, 9)
+    p = Plan(torch, 16, *case)
+    size = qimm.page_plan_work(n)
+    room = torch.full((size + 8,), -99, dtype=torch.int32, device="cuda")
+    p.call.work = room[at:].data_ptr()
+    qctx.page_plan(p.call, stream(torch))
+    p.check(paged_ref.plan(16, len(case[3]), *case))
+    assert (host(room)[:at] == -99).all() and (host(room)[at + size:] == -99).all()
