@@ -1061,7 +1061,7 @@ size_t paged_attention_scratch(int d) {
 hipError_t launch_paged_attention(const PageDims &d, const uint8_t *layer, const PagedAttnArgs &x, void *scratch,
                                   hipStream_t stream) {
     if (x.rows <= 0 || x.requests <= 0) return hipSuccess;
-    const int64_t g = x.heads / d.kv_heads, cap = std::min<int64_t>(x.max_pages * d.page_size, 0x7fffffff - 64);
+    const int64_t g = x.heads / d.kv_heads, cap = std::min<int64_t>(std::min<int64_t>(x.max_pages, 0x7fffffff) * d.page_size, 0x7fffffff - 64);
     const int ps16 = d.page_size / 16;
     Attn a{x.q, x.q_row, x.q_head, layer, d.pages, x.tables, x.max_pages, x.lengths, x.starts, (int32_t)x.requests,
            (int32_t)x.rows, d.kv_heads, (int32_t)g, ps16, (uint32_t)(((1ull << 32) + ps16 - 1) / ps16),
