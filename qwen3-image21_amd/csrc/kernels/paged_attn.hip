@@ -404,10 +404,11 @@ __device__ __forceinline__ void join_vectors(const Part &pb, int n, uint32_t ste
                 uint32_t at;
                 int p, d;
                 vector_at<F, D>(I0 + i, at, p, d);
-                const float f = s0 + s < n && p < pairs ? fac[(s0 + s) * F::TM + p] : 0.f;
-                if (f != 0.f)  // (an infinity of a share that does not count would be NaN)
+                if (s0 + s >= n) continue;  // (read once more)
+                // a share that weighs nothing counts too: what it has seen may be no number
+                const float f = p < pairs ? fac[(s0 + s) * F::TM + p] : 0.f;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) x[i][e] += y[s][i][e] * f;
+                for (int e = 0; e < 4; e++) x[i][e] += y[s][i][e] * f;
             }
     }
 #pragma unroll
