@@ -365,11 +365,12 @@ int qimm_pages_load(const qimm_pages *pg, int64_t layer, uint16_t *k, uint16_t *
  * (qimm_page_plan's lengths_out); starts as qimm_page_plan's, or NULL where row r is request r's one.
  * Row i of a request's n rows is its token p = length - n + i. It sees every key of its request, or
  * (causal) keys j <= p; in a window (> 0) of them j > p - window, and the first `sinks` keys,
- * j < sinks. A row that sees no key (p < 0) gives zeros; rows of no request are left as they were.
- * What keys hold that a row does not see does not count, NaN and infinities either. A table entry
- * outside the pages hides its keys. Lengths past the table are cut to it. scale: positive. Rows of
- * a refused request are of no use. Requests may have pages in common. q, its
- * strides and out are 16-byte aligned; up to 65536 requests. Allocates nothing and can be captured. */
+ * j < sinks. A row that sees no key (p < 0) gives zeros, one that sees only scores of -infinity NaN; rows
+ * of no request are left as they were. What keys hold that a row does not see does not count, NaN and
+ * infinities either. A table entry outside the pages hides its keys. Lengths past the table are cut to it.
+ * scale: positive; scores times scale are f32, below 2^30 where they are finite. Rows of a refused request
+ * are of no use. Requests may have pages in common. q, its strides and out are 16-byte aligned; up to
+ * 65536 requests. Allocates nothing and can be captured. */
 typedef struct {
     const uint16_t *q;
     int64_t q_row, q_head;
