@@ -19,6 +19,8 @@ int set_err(qimm_ctx *ctx, int status, const std::string &msg) {
 }
 
 int hip_err(qimm_ctx *ctx, hipError_t e, const char *what) {
+    // HIP keeps the error for the next hipGetLastError, which a launch asks, the caller's own too: it is told here
+    (void)hipGetLastError();
     char buf[512];
     snprintf(buf, sizeof(buf), "HIP error %d (%s) in %s", (int)e, hipGetErrorString(e), what);
     return set_err(ctx, e == hipErrorOutOfMemory ? QIMM_ERR_OOM : QIMM_ERR_HIP, buf);
