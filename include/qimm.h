@@ -369,8 +369,8 @@ int qimm_pages_load(const qimm_pages *pg, int64_t layer, uint16_t *k, uint16_t *
  * of no request are left as they were. What keys hold that a row does not see does not count, NaN and
  * infinities either. A table entry outside the pages hides its keys. Lengths past the table are cut to it.
  * scale: positive; scores times scale are f32, below 2^30 where they are finite. Rows of a refused request
- * are of no use. Requests may have pages in common. q, its strides and out are 16-byte aligned; up to
- * 65536 requests. Allocates nothing and can be captured. */
+ * are of no use. Requests may have pages in common. q, its strides and out are 16-byte aligned, out apart
+ * from q; up to 65536 requests. Allocates nothing and can be captured. */
 typedef struct {
     const uint16_t *q;
     int64_t q_row, q_head;

@@ -255,7 +255,8 @@ __device__ __forceinline__ T lane_of(T v, int lane) {
 
 // The piece of workgroup `item` of at most `most`, in request order; false: there is none. Up to 64
 // requests every wave counts them by itself, a lane each; of more, every thread counts its share and the one whose
-// share has the piece looks which.
+// share has the piece looks which: as much work as requests times workgroups. A token of each of 2048 requests of 100
+// to 2000 keys of 8 heads 988 us, their bytes 1033; but 16384 of up to 520 keys 12 ms, their bytes 0.6.
 template <typename F>
 __device__ __forceinline__ bool piece_of(const Attn &a, int item, int most, Piece &out) {
     if (!F::ROWS && !a.starts && !a.count) {

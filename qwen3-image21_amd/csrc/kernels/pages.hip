@@ -10,7 +10,8 @@
 // The store. Bound by bytes. Where 16 rows are the 16 slots of a granule, in order, a wave takes them: keys as
 // they are read are written 1 KB in a row, values are turned over in registers, four rows and eight dims a
 // lane, and gathered in LDS (paged.h). Other rows, the ends of a request and single tokens, are
-// written 16 B of a key and 2 B of a value at a time.
+// written 16 B of a key and 2 B of a value at a time. 8395 rows of 32 heads of 128: f32 88 us (4.7 TB/s), bf16
+// 55 to 60, f16 59 to 65, back 51.
 #include <algorithm>
 #include <type_traits>
 
